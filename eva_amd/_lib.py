@@ -19,6 +19,7 @@ EVAMX_OK, EVAMX_EINVAL, EVAMX_ELAUNCH, EVAMX_ENOSPACE = 0, -1, -2, -3
 DTYPE_F16, DTYPE_BF16 = 0, 1
 SCORE_SIGMOID, SCORE_SQRT_SOFTPLUS = 0, 1
 ERR_EXPERT_RANGE, ERR_RATE = 1, 2
+W4_MAX_DIM, W4_MAX_COUNT = 1 << 18, 1024       # EVAMX_W4_MAX_DIM, matrices of a stack
 STRICT_MAX_ROWS, STRICT_MAX_SLOTS = 64, 256      # EVAMX_STRICT_MAX_ROWS / EVAMX_STRICT_MAX_SLOTS
 
 _vp = ctypes.c_void_p
@@ -44,6 +45,12 @@ class MoeArgs(ctypes.Structure):
                 ("shared_gate_w", _vp)]
 
 
+class W4Desc(ctypes.Structure):
+    """evamx_w4_weight."""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("zeros", _vp), ("count", _i32), ("n_out", _i32), ("n_in", _i32),
+                ("group", _i32), ("scale_dtype", _i32)]
+
+
 class EvamxError(RuntimeError):
     pass
 
@@ -58,6 +65,14 @@ _SIGNATURES = {
     "evamx_exl3_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "evamx_exl3_linear": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _f32,
                                          _vp, _vp, ctypes.c_size_t, _vp]),
+    "evamx_w4_stored_group": (ctypes.c_int, [ctypes.c_int]),
+    "evamx_w4_code_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "evamx_w4_group_count": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "evamx_w4_pack": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.POINTER(W4Desc), _vp]),
+    "evamx_w4_dequant": (ctypes.c_int, [ctypes.POINTER(W4Desc), _vp, _vp]),
+    "evamx_w4_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),
+    "evamx_w4_linear": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.POINTER(W4Desc), _vp,
+                                       _vp, ctypes.c_int64, _vp, ctypes.c_size_t, _vp]),
     "evamx_router_logits": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int,
                                            ctypes.c_int, _vp, _vp]),
     "evamx_route_topk": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _f32,

@@ -10,7 +10,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import MoeArgs, MoeShape, check, lib, ptr, stream_handle
+from ._lib import MoeArgs, MoeShape, W4Desc, check, lib, ptr, stream_handle
 
 SCORE_FNS = {"sigmoid": _lib.SCORE_SIGMOID, "sqrt_softplus": _lib.SCORE_SQRT_SOFTPLUS}
 RATES = (2.0, 3.0, 4.0, 5.0)
@@ -71,6 +71,121 @@ def exl3_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, svh: 
     _dev(workspace, "workspace", torch.uint8, 1)
     check(lib().evamx_exl3_linear(ptr(x), m, n_in, n_out, ptr(trellis), ptr(suh), ptr(svh), float(bits), ptr(out),
                                   ptr(workspace), workspace.numel(), stream_handle(x.device)), "evamx_exl3_linear")
+    return out
+
+
+class W4Weight:
+    """A stack of 4-bit matrices with group scales in the layout the kernels read (``w4_pack`` makes it):
+    ``W[n, k] = scale[n, k // group] * (code[n, k] - zero[n, k // group])``, zero 8 without zero points."""
+
+    def __init__(self, count: int, n_out: int, n_in: int, group: int, scale_dtype: torch.dtype, zeros: bool, device):
+        stored = lib().evamx_w4_stored_group(group)
+        if stored == 0:
+            raise ValueError(f"group {group} is not a positive multiple of 32")
+        if scale_dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("scales must be fp16 or bf16")
+        nbytes, groups = lib().evamx_w4_code_bytes(count, n_out, n_in), lib().evamx_w4_group_count(count, n_out, n_in, stored)
+        if nbytes == 0:
+            raise ValueError(f"{count} matrices [{n_out}, {n_in}] outside 1..{_lib.W4_MAX_COUNT} and 1..{_lib.W4_MAX_DIM}")
+        self.count, self.n_out, self.n_in, self.group = count, n_out, n_in, group
+        self.device = torch.device(device)
+        self.codes = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.scales = torch.empty(groups, dtype=scale_dtype, device=device)
+        self.zeros = torch.empty(groups, dtype=torch.uint8, device=device) if zeros else None
+        self.desc = W4Desc(ptr(self.codes), ptr(self.scales), ptr(self.zeros), count, n_out, n_in, stored,
+                           _DTYPES[scale_dtype])
+
+
+_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def w4_pack(codes: torch.Tensor, scales: torch.Tensor, *, n_in: int, group: int, zeros: torch.Tensor | None = None) -> W4Weight:
+    """Lay 4-bit weights out for ``w4_linear`` / ``w4_moe_forward``. ``codes`` uint8 ``[(count,) n_out,
+    ceil(n_in / 2)]``, two codes of a row to a byte, the even one in the lower half; ``scales`` fp16 or
+    bf16 ``[(count,) n_out, ceil(n_in / group)]``; ``zeros`` uint8 like the scales, the codes that stand
+    for zero (0..15; without them 8). ``group``: a multiple of 32 input features that share a scale."""
+    _dev(codes, "codes", torch.uint8)
+    if codes.ndim not in (2, 3):
+        raise ValueError("codes must be [n_out, ceil(n_in / 2)] or a stack of such")
+    _dev(scales, "scales", None, codes.ndim)
+    if group < 32 or group % 32:
+        raise ValueError(f"group {group} is not a positive multiple of 32")
+    lead, n_out = tuple(codes.shape[:-2]), codes.shape[-2]
+    groups = (*lead, n_out, -(-n_in // group))
+    if codes.shape[-1] != (n_in + 1) // 2 or tuple(scales.shape) != groups:
+        raise ValueError(f"codes {tuple(codes.shape)} / scales {tuple(scales.shape)} disagree with n_in {n_in}, group {group}")
+    if zeros is not None:
+        _dev(zeros, "zeros", torch.uint8, codes.ndim)
+        if tuple(zeros.shape) != groups:
+            raise ValueError(f"zeros must have the scales' shape {groups}, got {tuple(zeros.shape)}")
+    for t, name in ((scales, "scales"), (zeros, "zeros")):
+        if t is not None and t.device != codes.device:
+            raise ValueError(f"{name} is on {t.device}, the codes on {codes.device}")
+    w = W4Weight(lead[0] if lead else 1, n_out, n_in, group, scales.dtype, zeros is not None, codes.device)
+    with torch.cuda.device(w.device):
+        check(lib().evamx_w4_pack(ptr(codes), ptr(scales), ptr(zeros), group, ctypes.byref(w.desc),
+                                  stream_handle(w.device)), "evamx_w4_pack")
+    return w
+
+
+def w4_dequant(weight: W4Weight) -> torch.Tensor:
+    """fp32 ``[count, n_out, n_in]`` of packed 4-bit weights."""
+    out = torch.empty(weight.count, weight.n_out, weight.n_in, dtype=torch.float32, device=weight.device)
+    with torch.cuda.device(weight.device):
+        check(lib().evamx_w4_dequant(ctypes.byref(weight.desc), ptr(out), stream_handle(weight.device)), "evamx_w4_dequant")
+    return out
+
+
+def _row_stride(t: torch.Tensor, name: str, dtype=None) -> int:
+    """Row stride of a 2-dim device tensor whose rows are contiguous and do not overlap (a single row: any)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.ndim != 2:
+        raise ValueError(f"{name} must be a 2-dim device tensor")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    rows, cols = t.shape
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"{name} must have unit column stride and non-overlapping rows")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _no_grad(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} has no backward: call it under torch.no_grad() or with detached tensors")
+
+
+def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ W.T + bias`` on 4-bit weights with group scales: ``x`` fp16 or bf16 ``[1..65536, n_in]``
+    (rows of any stride), ``bias`` and the result of x's dtype, summed in fp32 and rounded once. ``out``
+    must not overlap ``x``."""
+    x_stride = _row_stride(x, "x")
+    if x.dtype not in _DTYPES:
+        raise ValueError("x must be fp16 or bf16")
+    rows = x.shape[0]
+    if weight.count != 1 or x.shape[1] != weight.n_in:
+        raise ValueError(f"x {tuple(x.shape)} does not fit {weight.count} matrices [{weight.n_out}, {weight.n_in}]")
+    if not 1 <= rows <= 65536:
+        raise ValueError(f"x has {rows} rows, a call takes 1..65536")
+    if bias is not None:
+        _dev(bias, "bias", x.dtype, 1)
+        if bias.numel() != weight.n_out:
+            raise ValueError(f"bias must be [{weight.n_out}]")
+    if out is None:
+        out = torch.empty(rows, weight.n_out, dtype=x.dtype, device=x.device)
+    out_stride = _row_stride(out, "out", x.dtype)
+    if tuple(out.shape) != (rows, weight.n_out):
+        raise ValueError(f"out must be [{rows}, {weight.n_out}]")
+    _no_grad("w4_linear", x, bias, out)
+    if workspace is None:
+        workspace = torch.empty(lib().evamx_w4_linear_workspace_bytes(rows, weight.n_in), dtype=torch.uint8, device=x.device)
+    _dev(workspace, "workspace", torch.uint8, 1)
+    for t, name in ((weight, "weight"), (bias, "bias"), (out, "out"), (workspace, "workspace")):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    with torch.cuda.device(x.device):
+        check(lib().evamx_w4_linear(ptr(x), _DTYPES[x.dtype], x_stride, rows, ctypes.byref(weight.desc), ptr(bias), ptr(out),
+                                    out_stride, ptr(workspace), workspace.numel(), stream_handle(x.device)),
+              "evamx_w4_linear")
     return out
 
 

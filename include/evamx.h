@@ -72,6 +72,44 @@ int evamx_exl3_linear(const void* x_fp16, int rows, int in_features, int out_fea
                       const void* trellis, const void* suh_fp16, const void* svh_fp16, float bits,
                       void* y_fp16, void* workspace, size_t workspace_bytes, evamx_stream_t stream);
 
+/* ---- linear on 4-bit weights with group scales --------------------------------------------- */
+
+/* W[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), codes 0..15; without zero
+ * points zero is 8. A stack of `count` matrices [n_out][n_in] in the layout the kernels read,
+ * made by evamx_w4_pack; all pointers device, 16-byte aligned. */
+enum { EVAMX_W4_MAX_DIM = 1 << 18 };
+typedef struct evamx_w4_weight {
+    const void* codes;    /* evamx_w4_code_bytes(count, n_out, n_in) bytes */
+    const void* scales;   /* evamx_w4_group_count(count, n_out, n_in, group) values of scale_dtype */
+    const void* zeros;    /* as many bytes, or NULL (zero = 8) */
+    int32_t count, n_out, n_in;
+    int32_t group;        /* the stored group size: 32, 64 or 128 (evamx_w4_stored_group) */
+    int32_t scale_dtype;  /* EVAMX_DTYPE_F16 or EVAMX_DTYPE_BF16 */
+} evamx_w4_weight;
+
+/* The group size a matrix with groups of `group` (a multiple of 32) is stored with: the largest of
+ * 32, 64 and 128 that divides it (its scales are repeated); 0 for a group that is not supported. */
+int evamx_w4_stored_group(int group);
+/* Sizes of a packed stack; 0 for sizes outside 1..1024 matrices and 1..EVAMX_W4_MAX_DIM. */
+size_t evamx_w4_code_bytes(int count, int n_out, int n_in);
+size_t evamx_w4_group_count(int count, int n_out, int n_in, int group);
+/* Lay a stack out: codes uint8 [count][n_out][ceil(n_in / 2)] (the lower half of a byte is the even
+ * k), scales [count][n_out][ceil(n_in / group)] of w->scale_dtype, zeros likewise uint8 (codes
+ * 0..15) or NULL, written to the buffers of w. */
+int evamx_w4_pack(const uint8_t* codes, const void* scales, const uint8_t* zeros, int group,
+                  const evamx_w4_weight* w, evamx_stream_t stream);
+/* fp32 W[count][n_out][n_in] of a packed stack. */
+int evamx_w4_dequant(const evamx_w4_weight* w, float* out, evamx_stream_t stream);
+
+size_t evamx_w4_linear_workspace_bytes(int rows, int n_in);
+/* y[r][n] = sum_k x[r][k] W[n][k] + bias[n] for one matrix, summed in fp32 and rounded once. x and y
+ * fp16 or bf16 (x_dtype; the bias too), rows of x_stride and y_stride elements of any alignment;
+ * bias [n_out] or NULL; rows in 1..65536. A row's values are scaled by a power of two into fp16's
+ * range for the products, so bf16 values keep their bits down to 2^-28 of the row's largest. */
+int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int rows, const evamx_w4_weight* w,
+                    const void* bias, void* y, int64_t y_stride, void* workspace, size_t workspace_bytes,
+                    evamx_stream_t stream);
+
 /* ---- router ------------------------------------------------------------------------------ */
 
 /* logits[r][e] = sum_k float(x[r][k]) * gate_w[e][k] (fp32): the router gate GEMV of
