@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(HERE, "libevamx.so")
 ABI_VERSION = 5
 
 EVAMX_OK, EVAMX_EINVAL, EVAMX_ELAUNCH, EVAMX_ENOSPACE = 0, -1, -2, -3
-DTYPE_F16, DTYPE_BF16 = 0, 1
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 SCORE_SIGMOID, SCORE_SQRT_SOFTPLUS = 0, 1
 ERR_EXPERT_RANGE, ERR_RATE = 1, 2
 W4_MAX_DIM, W4_MAX_COUNT = 1 << 18, 1024       # EVAMX_W4_MAX_DIM, matrices of a stack
@@ -77,6 +77,11 @@ _SIGNATURES = {
                                            ctypes.c_int, _vp, _vp]),
     "evamx_route_topk": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _f32,
                                         _vp, _vp, _vp, _vp]),
+    "evamx_balance_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "evamx_balance_loss": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int,
+                                          ctypes.c_int, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "evamx_balance_grad": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                          ctypes.c_int, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp]),
     "evamx_prepare_routes_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),
     "evamx_prepare_routes": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                             _vp, _vp, ctypes.c_size_t, _vp]),

@@ -238,6 +238,111 @@ def route(x: torch.Tensor, gate_w: torch.Tensor, gate_b: torch.Tensor | None, to
     return w, idx
 
 
+_LOGIT_DTYPES = {torch.float32: _lib.DTYPE_F32, **_DTYPES}
+
+
+def _balance_args(logits, score_fn, seq_starts, token_mask):
+    """Checked (stride, sequences, starts, mask bytes) of a balance call."""
+    stride = _row_stride(logits, "logits")
+    if logits.dtype not in _LOGIT_DTYPES:
+        raise ValueError("logits must be fp32, bf16 or fp16")
+    if score_fn not in SCORE_FNS:
+        raise ValueError(f"score_fn {score_fn!r} not in {sorted(SCORE_FNS)}")
+    n = 1
+    if seq_starts is not None:
+        _dev(seq_starts, "seq_starts", torch.int32, 1)
+        n = seq_starts.numel() - 1
+        if n < 1:
+            raise ValueError("seq_starts must hold the start of each sequence and the last one's end")
+    if token_mask is not None:
+        _dev(token_mask, "token_mask", torch.bool, 1)
+        if token_mask.numel() != logits.shape[0]:
+            raise ValueError(f"token_mask must be [{logits.shape[0]}]")
+    for t, name in ((seq_starts, "seq_starts"), (token_mask, "token_mask")):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"{name} is on {t.device}, logits on {logits.device}")
+    return stride, n
+
+
+def balance_stats(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "sigmoid", seq_starts: torch.Tensor | None = None,
+                  token_mask: torch.Tensor | None = None):
+    """``(loss fp32 [S], counts int32 [S, E], tokens int32 [S])`` of ``balance_loss``, outside autograd."""
+    stride, n = _balance_args(logits, score_fn, seq_starts, token_mask)
+    rows, experts = logits.shape
+    _dev(sel, "sel", torch.int64, 2)
+    if sel.shape[0] != rows or sel.device != logits.device:
+        raise ValueError(f"sel must be [{rows}, topk] on {logits.device}, got {tuple(sel.shape)} on {sel.device}")
+    dev = logits.device
+    loss = torch.empty(n, dtype=torch.float32, device=dev)
+    counts = torch.empty(n, experts, dtype=torch.int32, device=dev)
+    tokens = torch.empty(n, dtype=torch.int32, device=dev)
+    ws = torch.empty(lib().evamx_balance_workspace_bytes(rows, experts, n), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        check(lib().evamx_balance_loss(ptr(logits), _LOGIT_DTYPES[logits.dtype], stride, rows, experts, ptr(sel), sel.shape[1],
+                                       SCORE_FNS[score_fn], ptr(seq_starts), n, ptr(token_mask), ptr(loss), ptr(counts), ptr(tokens),
+                                       ptr(ws), ws.numel(), stream_handle(dev)), "evamx_balance_loss")
+    return loss, counts, tokens
+
+
+def balance_loss_grad(grad_loss: torch.Tensor, logits: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor, topk: int, *,
+                      score_fn: str = "sigmoid", seq_starts: torch.Tensor | None = None,
+                      token_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of ``(grad_loss * loss).sum()`` with respect to the logits, for the ``counts`` and
+    ``tokens`` that ``balance_stats`` gave for the same arguments; zero for rows that do not count."""
+    stride, n = _balance_args(logits, score_fn, seq_starts, token_mask)
+    rows, experts = logits.shape
+    for t, name, dtype, shape in ((grad_loss, "grad_loss", torch.float32, (n,)), (counts, "counts", torch.int32, (n, experts)),
+                                  (tokens, "tokens", torch.int32, (n,))):
+        _dev(t, name, dtype)
+        if tuple(t.shape) != shape or t.device != logits.device:
+            raise ValueError(f"{name} must be {shape} on {logits.device}, got {tuple(t.shape)} on {t.device}")
+    grad = torch.empty(rows, experts, dtype=logits.dtype, device=logits.device)
+    with torch.cuda.device(logits.device):
+        check(lib().evamx_balance_grad(ptr(grad_loss), ptr(logits), _LOGIT_DTYPES[logits.dtype], stride, rows, experts, topk,
+                                       SCORE_FNS[score_fn], ptr(seq_starts), n, ptr(token_mask), ptr(counts), ptr(tokens), ptr(grad),
+                                       stream_handle(logits.device)), "evamx_balance_grad")
+    return grad
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, sel, score_fn, seq_starts, token_mask):
+        loss, counts, tokens = balance_stats(logits, sel, score_fn=score_fn, seq_starts=seq_starts, token_mask=token_mask)
+        ctx.save_for_backward(logits, counts, tokens, seq_starts, token_mask)
+        ctx.topk, ctx.score_fn = sel.shape[1], score_fn
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss, _):
+        logits, counts, tokens, seq_starts, token_mask = ctx.saved_tensors
+        grad = balance_loss_grad(grad_loss.contiguous(), logits, counts, tokens, ctx.topk, score_fn=ctx.score_fn,
+                                 seq_starts=seq_starts, token_mask=token_mask)
+        return grad, None, None, None, None
+
+
+def balance_loss(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "sigmoid", seq_starts: torch.Tensor | None = None,
+                 token_mask: torch.Tensor | None = None):
+    """Balance loss of each sequence and the picks of each expert, ``(loss fp32 [S], counts int32 [S, E])``,
+    for router ``logits [T, E]`` (fp32, bf16 or fp16) and their routes ``sel`` int64 ``[T, topk]`` (``route_topk``).
+
+    With ``p = score / score.sum(1)``, ``n`` tokens and ``c_e`` picks of expert e in a sequence, the loss is
+    ``sum_e (E c_e / (topk n)) (sum_t p_te / n)``: 1 where picks and shares are even, larger where the experts
+    that are picked often also have large scores. It is differentiable in the logits; the counts (which serve
+    a selection bias as well as the loss) are constants. ``seq_starts`` int32 ``[S + 1]`` ascending: sequence
+    s is rows ``seq_starts[s]`` to ``seq_starts[s + 1]``, and rows of none count nowhere; without it all rows
+    are one sequence. ``token_mask`` bool ``[T]``: rows that count. A sequence without such rows has loss 0.
+    Picks outside ``[0, E)`` are not counted.
+
+    The backward pass is not for a graph capture (autograd's own streams and accumulators are not): there call
+    ``balance_stats`` and ``balance_loss_grad``."""
+    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad and logits.is_cuda and \
+            torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("balance_loss is not captured with a backward pass: call balance_stats and balance_loss_grad")
+    return _BalanceLoss.apply(logits, sel, score_fn, seq_starts, token_mask)
+
+
 def prepare_routes_workspace_bytes(capacity: int, topk: int) -> int:
     n = lib().evamx_prepare_routes_workspace_bytes(capacity, topk)
     if n == 0:

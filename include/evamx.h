@@ -38,7 +38,7 @@ extern "C" {
 typedef struct ihipStream_t* evamx_stream_t; /* hipStream_t */
 
 enum { EVAMX_OK = 0, EVAMX_EINVAL = -1, EVAMX_ELAUNCH = -2, EVAMX_ENOSPACE = -3 };
-enum { EVAMX_DTYPE_F16 = 0, EVAMX_DTYPE_BF16 = 1 };
+enum { EVAMX_DTYPE_F16 = 0, EVAMX_DTYPE_BF16 = 1, EVAMX_DTYPE_F32 = 2 }; /* x: the first two */
 enum { EVAMX_SCORE_SIGMOID = 0, EVAMX_SCORE_SQRT_SOFTPLUS = 1 };
 /* Device-side error flags (sticky bits in the workspace, read with evamx_moe_flags_ptr). */
 enum { EVAMX_ERR_EXPERT_RANGE = 1, EVAMX_ERR_RATE = 2 };
@@ -126,6 +126,28 @@ int evamx_router_logits(const void* x, int x_dtype, int x_stride, int rows, cons
 int evamx_route_topk(const float* logits, const float* sel_bias, int rows, int n_experts, int topk,
                      int score_fn, float route_scale, int64_t* indices, float* weights, void* rw_fp16,
                      evamx_stream_t stream);
+
+/* Balance of a router: with a = score(logits), p = a / sum a, c[s][e] the picks of expert e among
+ * the n valid tokens of sequence s (sel entries outside [0, experts) are no pick),
+ *   loss[s] = sum_e f_e P_e,  f_e = experts * c_e / (topk * n),  P_e = sum_t p_te / n
+ * (1 for even picks and shares; 0 for a sequence without tokens). logits: device fp32, bf16 or fp16
+ * [rows][stride]; sel: int64 [rows][topk]; sequence s is rows starts[s] .. starts[s + 1] - 1 (int32
+ * [sequences + 1], ascending; values are taken into 0..rows), or all rows for one sequence with
+ * starts NULL; rows outside every sequence and rows whose mask byte is 0 are not read into any
+ * result. A row of -inf alone has no shares (p = 0), only picks. Writes loss fp32 [sequences],
+ * counts int32 [sequences][experts] and tokens (n) int32 [sequences]; sums run in a fixed order, so
+ * a call repeats its bits. rows may be 0. */
+enum { EVAMX_BALANCE_MAX_ROWS = 1 << 24, EVAMX_BALANCE_MAX_SEQUENCES = 1 << 16 };
+size_t evamx_balance_workspace_bytes(int rows, int experts, int sequences);
+int evamx_balance_loss(const void* logits, int dtype, int64_t stride, int rows, int experts, const int64_t* sel,
+                       int topk, int score_fn, const int32_t* starts, int sequences, const uint8_t* mask,
+                       float* loss, int32_t* counts, int32_t* tokens, void* workspace, size_t workspace_bytes,
+                       evamx_stream_t stream);
+/* grad[rows][experts] (contiguous, the logits' type) = sum_s grad_loss[s] dloss[s]/dlogits, the counts
+ * and tokens of evamx_balance_loss held constant; zero for rows of no sequence and masked rows. */
+int evamx_balance_grad(const float* grad_loss, const void* logits, int dtype, int64_t stride, int rows, int experts,
+                       int topk, int score_fn, const int32_t* starts, int sequences, const uint8_t* mask,
+                       const int32_t* counts, const int32_t* tokens, void* grad, evamx_stream_t stream);
 
 /* ---- slot grouping (the reference's run table) ------------------------------------------- */
 
