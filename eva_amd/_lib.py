@@ -19,7 +19,8 @@ EVAMX_OK, EVAMX_EINVAL, EVAMX_ELAUNCH, EVAMX_ENOSPACE = 0, -1, -2, -3
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 SCORE_SIGMOID, SCORE_SQRT_SOFTPLUS = 0, 1
 ERR_EXPERT_RANGE, ERR_RATE = 1, 2
-W4_MAX_DIM, W4_MAX_COUNT = 1 << 18, 1024       # EVAMX_W4_MAX_DIM, matrices of a stack
+W4_MAX_DIM, W4_MAX_COUNT = 1 << 18, 1024         # EVAMX_W4_MAX_DIM, matrices of a stack
+W4_MOE_MAX_SLOTS = 65536                         # EVAMX_W4_MOE_MAX_SLOTS
 STRICT_MAX_ROWS, STRICT_MAX_SLOTS = 64, 256      # EVAMX_STRICT_MAX_ROWS / EVAMX_STRICT_MAX_SLOTS
 
 _vp = ctypes.c_void_p
@@ -49,6 +50,13 @@ class W4Desc(ctypes.Structure):
     """evamx_w4_weight."""
     _fields_ = [("codes", _vp), ("scales", _vp), ("zeros", _vp), ("count", _i32), ("n_out", _i32), ("n_in", _i32),
                 ("group", _i32), ("scale_dtype", _i32)]
+
+
+class W4MoeArgs(ctypes.Structure):
+    _fields_ = [("x", _vp), ("sel", _vp), ("weights", _vp), ("gate", ctypes.POINTER(W4Desc)), ("up", ctypes.POINTER(W4Desc)),
+                ("down", ctypes.POINTER(W4Desc)), ("out", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+                ("x_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("first_expert", ctypes.c_int64),
+                ("x_dtype", _i32), ("rows", _i32), ("topk", _i32), ("n_shared", _i32), ("limit", _f32)]
 
 
 class EvamxError(RuntimeError):
@@ -94,6 +102,8 @@ _SIGNATURES = {
     "evamx_moe_flags_ptr": (_vp, [ctypes.POINTER(MoeShape), _vp]),
     "evamx_moe_logits_ptr": (_vp, [ctypes.POINTER(MoeShape), _vp]),
     "evamx_moe_rotated_ptr": (_vp, [ctypes.POINTER(MoeShape), _vp]),
+    "evamx_w4_moe_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "evamx_w4_moe_forward": (ctypes.c_int, [ctypes.POINTER(W4MoeArgs), _vp]),
     "evamx_bench_decode": (ctypes.c_int, [_f32, ctypes.c_int, ctypes.c_int, _vp, _vp]),
     "evamx_bench_read": (ctypes.c_int, [_vp, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]),
 }

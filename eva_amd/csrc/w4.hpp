@@ -14,6 +14,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/evamx.h"
 
 namespace evamx {
@@ -131,6 +133,38 @@ __device__ __forceinline__ void w4_accumulate(w4_f32x4& acc, const W4Mat& m, siz
             }
         }
     }
+}
+
+// A result of x's type, to nearest even; NaN stays.
+__device__ __forceinline__ void w4_store(void* y, size_t at, float v, int bf16)
+{
+    if (bf16) {
+        uint32_t b = __builtin_bit_cast(uint32_t, v);
+        b = (b & 0x7fffffffu) > 0x7f800000u ? 0x7fc00000u : b + 0x7fffu + ((b >> 16) & 1);
+        ((uint16_t*)y)[at] = (uint16_t)(b >> 16);
+    } else {
+        ((w4_half*)y)[at] = (w4_half)v;
+    }
+}
+
+// Exponent that takes a row whose largest finite magnitude has the bits `top` into [2^14, 2^15).
+__device__ __forceinline__ int w4_exponent(uint32_t top)
+{
+    const int e = (int)(top >> 23) - 127 - 14;
+    return top == 0 ? 0 : e < -126 ? -126 : e;            // 2^-e stays finite, 2^e normal
+}
+
+// f(groups per k-tile, zero points or none) with both as types, for the kernels built for them.
+template <class F>
+inline void w4_dispatch(const evamx_w4_weight& w, F f)
+{
+    using std::integral_constant;
+    const std::true_type yes;
+    const std::false_type no;
+    auto pick = [&](auto sg) { if (w.zeros) f(sg, yes); else f(sg, no); };
+    if (w.group == 32) pick(integral_constant<int, 4>());
+    else if (w.group == 64) pick(integral_constant<int, 2>());
+    else pick(integral_constant<int, 1>());
 }
 
 // Rows of activations made ready for the products: fp16 [rows][kt * 128] of x * 2^-e, zeros past n_in, and 2^e per row,

@@ -4,17 +4,6 @@
 
 namespace evamx {
 
-__device__ __forceinline__ void w4_store(void* y, size_t at, float v, int bf16)
-{
-    if (bf16) {
-        uint32_t b = __builtin_bit_cast(uint32_t, v);
-        b = (b & 0x7fffffffu) > 0x7f800000u ? 0x7fc00000u : b + 0x7fffu + ((b >> 16) & 1);     // to nearest even; NaN stays
-        ((uint16_t*)y)[at] = (uint16_t)(b >> 16);
-    } else {
-        ((w4_half*)y)[at] = (w4_half)v;
-    }
-}
-
 __device__ __forceinline__ float w4_bias(const void* b, int n, int bf16)
 {
     return bf16 ? __builtin_bit_cast(float, (uint32_t)((const uint16_t*)b)[n] << 16) : (float)((const w4_half*)b)[n];
@@ -40,15 +29,6 @@ __global__ __launch_bounds__(256) void w4_linear_kernel(const w4_half* __restric
     v *= row_scale[r0 + r];
     if (bias) v += w4_bias(bias, n, bf16);
     w4_store(y, (size_t)(r0 + r) * y_stride + n, v, bf16);
-}
-
-template <int SG>
-static void w4_launch_linear(const w4_half* x, const float* rs, int rows, const W4Mat& m, const void* bias, void* y, size_t y_stride,
-                             int bf16, hipStream_t stream)
-{
-    const dim3 grid(w4_ceil(m.n_out, W4_TILE_N), w4_ceil(rows, 16));
-    if (m.zeros) w4_linear_kernel<SG, true><<<grid, 256, 0, stream>>>(x, rs, rows, m, bias, y, y_stride, bf16);
-    else w4_linear_kernel<SG, false><<<grid, 256, 0, stream>>>(x, rs, rows, m, bias, y, y_stride, bf16);
 }
 
 }  // namespace evamx
@@ -80,10 +60,9 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
     const int bf16 = x_dtype == EVAMX_DTYPE_BF16;
     w4_launch_rows(x, x_dtype, (size_t)x_stride, rows, w->n_in, xh, rs, s);
     const W4Mat m = w4_mat(*w);
-    switch (w->group) {
-    case 32: w4_launch_linear<4>(xh, rs, rows, m, bias, y, (size_t)y_stride, bf16, s); break;
-    case 64: w4_launch_linear<2>(xh, rs, rows, m, bias, y, (size_t)y_stride, bf16, s); break;
-    default: w4_launch_linear<1>(xh, rs, rows, m, bias, y, (size_t)y_stride, bf16, s);
-    }
+    const dim3 grid(w4_ceil(m.n_out, W4_TILE_N), w4_ceil(rows, 16));
+    w4_dispatch(*w, [&](auto sg, auto zero) {
+        w4_linear_kernel<decltype(sg)::value, decltype(zero)::value><<<grid, 256, 0, s>>>(xh, rs, rows, m, bias, y, (size_t)y_stride, bf16);
+    });
     return launched("w4_linear");
 }

@@ -96,9 +96,7 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(const char* __restrict__ s
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
     for (int i = 0; i < 4; ++i) top = part[i] > top ? part[i] : top;
-    int e = (int)(top >> 23) - 127 - 14;
-    if (top == 0) e = 0;
-    if (e < -126) e = -126;                              // 2^-e stays finite, 2^e normal
+    const int e = w4_exponent(top);
     const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
     for (int k = threadIdx.x; k < n_pad; k += 256)
         dst[blockIdx.x * (size_t)n_pad + k] = k < n_in ? (w4_half)(w4_src<SRC>(row, k) * down) : (w4_half)0.0f;

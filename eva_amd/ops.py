@@ -10,7 +10,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import MoeArgs, MoeShape, W4Desc, check, lib, ptr, stream_handle
+from ._lib import MoeArgs, MoeShape, W4Desc, W4MoeArgs, check, lib, ptr, stream_handle
 
 SCORE_FNS = {"sigmoid": _lib.SCORE_SIGMOID, "sqrt_softplus": _lib.SCORE_SQRT_SOFTPLUS}
 RATES = (2.0, 3.0, 4.0, 5.0)
@@ -608,6 +608,48 @@ def moe_forward_static(shape: MoeShape, x: torch.Tensor, tables: torch.Tensor, o
                         residual, gate_w, bits_down, k2_down_per_expert, shared_bits_down, shared_gate_w)
     check(lib().evamx_moe_forward_static(ctypes.byref(a), stream_handle(x.device)), "evamx_moe_forward_static")
     del keep
+    return out
+
+
+def w4_moe_forward(x: torch.Tensor, gate: W4Weight, up: W4Weight, down: W4Weight, sel: torch.Tensor, weights: torch.Tensor, *,
+                   n_shared: int = 0, first_expert: int = 0, limit: float = 0.0, out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """One MoE layer's experts on 4-bit weights with group scales, for given routes: ``x`` fp16 or bf16
+    ``[rows, hidden]``, ``sel`` int64 and ``weights`` fp32 ``[rows, topk]`` (``route`` / ``route_topk``), the
+    result of x's dtype. ``gate`` and ``up`` are stacks ``[inter, hidden]``, ``down`` ``[hidden, inter]``: the
+    experts ``first_expert`` and up, then ``n_shared`` shared experts that every token takes with weight 1.
+    Slots of other experts add nothing (expert parallelism). ``limit`` clamps as in ``moe_forward``. ``out``
+    must not overlap ``x``. At most 65536 slots a call (``W4Experts`` splits larger ones)."""
+    x_stride = _row_stride(x, "x")
+    if x.dtype not in _DTYPES:
+        raise ValueError("x must be fp16 or bf16")
+    rows, hidden = x.shape
+    _dev(sel, "sel", torch.int64, 2)
+    _dev(weights, "weights", torch.float32, 2)
+    if sel.shape[0] != rows or weights.shape != sel.shape:
+        raise ValueError(f"sel {tuple(sel.shape)} and weights {tuple(weights.shape)} must be [{rows}, topk]")
+    if gate.n_in != hidden:
+        raise ValueError(f"x has {hidden} features, the experts {gate.n_in}")
+    if out is None:
+        out = torch.empty(rows, hidden, dtype=x.dtype, device=x.device)
+    out_stride = _row_stride(out, "out", x.dtype)
+    if tuple(out.shape) != (rows, hidden):
+        raise ValueError(f"out must be [{rows}, {hidden}]")
+    _no_grad("w4_moe_forward", x, weights, out)
+    if workspace is None:
+        need = lib().evamx_w4_moe_workspace_bytes(rows, sel.shape[1], n_shared, hidden, gate.n_out)
+        if need == 0:
+            raise ValueError(lib().evamx_last_error().decode())
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _dev(workspace, "workspace", torch.uint8, 1)
+    for t, name in ((sel, "sel"), (weights, "weights"), (gate, "gate"), (up, "up"), (down, "down"), (out, "out"), (workspace, "workspace")):
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    a = W4MoeArgs(ptr(x), ptr(sel), ptr(weights), ctypes.pointer(gate.desc), ctypes.pointer(up.desc), ctypes.pointer(down.desc), ptr(out),
+                  ptr(workspace), workspace.numel(), x_stride, out_stride, first_expert, _DTYPES[x.dtype], rows, sel.shape[1], n_shared,
+                  float(limit))
+    with torch.cuda.device(x.device):
+        check(lib().evamx_w4_moe_forward(ctypes.byref(a), stream_handle(x.device)), "evamx_w4_moe_forward")
     return out
 
 

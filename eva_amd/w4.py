@@ -32,3 +32,41 @@ class W4Linear:
         return y.reshape(*x.shape[:-1], self.out_features)
 
     __call__ = forward
+
+
+class W4Experts:
+    """The experts of an MoE layer: stacks ``gate`` and ``up`` ``[inter, hidden]`` and ``down`` ``[hidden, inter]``,
+    of which the last ``n_shared`` are shared experts and the others have the router's indices ``first_expert``
+    and up (one rank's experts; slots of others add nothing)."""
+
+    def __init__(self, gate: ops.W4Weight, up: ops.W4Weight, down: ops.W4Weight, *, n_shared: int = 0, first_expert: int = 0):
+        shape = (gate.count, gate.n_out, gate.n_in)
+        if (up.count, up.n_out, up.n_in) != shape or (down.count, down.n_in, down.n_out) != shape:
+            raise ValueError("gate and up must be stacks [inter, hidden], down [hidden, inter], of as many matrices")
+        if up.desc.group != gate.desc.group or (up.zeros is None) != (gate.zeros is None):
+            raise ValueError("gate and up must agree in their group size and in having zero points")
+        if not 0 <= n_shared <= gate.count:
+            raise ValueError(f"{n_shared} shared experts of {gate.count}")
+        self.gate, self.up, self.down = gate, up, down
+        self.n_shared, self.first_expert = n_shared, first_expert
+        self.hidden, self.inter, self.n_local = gate.n_in, gate.n_out, gate.count - n_shared
+
+    def forward(self, x: torch.Tensor, sel: torch.Tensor, weights: torch.Tensor, limit: float = 0.0) -> torch.Tensor:
+        """Experts of x ``[..., hidden]`` (fp16 or bf16) for routes ``sel`` (integers) and ``weights`` ``[..., topk]``."""
+        if x.shape[-1] != self.hidden:
+            raise ValueError(f"x has {x.shape[-1]} features, the experts {self.hidden}")
+        flat, topk = x.reshape(-1, self.hidden), sel.shape[-1]
+        if (flat.shape[1] > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < self.hidden):
+            flat = flat.contiguous()
+        rows = flat.shape[0]
+        sel = sel.reshape(rows, topk).to(torch.int64).contiguous()
+        weights = weights.reshape(rows, topk).to(torch.float32).contiguous()
+        out = torch.empty(rows, self.hidden, dtype=x.dtype, device=x.device)
+        step = ops._lib.W4_MOE_MAX_SLOTS // (topk + self.n_shared)
+        for r0 in range(0, rows, step):
+            part = slice(r0, r0 + step)
+            ops.w4_moe_forward(flat[part], self.gate, self.up, self.down, sel[part], weights[part], n_shared=self.n_shared,
+                               first_expert=self.first_expert, limit=limit, out=out[part])
+        return out.reshape(*x.shape[:-1], self.hidden)
+
+    __call__ = forward

@@ -282,6 +282,33 @@ float* evamx_moe_logits_ptr(const evamx_moe_shape* shape, void* workspace);
  * of 1-2 rows, whose waves rotate their inputs in LDS. */
 const void* evamx_moe_rotated_ptr(const evamx_moe_shape* shape, void* workspace);
 
+/* ---- MoE experts on 4-bit weights with group scales ----------------------------------------- */
+
+/* out[t] = sum_k weights[t][k] * D_e(act(G_e x_t, U_e x_t)), e = sel[t][k] - first_expert, over the slots
+ * with e in [0, n_local), n_local = count - n_shared; other slots (another rank's experts) add 0. The
+ * last n_shared matrices of the stacks are shared experts: every token takes each with weight 1.
+ * act = min(silu(g), limit) * clamp(u, -limit, limit), the shared experts' min(g, limit) before SiLU
+ * (limit 0: no clamping; a NaN stays NaN). fp32 sums, fp16 hidden activations with a power-of-two
+ * factor per row (they neither overflow nor vanish), routing weights as given, slots added in slot
+ * order, one rounding to x's type. */
+enum { EVAMX_W4_MOE_MAX_SLOTS = 65536 };   /* rows * (topk + n_shared) of a call */
+typedef struct evamx_w4_moe_args {
+    const void* x;                /* device fp16/bf16 [rows][x_stride] */
+    const int64_t* sel;           /* device [rows][topk] */
+    const float* weights;         /* device [rows][topk] */
+    const evamx_w4_weight* gate;  /* HOST: stacks of `count` [inter][hidden], [inter][hidden], [hidden][inter]; gate */
+    const evamx_w4_weight* up;    /* and up alike in group size and in having zero points */
+    const evamx_w4_weight* down;
+    void* out;                    /* device, x's type, [rows][out_stride]; must not overlap x */
+    void* workspace;              /* device, evamx_w4_moe_workspace_bytes bytes, 16-byte aligned; needs no clearing */
+    size_t workspace_bytes;
+    int64_t x_stride, out_stride, first_expert;
+    int32_t x_dtype, rows, topk, n_shared;
+    float limit;
+} evamx_w4_moe_args;
+size_t evamx_w4_moe_workspace_bytes(int rows, int topk, int n_shared, int hidden, int inter);
+int evamx_w4_moe_forward(const evamx_w4_moe_args* args, evamx_stream_t stream);
+
 /* ---- measurement --------------------------------------------------------------------------- */
 
 /* No counterpart in the reference: a benchmark kernel for the arithmetic bound of the decode

@@ -60,3 +60,56 @@ def test_linear_is_checked():
     sizes = [L.evamx_w4_linear_workspace_bytes(r, 512) for r in (1, 2, 16, 17, 65536)]
     assert all(a <= b for a, b in zip(sizes, sizes[1:])) and sizes[0] > 0
     assert L.evamx_w4_linear_workspace_bytes(0, 512) == 0 and L.evamx_w4_linear_workspace_bytes(65537, 512) == 0
+
+
+def _moe(**kw):
+    w = {n: _weight(count=9, n_out=o, n_in=i) for n, o, i in (("gate", 256, 512), ("up", 256, 512), ("down", 512, 256))}
+    for n in ("gate", "up", "down"):
+        for f, v in kw.pop(n, {}).items():
+            setattr(w[n], f, v)
+    a = _lib.W4MoeArgs(x=FAKE, sel=FAKE, weights=FAKE, gate=ctypes.pointer(w["gate"]), up=ctypes.pointer(w["up"]),
+                       down=ctypes.pointer(w["down"]), out=FAKE, workspace=FAKE, workspace_bytes=1 << 40, x_stride=512, out_stride=512,
+                       first_expert=0, x_dtype=1, rows=4, topk=2, n_shared=1, limit=10.0)
+    for f, v in kw.items():
+        setattr(a, f, v)
+    return _lib.lib().evamx_w4_moe_forward(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(x=0), dict(sel=0), dict(weights=0), dict(out=0), dict(workspace=0), dict(workspace=FAKE + 4), dict(x_stride=511), dict(out_stride=511),
+    dict(x_dtype=2), dict(rows=0), dict(rows=21846), dict(topk=0), dict(topk=33), dict(n_shared=-1), dict(n_shared=10), dict(limit=-1.0),
+    dict(limit=float("inf")), dict(limit=float("nan")), dict(gate=dict(codes=0)), dict(up=dict(group=48)), dict(down=dict(n_out=500)),
+    dict(up=dict(n_out=255)), dict(down=dict(count=8)), dict(up=dict(group=64)), dict(up=dict(zeros=FAKE)), dict(down=dict(scale_dtype=5)),
+])
+def test_moe_is_checked(bad):
+    assert _moe(**bad) == _lib.EVAMX_EINVAL
+    assert _lib.lib().evamx_last_error()
+
+
+def test_moe_workspace():
+    L = _lib.lib()
+    assert _moe(workspace_bytes=1000) == _lib.EVAMX_ENOSPACE
+    assert L.evamx_w4_moe_forward(None, None) == _lib.EVAMX_EINVAL
+    sizes = [L.evamx_w4_moe_workspace_bytes(r, 8, 1, 7168, 2048) for r in (1, 2, 16, 17, 512, 7281)]
+    assert sizes[0] > 0 and all(a <= b for a, b in zip(sizes, sizes[1:]))
+    for bad in ((0, 8, 1, 64, 64), (7282, 8, 1, 64, 64), (1, 0, 0, 64, 64), (1, 8, 33, 64, 64), (1, 8, 0, 0, 64), (1, 8, 0, 64, 1 << 19)):
+        assert L.evamx_w4_moe_workspace_bytes(*bad) == 0, bad
+
+
+def test_struct_layouts_match_the_header(tmp_path):
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    structs = {"evamx_w4_weight": _lib.W4Desc, "evamx_w4_moe_args": _lib.W4MoeArgs}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "evamx.h"', 'int main(void) {']
+    for st, cls in structs.items():
+        lines.append(f'printf("{st} size %zu\\n", sizeof({st}));')
+        lines += [f'printf("{st} {f} %zu\\n", offsetof({st}, {f}));' for f, _ in cls._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c99", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+    got = dict(l.rsplit(" ", 1) for l in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines())
+    for st, cls in structs.items():
+        assert int(got[f"{st} size"]) == ctypes.sizeof(cls)
+        for f, _ in cls._fields_:
+            assert int(got[f"{st} {f}"]) == getattr(cls, f).offset, (st, f)

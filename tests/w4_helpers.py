@@ -50,3 +50,54 @@ def check_linear(y, x, w, bias=None, input_error=0.0):
     tol = tol + half_step(y.dtype) * (ref.abs() + tol) + torch.finfo(y.dtype).smallest_normal * half_step(y.dtype)
     off = (y.double().cpu() - ref).abs()
     assert (off <= tol).all(), float((off / tol).max())
+
+
+class Experts:
+    """An MoE layer's experts on such matrices."""
+
+    def __init__(self, gen, hidden, inter, count, group, *, zeros=False, dtype=torch.bfloat16, down_group=None, down_zeros=None, scale=None):
+        kw = dict(count=count, zeros=zeros, dtype=dtype, scale=scale)
+        self.gate, self.up = Matrix(gen, inter, hidden, group, **kw), Matrix(gen, inter, hidden, group, **kw)
+        kw["zeros"] = zeros if down_zeros is None else down_zeros
+        self.down = Matrix(gen, hidden, inter, group if down_group is None else down_group, **kw)
+        self.hidden, self.inter, self.count = hidden, inter, count
+
+    def module(self, dev, **kw):
+        from eva_amd.w4 import W4Experts
+        return W4Experts(self.gate.pack(dev), self.up.pack(dev), self.down.pack(dev), **kw)
+
+    def reference(self, x, sel, weights, *, n_shared=0, first_expert=0, limit=0.0, dtype=torch.bfloat16):
+        """(out, tolerance) in 64 bits on the CPU. The tolerance carries the sums' errors and the hidden
+        activations' rounding to fp16 (half a step, relative; the row's factor keeps them from underflow) to the
+        output, whose own rounding is half a step of its type."""
+        x, weights = x.double().cpu(), weights.double().cpu()
+        out, tol = torch.zeros_like(x), torch.zeros_like(x)
+        local = self.count - n_shared
+        for e in range(self.count):
+            if e < local:
+                t, k = (sel.cpu() == e + first_expert).nonzero(as_tuple=True)
+                w = weights[t, k]
+            else:
+                t = torch.arange(x.shape[0])
+                w = torch.ones(len(t), dtype=torch.float64)
+            if not len(t):
+                continue
+            a, unit = x[t], sum_error(self.hidden)
+            g, u = a @ self.gate.w[e].t(), a @ self.up.w[e].t()
+            dg, du = unit * (a.abs() @ self.gate.w[e].abs().t()), unit * (a.abs() @ self.up.w[e].abs().t())
+            if limit:
+                u = u.clamp(-limit, limit)
+                if e >= local:
+                    g = g.clamp(max=limit)
+            s = g * torch.sigmoid(g)
+            if limit and e < local:
+                s = s.clamp(max=limit)
+            h = s * u
+            # SiLU's slope is below 1.1; exp and the quotient a few steps of 2^-22 each
+            dh = 1.1 * dg * (u.abs() + du) + s.abs() * du + h.abs() * (2.0 ** -20 + half_step(torch.float16))
+            dh = dh + h.abs().amax(1, keepdim=True) * 2.0 ** -39
+            d = self.down.w[e]
+            y, mag = h @ d.t(), h.abs() @ d.abs().t()
+            out.index_add_(0, t, w[:, None] * y)
+            tol.index_add_(0, t, w.abs()[:, None] * (dh @ d.abs().t() + (sum_error(self.inter) + 2.0 ** -20) * mag))
+        return out, tol + half_step(dtype) * (out.abs() + tol) + torch.finfo(dtype).smallest_normal * half_step(dtype)
