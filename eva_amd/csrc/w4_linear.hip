@@ -4,31 +4,116 @@
 
 namespace evamx {
 
+struct W4LinearParams {
+    const void* x;               // as given
+    size_t x_stride;
+    const w4_half* xh;           // made ready: rows of kt * 128
+    const float* row_scale;      // NULL: 1
+    int rows, aligned, bf16;
+    const void* bias;
+    void* y;
+    size_t y_stride;
+};
+
 __device__ __forceinline__ float w4_bias(const void* b, int n, int bf16)
 {
     return bf16 ? __builtin_bit_cast(float, (uint32_t)((const uint16_t*)b)[n] << 16) : (float)((const w4_half*)b)[n];
 }
 
-// One workgroup 16 columns by 16 rows, its four waves every fourth quad of k-tiles.
-template <int SG, bool ZERO>
-__global__ __launch_bounds__(256) void w4_linear_kernel(const w4_half* __restrict__ x, const float* __restrict__ row_scale, int rows,
-                                                        W4Mat m, const void* __restrict__ bias, void* __restrict__ y, size_t y_stride,
-                                                        int bf16)
+__device__ __forceinline__ void w4_linear_store(const W4LinearParams& p, const W4Mat& m, int row, int n, float v, float scale)
 {
-    __shared__ w4_f32x4 part[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int nt = blockIdx.x, r0 = 16 * blockIdx.y, row = r0 + (lane & 15);
-    w4_f32x4 acc = {0, 0, 0, 0};
-    w4_accumulate<SG, ZERO>(acc, m, 0, nt, row < rows ? x + (size_t)row * m.kt * W4_TILE_K + 8 * (lane >> 4) : nullptr, wave, 4);
-    part[wave][lane] = acc;
+    v *= scale;
+    if (p.bias) v += w4_bias(p.bias, n, p.bf16);
+    w4_store(p.y, (size_t)row * p.y_stride + n, v, p.bf16);
+}
+
+// Up to four rows: one launch. A workgroup takes 16 NB columns, a wave one part of the k-tiles; the rows are made ready in LDS
+// while the first tiles are on their way, and each stands in four of the 16 rows of a matrix operand, so that one of the four
+// accumulators of a lane is all there is to scale.
+template <int SG, bool ZERO, int NB>
+__global__ __launch_bounds__(512) void w4_linear_few_kernel(W4LinearParams p, W4Mat m)
+{
+    extern __shared__ w4_half xs[];
+    __shared__ uint32_t top[W4_MAX_PARTS][4];
+    __shared__ float scale[4], part[W4_MAX_PARTS][NB][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, parts = blockDim.x >> 6, ld = m.kt * W4_TILE_K + W4_STAGE_PAD;
+    const int k0 = w4_part_begin(m.kt, parts, wave), k1 = w4_part_begin(m.kt, parts, wave + 1);
+    W4Stage stage{(const uint16_t*)p.x, p.x_stride, p.rows, m.n_in, m.kt, p.bf16, p.aligned};
+    stage.load();
+    W4Stream st[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int nt = NB * blockIdx.x + b;
+        st[b] = w4_stream<SG, ZERO>(m, 0, nt < m.nt ? nt : m.nt - 1, k1);
+    }
+    const int row = (lane & 15) >> 2;
+    const w4_half* a = xs + (row < p.rows ? row : p.rows - 1) * ld + 8 * (lane >> 4);
+    w4_f32x4 acc[NB][1] = {};
+    w4_run<2, SG, ZERO, NB, 1, 1, false>(
+        acc, st, k0, k1, m.bf16, [](int, int) {},
+        [&](int, int kt, w4_half8 (&x)[1][4], w4_half8 (&)[1][4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[0][j] = *(const w4_half8*)(a + kt * W4_TILE_K + 32 * j);
+        },
+        [&] { stage.finish(xs, top, scale); });
+#pragma unroll
+    for (int b = 0; b < NB; ++b) part[wave][b][lane] = acc[b][0][0];
     __syncthreads();
-    const int r = 4 * (lane >> 4) + wave, n = 16 * nt + (lane & 15);      // wave w joins and stores rows 4 g + w
-    if (r0 + r >= rows || n >= m.n_out) return;
+    if (threadIdx.x >= 64 * NB) return;
+    const int r = lane >> 4, n = 16 * (NB * blockIdx.x + wave) + (lane & 15);
+    if (r >= p.rows || n >= m.n_out) return;
     float v = 0;
-    for (int w = 0; w < 4; ++w) v += part[w][lane][wave];
-    v *= row_scale[r0 + r];
-    if (bias) v += w4_bias(bias, n, bf16);
-    w4_store(y, (size_t)(r0 + r) * y_stride + n, v, bf16);
+    for (int w = 0; w < parts; ++w) v += part[w][wave][lane];
+    w4_linear_store(p, m, r, n, v, scale[r]);
+}
+
+// 16 MB rows by 16 NB columns a workgroup, a wave one part of the k-tiles; the rows come ready from memory with the tiles.
+template <int SG, bool ZERO, int NB, int MB>
+__global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat m)
+{
+    constexpr int RING = MB == 1 ? 1 : 2;
+    extern __shared__ w4_f32x4 part[];                       // [parts][NB][MB][64]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, parts = blockDim.x >> 6;
+    const int k0 = w4_part_begin(m.kt, parts, wave), k1 = w4_part_begin(m.kt, parts, wave + 1), r0 = 16 * MB * blockIdx.y;
+    W4Stream st[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int nt = NB * blockIdx.x + b;
+        st[b] = w4_stream<SG, ZERO>(m, 0, nt < m.nt ? nt : m.nt - 1, k1);
+    }
+    W4GlobalRows<RING, MB, false> rows;
+    rows.src = w4_rsrc(p.xh + (size_t)r0 * m.kt * W4_TILE_K, (uint32_t)(p.rows - r0 < 16 * MB ? p.rows - r0 : 16 * MB) * m.kt * (W4_TILE_K * 2));
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        const int r = 16 * mb + (lane & 15);
+        rows.at[mb] = (uint32_t)(r0 + r < p.rows ? r : p.rows - 1 - r0) * m.kt * (W4_TILE_K * 2) + 16 * (lane >> 4);
+    }
+    w4_f32x4 acc[NB][MB] = {};
+    w4_run<RING, SG, ZERO, NB, MB, 4, false>(
+        acc, st, k0, k1, m.bf16, [&](int d, int kt) { rows.request(d, kt); },
+        [&](int d, int, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) { rows.take(d, x, lo); }, [] {});
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) part[((wave * NB + b) * MB + mb) * 64 + lane] = acc[b][mb];
+    __syncthreads();
+    for (int t = wave; t < NB * MB * 4; t += parts) {        // value i of block mb and stream b
+        const int i = t & 3, mb = (t >> 2) % MB, b = (t >> 2) / MB;
+        const int r = r0 + 16 * mb + 4 * (lane >> 4) + i, n = 16 * (NB * blockIdx.x + b) + (lane & 15);
+        if (r >= p.rows || n >= m.n_out) continue;
+        float v = 0;
+        for (int w = 0; w < parts; ++w) v += part[((w * NB + b) * MB + mb) * 64 + lane][i];
+        w4_linear_store(p, m, r, n, v, p.row_scale ? p.row_scale[r] : 1.0f);
+    }
+}
+
+template <int NB, int MB>
+static void w4_launch_linear(const W4LinearParams& p, const W4Mat& m, const evamx_w4_weight& w, int parts, hipStream_t s)
+{
+    const dim3 grid(w4_ceil(m.nt, NB), w4_ceil(p.rows, 16 * MB));
+    w4_dispatch(w, [&](auto sg, auto zero) {
+        w4_linear_kernel<decltype(sg)::value, decltype(zero)::value, NB, MB><<<grid, 64 * parts, parts * NB * MB * 1024, s>>>(p, m);
+    });
 }
 
 }  // namespace evamx
@@ -55,14 +140,32 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
     const size_t need = evamx_w4_linear_workspace_bytes(rows, w->n_in);
     if (workspace_bytes < need) { set_error("evamx_w4_linear: workspace %zu bytes < %zu", workspace_bytes, need); return EVAMX_ENOSPACE; }
     const hipStream_t s = (hipStream_t)stream;
-    float* rs = (float*)workspace;
-    w4_half* xh = (w4_half*)((char*)workspace + w4_align((size_t)rows * 4));
-    const int bf16 = x_dtype == EVAMX_DTYPE_BF16;
-    w4_launch_rows(x, x_dtype, (size_t)x_stride, rows, w->n_in, xh, rs, s);
     const W4Mat m = w4_mat(*w);
-    const dim3 grid(w4_ceil(m.n_out, W4_TILE_N), w4_ceil(rows, 16));
-    w4_dispatch(*w, [&](auto sg, auto zero) {
-        w4_linear_kernel<decltype(sg)::value, decltype(zero)::value><<<grid, 256, 0, s>>>(xh, rs, rows, m, bias, y, (size_t)y_stride, bf16);
-    });
+    const int parts = w4_parts(m.kt);
+    W4LinearParams p;
+    p.x = x; p.x_stride = (size_t)x_stride; p.rows = rows; p.bf16 = x_dtype == EVAMX_DTYPE_BF16;
+    p.aligned = (((uintptr_t)x | (uintptr_t)(2 * x_stride)) & 15) == 0;
+    p.bias = bias; p.y = y; p.y_stride = (size_t)y_stride; p.xh = nullptr; p.row_scale = nullptr;
+    if (w4_stage_fits(rows, m.kt, parts)) {
+        w4_dispatch(*w, [&](auto sg, auto zero) {
+            w4_linear_few_kernel<decltype(sg)::value, decltype(zero)::value, 1><<<m.nt, 64 * parts, w4_stage_bytes(rows, m.kt), s>>>(p, m);
+        });
+        return launched("w4_linear");
+    }
+    if (w4_rows_ready(x, x_dtype, x_stride, m.n_in)) {
+        p.xh = (const w4_half*)x;
+    } else {
+        float* rs = (float*)workspace;
+        w4_half* xh = (w4_half*)((char*)workspace + w4_align((size_t)rows * 4));
+        w4_launch_rows(x, x_dtype, (size_t)x_stride, rows, w->n_in, xh, rs, s);
+        p.xh = xh;
+        p.row_scale = rs;
+    }
+    // fewer than two workgroups a CU otherwise: 16 columns each (5001 -> 2303 at 13 rows: 12.3 us against 14.9 with 32), else
+    // 32 on the same rows (7168 -> 18432 at 5 rows: 21.8 us against 25.8 with 16)
+    if (rows <= 16 && m.nt < 1024) w4_launch_linear<1, 1>(p, m, *w, parts, s);
+    else if (rows <= 16) w4_launch_linear<2, 1>(p, m, *w, parts, s);
+    else if (rows <= 32) w4_launch_linear<2, 2>(p, m, *w, parts, s);
+    else w4_launch_linear<2, 4>(p, m, *w, parts < 4 ? parts : 4, s);
     return launched("w4_linear");
 }

@@ -4,22 +4,34 @@
 // their gate clamped before SiLU (both as evamx_moe_forward has them). L = 0: no clamping.
 #include <cmath>
 
+#include "evamx_gemv.hpp"
 #include "evamx_internal.hpp"
 #include "w4.hpp"
 
 namespace evamx {
 
+struct W4Unit {
+    int expert, r0, rows, pad;   // rows slots from order[r0] on, all of one expert; expert -1: none
+};
+
 struct W4MoeParams {
     int rows, topk, n_shared, kt_slots, slots, n_local, count, hidden, inter, bf16;   // kt_slots = topk + n_shared per token
+    uint32_t recip;              // ceil(2^32 / kt_slots)
     long long first;
     float limit;
     const int64_t* sel;
     const float* weights;
-    int* offsets;                // [count + 1]: positions of an expert's slots in `order`; the last is their number
-    int* order;                  // [slots]: slots by (expert, slot)
-    const w4_half* x;            // [rows][k of gate, padded], with a factor per row
+    W4Unit* units;
+    const int* units_in_use;     // their number, or NULL: one for each slot
+    int* n_units;
+    int* order;                  // slots by (expert, slot)
+    const void* x_in;            // as given
+    size_t x_stride;
+    int aligned;
+    const w4_half* x;            // [rows][k of gate, padded], with a factor per row (NULL: 1)
     const float* xs;
-    float* h;                    // [positions][inter]
+    float* h;                    // [slots][h_ld]
+    int h_ld;
     w4_half* hh;                 // the same, ready for the down products, with a factor per row
     float* hs;
     float* y;                    // [slots][hidden]
@@ -27,82 +39,95 @@ struct W4MoeParams {
     size_t out_stride;
 };
 
+// Token of a slot: a division by a constant of the call as one high product (exact below 2^16).
+__device__ __forceinline__ int w4_token(const W4MoeParams& p, int s) { return p.kt_slots == 1 ? s : (int)__umulhi((uint32_t)s, p.recip); }
+
 // Matrix of slot s, or -1.
 __device__ __forceinline__ int w4_slot_expert(const W4MoeParams& p, int s)
 {
-    const int t = s / p.kt_slots, k = s - t * p.kt_slots;
-    if (k >= p.topk) return p.n_local + k - p.topk;
-    const unsigned long long e = (unsigned long long)p.sel[(size_t)t * p.topk + k] - (unsigned long long)p.first;    // wraps
+    int at = s;
+    if (p.n_shared) {
+        const int t = w4_token(p, s), k = s - t * p.kt_slots;
+        if (k >= p.topk) return p.n_local + k - p.topk;
+        at = t * p.topk + k;
+    }
+    const unsigned long long e = (unsigned long long)p.sel[at] - (unsigned long long)p.first;    // wraps
     return e < (unsigned)p.n_local ? (int)e : -1;
 }
 
-// Stable grouping, one workgroup an expert: it counts the slots of smaller experts and its own, then writes its own in
-// order. count x slots reads from L2, far below the products that follow.
-__global__ __launch_bounds__(256) void w4_group_kernel(W4MoeParams p)
+// What a call of more than W4_FEW_ROWS tokens needs before its products, one launch: workgroups 0 .. count - 1 group the slots
+// stably by expert and cut each expert's into units of `tile` rows; the others make a row of x ready each.
+//
+// The workgroup of expert e reads every slot (from L2; far below the products that follow): a histogram gives the places of its
+// slots and units, each wave counts its own range's slots of e, then writes them in order.
+constexpr int W4_PREP_THREADS = 512;
+
+template <int SRC>
+__global__ __launch_bounds__(W4_PREP_THREADS) void w4_prep_kernel(W4MoeParams p, int tile, w4_half* __restrict__ xh, float* __restrict__ xs, int n_pad)
 {
-    __shared__ int part[4], wave_n[4];
+    constexpr int WAVES = W4_PREP_THREADS / 64;
+    __shared__ uint32_t top[WAVES];
+    if ((int)blockIdx.x >= p.count) {
+        const int t = blockIdx.x - p.count;
+        W4ReadyRow<SRC, W4_PREP_THREADS, false> row{(const char*)p.x_in + t * p.x_stride * 2, p.hidden, n_pad, (bool)p.aligned, (int)threadIdx.x};
+        row.load();
+        const float f = row.finish(xh + (size_t)t * n_pad, 0, top);
+        if (threadIdx.x == 0) xs[t] = f;
+        return;
+    }
+    __shared__ int hist[1024], mine_n[WAVES], sums[3][WAVES];
     const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int less = 0;
-    for (int s = threadIdx.x; s < p.slots; s += 256) {
-        const int v = w4_slot_expert(p, s);
-        less += v >= 0 && v < e;
-    }
-    for (int i = 32; i; i >>= 1) less += __shfl_xor(less, i);
-    if (lane == 0) part[wave] = less;
+    for (int i = threadIdx.x; i < p.count; i += W4_PREP_THREADS) hist[i] = 0;
     __syncthreads();
-    int at = part[0] + part[1] + part[2] + part[3];
-    if (threadIdx.x == 0) p.offsets[e] = at;
-    for (int s0 = 0; s0 < p.slots; s0 += 256) {
-        const int s = s0 + threadIdx.x;
-        const bool mine = s < p.slots && w4_slot_expert(p, s) == e;
-        const unsigned long long b = __ballot(mine);
-        if (lane == 0) wave_n[wave] = __popcll(b);
-        __syncthreads();
-        int pos = at + __popcll(b & ((1ull << lane) - 1));
-        for (int w = 0; w < wave; ++w) pos += wave_n[w];
-        if (mine) p.order[pos] = s;
-        at += wave_n[0] + wave_n[1] + wave_n[2] + wave_n[3];
-        __syncthreads();
+    const int span = (w4_ceil(p.slots, WAVES) + 63) & ~63, s0 = wave * span, s1 = s0 + span < p.slots ? s0 + span : p.slots;
+    int own = 0;
+    for (int s = s0 + lane; s < s1; s += 64) {
+        const int v = w4_slot_expert(p, s);
+        if (v >= 0) atomicAdd(&hist[v], 1);
+        own += v == e;
     }
-    if (e == p.count - 1 && threadIdx.x == 0) p.offsets[p.count] = at;
-}
-
-struct W4Unit {
-    int expert, r0, rows;        // positions r0 .. r0 + rows - 1 of the order; expert -1: past the last unit
-};
-
-// The unit'th block of at most `tile` positions of one expert, found by every wave on its own.
-__device__ __forceinline__ W4Unit w4_unit(const int* __restrict__ offsets, int count, int tile, int unit)
-{
-    const int lane = threadIdx.x & 63, per = (count + 63) / 64;
-    int n = 0;
-    for (int i = 0; i < per; ++i) {
-        const int e = lane * per + i;
-        if (e < count) n += (offsets[e + 1] - offsets[e] + tile - 1) / tile;
-    }
-    int incl = n;
-    for (int s = 1; s < 64; s <<= 1) {
-        const int v = __shfl_up(incl, s);
-        if (lane >= s) incl += v;
-    }
-    const unsigned long long here = __ballot(incl > unit);
-    if (!here) return {-1, 0, 0};
-    const int owner = __builtin_ctzll(here);
-    W4Unit u = {-1, 0, 0};
-    if (lane == owner) {
-        int left = unit - (incl - n);
-        for (int i = 0; i < per; ++i) {
-            const int e = lane * per + i;
-            if (e >= count) break;
-            const int o = offsets[e], c = offsets[e + 1] - o, t = (c + tile - 1) / tile;
-            if (left < t) {
-                u = {e, o + left * tile, c - left * tile < tile ? c - left * tile : tile};
-                break;
-            }
-            left -= t;
+    for (int i = 32; i; i >>= 1) own += __shfl_xor(own, i);
+    if (lane == 0) mine_n[wave] = own;
+    __syncthreads();
+    int slots = 0, units = 0, all = 0;
+    for (int i = threadIdx.x; i < p.count; i += W4_PREP_THREADS) {
+        const int n = hist[i], u = (n + tile - 1) / tile;
+        all += u;
+        if (i < e) {
+            slots += n;
+            units += u;
         }
     }
-    return {__shfl(u.expert, owner), __shfl(u.r0, owner), __shfl(u.rows, owner)};
+    for (int i = 32; i; i >>= 1) {
+        slots += __shfl_xor(slots, i);
+        units += __shfl_xor(units, i);
+        all += __shfl_xor(all, i);
+    }
+    if (lane == 0) {
+        sums[0][wave] = slots;
+        sums[1][wave] = units;
+        sums[2][wave] = all;
+    }
+    __syncthreads();
+    slots = units = all = 0;
+    for (int w = 0; w < WAVES; ++w) {
+        slots += sums[0][w];
+        units += sums[1][w];
+        all += sums[2][w];
+    }
+    const int n = hist[e];
+    if (e == 0 && threadIdx.x == 0) *p.n_units = all;
+    for (int i = threadIdx.x; i * tile < n; i += W4_PREP_THREADS)
+        p.units[units + i] = W4Unit{e, slots + i * tile, n - i * tile < tile ? n - i * tile : tile, 0};
+    int at = slots;
+    for (int w = 0; w < wave; ++w) at += mine_n[w];
+    for (int b0 = s0; b0 < s1; b0 += 64) {
+        const int s = b0 + lane;
+        const bool mine = s < s1 && w4_slot_expert(p, s) == e;
+        const unsigned long long b = __ballot(mine);
+        if (mine) p.order[at + __popcll(b & ((1ull << lane) - 1))] = s;
+        at += __popcll(b);
+    }
 }
 
 __device__ __forceinline__ float w4_clamp(float v, float lo, float hi) { return v < lo ? lo : v > hi ? hi : v; }    // NaN stays
@@ -118,97 +143,311 @@ __device__ __forceinline__ float w4_swiglu(float g, float u, float limit, bool s
     return a * u;
 }
 
-// 16 columns of gate and up by 16 positions of one expert; the four waves take every fourth quad of k-tiles.
+// Waves of a workgroup: parts of the k-tiles times column groups. The parts depend on the matrix alone (w4_part_begin), and a
+// wave has at least some twenty tiles to make up for its start.
+constexpr int W4_WAVES = 4;
+inline int w4_moe_parts(int kt) { return kt >= 48 ? 4 : kt >= 24 ? 2 : 1; }
+
+// Column tiles a wave takes at once, of gate and up each and of down. The rows' operands come from L2 with every tile, four
+// times the bytes of one column tile's codes, so more columns for the same operands win (16 tokens of a 7168 x 2048 layer of
+// 256 experts: 405 us with 1 and 2, 391 with 1 and 4, 369 with 2 and 4), while tiles requested further ahead cost the
+// registers of waves that hide more (with two tiles in flight a stream instead of one: 374 us, with four 442).
+constexpr int W4_GU_CT = 2, W4_DOWN_NB = 4;
+
+// Up to W4_FEW_ROWS tokens, without a launch before it: 16 columns of gate and up of one expert a column group, the tokens' rows
+// in LDS (w4_linear_few_kernel's scheme). Unit u is the expert of slot u, if no slot before it has that expert; with one token
+// every slot is a unit.
+constexpr int W4_FEW_ROWS = 4, W4_FEW_SLOTS = W4_FEW_ROWS * 64;
+
 template <int SG, bool ZERO>
-__global__ __launch_bounds__(256) void w4_gate_up_kernel(W4MoeParams p, W4Mat gate, W4Mat up)
+__global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_few_kernel(W4MoeParams p, W4Mat gate, W4Mat up, int parts)
 {
-    __shared__ w4_f32x4 part[4][2][64];
-    const W4Unit u = w4_unit(p.offsets, p.count, 16, blockIdx.y);
-    if (u.expert < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = blockIdx.x;
-    const w4_half* a = nullptr;
-    if ((lane & 15) < u.rows) {
-        const int t = p.order[u.r0 + (lane & 15)] / p.kt_slots;
-        a = p.x + (size_t)t * gate.kt * W4_TILE_K + 8 * (lane >> 4);
+    extern __shared__ w4_half xs[];
+    __shared__ uint32_t top[W4_MAX_PARTS][4];
+    __shared__ float scale[4], part[W4_WAVES][2][64];
+    __shared__ int list[W4_FEW_SLOTS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = W4_WAVES / parts, ld = gate.kt * W4_TILE_K + W4_STAGE_PAD;
+    const int q = wave % parts, nt = blockIdx.x * groups + wave / parts;
+    const int k0 = w4_part_begin(gate.kt, parts, q), k1 = w4_part_begin(gate.kt, parts, q + 1);
+    const int e = __builtin_amdgcn_readfirstlane(w4_slot_expert(p, blockIdx.y));
+    W4Stage stage{(const uint16_t*)p.x_in, p.x_stride, p.rows, gate.n_in, gate.kt, p.bf16, p.aligned};
+    stage.load();
+    const bool tell = blockIdx.x == 0 && wave == 0;           // the down products take the units from here
+    if (e < 0) {
+        if (tell && lane == 0) p.units[blockIdx.y] = W4Unit{-1, 0, 0, 0};
+        return;
     }
-    w4_f32x4 g = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-    w4_accumulate<SG, ZERO>(g, gate, u.expert, nt, a, wave, 4);
-    w4_accumulate<SG, ZERO>(v, up, u.expert, nt, a, wave, 4);
-    part[wave][0][lane] = g;
-    part[wave][1][lane] = v;
-    __syncthreads();
-    const int r = 4 * (lane >> 4) + wave, n = 16 * nt + (lane & 15);
-    if (r >= u.rows || n >= p.inter) return;
-    float gs = 0, us = 0;
-    for (int w = 0; w < 4; ++w) {
-        gs += part[w][0][lane][wave];
-        us += part[w][1][lane][wave];
+    int rows = 1;
+    if (p.rows == 1) {
+        list[0] = blockIdx.y;
+    } else {
+        rows = 0;
+        bool first = true;
+        int v[W4_FEW_ROWS];
+#pragma unroll
+        for (int c = 0; c < W4_FEW_ROWS; ++c) v[c] = 64 * c + lane < p.slots ? w4_slot_expert(p, 64 * c + lane) : -1;
+#pragma unroll
+        for (int c = 0; c < W4_FEW_ROWS; ++c) {
+            const unsigned long long b = __ballot(v[c] == e);
+            const int below = (int)blockIdx.y - 64 * c;
+            if (v[c] == e) list[rows + __popcll(b & ((1ull << lane) - 1))] = 64 * c + lane;
+            rows += __popcll(b);
+            if (below >= 64 ? b != 0 : below > 0 && (b & ((1ull << below) - 1)) != 0) first = false;
+        }
+        if (!first) {
+            if (tell && lane == 0) p.units[blockIdx.y] = W4Unit{-1, 0, 0, 0};
+            return;
+        }
     }
-    const float xs = p.xs[p.order[u.r0 + r] / p.kt_slots];
-    p.h[(size_t)(u.r0 + r) * p.inter + n] = w4_swiglu(gs * xs, us * xs, p.limit, u.expert >= p.n_local);
+    wave_lds_fence();
+    if (tell) {
+        if (lane == 0) p.units[blockIdx.y] = W4Unit{e, (int)blockIdx.y * p.slots, rows, 0};
+        for (int i = lane; i < rows; i += 64) p.order[blockIdx.y * p.slots + i] = list[i];
+    }
+    const int ntc = nt < gate.nt ? nt : gate.nt - 1;
+    const W4Stream st[2] = {w4_stream<SG, ZERO>(gate, e, ntc, k1), w4_stream<SG, ZERO>(up, e, ntc, k1)};
+    auto block = [&](int r0, auto begin) {
+        const int mine = r0 + ((lane & 15) >> 2), token = w4_token(p, list[mine < rows ? mine : rows - 1]);
+        const w4_half* a = xs + token * ld + 8 * (lane >> 4);
+        w4_f32x4 acc[2][1] = {};
+        w4_run<2, SG, ZERO, 2, 1, 1, false>(
+            acc, st, k0, k1, gate.bf16, [](int, int) {},
+            [&](int, int kt, w4_half8 (&x)[1][4], w4_half8 (&)[1][4]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[0][j] = *(const w4_half8*)(a + kt * W4_TILE_K + 32 * j);
+            },
+            begin);
+        part[wave][0][lane] = acc[0][0][0];
+        part[wave][1][lane] = acc[1][0][0];
+        __syncthreads();
+        const int r = r0 + (lane >> 4), n = 16 * nt + (lane & 15);
+        if (q == 0 && r < rows && n < p.inter) {
+            float g = 0, v = 0;
+            for (int w = 0; w < parts; ++w) {
+                g += part[wave + w][0][lane];
+                v += part[wave + w][1][lane];
+            }
+            const int s = list[r];
+            const float f = scale[w4_token(p, s)];
+            p.h[(size_t)s * p.h_ld + n] = w4_swiglu(g * f, v * f, p.limit, e >= p.n_local);
+        }
+        __syncthreads();
+    };
+    block(0, [&] { stage.finish(xs, top, scale); });
+    for (int r0 = 4; r0 < rows; r0 += 4) block(r0, [] {});          // only where a token repeats an expert
 }
 
-// The hidden activations of the positions there are, ready for the down products (w4_rows_kernel's scheme).
+// 16 CT columns of gate and up a column group, by a unit of up to 16 MB rows.
+template <int RING, int SG, bool ZERO, int CT, int MB>
+__global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_kernel(W4MoeParams p, W4Mat gate, W4Mat up, int parts)
+{
+    __shared__ w4_f32x4 part[W4_WAVES][2 * CT][MB][64];
+    if ((int)blockIdx.y >= *p.units_in_use) return;
+    const W4Unit u = p.units[blockIdx.y];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = W4_WAVES / parts;
+    const int q = wave % parts, nt = CT * (blockIdx.x * groups + wave / parts);
+    const int k0 = w4_part_begin(gate.kt, parts, q), k1 = w4_part_begin(gate.kt, parts, q + 1);
+    W4Stream st[2 * CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        const int t = nt + c < gate.nt ? nt + c : gate.nt - 1;
+        st[2 * c] = w4_stream<SG, ZERO>(gate, u.expert, t, k1);
+        st[2 * c + 1] = w4_stream<SG, ZERO>(up, u.expert, t, k1);
+    }
+    W4GlobalRows<RING, MB, false> rows;
+    rows.src = w4_rsrc(p.x, (uint32_t)p.rows * gate.kt * (W4_TILE_K * 2));
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        const int r = 16 * mb + (lane & 15), t = w4_token(p, p.order[u.r0 + (r < u.rows ? r : u.rows - 1)]);
+        rows.at[mb] = (uint32_t)t * gate.kt * (W4_TILE_K * 2) + 16 * (lane >> 4);
+    }
+    w4_f32x4 acc[2 * CT][MB] = {};
+    w4_run<RING, SG, ZERO, 2 * CT, MB, 4, false>(
+        acc, st, k0, k1, gate.bf16, [&](int d, int kt) { rows.request(d, kt); },
+        [&](int d, int, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) { rows.take(d, x, lo); }, [] {});
+#pragma unroll
+    for (int b = 0; b < 2 * CT; ++b)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) part[wave][b][mb][lane] = acc[b][mb];
+    __syncthreads();
+    for (int t = q; t < CT * MB * 4; t += parts) {           // the parts share the values of their column group
+        const int i = t & 3, mb = (t >> 2) % MB, c = (t >> 2) / MB, r = 16 * mb + 4 * (lane >> 4) + i, n = 16 * (nt + c) + (lane & 15);
+        if (r >= u.rows || n >= p.inter) continue;
+        float g = 0, v = 0;
+        for (int w = wave - q; w < wave - q + parts; ++w) {
+            g += part[w][2 * c][mb][lane][i];
+            v += part[w][2 * c + 1][mb][lane][i];
+        }
+        const int s = p.order[u.r0 + r];
+        const float f = p.xs ? p.xs[w4_token(p, s)] : 1.0f;
+        p.h[(size_t)s * p.h_ld + n] = w4_swiglu(g * f, v * f, p.limit, u.expert >= p.n_local);
+    }
+}
+
+// The hidden activations of the slots there are, ready for the down products. HL, for fp16 calls: what rounding them to 11 bits
+// leaves is kept in a second half, since their results' own rounding is no coarser (relative error of a layer 2.9e-4 with one
+// half, 2.1e-4 being the results' rounding; of bf16 results 1.7e-3 with one half or two).
+template <bool HL>
 __global__ __launch_bounds__(256) void w4_hidden_kernel(W4MoeParams p, int n_pad)
 {
     __shared__ uint32_t part[4];
-    if ((int)blockIdx.x >= p.offsets[p.count]) return;
-    const float* row = p.h + (size_t)blockIdx.x * p.inter;
-    uint32_t top = 0;
-    for (int k = threadIdx.x; k < p.inter; k += 256) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, row[k]) & 0x7fffffffu;
-        if (b < 0x7f800000u && b > top) top = b;
-    }
-    for (int s = 32; s; s >>= 1) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)top, s);
-        top = o > top ? o : top;
-    }
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) top = part[i] > top ? part[i] : top;
-    const int e = w4_exponent(top);
-    const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-    for (int k = threadIdx.x; k < n_pad; k += 256)
-        p.hh[blockIdx.x * (size_t)n_pad + k] = k < p.inter ? (w4_half)(row[k] * down) : (w4_half)0.0f;
-    if (threadIdx.x == 0) p.hs[blockIdx.x] = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+    const int s = blockIdx.x;
+    if (w4_slot_expert(p, s) < 0) return;
+    W4ReadyRow<W4_SRC_F32, 256, HL> row{(const char*)(p.h + (size_t)s * p.h_ld), p.inter, n_pad, true, (int)threadIdx.x};
+    row.load();
+    const float f = row.finish(p.hh + s * (size_t)(HL ? 2 * n_pad : n_pad), n_pad, part);
+    if (threadIdx.x == 0) p.hs[s] = f;
 }
 
-template <int SG, bool ZERO>
-__global__ __launch_bounds__(256) void w4_down_kernel(W4MoeParams p, W4Mat down)
+// 16 NB columns of the output a column group, by a unit of up to 16 MB rows.
+template <int RING, int SG, bool ZERO, int NB, int MB, bool HL>
+__global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W4Mat down, int parts)
 {
-    __shared__ w4_f32x4 part[4][64];
-    const W4Unit u = w4_unit(p.offsets, p.count, 16, blockIdx.y);
+    __shared__ w4_f32x4 part[W4_WAVES][NB][MB][64];
+    if (p.units_in_use && (int)blockIdx.y >= *p.units_in_use) return;
+    const W4Unit u = p.units[blockIdx.y];
     if (u.expert < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = blockIdx.x;
-    w4_f32x4 acc = {0, 0, 0, 0};
-    w4_accumulate<SG, ZERO>(acc, down, u.expert, nt,
-                            (lane & 15) < u.rows ? p.hh + (size_t)(u.r0 + (lane & 15)) * down.kt * W4_TILE_K + 8 * (lane >> 4) : nullptr, wave, 4);
-    part[wave][lane] = acc;
-    __syncthreads();
-    const int r = 4 * (lane >> 4) + wave, n = 16 * nt + (lane & 15);
-    if (r >= u.rows || n >= p.hidden) return;
-    float v = 0;
-    for (int w = 0; w < 4; ++w) v += part[w][lane][wave];
-    p.y[(size_t)p.order[u.r0 + r] * p.hidden + n] = v * p.hs[u.r0 + r];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = W4_WAVES / parts;
+    const int q = wave % parts, nt = NB * (blockIdx.x * groups + wave / parts), n_pad = down.kt * W4_TILE_K;
+    const int k0 = w4_part_begin(down.kt, parts, q), k1 = w4_part_begin(down.kt, parts, q + 1);
+    W4Stream st[NB];
+#pragma unroll
+    for (int c = 0; c < NB; ++c) st[c] = w4_stream<SG, ZERO>(down, u.expert, nt + c < down.nt ? nt + c : down.nt - 1, k1);
+    W4GlobalRows<RING, MB, HL> rows;
+    const uint32_t ld = (HL ? 4 : 2) * n_pad;
+    rows.src = w4_rsrc(p.hh, (uint32_t)p.slots * ld);
+    rows.lo_off = 2 * n_pad;
+    for (int r0 = 0; r0 < u.rows; r0 += 16 * MB) {           // once, but for few tokens that repeat an expert
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+            const int r = r0 + 16 * mb + (lane & 15), s = p.order[u.r0 + (r < u.rows ? r : u.rows - 1)];
+            rows.at[mb] = (uint32_t)s * ld + 16 * (lane >> 4);
+        }
+        w4_f32x4 acc[NB][MB] = {};
+        w4_run<RING, SG, ZERO, NB, MB, 4, HL>(
+            acc, st, k0, k1, down.bf16, [&](int d, int kt) { rows.request(d, kt); },
+            [&](int d, int, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) { rows.take(d, x, lo); }, [] {});
+#pragma unroll
+        for (int c = 0; c < NB; ++c)
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) part[wave][c][mb][lane] = acc[c][mb];
+        __syncthreads();
+        for (int t = q; t < NB * MB * 4; t += parts) {
+            const int i = t & 3, mb = (t >> 2) % MB, b = (t >> 2) / MB;
+            const int r = r0 + 16 * mb + 4 * (lane >> 4) + i, n = 16 * (nt + b) + (lane & 15);
+            if (r >= u.rows || n >= p.hidden) continue;
+            float v = 0;
+            for (int w = wave - q; w < wave - q + parts; ++w) v += part[w][b][mb][lane][i];
+            const int s = p.order[u.r0 + r];
+            p.y[(size_t)s * p.hidden + n] = v * p.hs[s];
+        }
+        __syncthreads();
+    }
 }
 
-// out[t] = the slots' outputs in slot order times their routing weights (fp32, as given), rounded once.
+// One token: 16 NB columns of the output, a wave a slot (up to 16, then the next ones), its parts of the k-tiles one after the
+// other; the slots' sums meet in LDS, so that no launch follows.
+constexpr int W4_ONE_WAVES = 16, W4_ONE_NB = 2;
+
+template <int SG, bool ZERO, bool HL>
+__global__ __launch_bounds__(64 * W4_ONE_WAVES) void w4_down_one_kernel(W4MoeParams p, W4Mat down, int parts)
+{
+    extern __shared__ w4_half hs[];                          // per wave, its slot's activations
+    __shared__ float y[64][W4_ONE_NB][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, n_pad = down.kt * W4_TILE_K;
+    w4_half* mine = hs + wave * (HL ? 2 * n_pad : n_pad);
+    const w4_half* a = mine + 8 * (lane >> 4);
+    for (int s = wave; s < p.kt_slots; s += waves) {
+        const int e = __builtin_amdgcn_readfirstlane(w4_slot_expert(p, s));
+        if (e < 0) continue;
+        W4ReadyRow<W4_SRC_F32, 64, HL> row{(const char*)(p.h + (size_t)s * p.h_ld), p.inter, n_pad, true, lane};
+        row.load();
+        W4Stream st[W4_ONE_NB];
+#pragma unroll
+        for (int b = 0; b < W4_ONE_NB; ++b) {
+            const int nt = W4_ONE_NB * blockIdx.x + b;
+            st[b] = w4_stream<SG, ZERO>(down, e, nt < down.nt ? nt : down.nt - 1, down.kt);
+        }
+        float f = 0, v[W4_ONE_NB] = {};
+        auto part = [&](int q, auto begin) {
+            w4_f32x4 acc[W4_ONE_NB][1] = {};
+            w4_run<2, SG, ZERO, W4_ONE_NB, 1, 1, HL>(
+                acc, st, w4_part_begin(down.kt, parts, q), w4_part_begin(down.kt, parts, q + 1), down.bf16, [](int, int) {},
+                [&](int, int kt, w4_half8 (&x)[1][4], w4_half8 (&lo)[1][4]) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[0][j] = *(const w4_half8*)(a + kt * W4_TILE_K + 32 * j);
+                        if constexpr (HL) lo[0][j] = *(const w4_half8*)(a + n_pad + kt * W4_TILE_K + 32 * j);
+                    }
+                },
+                begin);
+#pragma unroll
+            for (int b = 0; b < W4_ONE_NB; ++b) v[b] += acc[b][0][0];
+        };
+        part(0, [&] {
+            f = row.finish(mine, n_pad, nullptr);
+            wave_lds_fence();
+        });
+        for (int q = 1; q < parts; ++q) part(q, [] {});
+        if (lane < 16)
+#pragma unroll
+            for (int b = 0; b < W4_ONE_NB; ++b) y[s][b][lane] = v[b] * f;
+        wave_lds_fence();
+    }
+    __syncthreads();
+    const int b = threadIdx.x >> 4, c = threadIdx.x & 15, n = 16 * (W4_ONE_NB * blockIdx.x + b) + c;
+    if (threadIdx.x >= 16 * W4_ONE_NB || n >= p.hidden) return;
+    float v = 0;
+    for (int k = 0; k < p.kt_slots; ++k)
+        if (w4_slot_expert(p, k) >= 0) v = __builtin_fmaf(k < p.topk ? p.weights[k] : 1.0f, y[k][b][c], v);
+    w4_store(p.out, n, v, p.bf16);
+}
+
+// out[t] = the slots' outputs in slot order times their routing weights (fp32, as given), rounded once. Four columns a thread;
+// the token's weights come first, so that all its slots' outputs are on their way at once.
 __global__ __launch_bounds__(256) void w4_combine_kernel(W4MoeParams p)
 {
-    const int t = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= p.hidden) return;
-    float v = 0;
-    for (int k = 0; k < p.kt_slots; ++k) {
-        const int s = t * p.kt_slots + k;
-        if (w4_slot_expert(p, s) < 0) continue;
-        v += (k < p.topk ? p.weights[(size_t)t * p.topk + k] : 1.0f) * p.y[(size_t)s * p.hidden + n];
+    __shared__ float w[64];
+    __shared__ int use[64];
+    const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if ((int)threadIdx.x < p.kt_slots) {
+        const int k = threadIdx.x;
+        use[k] = w4_slot_expert(p, t * p.kt_slots + k) >= 0;
+        w[k] = k < p.topk ? p.weights[(size_t)t * p.topk + k] : 1.0f;
     }
-    w4_store(p.out, (size_t)t * p.out_stride + n, v, p.bf16);
+    __syncthreads();
+    if (n >= p.hidden) return;
+    const float* y = p.y + (size_t)t * p.kt_slots * p.hidden + n;
+    float v[4] = {0, 0, 0, 0};
+    if ((p.hidden & 3) == 0) {
+#pragma unroll 8
+        for (int k = 0; k < p.kt_slots; ++k) {
+            if (!use[k]) continue;
+            const w4_f32x4 a = *(const w4_f32x4*)(y + (size_t)k * p.hidden);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(w[k], a[i], v[i]);
+        }
+    } else {
+        for (int k = 0; k < p.kt_slots; ++k)
+            if (use[k])
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < p.hidden) v[i] = __builtin_fmaf(w[k], y[(size_t)k * p.hidden + i], v[i]);
+    }
+    for (int i = 0; i < 4; ++i)
+        if (n + i < p.hidden) w4_store(p.out, (size_t)t * p.out_stride + n + i, v[i], p.bf16);
 }
 
 struct W4MoeLayout {
-    size_t offsets, order, xs, x, h, hs, hh, y, total;
+    size_t n_units, units, order, xs, x, h, hs, hh, y, total;
 };
+
+constexpr int W4_UNIT_ROWS = 16;
+
+// Units of a call, whatever its routes: each slot one of a few tokens'; else every used expert's last, and the full ones.
+static size_t w4_max_units(size_t slots, size_t count, bool few)
+{
+    return few ? slots : (slots < count ? slots : count) + slots / W4_UNIT_ROWS;
+}
 
 static W4MoeLayout w4_moe_layout(int rows, int topk, int n_shared, int hidden, int inter)
 {
@@ -217,13 +456,14 @@ static W4MoeLayout w4_moe_layout(int rows, int topk, int n_shared, int hidden, i
     W4MoeLayout l;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += w4_align(bytes); return o; };
-    l.offsets = take(1025 * 4);
-    l.order = take(slots * 4);
+    l.n_units = take(4);
+    l.units = take(w4_max_units(slots, slots, false) * sizeof(W4Unit));
+    l.order = take((rows <= W4_FEW_ROWS ? slots * slots : slots) * 4);
     l.xs = take((size_t)rows * 4);
     l.x = take(rows * kx * 2);
-    l.h = take(slots * inter * 4);
+    l.h = take(slots * kh * 4);
     l.hs = take(slots * 4);
-    l.hh = take(slots * kh * 2);
+    l.hh = take(slots * kh * 4);                             // fp16 calls keep two halves a value
     l.y = take(slots * hidden * 4);
     l.total = at;
     return l;
@@ -237,19 +477,12 @@ static bool w4_moe_shape_ok(int rows, int topk, int n_shared, int hidden, int in
         return false;
     }
     if (hidden < 1 || hidden > EVAMX_W4_MAX_DIM || inter < 1 || inter > EVAMX_W4_MAX_DIM) { set_error("%s: hidden %d or inter %d", who, hidden, inter); return false; }
+    const long kx = w4_ceil(hidden, W4_TILE_K) * (long)W4_TILE_K, kh = w4_ceil(inter, W4_TILE_K) * (long)W4_TILE_K;
+    if (rows * kx >= 1l << 31 || (long)rows * (topk + n_shared) * kh >= 1l << 30) {
+        set_error("%s: %d rows of %d features or their hidden activations exceed 2^31 or 2^30 values", who, rows, hidden);
+        return false;
+    }
     return true;
-}
-
-template <int SG, bool ZERO>
-static void w4_launch_gate_up(const W4MoeParams& p, const W4Mat& gate, const W4Mat& up, int units, hipStream_t s)
-{
-    w4_gate_up_kernel<SG, ZERO><<<dim3(w4_ceil(p.inter, 16), units), 256, 0, s>>>(p, gate, up);
-}
-
-template <int SG, bool ZERO>
-static void w4_launch_down(const W4MoeParams& p, const W4Mat& down, int units, hipStream_t s)
-{
-    w4_down_kernel<SG, ZERO><<<dim3(w4_ceil(p.hidden, 16), units), 256, 0, s>>>(p, down);
 }
 
 }  // namespace evamx
@@ -292,20 +525,65 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
     W4MoeParams p;
     p.rows = a->rows; p.topk = a->topk; p.n_shared = a->n_shared; p.kt_slots = a->topk + a->n_shared; p.slots = a->rows * p.kt_slots;
     p.count = g.count; p.n_local = g.count - a->n_shared; p.hidden = g.n_in; p.inter = g.n_out; p.bf16 = a->x_dtype == EVAMX_DTYPE_BF16;
+    p.recip = (uint32_t)(((1ull << 32) + p.kt_slots - 1) / p.kt_slots);
     p.first = a->first_expert; p.limit = a->limit; p.sel = a->sel; p.weights = a->weights;
-    p.offsets = (int*)(ws + l.offsets); p.order = (int*)(ws + l.order);
+    p.n_units = (int*)(ws + l.n_units); p.units = (W4Unit*)(ws + l.units); p.order = (int*)(ws + l.order);
     p.x = (const w4_half*)(ws + l.x); p.xs = (const float*)(ws + l.xs);
     p.h = (float*)(ws + l.h); p.hh = (w4_half*)(ws + l.hh); p.hs = (float*)(ws + l.hs); p.y = (float*)(ws + l.y);
     p.out = a->out; p.out_stride = (size_t)a->out_stride;
     const hipStream_t s = (hipStream_t)stream;
     const W4Mat gm = w4_mat(g), um = w4_mat(u), dm = w4_mat(d);
-    const int units = (p.slots < p.count ? p.slots : p.count) + p.slots / 16;
+    p.x_in = a->x; p.x_stride = (size_t)a->x_stride;
+    p.aligned = (((uintptr_t)a->x | (uintptr_t)(2 * a->x_stride)) & 15) == 0;
+    const int gp = w4_moe_parts(gm.kt), dp = w4_moe_parts(dm.kt), h_pad = dm.kt * W4_TILE_K;
+    p.h_ld = h_pad;
+    const bool few = w4_stage_fits(p.rows, gm.kt, W4_WAVES);
+    const unsigned units = (unsigned)w4_max_units(p.slots, p.count, few);
+    p.units_in_use = few ? nullptr : p.n_units;
 
-    w4_launch_rows(a->x, a->x_dtype, (size_t)a->x_stride, p.rows, p.hidden, ws + l.x, (float*)(ws + l.xs), s);
-    w4_group_kernel<<<p.count, 256, 0, s>>>(p);
-    w4_dispatch(g, [&](auto sg, auto zero) { w4_launch_gate_up<decltype(sg)::value, decltype(zero)::value>(p, gm, um, units, s); });
-    w4_hidden_kernel<<<p.slots, 256, 0, s>>>(p, dm.kt * W4_TILE_K);
-    w4_dispatch(d, [&](auto sg, auto zero) { w4_launch_down<decltype(sg)::value, decltype(zero)::value>(p, dm, units, s); });
-    w4_combine_kernel<<<dim3(w4_ceil(p.hidden, 256), p.rows), 256, 0, s>>>(p);
+    // gate and up
+    const dim3 gu_grid(w4_ceil(gm.nt, W4_WAVES / gp), units);
+    if (few) {
+        w4_dispatch(g, [&](auto sg, auto zero) {
+            w4_gate_up_few_kernel<decltype(sg)::value, decltype(zero)::value>
+                <<<gu_grid, 64 * W4_WAVES, w4_stage_bytes(p.rows, gm.kt), s>>>(p, gm, um, gp);
+        });
+    } else {
+        const bool ready = w4_rows_ready(a->x, a->x_dtype, a->x_stride, p.hidden);
+        const int blocks = p.count + (ready ? 0 : p.rows), x_pad = gm.kt * W4_TILE_K;
+        w4_half* xh = (w4_half*)(ws + l.x);
+        float* xs = (float*)(ws + l.xs);
+        if (p.bf16) w4_prep_kernel<EVAMX_DTYPE_BF16><<<blocks, W4_PREP_THREADS, 0, s>>>(p, W4_UNIT_ROWS, xh, xs, x_pad);
+        else w4_prep_kernel<EVAMX_DTYPE_F16><<<blocks, W4_PREP_THREADS, 0, s>>>(p, W4_UNIT_ROWS, xh, xs, x_pad);
+        p.x = ready ? (const w4_half*)a->x : xh;
+        p.xs = ready ? nullptr : xs;
+        w4_dispatch(g, [&](auto sg, auto zero) {
+            w4_gate_up_kernel<1, decltype(sg)::value, decltype(zero)::value, W4_GU_CT, 1><<<dim3(w4_ceil(gm.nt, W4_GU_CT * (W4_WAVES / gp)), units), 64 * W4_WAVES, 0, s>>>(p, gm, um, gp);
+        });
+    }
+
+    // down
+    const int one_waves = p.kt_slots < W4_ONE_WAVES ? p.kt_slots : W4_ONE_WAVES;
+    const size_t one_bytes = (size_t)one_waves * h_pad * (p.bf16 ? 2 : 4);
+    if (p.rows == 1 && one_bytes <= 56 * 1024) {
+        w4_dispatch(d, [&](auto sg, auto zero) {
+            constexpr int SG = decltype(sg)::value;
+            constexpr bool ZERO = decltype(zero)::value;
+            const int blocks = w4_ceil(dm.nt, W4_ONE_NB);
+            if (p.bf16) w4_down_one_kernel<SG, ZERO, false><<<blocks, 64 * one_waves, one_bytes, s>>>(p, dm, dp);
+            else w4_down_one_kernel<SG, ZERO, true><<<blocks, 64 * one_waves, one_bytes, s>>>(p, dm, dp);
+        });
+        return launched("w4_moe_forward");
+    }
+    if (p.bf16) w4_hidden_kernel<false><<<p.slots, 256, 0, s>>>(p, h_pad);
+    else w4_hidden_kernel<true><<<p.slots, 256, 0, s>>>(p, h_pad);
+    const dim3 d_grid(w4_ceil(dm.nt, W4_DOWN_NB * (W4_WAVES / dp)), units);
+    w4_dispatch(d, [&](auto sg, auto zero) {
+        constexpr int SG = decltype(sg)::value;
+        constexpr bool ZERO = decltype(zero)::value;
+        if (p.bf16) w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, false><<<d_grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
+        else w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, true><<<d_grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
+    });
+    w4_combine_kernel<<<dim3(w4_ceil(p.hidden, 1024), p.rows), 256, 0, s>>>(p);
     return launched("w4_moe_forward");
 }

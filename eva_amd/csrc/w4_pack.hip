@@ -36,13 +36,13 @@ __global__ __launch_bounds__(256) void w4_pack_groups_kernel(const uint16_t* __r
                                                              int src_group, W4Mat m, int sg, uint16_t* __restrict__ out_s,
                                                              uint8_t* __restrict__ out_z, size_t total)
 {
-    const int per = W4_QUAD * sg, group = W4_TILE_K / sg, src_n = (m.n_in + src_group - 1) / src_group;
+    const int group = W4_TILE_K / sg, src_n = (m.n_in + src_group - 1) / src_group;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
         const size_t mat = i / m.groups, r = i % m.groups;
-        const int g = (int)(r % per), col = (int)(r / per % W4_TILE_N);
-        const size_t quads = r / (per * W4_TILE_N);
-        const size_t n = quads / m.qt * W4_TILE_N + col;
-        const int k = (int)(quads % m.qt) * (W4_QUAD * W4_TILE_K) + g * group;
+        const int g = (int)(r % sg), col = (int)(r / sg % W4_TILE_N);
+        const size_t tile = r / (sg * W4_TILE_N);
+        const size_t n = tile / m.kt * W4_TILE_N + col;
+        const int k = (int)(tile % m.kt) * W4_TILE_K + g * group;
         const bool in = n < (size_t)m.n_out && k < m.n_in;
         const size_t at = in ? (mat * m.n_out + n) * src_n + k / src_group : 0;
         out_s[i] = in ? scales[at] : 0;
@@ -53,7 +53,6 @@ __global__ __launch_bounds__(256) void w4_pack_groups_kernel(const uint16_t* __r
 // W in fp32, one thread a value: scale * (code - zero), both exact before the one rounding of the product.
 __global__ __launch_bounds__(256) void w4_dequant_kernel(W4Mat m, int sg, float* __restrict__ out, size_t total)
 {
-    const int per = W4_QUAD * sg;
     const size_t mat_size = (size_t)m.n_out * m.n_in;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
         const size_t mat = i / mat_size, r = i % mat_size;
@@ -61,57 +60,34 @@ __global__ __launch_bounds__(256) void w4_dequant_kernel(W4Mat m, int sg, float*
         const int k = (int)(r % m.n_in), nt = (int)(n / W4_TILE_N), col = (int)(n % W4_TILE_N);
         const int kt = k / W4_TILE_K, in_tile = k % W4_TILE_K;
         const int j = in_tile / 32, g = in_tile / 8 % 4, e = in_tile % 8;
-        const uint32_t w = m.codes[(mat * m.tiles + (size_t)nt * m.kt + kt) * W4_TILE_DWORDS + (col + 16 * g) * 4 + j];
+        const size_t tile = (size_t)nt * m.kt + kt;
+        const uint32_t w = m.codes[(mat * m.tiles + tile) * W4_TILE_DWORDS + (col + 16 * g) * 4 + j];
         const int q = (w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15;
-        const size_t at = mat * m.groups + (((size_t)nt * m.qt + kt / W4_QUAD) * W4_TILE_N + col) * per + kt % W4_QUAD * sg +
-                          in_tile * sg / W4_TILE_K;
+        const size_t at = mat * m.groups + (tile * W4_TILE_N + col) * sg + in_tile * sg / W4_TILE_K;
         out[i] = w4_scale(m.scales[at], m.bf16) * (float)(q - (m.zeros ? (int)m.zeros[at] : 8));
     }
 }
 
+// One workgroup a row.
 template <int SRC>
-__device__ __forceinline__ float w4_src(const void* row, int k)
-{
-    if constexpr (SRC == EVAMX_DTYPE_F16) return (float)((const w4_half*)row)[k];
-    else if constexpr (SRC == EVAMX_DTYPE_BF16) return __builtin_bit_cast(float, (uint32_t)((const uint16_t*)row)[k] << 16);
-    else return ((const float*)row)[k];
-}
-
-// One workgroup a row: the largest finite magnitude, then the scaled values. Two passes over a row of a few KiB.
-template <int SRC>
-__global__ __launch_bounds__(256) void w4_rows_kernel(const char* __restrict__ src, size_t stride_bytes, int n_in, int n_pad,
+__global__ __launch_bounds__(256) void w4_rows_kernel(const char* __restrict__ src, size_t stride, bool aligned, int n_in, int n_pad,
                                                       w4_half* __restrict__ dst, float* __restrict__ scale)
 {
     __shared__ uint32_t part[4];
-    const char* row = src + blockIdx.x * stride_bytes;
-    uint32_t top = 0;
-    for (int k = threadIdx.x; k < n_in; k += 256) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, w4_src<SRC>(row, k)) & 0x7fffffffu;
-        if (b < 0x7f800000u && b > top) top = b;
-    }
-    for (int s = 32; s; s >>= 1) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)top, s);
-        top = o > top ? o : top;
-    }
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) top = part[i] > top ? part[i] : top;
-    const int e = w4_exponent(top);
-    const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-    for (int k = threadIdx.x; k < n_pad; k += 256)
-        dst[blockIdx.x * (size_t)n_pad + k] = k < n_in ? (w4_half)(w4_src<SRC>(row, k) * down) : (w4_half)0.0f;
-    if (threadIdx.x == 0) scale[blockIdx.x] = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+    W4ReadyRow<SRC, 256, false> row{src + blockIdx.x * stride, n_in, n_pad, aligned, (int)threadIdx.x};
+    row.load();
+    const float f = row.finish(dst + blockIdx.x * (size_t)n_pad, 0, part);
+    if (threadIdx.x == 0) scale[blockIdx.x] = f;
 }
 
 void w4_launch_rows(const void* src, int src_dtype, size_t src_stride, int rows, int n_in, void* dst, float* scale, hipStream_t stream)
 {
     const int n_pad = w4_ceil(n_in, W4_TILE_K) * W4_TILE_K;
+    const bool aligned = (((uintptr_t)src | (2 * src_stride)) & 15) == 0;
     if (src_dtype == EVAMX_DTYPE_F16)
-        w4_rows_kernel<EVAMX_DTYPE_F16><<<rows, 256, 0, stream>>>((const char*)src, src_stride * 2, n_in, n_pad, (w4_half*)dst, scale);
-    else if (src_dtype == EVAMX_DTYPE_BF16)
-        w4_rows_kernel<EVAMX_DTYPE_BF16><<<rows, 256, 0, stream>>>((const char*)src, src_stride * 2, n_in, n_pad, (w4_half*)dst, scale);
+        w4_rows_kernel<EVAMX_DTYPE_F16><<<rows, 256, 0, stream>>>((const char*)src, src_stride * 2, aligned, n_in, n_pad, (w4_half*)dst, scale);
     else
-        w4_rows_kernel<W4_SRC_F32><<<rows, 256, 0, stream>>>((const char*)src, src_stride * 4, n_in, n_pad, (w4_half*)dst, scale);
+        w4_rows_kernel<EVAMX_DTYPE_BF16><<<rows, 256, 0, stream>>>((const char*)src, src_stride * 2, aligned, n_in, n_pad, (w4_half*)dst, scale);
 }
 
 static int w4_grid(size_t total)
@@ -161,8 +137,7 @@ extern "C" size_t evamx_w4_code_bytes(int count, int n_out, int n_in)
 extern "C" size_t evamx_w4_group_count(int count, int n_out, int n_in, int group)
 {
     if (!w4_stored_group(group) || evamx_w4_code_bytes(count, n_out, n_in) == 0) return 0;
-    return (size_t)count * w4_ceil(n_out, W4_TILE_N) * w4_ceil(n_in, W4_TILE_K * W4_QUAD) *
-           (W4_TILE_N * W4_QUAD * (W4_TILE_K / group));
+    return (size_t)count * w4_ceil(n_out, W4_TILE_N) * w4_ceil(n_in, W4_TILE_K) * (W4_TILE_N * (W4_TILE_K / group));
 }
 
 extern "C" int evamx_w4_pack(const uint8_t* codes, const void* scales, const uint8_t* zeros, int group, const evamx_w4_weight* w,

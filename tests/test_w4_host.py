@@ -19,7 +19,7 @@ def test_stored_groups_and_sizes():
     assert [L.evamx_w4_stored_group(g) for g in (32, 64, 96, 128, 160, 192, 256, 384, 1024)] == [32, 64, 32, 128, 32, 64, 128, 128, 128]
     assert [L.evamx_w4_stored_group(g) for g in (0, -32, 16, 33, 48)] == [0] * 5
     assert L.evamx_w4_code_bytes(1, 16, 128) == 1024 and L.evamx_w4_code_bytes(3, 17, 129) == 3 * 4 * 1024
-    assert L.evamx_w4_group_count(1, 16, 128, 128) == 64 and L.evamx_w4_group_count(2, 17, 513, 32) == 2 * 2 * 2 * 256
+    assert L.evamx_w4_group_count(1, 16, 128, 128) == 16 and L.evamx_w4_group_count(2, 17, 513, 32) == 2 * 2 * 5 * 64
     big = _lib.W4_MAX_DIM
     assert L.evamx_w4_code_bytes(1024, big, big) == 1024 * big * big // 2       # sizes do not wrap at 32 bits
     for bad in ((0, 16, 16), (1025, 16, 16), (1, 0, 16), (1, 16, 0), (1, big + 1, 16), (1, 16, big + 1)):
