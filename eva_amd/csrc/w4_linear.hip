@@ -1,6 +1,6 @@
 // y = x W^T (+ bias) on 4-bit weights with group scales (w4.hpp).
 #include "evamx_internal.hpp"
-#include "w4.hpp"
+#include "w4_gemm.hpp"
 
 namespace evamx {
 
@@ -107,6 +107,54 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat 
     }
 }
 
+constexpr int W4G_MIN_TILES = 200;
+
+// Long calls: 64 rows by 256 columns a workgroup (w4_gemm.hpp). Consecutive workgroups go to the eight XCDs in turn, so each XCD
+// takes a contiguous run of tiles, eight row tiles by all columns at a time: its rows' tiles stay in its L2 while it passes over
+// the columns.
+template <int SG, bool ZERO, int MB>
+__device__ __forceinline__ void w4_linear_gemm(const W4LinearParams& p, const W4Mat& m, int r0, int have, int nt0, char* lds)
+{
+    W4Stream st[W4G_NB];
+#pragma unroll
+    for (int b = 0; b < W4G_NB; ++b) st[b] = w4_stream<SG, ZERO>(m, 0, nt0 + b < m.nt ? nt0 + b : m.nt - 1, m.kt);
+    W4GemmRows<MB> rows;
+    const uint32_t ld = m.kt * (W4_TILE_K * 2);
+    rows.src = w4_rsrc(p.xh + (size_t)r0 * m.kt * W4_TILE_K, have * ld);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) rows.at[i] = (w4g_row<MB>(i) < have ? w4g_row<MB>(i) : have - 1) * ld + w4g_chunk<MB>(i);
+    w4_f32x4 acc[W4G_NB][MB] = {};
+    w4g_run<SG, ZERO, false, MB>(acc, st, rows, lds, m.kt, m.bf16);
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + 16 * mb + 4 * (lane >> 4) + i;
+            if (r >= p.rows) continue;
+            const float f = p.row_scale ? p.row_scale[r] : 1.0f;
+#pragma unroll
+            for (int b = 0; b < W4G_NB; ++b) {
+                const int n = 16 * (nt0 + b) + (lane & 15);
+                if (n < m.n_out) w4_linear_store(p, m, r, n, acc[b][mb][i], f);
+            }
+        }
+}
+
+template <int SG, bool ZERO>
+__global__ __launch_bounds__(256, 2) void w4_linear_gemm_kernel(W4LinearParams p, W4Mat m, int row_tiles, int col_tiles)
+{
+    __shared__ __attribute__((aligned(128))) char lds[W4G_STAGES * W4G_STAGE];
+    const int total = row_tiles * col_tiles, per = w4_ceil(total, 8), t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || t >= total) return;
+    const int band = t / (8 * col_tiles), in_band = t - band * 8 * col_tiles, deep = row_tiles - 8 * band < 8 ? row_tiles - 8 * band : 8;
+    const int r0 = W4G_ROWS * (8 * band + in_band % deep), have = p.rows - r0 < W4G_ROWS ? p.rows - r0 : W4G_ROWS;
+    const int nt0 = W4G_COLS / 16 * (in_band / deep) + (threadIdx.x >> 6) * W4G_NB;
+    if (have > 32) w4_linear_gemm<SG, ZERO, 4>(p, m, r0, have, nt0, lds);
+    else if (have > 16) w4_linear_gemm<SG, ZERO, 2>(p, m, r0, have, nt0, lds);
+    else w4_linear_gemm<SG, ZERO, 1>(p, m, r0, have, nt0, lds);
+}
+
 template <int NB, int MB>
 static void w4_launch_linear(const W4LinearParams& p, const W4Mat& m, const evamx_w4_weight& w, int parts, hipStream_t s)
 {
@@ -165,6 +213,12 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
     // 32 on the same rows (7168 -> 18432 at 5 rows: 21.8 us against 25.8 with 16)
     if (rows <= 16 && m.nt < 1024) w4_launch_linear<1, 1>(p, m, *w, parts, s);
     else if (rows <= 16) w4_launch_linear<2, 1>(p, m, *w, parts, s);
+    else if ((long)w4_ceil(rows, W4G_ROWS) * w4_ceil(m.n_out, W4G_COLS) >= W4G_MIN_TILES) {
+        const int rt = w4_ceil(rows, W4G_ROWS), ct = w4_ceil(m.n_out, W4G_COLS);
+        w4_dispatch(*w, [&](auto sg, auto zero) {
+            w4_linear_gemm_kernel<decltype(sg)::value, decltype(zero)::value><<<8 * w4_ceil(rt * ct, 8), 256, 0, s>>>(p, m, rt, ct);
+        });
+    }
     else if (rows <= 32) w4_launch_linear<2, 2>(p, m, *w, parts, s);
     else w4_launch_linear<2, 4>(p, m, *w, parts < 4 ? parts : 4, s);
     return launched("w4_linear");

@@ -6,7 +6,7 @@
 
 #include "evamx_gemv.hpp"
 #include "evamx_internal.hpp"
-#include "w4.hpp"
+#include "w4_gemm.hpp"
 
 namespace evamx {
 
@@ -21,9 +21,9 @@ struct W4MoeParams {
     float limit;
     const int64_t* sel;
     const float* weights;
-    W4Unit* units;
-    const int* units_in_use;     // their number, or NULL: one for each slot
-    int* n_units;
+    W4Unit *units, *big;         // of up to 16 rows (W4_UNIT_ROWS) and up to 64 (W4G_ROWS)
+    const int* units_in_use;     // number of the former, or NULL: one for each slot
+    int* n_units;                // [2]
     int* order;                  // slots by (expert, slot)
     const void* x_in;            // as given
     size_t x_stride;
@@ -56,14 +56,21 @@ __device__ __forceinline__ int w4_slot_expert(const W4MoeParams& p, int s)
 }
 
 // What a call of more than W4_FEW_ROWS tokens needs before its products, one launch: workgroups 0 .. count - 1 group the slots
-// stably by expert and cut each expert's into units of `tile` rows; the others make a row of x ready each.
+// stably by expert and cut each expert's into units; the others make a row of x ready each. An expert of at most `small` rows has
+// units of 16 rows, one of more units of 64 (the last of any size). In a call of up to 16 tokens all are of 16, whatever an expert
+// gets: a token's arithmetic is then the one it has alone.
 //
 // The workgroup of expert e reads every slot (from L2; far below the products that follow): a histogram gives the places of its
 // slots and units, each wave counts its own range's slots of e, then writes them in order.
-constexpr int W4_PREP_THREADS = 512;
+constexpr int W4_PREP_THREADS = 512, W4_UNIT_ROWS = 16;
+
+// Experts of up to this many rows go to the kernels of 16-row units, which keep more of the memory busy; larger ones would read
+// their weights twice there (7168 x 2048, 256 experts of 19 rows on average: 1365 us with 16, 1684 with 24; of 9 rows: 1298 and
+// 1248).
+constexpr int W4_REST_ROWS = 16;
 
 template <int SRC>
-__global__ __launch_bounds__(W4_PREP_THREADS) void w4_prep_kernel(W4MoeParams p, int tile, w4_half* __restrict__ xh, float* __restrict__ xs, int n_pad)
+__global__ __launch_bounds__(W4_PREP_THREADS) void w4_prep_kernel(W4MoeParams p, int small, w4_half* __restrict__ xh, float* __restrict__ xs, int n_pad)
 {
     constexpr int WAVES = W4_PREP_THREADS / 64;
     __shared__ uint32_t top[WAVES];
@@ -75,50 +82,55 @@ __global__ __launch_bounds__(W4_PREP_THREADS) void w4_prep_kernel(W4MoeParams p,
         if (threadIdx.x == 0) xs[t] = f;
         return;
     }
-    __shared__ int hist[1024], mine_n[WAVES], sums[3][WAVES];
+    __shared__ int hist[1024], mine_n[WAVES], sums[5][WAVES];
     const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < p.count; i += W4_PREP_THREADS) hist[i] = 0;
     __syncthreads();
     const int span = (w4_ceil(p.slots, WAVES) + 63) & ~63, s0 = wave * span, s1 = s0 + span < p.slots ? s0 + span : p.slots;
     int own = 0;
     for (int s = s0 + lane; s < s1; s += 64) {
-        const int v = w4_slot_expert(p, s);
-        if (v >= 0) atomicAdd(&hist[v], 1);
-        own += v == e;
+        const int x = w4_slot_expert(p, s);
+        if (x >= 0) atomicAdd(&hist[x], 1);
+        own += x == e;
     }
     for (int i = 32; i; i >>= 1) own += __shfl_xor(own, i);
     if (lane == 0) mine_n[wave] = own;
     __syncthreads();
-    int slots = 0, units = 0, all = 0;
+    auto bigs = [&](int n) { return n <= small ? 0 : (n + W4G_ROWS - 1) / W4G_ROWS; };
+    auto smalls = [&](int n) { return n <= small ? (n + W4_UNIT_ROWS - 1) / W4_UNIT_ROWS : 0; };
+    int v[5] = {0, 0, 0, 0, 0};                              // before e: slots, units, big units; in all: units, big units
     for (int i = threadIdx.x; i < p.count; i += W4_PREP_THREADS) {
-        const int n = hist[i], u = (n + tile - 1) / tile;
-        all += u;
+        const int n = hist[i], u = smalls(n), b = bigs(n);
+        v[3] += u;
+        v[4] += b;
         if (i < e) {
-            slots += n;
-            units += u;
+            v[0] += n;
+            v[1] += u;
+            v[2] += b;
         }
     }
-    for (int i = 32; i; i >>= 1) {
-        slots += __shfl_xor(slots, i);
-        units += __shfl_xor(units, i);
-        all += __shfl_xor(all, i);
-    }
-    if (lane == 0) {
-        sums[0][wave] = slots;
-        sums[1][wave] = units;
-        sums[2][wave] = all;
+#pragma unroll
+    for (int c = 0; c < 5; ++c) {
+        for (int i = 32; i; i >>= 1) v[c] += __shfl_xor(v[c], i);
+        if (lane == 0) sums[c][wave] = v[c];
     }
     __syncthreads();
-    slots = units = all = 0;
-    for (int w = 0; w < WAVES; ++w) {
-        slots += sums[0][w];
-        units += sums[1][w];
-        all += sums[2][w];
+#pragma unroll
+    for (int c = 0; c < 5; ++c) {
+        v[c] = 0;
+        for (int w = 0; w < WAVES; ++w) v[c] += sums[c][w];
     }
-    const int n = hist[e];
-    if (e == 0 && threadIdx.x == 0) *p.n_units = all;
-    for (int i = threadIdx.x; i * tile < n; i += W4_PREP_THREADS)
-        p.units[units + i] = W4Unit{e, slots + i * tile, n - i * tile < tile ? n - i * tile : tile, 0};
+    const int n = hist[e], slots = v[0], nb = bigs(n), done = nb ? n : 0;
+    if (e == 0 && threadIdx.x == 0) {
+        p.n_units[0] = v[3];
+        p.n_units[1] = v[4];
+    }
+    for (int i = threadIdx.x; i < nb; i += W4_PREP_THREADS)
+        p.big[v[2] + i] = W4Unit{e, slots + i * W4G_ROWS, n - i * W4G_ROWS < W4G_ROWS ? n - i * W4G_ROWS : W4G_ROWS, 0};
+    for (int i = threadIdx.x; done + i * W4_UNIT_ROWS < n; i += W4_PREP_THREADS) {
+        const int r = done + i * W4_UNIT_ROWS;
+        p.units[v[1] + i] = W4Unit{e, slots + r, n - r < W4_UNIT_ROWS ? n - r : W4_UNIT_ROWS, 0};
+    }
     int at = slots;
     for (int w = 0; w < wave; ++w) at += mine_n[w];
     for (int b0 = s0; b0 < s1; b0 += 64) {
@@ -345,6 +357,102 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W
     }
 }
 
+// 128 columns of gate and up by a unit of up to 64 rows: the streams of a wave are gate and up of two column tiles.
+template <int SG, bool ZERO, int MB>
+__device__ __forceinline__ void w4_gate_up_gemm(const W4MoeParams& p, const W4Mat& gate, const W4Mat& up, const W4Unit& u, char* lds)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = (blockIdx.x * W4G_WAVES + wave) * (W4G_NB / 2);
+    W4Stream st[W4G_NB];
+#pragma unroll
+    for (int c = 0; c < W4G_NB / 2; ++c) {
+        const int t = nt + c < gate.nt ? nt + c : gate.nt - 1;
+        st[2 * c] = w4_stream<SG, ZERO>(gate, u.expert, t, gate.kt);
+        st[2 * c + 1] = w4_stream<SG, ZERO>(up, u.expert, t, gate.kt);
+    }
+    W4GemmRows<MB> rows;
+    const uint32_t ld = gate.kt * (W4_TILE_K * 2);
+    rows.src = w4_rsrc(p.x, p.rows * ld);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const int r = w4g_row<MB>(i);
+        rows.at[i] = w4_token(p, p.order[u.r0 + (r < u.rows ? r : u.rows - 1)]) * ld + w4g_chunk<MB>(i);
+    }
+    w4_f32x4 acc[W4G_NB][MB] = {};
+    w4g_run<SG, ZERO, false, MB>(acc, st, rows, lds, gate.kt, gate.bf16);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 16 * mb + 4 * (lane >> 4) + i;
+            if (r >= u.rows) continue;
+            const int s = p.order[u.r0 + r];
+            const float f = p.xs ? p.xs[w4_token(p, s)] : 1.0f;
+#pragma unroll
+            for (int c = 0; c < W4G_NB / 2; ++c) {
+                const int n = 16 * (nt + c) + (lane & 15);
+                if (n < p.inter)
+                    p.h[(size_t)s * p.h_ld + n] = w4_swiglu(acc[2 * c][mb][i] * f, acc[2 * c + 1][mb][i] * f, p.limit, u.expert >= p.n_local);
+            }
+        }
+}
+
+template <int SG, bool ZERO>
+__global__ __launch_bounds__(64 * W4G_WAVES, 2) void w4_gate_up_gemm_kernel(W4MoeParams p, W4Mat gate, W4Mat up)
+{
+    __shared__ __attribute__((aligned(128))) char lds[W4G_STAGES * W4G_STAGE];
+    if ((int)blockIdx.y >= p.n_units[1]) return;
+    const W4Unit u = p.big[blockIdx.y];
+    if (u.rows > 32) w4_gate_up_gemm<SG, ZERO, 4>(p, gate, up, u, lds);
+    else if (u.rows > 16) w4_gate_up_gemm<SG, ZERO, 2>(p, gate, up, u, lds);
+    else w4_gate_up_gemm<SG, ZERO, 1>(p, gate, up, u, lds);
+}
+
+// 256 columns of the output by a unit of up to 64 rows.
+template <int SG, bool ZERO, bool HL, int MB>
+__device__ __forceinline__ void w4_down_gemm(const W4MoeParams& p, const W4Mat& down, const W4Unit& u, char* lds)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = (blockIdx.x * W4G_WAVES + wave) * W4G_NB;
+    W4Stream st[W4G_NB];
+#pragma unroll
+    for (int b = 0; b < W4G_NB; ++b) st[b] = w4_stream<SG, ZERO>(down, u.expert, nt + b < down.nt ? nt + b : down.nt - 1, down.kt);
+    W4GemmRows<MB> rows;
+    const uint32_t half = down.kt * (W4_TILE_K * 2), ld = HL ? 2 * half : half;
+    rows.src = w4_rsrc(p.hh, p.slots * ld);
+    rows.lo_off = half;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const int r = w4g_row<MB>(i);
+        rows.at[i] = p.order[u.r0 + (r < u.rows ? r : u.rows - 1)] * ld + w4g_chunk<MB>(i);
+    }
+    w4_f32x4 acc[W4G_NB][MB] = {};
+    w4g_run<SG, ZERO, HL, MB>(acc, st, rows, lds, down.kt, down.bf16);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 16 * mb + 4 * (lane >> 4) + i;
+            if (r >= u.rows) continue;
+            const int s = p.order[u.r0 + r];
+            const float f = p.hs[s];
+#pragma unroll
+            for (int b = 0; b < W4G_NB; ++b) {
+                const int n = 16 * (nt + b) + (lane & 15);
+                if (n < p.hidden) p.y[(size_t)s * p.hidden + n] = acc[b][mb][i] * f;
+            }
+        }
+}
+
+template <int SG, bool ZERO, bool HL>
+__global__ __launch_bounds__(64 * W4G_WAVES, HL ? 1 : 2) void w4_down_gemm_kernel(W4MoeParams p, W4Mat down)
+{
+    __shared__ __attribute__((aligned(128))) char lds[W4G_STAGES * W4G_STAGE * (HL ? 2 : 1)];
+    if ((int)blockIdx.y >= p.n_units[1]) return;
+    const W4Unit u = p.big[blockIdx.y];
+    if (u.rows > 32) w4_down_gemm<SG, ZERO, HL, 4>(p, down, u, lds);
+    else if (u.rows > 16) w4_down_gemm<SG, ZERO, HL, 2>(p, down, u, lds);
+    else w4_down_gemm<SG, ZERO, HL, 1>(p, down, u, lds);
+}
+
 // One token: 16 NB columns of the output, a wave a slot (up to 16, then the next ones), its parts of the k-tiles one after the
 // other; the slots' sums meet in LDS, so that no launch follows.
 constexpr int W4_ONE_WAVES = 16, W4_ONE_NB = 2;
@@ -438,16 +546,19 @@ __global__ __launch_bounds__(256) void w4_combine_kernel(W4MoeParams p)
 }
 
 struct W4MoeLayout {
-    size_t n_units, units, order, xs, x, h, hs, hh, y, total;
+    size_t n_units, units, big, order, xs, x, h, hs, hh, y, total;
 };
 
-constexpr int W4_UNIT_ROWS = 16;
-
-// Units of a call, whatever its routes: each slot one of a few tokens'; else every used expert's last, and the full ones.
-static size_t w4_max_units(size_t slots, size_t count, bool few)
+// The most units a call can have, whatever its routes: few tokens have one for each slot; else an expert has at most
+// W4_REST_ROWS rows in units of 16, and one with units of 64 has more than W4_REST_ROWS rows for each.
+static size_t w4_max_units(size_t slots, size_t count, bool few, bool all_small)
 {
-    return few ? slots : (slots < count ? slots : count) + slots / W4_UNIT_ROWS;
+    if (few) return slots;
+    const size_t rests = all_small ? (slots < count ? slots : count) + slots / W4_UNIT_ROWS : count * ((W4_REST_ROWS + W4_UNIT_ROWS - 1) / W4_UNIT_ROWS);
+    return slots < rests ? slots : rests;
 }
+
+static size_t w4_max_big(size_t slots) { return slots / (W4_REST_ROWS + 1); }
 
 static W4MoeLayout w4_moe_layout(int rows, int topk, int n_shared, int hidden, int inter)
 {
@@ -456,8 +567,9 @@ static W4MoeLayout w4_moe_layout(int rows, int topk, int n_shared, int hidden, i
     W4MoeLayout l;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += w4_align(bytes); return o; };
-    l.n_units = take(4);
-    l.units = take(w4_max_units(slots, slots, false) * sizeof(W4Unit));
+    l.n_units = take(8);
+    l.units = take(slots * sizeof(W4Unit));
+    l.big = take(w4_max_big(slots) * sizeof(W4Unit));
     l.order = take((rows <= W4_FEW_ROWS ? slots * slots : slots) * 4);
     l.xs = take((size_t)rows * 4);
     l.x = take(rows * kx * 2);
@@ -527,7 +639,7 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
     p.count = g.count; p.n_local = g.count - a->n_shared; p.hidden = g.n_in; p.inter = g.n_out; p.bf16 = a->x_dtype == EVAMX_DTYPE_BF16;
     p.recip = (uint32_t)(((1ull << 32) + p.kt_slots - 1) / p.kt_slots);
     p.first = a->first_expert; p.limit = a->limit; p.sel = a->sel; p.weights = a->weights;
-    p.n_units = (int*)(ws + l.n_units); p.units = (W4Unit*)(ws + l.units); p.order = (int*)(ws + l.order);
+    p.n_units = (int*)(ws + l.n_units); p.units = (W4Unit*)(ws + l.units); p.big = (W4Unit*)(ws + l.big); p.order = (int*)(ws + l.order);
     p.x = (const w4_half*)(ws + l.x); p.xs = (const float*)(ws + l.xs);
     p.h = (float*)(ws + l.h); p.hh = (w4_half*)(ws + l.hh); p.hs = (float*)(ws + l.hs); p.y = (float*)(ws + l.y);
     p.out = a->out; p.out_stride = (size_t)a->out_stride;
@@ -538,51 +650,58 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
     const int gp = w4_moe_parts(gm.kt), dp = w4_moe_parts(dm.kt), h_pad = dm.kt * W4_TILE_K;
     p.h_ld = h_pad;
     const bool few = w4_stage_fits(p.rows, gm.kt, W4_WAVES);
-    const unsigned units = (unsigned)w4_max_units(p.slots, p.count, few);
+    const bool all_small = p.rows <= W4_UNIT_ROWS || p.slots <= W4_REST_ROWS;
+    const unsigned units = (unsigned)w4_max_units(p.slots, p.count, few, all_small), bigs = few || all_small ? 0 : (unsigned)w4_max_big(p.slots);
     p.units_in_use = few ? nullptr : p.n_units;
 
-    // gate and up
-    const dim3 gu_grid(w4_ceil(gm.nt, W4_WAVES / gp), units);
+    // a few tokens: their rows in LDS; one token: two launches in all
     if (few) {
         w4_dispatch(g, [&](auto sg, auto zero) {
             w4_gate_up_few_kernel<decltype(sg)::value, decltype(zero)::value>
-                <<<gu_grid, 64 * W4_WAVES, w4_stage_bytes(p.rows, gm.kt), s>>>(p, gm, um, gp);
+                <<<dim3(w4_ceil(gm.nt, W4_WAVES / gp), units), 64 * W4_WAVES, w4_stage_bytes(p.rows, gm.kt), s>>>(p, gm, um, gp);
         });
+        const int one_waves = p.kt_slots < W4_ONE_WAVES ? p.kt_slots : W4_ONE_WAVES;
+        const size_t one_bytes = (size_t)one_waves * h_pad * (p.bf16 ? 2 : 4);
+        if (p.rows == 1 && one_bytes <= 56 * 1024) {
+            w4_dispatch(d, [&](auto sg, auto zero) {
+                constexpr int SG = decltype(sg)::value;
+                constexpr bool ZERO = decltype(zero)::value;
+                const int blocks = w4_ceil(dm.nt, W4_ONE_NB);
+                if (p.bf16) w4_down_one_kernel<SG, ZERO, false><<<blocks, 64 * one_waves, one_bytes, s>>>(p, dm, dp);
+                else w4_down_one_kernel<SG, ZERO, true><<<blocks, 64 * one_waves, one_bytes, s>>>(p, dm, dp);
+            });
+            return launched("w4_moe_forward");
+        }
     } else {
         const bool ready = w4_rows_ready(a->x, a->x_dtype, a->x_stride, p.hidden);
-        const int blocks = p.count + (ready ? 0 : p.rows), x_pad = gm.kt * W4_TILE_K;
+        const int blocks = p.count + (ready ? 0 : p.rows), x_pad = gm.kt * W4_TILE_K, rest = all_small ? p.slots : W4_REST_ROWS;
         w4_half* xh = (w4_half*)(ws + l.x);
         float* xs = (float*)(ws + l.xs);
-        if (p.bf16) w4_prep_kernel<EVAMX_DTYPE_BF16><<<blocks, W4_PREP_THREADS, 0, s>>>(p, W4_UNIT_ROWS, xh, xs, x_pad);
-        else w4_prep_kernel<EVAMX_DTYPE_F16><<<blocks, W4_PREP_THREADS, 0, s>>>(p, W4_UNIT_ROWS, xh, xs, x_pad);
+        if (p.bf16) w4_prep_kernel<EVAMX_DTYPE_BF16><<<blocks, W4_PREP_THREADS, 0, s>>>(p, rest, xh, xs, x_pad);
+        else w4_prep_kernel<EVAMX_DTYPE_F16><<<blocks, W4_PREP_THREADS, 0, s>>>(p, rest, xh, xs, x_pad);
         p.x = ready ? (const w4_half*)a->x : xh;
         p.xs = ready ? nullptr : xs;
         w4_dispatch(g, [&](auto sg, auto zero) {
-            w4_gate_up_kernel<1, decltype(sg)::value, decltype(zero)::value, W4_GU_CT, 1><<<dim3(w4_ceil(gm.nt, W4_GU_CT * (W4_WAVES / gp)), units), 64 * W4_WAVES, 0, s>>>(p, gm, um, gp);
-        });
-    }
-
-    // down
-    const int one_waves = p.kt_slots < W4_ONE_WAVES ? p.kt_slots : W4_ONE_WAVES;
-    const size_t one_bytes = (size_t)one_waves * h_pad * (p.bf16 ? 2 : 4);
-    if (p.rows == 1 && one_bytes <= 56 * 1024) {
-        w4_dispatch(d, [&](auto sg, auto zero) {
             constexpr int SG = decltype(sg)::value;
             constexpr bool ZERO = decltype(zero)::value;
-            const int blocks = w4_ceil(dm.nt, W4_ONE_NB);
-            if (p.bf16) w4_down_one_kernel<SG, ZERO, false><<<blocks, 64 * one_waves, one_bytes, s>>>(p, dm, dp);
-            else w4_down_one_kernel<SG, ZERO, true><<<blocks, 64 * one_waves, one_bytes, s>>>(p, dm, dp);
+            if (bigs) w4_gate_up_gemm_kernel<SG, ZERO><<<dim3(w4_ceil(gm.nt, W4G_WAVES * W4G_NB / 2), bigs), 64 * W4G_WAVES, 0, s>>>(p, gm, um);
+            w4_gate_up_kernel<1, SG, ZERO, W4_GU_CT, 1>
+                <<<dim3(w4_ceil(gm.nt, W4_GU_CT * (W4_WAVES / gp)), units), 64 * W4_WAVES, 0, s>>>(p, gm, um, gp);
         });
-        return launched("w4_moe_forward");
     }
     if (p.bf16) w4_hidden_kernel<false><<<p.slots, 256, 0, s>>>(p, h_pad);
     else w4_hidden_kernel<true><<<p.slots, 256, 0, s>>>(p, h_pad);
-    const dim3 d_grid(w4_ceil(dm.nt, W4_DOWN_NB * (W4_WAVES / dp)), units);
     w4_dispatch(d, [&](auto sg, auto zero) {
         constexpr int SG = decltype(sg)::value;
         constexpr bool ZERO = decltype(zero)::value;
-        if (p.bf16) w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, false><<<d_grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
-        else w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, true><<<d_grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
+        const dim3 grid(w4_ceil(dm.nt, W4_DOWN_NB * (W4_WAVES / dp)), units), big_grid(w4_ceil(dm.nt, W4G_WAVES * W4G_NB), bigs);
+        if (p.bf16) {
+            if (bigs) w4_down_gemm_kernel<SG, ZERO, false><<<big_grid, 64 * W4G_WAVES, 0, s>>>(p, dm);
+            w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, false><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
+        } else {
+            if (bigs) w4_down_gemm_kernel<SG, ZERO, true><<<big_grid, 64 * W4G_WAVES, 0, s>>>(p, dm);
+            w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, true><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
+        }
     });
     w4_combine_kernel<<<dim3(w4_ceil(p.hidden, 1024), p.rows), 256, 0, s>>>(p);
     return launched("w4_moe_forward");
