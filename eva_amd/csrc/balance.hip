@@ -8,6 +8,9 @@
 //   dlog a/dz = sigma(-z) for sigmoid, sigma(z) / (2 softplus(z)) for sqrt(softplus).
 #include <cstring>
 
+#include <type_traits>
+
+#include "evamx_device.hpp"
 #include "evamx_internal.hpp"
 
 namespace evamx {
@@ -26,20 +29,31 @@ struct BalanceParams {
     int32_t* tokens;            // [sequences]
     const float* grad_loss;
     void* grad;
+    // work: chunks of `chunk` rows, a workgroup each; the part of sequence s in chunk w is piece w + s (an ascending walk over
+    // both, so no two parts share one)
+    int chunk;
+    uint32_t recip;             // ceil(2^32 / topk)
+    float* share;               // [pieces][experts]: sum of p
+    int32_t* picks;             // [pieces][experts]
+    int32_t* piece_tokens;      // [pieces]
+    float* group_loss;          // [sequences][groups of 64 experts]
+    unsigned long long* arrive; // [sequences], ARRIVE_STRIDE words apart
 };
 
-__device__ __forceinline__ float bal_load(const void* p, size_t at, int dtype)
+template <int DT>
+__device__ __forceinline__ float bal_load(const void* p, size_t at)
 {
-    if (dtype == EVAMX_DTYPE_F32) return ((const float*)p)[at];
-    if (dtype == EVAMX_DTYPE_BF16) return __builtin_bit_cast(float, (uint32_t)((const uint16_t*)p)[at] << 16);
-    return (float)((const _Float16*)p)[at];
+    if constexpr (DT == EVAMX_DTYPE_F32) return ((const float*)p)[at];
+    else if constexpr (DT == EVAMX_DTYPE_BF16) return __builtin_bit_cast(float, (uint32_t)((const uint16_t*)p)[at] << 16);
+    else return (float)((const _Float16*)p)[at];
 }
 
-__device__ __forceinline__ void bal_store(void* p, size_t at, float v, int dtype)
+template <int DT>
+__device__ __forceinline__ void bal_store(void* p, size_t at, float v)
 {
-    if (dtype == EVAMX_DTYPE_F32) {
+    if constexpr (DT == EVAMX_DTYPE_F32) {
         ((float*)p)[at] = v;
-    } else if (dtype == EVAMX_DTYPE_BF16) {
+    } else if constexpr (DT == EVAMX_DTYPE_BF16) {
         uint32_t b = __builtin_bit_cast(uint32_t, v);
         b = (b & 0x7fffffffu) > 0x7f800000u ? 0x7fc00000u : b + 0x7fffu + ((b >> 16) & 1);
         ((uint16_t*)p)[at] = (uint16_t)(b >> 16);
@@ -56,131 +70,340 @@ __device__ __forceinline__ int bal_start(const BalanceParams& p, int s)
     return v < 0 ? 0 : v > p.rows ? p.rows : v;
 }
 
-// score(z) * 2^(shift): the row's shift lifts rows whose scores would all underflow; it drops out of the shares.
-__device__ __forceinline__ float bal_score(float z, float lift, int score)
-{
-    const float e = expf(-fabsf(z));                                     // in (0, 1]; 0 at infinity
-    if (score == EVAMX_SCORE_SIGMOID) return z >= 0 ? 1.0f / (1.0f + e) : expf(z + lift) / (1.0f + e);
-    if (z >= -16.0f) return sqrtf(fmaxf(z, 0.0f) + log1pf(e)) * expf(0.5f * lift);
-    return expf(0.5f * (z + lift));                                      // softplus(z) = e^z (1 - e^z / 2 ..)
-}
-
-__device__ __forceinline__ float bal_slope(float z, int score)
-{
-    const float e = expf(-fabsf(z)), d = 1.0f / (1.0f + e);
-    if (score == EVAMX_SCORE_SIGMOID) return z >= 0 ? e * d : d;
-    if (z < -16.0f) return 0.5f;
-    return 0.5f * (z >= 0 ? d : e * d) / (fmaxf(z, 0.0f) + log1pf(e));
-}
-
-template <class T, class F>
-__device__ __forceinline__ T wave_all(T v, F f)
-{
-    for (int s = 32; s; s >>= 1) v = f(v, __shfl_xor(v, s));
-    return v;
-}
-
-// The row's shares in a wave's lanes: p[i] is expert lane + 64 i. A row whose logits are all -inf has none (zeros).
-__device__ __forceinline__ void bal_shares(const BalanceParams& q, int row, float (&z)[BAL_MAX_EXPERTS / 64], float (&p)[BAL_MAX_EXPERTS / 64])
+// The sequence that holds a row: the last that starts at or before it (-1 before the first, `sequences` behind the last). Each
+// step's 64 probes leave a 64th of the table.
+__device__ __forceinline__ int bal_sequence(const BalanceParams& p, int row)
 {
     const int lane = threadIdx.x & 63;
-    const float inf = __builtin_inff();
-    float top = -inf;
-#pragma unroll
-    for (int i = 0; i < BAL_MAX_EXPERTS / 64; ++i) {
-        const int e = lane + 64 * i;
-        z[i] = e < q.experts ? bal_load(q.logits, row * q.stride + e, q.dtype) : -inf;
-        top = fmaxf(top, z[i]);
+    int lo = 0, n = p.sequences + 1;                          // starts[lo .. lo + n) hold the first one past the row
+    while (n > 0) {
+        const int step = (n + 63) / 64, at = lo + lane * step;
+        const bool past = at >= lo + n || bal_start(p, at) > row;
+        const unsigned long long b = __ballot(past);
+        const int first = b ? __builtin_ctzll(b) : 64;        // probes before it start at or before the row
+        if (first == 0) break;
+        const int next = lo + (first - 1) * step + 1;
+        n = (first - 1) * step + step < n ? step - 1 : n - (next - lo);
+        lo = next;
     }
-    top = wave_all(top, [](float a, float b) { return fmaxf(a, b); });
-    const float lift = top < 0 && top > -inf ? -top : 0.0f;
+    return lo - 1;
+}
+
+// Sum over a wave in a fixed order, the same in every lane.
+__device__ __forceinline__ float bal_wave_sum(float v)
+{
+    auto step = [](float a, auto ctrl) {
+        return a + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, a), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    v = step(v, std::integral_constant<int, 0xb1>());         // lane ^ 1
+    v = step(v, std::integral_constant<int, 0x4e>());         // lane ^ 2
+    v = step(v, std::integral_constant<int, 0x141>());        // the half row mirrored
+    v = step(v, std::integral_constant<int, 0x140>());        // the row of 16 mirrored
+    const int b = __builtin_bit_cast(int, v);
+    const float r0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 0)), r1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16));
+    const float r2 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 32)), r3 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48));
+    return (r0 + r1) + (r2 + r3);
+}
+
+// log(1 + e) for e in [0, 1], to a few fp32 steps: log(u) e / (u - 1) with u = 1 + e as rounded, whose error in u cancels.
+__device__ __forceinline__ float bal_log1p(float e)
+{
+    const float u = 1.0f + e, d = u - 1.0f;
+    return d == 0.0f ? e : __logf(u) * (e * __builtin_amdgcn_rcpf(d));
+}
+
+// The score of a logit and d log(score) / dz, by the hardware's exp2, log2, reciprocal and root (about one fp32 step each).
+__device__ __forceinline__ void bal_score(float z, int score, float& a, float& slope)
+{
+    const float e = __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+    const float up = z >= 0 ? r : er, down = z >= 0 ? er : r;                       // sigma(z), sigma(-z)
+    if (score == EVAMX_SCORE_SIGMOID) {
+        a = up;
+        slope = down;
+    } else {
+        const float sp = fmaxf(z, 0.0f) + bal_log1p(e);
+        a = __builtin_amdgcn_sqrtf(sp);
+        slope = z < -16.0f ? 0.5f : 0.5f * up * __builtin_amdgcn_rcpf(sp);           // 1 - e^z / 4 ..
+    }
+}
+
+// The same for a row whose scores may all underflow: times 2^(lift / ln 2) (its root), which drops out of the shares, with the
+// limit of the slope far below zero.
+__device__ __forceinline__ float bal_score_far(float z, float lift, int score, float& slope)
+{
+    const float e = expf(-fabsf(z)), d = 1.0f / (1.0f + e);
+    if (score == EVAMX_SCORE_SIGMOID) {
+        slope = z >= 0 ? e * d : d;
+        return z >= 0 ? d : expf(z + lift) * d;
+    }
+    const float sp = fmaxf(z, 0.0f) + log1pf(e);
+    slope = z < -16.0f ? 0.5f : 0.5f * (z >= 0 ? d : e * d) / sp;
+    return z < -16.0f ? expf(0.5f * (z + lift)) : sqrtf(sp) * expf(0.5f * lift);     // softplus(z) = e^z (1 - e^z / 2 ..)
+}
+
+// The shares of a row and the slopes, expert lane + 64 i in element i; z: the row's logits, -inf past the experts. A row whose
+// logits are all -inf has none (zeros). Scores that underflow beside a sum over the threshold are below 2^-26 of it; smaller
+// sums are made again relative to the row's largest logit.
+template <int N>
+__device__ __forceinline__ void bal_shares(const float (&z)[N], int score, float (&p)[N], float (&slope)[N])
+{
     float sum = 0;
 #pragma unroll
-    for (int i = 0; i < BAL_MAX_EXPERTS / 64; ++i) {
-        p[i] = bal_score(z[i], lift, q.score);
+    for (int i = 0; i < N; ++i) {
+        bal_score(z[i], score, p[i], slope[i]);
         sum += p[i];
     }
-    sum = wave_all(sum, [](float a, float b) { return a + b; });
-    const float inv = top == -inf && sum == 0 ? 0.0f : 1.0f / sum;
+    sum = bal_wave_sum(sum);
+    float inv = __builtin_amdgcn_rcpf(sum);
+    if (!(sum >= (score == EVAMX_SCORE_SIGMOID ? 1e-30f : 1e-11f))) {
+        const float inf = __builtin_inff();
+        float top = -inf;
 #pragma unroll
-    for (int i = 0; i < BAL_MAX_EXPERTS / 64; ++i) p[i] *= inv;
-}
-
-// One workgroup a sequence: its four waves take every fourth token, their sums meet in LDS in a fixed order.
-__global__ __launch_bounds__(256) void balance_kernel(BalanceParams q)
-{
-    constexpr int N = BAL_MAX_EXPERTS / 64;
-    __shared__ float share[4][BAL_MAX_EXPERTS];
-    __shared__ int picks[BAL_MAX_EXPERTS], total;
-    __shared__ float part[4];
-    const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int e = threadIdx.x; e < BAL_MAX_EXPERTS; e += 256) picks[e] = 0;
-    if (threadIdx.x == 0) total = 0;
-    __syncthreads();
-    const int t0 = bal_start(q, s), t1 = bal_start(q, s + 1);
-    float acc[N] = {};
-    int n = 0;
-    for (int t = t0 + wave; t < t1; t += 4) {
-        if (q.mask && !q.mask[t]) continue;
-        ++n;
-        float z[N], p[N];
-        bal_shares(q, t, z, p);
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] += p[i];
-        if (lane < q.topk) {
-            const int64_t e = q.sel[(size_t)t * q.topk + lane];
-            if (e >= 0 && e < q.experts) atomicAdd(&picks[e], 1);
-        }
-    }
-    if (lane == 0 && n) atomicAdd(&total, n);
-#pragma unroll
-    for (int i = 0; i < N; ++i) share[wave][lane + 64 * i] = acc[i];
-    __syncthreads();
-    float v = 0;
-    for (int e = threadIdx.x; e < q.experts; e += 256) {
-        v += (float)picks[e] * ((share[0][e] + share[1][e]) + (share[2][e] + share[3][e]));
-        q.counts[(size_t)s * q.experts + e] = picks[e];
-    }
-    v = wave_all(v, [](float a, float b) { return a + b; });
-    if (lane == 0) part[wave] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const float k = total ? (float)q.experts / ((float)q.topk * (float)total * (float)total) : 0.0f;
-        q.loss[s] = k * ((part[0] + part[1]) + (part[2] + part[3]));
-        q.tokens[s] = total;
-    }
-}
-
-// One wave a row. A row of no sequence, or masked, has a zero gradient.
-__global__ __launch_bounds__(256) void balance_grad_kernel(BalanceParams q)
-{
-    constexpr int N = BAL_MAX_EXPERTS / 64;
-    const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= q.rows) return;
-    int s = -1;
-    if (!q.mask || q.mask[t])
-        for (int i = 0; i < q.sequences; ++i)
-            if (t >= bal_start(q, i) && t < bal_start(q, i + 1)) s = i;
-    float g[N] = {};
-    if (s >= 0) {
-        float z[N], p[N], c[N], dot = 0;
-        bal_shares(q, t, z, p);
+        for (int i = 0; i < N; ++i) top = fmaxf(top, z[i]);
+        for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
+        const float lift = top < 0 && top > -inf ? -top : 0.0f;
+        sum = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int e = lane + 64 * i;
-            c[i] = e < q.experts ? (float)q.counts[(size_t)s * q.experts + e] : 0.0f;
-            dot += c[i] * p[i];
+            p[i] = bal_score_far(z[i], lift, score, slope[i]);
+            sum += p[i];
         }
-        dot = wave_all(dot, [](float a, float b) { return a + b; });
-        const float n = (float)q.tokens[s], k = q.grad_loss[s] * ((float)q.experts / ((float)q.topk * n * n));
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = k * p[i] * (c[i] - dot) * bal_slope(z[i], q.score);
+        sum = bal_wave_sum(sum);
+        inv = top == -inf && sum == 0 ? 0.0f : 1.0f / sum;
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] *= inv;
+}
+
+template <int N, int DT>
+__device__ __forceinline__ void bal_row(const BalanceParams& q, int row, float (&z)[N])
+{
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int e = lane + 64 * i;
-        if (e < q.experts) bal_store(q.grad, (size_t)t * q.experts + e, g[i], q.dtype);
+        z[i] = e < q.experts ? bal_load<DT>(q.logits, row * q.stride + e) : -__builtin_inff();
     }
+}
+
+constexpr int BAL_WAVES = 8;
+constexpr int bal_ahead(int n) { return n <= 4 ? 4 : 2; }     // rows a wave has on the way
+
+// Sums of a chunk, one piece for each sequence that it meets: a wave takes a few rows at a time, a lane its experts' shares in
+// registers; the waves meet in LDS in a fixed order, the picks are counted there (whole numbers: any order).
+template <int N, int DT>
+__global__ __launch_bounds__(64 * BAL_WAVES) void balance_kernel(BalanceParams q)
+{
+    constexpr int BAL_AHEAD = bal_ahead(N);
+    __shared__ float share[BAL_WAVES][64 * N];
+    __shared__ int picks[64 * N], total;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r0 = blockIdx.x * q.chunk, r1 = r0 + q.chunk < q.rows ? r0 + q.chunk : q.rows;
+    if (blockIdx.x == 0)                                     // sequences that hold no row at all leave their words at rest
+        for (int s = threadIdx.x; s < q.sequences; s += 64 * BAL_WAVES) q.arrive[(size_t)s * ARRIVE_STRIDE] = (unsigned long long)ARRIVE_REST << 32;
+    for (int s = bal_sequence(q, r0), at = r0; at < r1;) {
+        if (s >= q.sequences) break;
+        int end = bal_start(q, s + 1);                       // of the rows before the first sequence too (s = -1)
+        if (s < 0 || end <= at) {
+            at = s < 0 ? end : at;
+            ++s;
+            continue;
+        }
+        if (end > r1) end = r1;
+        for (int e = threadIdx.x; e < 64 * N; e += 64 * BAL_WAVES) picks[e] = 0;
+        if (threadIdx.x == 0) total = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < (end - at) * q.topk; i += 64 * BAL_WAVES) {
+            const int t = at + (q.topk == 1 ? i : (int)__umulhi((uint32_t)i, q.recip));
+            const int64_t e = q.sel[(size_t)at * q.topk + i];
+            if (e >= 0 && e < q.experts && (!q.mask || q.mask[t])) atomicAdd(&picks[e], 1);
+        }
+        float acc[N] = {};
+        int n = 0;
+        for (int t = at + wave * BAL_AHEAD; t < end; t += BAL_WAVES * BAL_AHEAD) {
+            float z[BAL_AHEAD][N];
+            bool use[BAL_AHEAD];
+#pragma unroll
+            for (int a = 0; a < BAL_AHEAD; ++a) {
+                use[a] = t + a < end && (!q.mask || q.mask[t + a]);
+                if (use[a]) bal_row<N, DT>(q, t + a, z[a]);
+            }
+#pragma unroll
+            for (int a = 0; a < BAL_AHEAD; ++a) {
+                if (!use[a]) continue;
+                ++n;
+                float p[N], slope[N];
+                bal_shares<N>(z[a], q.score, p, slope);
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] += p[i];
+            }
+        }
+        if (lane == 0 && n) atomicAdd(&total, n);
+#pragma unroll
+        for (int i = 0; i < N; ++i) share[wave][lane + 64 * i] = acc[i];
+        __syncthreads();
+        const size_t piece = (size_t)blockIdx.x + s;
+        for (int e = threadIdx.x; e < q.experts; e += 64 * BAL_WAVES) {
+            float v = 0;
+#pragma unroll
+            for (int w = 0; w < BAL_WAVES; ++w) v += share[w][e];
+            q.share[piece * q.experts + e] = v;
+            q.picks[piece * q.experts + e] = picks[e];
+        }
+        if (threadIdx.x == 0) q.piece_tokens[piece] = total;
+        __syncthreads();
+        at = end;
+        ++s;
+    }
+}
+
+// Joins the pieces of a sequence: one workgroup for 64 of its experts, BAL_JOIN lanes an expert over the pieces. The last workgroup
+// of a sequence to arrive adds the groups' products of picks and shares in order.
+constexpr int BAL_JOIN = 16;
+
+__global__ __launch_bounds__(64 * BAL_JOIN) void balance_join_kernel(BalanceParams q)
+{
+    __shared__ float share[BAL_JOIN][64];
+    __shared__ int picks[BAL_JOIN][64], tok[BAL_JOIN];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.x, groups = gridDim.y, e = 64 * blockIdx.y + lane;
+    const int t0 = bal_start(q, s), t1 = bal_start(q, s + 1), w0 = t0 / q.chunk, w1 = t1 > t0 ? (t1 - 1) / q.chunk + 1 : w0;
+    float p = 0;
+    int c = 0, n = 0;
+#pragma unroll 4
+    for (int w = w0 + wave; w < w1; w += BAL_JOIN) {
+        const size_t piece = (size_t)w + s;
+        if (e < q.experts) {
+            p += q.share[piece * q.experts + e];
+            c += q.picks[piece * q.experts + e];
+        }
+        n += q.piece_tokens[piece];
+    }
+    share[wave][lane] = p;
+    picks[wave][lane] = c;
+    if (lane == 0) tok[wave] = n;
+    __syncthreads();
+    if (wave) return;
+    p = 0;
+    c = n = 0;
+    for (int w = 0; w < BAL_JOIN; ++w) {
+        p += share[w][lane];
+        c += picks[w][lane];
+        n += tok[w];
+    }
+    if (e < q.experts) q.counts[(size_t)s * q.experts + e] = c;
+    const float part = bal_wave_sum((float)c * p), k = n ? (float)q.experts / ((float)q.topk * (float)n * (float)n) : 0.0f;
+    if (blockIdx.y == 0 && lane == 0) q.tokens[s] = n;
+    if (groups == 1) {
+        if (lane == 0) q.loss[s] = k * part;
+        return;
+    }
+    float* out = q.group_loss + (size_t)s * groups;
+    if (lane == 0) __hip_atomic_store(out + blockIdx.y, part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!wave_arrive_last(q.arrive + (size_t)s * ARRIVE_STRIDE, (unsigned)groups)) return;
+    float v = 0;
+    for (int g = 0; g < groups; ++g) v += __hip_atomic_load(out + g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (lane == 0) q.loss[s] = k * v;
+}
+
+// The gradient of a chunk's rows; a wave keeps the counts of the sequence it is in. Rows of no sequence, or masked, get zeros.
+template <int N, int DT>
+__global__ __launch_bounds__(64 * BAL_WAVES) void balance_grad_kernel(BalanceParams q)
+{
+    constexpr int BAL_AHEAD = bal_ahead(N);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r0 = blockIdx.x * q.chunk, r1 = r0 + q.chunk < q.rows ? r0 + q.chunk : q.rows;
+    for (int s = bal_sequence(q, r0), at = r0; at < r1;) {
+        int end = s >= q.sequences ? r1 : bal_start(q, s + 1);
+        if (end <= at) {
+            ++s;
+            continue;
+        }
+        if (end > r1) end = r1;
+        const bool in = s >= 0 && s < q.sequences;
+        float c[N] = {}, k = 0;
+        if (in) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) c[i] = lane + 64 * i < q.experts ? (float)q.counts[(size_t)s * q.experts + lane + 64 * i] : 0.0f;
+            const float n = (float)q.tokens[s];
+            k = q.grad_loss[s] * ((float)q.experts / ((float)q.topk * n * n));
+        }
+        for (int t = at + wave * BAL_AHEAD; t < end; t += BAL_WAVES * BAL_AHEAD) {
+            float z[BAL_AHEAD][N];
+            bool use[BAL_AHEAD];
+#pragma unroll
+            for (int a = 0; a < BAL_AHEAD; ++a) {
+                use[a] = in && t + a < end && (!q.mask || q.mask[t + a]);
+                if (use[a]) bal_row<N, DT>(q, t + a, z[a]);
+            }
+#pragma unroll
+            for (int a = 0; a < BAL_AHEAD; ++a) {
+                if (t + a >= end) continue;
+                float g[N] = {};
+                if (use[a]) {
+                    float p[N], slope[N], dot = 0;
+                    bal_shares<N>(z[a], q.score, p, slope);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) dot += c[i] * p[i];
+                    dot = bal_wave_sum(dot);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) g[i] = k * p[i] * (c[i] - dot) * slope[i];
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int e = lane + 64 * i;
+                    if (e < q.experts) bal_store<DT>(q.grad, (size_t)(t + a) * q.experts + e, g[i]);
+                }
+            }
+        }
+        at = end;
+        ++s;
+    }
+}
+
+// f(experts per lane, dtype) with both as types.
+template <class F>
+static void balance_dispatch(const BalanceParams& p, F f)
+{
+    using std::integral_constant;
+    auto type = [&](auto n) {
+        if (p.dtype == EVAMX_DTYPE_F32) f(n, integral_constant<int, EVAMX_DTYPE_F32>());
+        else if (p.dtype == EVAMX_DTYPE_BF16) f(n, integral_constant<int, EVAMX_DTYPE_BF16>());
+        else f(n, integral_constant<int, EVAMX_DTYPE_F16>());
+    };
+    if (p.experts <= 64) type(integral_constant<int, 1>());
+    else if (p.experts <= 128) type(integral_constant<int, 2>());
+    else if (p.experts <= 256) type(integral_constant<int, 4>());
+    else if (p.experts <= 384) type(integral_constant<int, 6>());
+    else type(integral_constant<int, 8>());
+}
+
+// Rows of a chunk: enough workgroups to fill the GPU twice, few enough that their pieces are quickly joined.
+static int balance_chunk(int rows)
+{
+    const int c = (rows + 511) / 512;
+    return c < 32 ? 32 : c;
+}
+
+static size_t balance_align(size_t v) { return (v + 255) & ~(size_t)255; }
+
+struct BalanceLayout {
+    size_t share, picks, tokens, group_loss, arrive, total;
+};
+
+static BalanceLayout balance_layout(int rows, int experts, int sequences)
+{
+    const int chunk = balance_chunk(rows);
+    const size_t pieces = (size_t)(rows + chunk - 1) / chunk + sequences;
+    BalanceLayout l;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t o = at; at += balance_align(bytes); return o; };
+    l.share = take(pieces * experts * 4);
+    l.picks = take(pieces * experts * 4);
+    l.tokens = take(pieces * 4);
+    l.group_loss = take((size_t)sequences * ((experts + 63) / 64) * 4);
+    l.arrive = take((size_t)sequences * ARRIVE_STRIDE * 8);
+    l.total = at;
+    return l;
 }
 
 }  // namespace evamx
@@ -209,13 +432,17 @@ static BalanceParams balance_params(const void* logits, int dtype, int64_t strid
     BalanceParams p;
     memset(&p, 0, sizeof p);
     p.logits = logits; p.dtype = dtype; p.stride = stride < 0 ? 0 : (size_t)stride; p.rows = rows; p.experts = experts;
+    p.chunk = balance_chunk(rows); p.recip = topk > 0 ? (uint32_t)(((1ull << 32) + topk - 1) / topk) : 0;
     p.sel = sel; p.topk = topk; p.score = score_fn; p.starts = starts; p.sequences = sequences; p.mask = mask;
     return p;
 }
 
 extern "C" size_t evamx_balance_workspace_bytes(int rows, int experts, int sequences)
 {
-    return 256;
+    if (rows < 0 || rows > EVAMX_BALANCE_MAX_ROWS || experts < 1 || experts > BAL_MAX_EXPERTS || sequences < 1 ||
+        sequences > EVAMX_BALANCE_MAX_SEQUENCES)
+        return 0;
+    return balance_layout(rows, experts, sequences).total;
 }
 
 extern "C" int evamx_balance_loss(const void* logits, int dtype, int64_t stride, int rows, int experts, const int64_t* sel, int topk,
@@ -226,10 +453,19 @@ extern "C" int evamx_balance_loss(const void* logits, int dtype, int64_t stride,
     BalanceParams p = balance_params(logits, dtype, stride, rows, experts, sel, topk, score_fn, starts, sequences, mask);
     p.loss = loss; p.counts = counts; p.tokens = tokens;
     if (!balance_ok(p, "evamx_balance_loss")) return EVAMX_EINVAL;
+    if ((uintptr_t)workspace & 15) { set_error("evamx_balance_loss: the workspace must be 16-byte aligned"); return EVAMX_EINVAL; }
     if (!loss || !workspace) { set_error("evamx_balance_loss: null pointer"); return EVAMX_EINVAL; }
     const size_t need = evamx_balance_workspace_bytes(rows, experts, sequences);
     if (workspace_bytes < need) { set_error("evamx_balance_loss: workspace %zu bytes < %zu", workspace_bytes, need); return EVAMX_ENOSPACE; }
-    balance_kernel<<<sequences, 256, 0, (hipStream_t)stream>>>(p);
+    char* ws = (char*)workspace;
+    const BalanceLayout l = balance_layout(rows, experts, sequences);
+    p.share = (float*)(ws + l.share); p.picks = (int32_t*)(ws + l.picks); p.piece_tokens = (int32_t*)(ws + l.tokens);
+    p.group_loss = (float*)(ws + l.group_loss); p.arrive = (unsigned long long*)(ws + l.arrive);
+    const int chunks = rows ? (rows + p.chunk - 1) / p.chunk : 1;
+    balance_dispatch(p, [&](auto n, auto dt) {
+        balance_kernel<decltype(n)::value, decltype(dt)::value><<<chunks, 64 * BAL_WAVES, 0, (hipStream_t)stream>>>(p);
+    });
+    balance_join_kernel<<<dim3(sequences, (experts + 63) / 64), 64 * BAL_JOIN, 0, (hipStream_t)stream>>>(p);
     return launched("balance_loss");
 }
 
@@ -244,6 +480,8 @@ extern "C" int evamx_balance_grad(const float* grad_loss, const void* logits, in
     if (!balance_ok(p, "evamx_balance_grad")) return EVAMX_EINVAL;
     if (!grad_loss || (!grad && rows)) { set_error("evamx_balance_grad: null pointer"); return EVAMX_EINVAL; }
     if (rows == 0) return EVAMX_OK;
-    balance_grad_kernel<<<(rows + 3) / 4, 256, 0, (hipStream_t)stream>>>(p);
+    balance_dispatch(p, [&](auto n, auto dt) {
+        balance_grad_kernel<decltype(n)::value, decltype(dt)::value><<<(rows + p.chunk - 1) / p.chunk, 64 * BAL_WAVES, 0, (hipStream_t)stream>>>(p);
+    });
     return launched("balance_grad");
 }

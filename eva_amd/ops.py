@@ -122,18 +122,24 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, *, n_in: int, group: int,
         if t is not None and t.device != codes.device:
             raise ValueError(f"{name} is on {t.device}, the codes on {codes.device}")
     w = W4Weight(lead[0] if lead else 1, n_out, n_in, group, scales.dtype, zeros is not None, codes.device)
-    with torch.cuda.device(w.device):
-        check(lib().evamx_w4_pack(ptr(codes), ptr(scales), ptr(zeros), group, ctypes.byref(w.desc),
-                                  stream_handle(w.device)), "evamx_w4_pack")
+    _launch(lib().evamx_w4_pack, "evamx_w4_pack", w.device, ptr(codes), ptr(scales), ptr(zeros), group, ctypes.byref(w.desc))
     return w
 
 
 def w4_dequant(weight: W4Weight) -> torch.Tensor:
     """fp32 ``[count, n_out, n_in]`` of packed 4-bit weights."""
     out = torch.empty(weight.count, weight.n_out, weight.n_in, dtype=torch.float32, device=weight.device)
-    with torch.cuda.device(weight.device):
-        check(lib().evamx_w4_dequant(ctypes.byref(weight.desc), ptr(out), stream_handle(weight.device)), "evamx_w4_dequant")
+    _launch(lib().evamx_w4_dequant, "evamx_w4_dequant", weight.device, ctypes.byref(weight.desc), ptr(out))
     return out
+
+
+def _launch(fn, what: str, device: torch.device, *args):
+    """One library call on the current stream of ``device``, which is made current if it is not."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what)
 
 
 def _row_stride(t: torch.Tensor, name: str, dtype=None) -> int:
@@ -149,8 +155,10 @@ def _row_stride(t: torch.Tensor, name: str, dtype=None) -> int:
 
 
 def _no_grad(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no backward: call it under torch.no_grad() or with detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no backward: call it under torch.no_grad() or with detached tensors")
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
@@ -166,26 +174,27 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
         raise ValueError(f"x {tuple(x.shape)} does not fit {weight.count} matrices [{weight.n_out}, {weight.n_in}]")
     if not 1 <= rows <= 65536:
         raise ValueError(f"x has {rows} rows, a call takes 1..65536")
+    device = x.device
     if bias is not None:
         _dev(bias, "bias", x.dtype, 1)
-        if bias.numel() != weight.n_out:
-            raise ValueError(f"bias must be [{weight.n_out}]")
+        if bias.numel() != weight.n_out or bias.device != device:
+            raise ValueError(f"bias must be [{weight.n_out}] on {device}")
     if out is None:
-        out = torch.empty(rows, weight.n_out, dtype=x.dtype, device=x.device)
-    out_stride = _row_stride(out, "out", x.dtype)
-    if tuple(out.shape) != (rows, weight.n_out):
-        raise ValueError(f"out must be [{rows}, {weight.n_out}]")
+        out = torch.empty(rows, weight.n_out, dtype=x.dtype, device=device)
+        out_stride = weight.n_out
+    else:
+        out_stride = _row_stride(out, "out", x.dtype)
+        if tuple(out.shape) != (rows, weight.n_out) or out.device != device:
+            raise ValueError(f"out must be [{rows}, {weight.n_out}] on {device}")
     _no_grad("w4_linear", x, bias, out)
     if workspace is None:
-        workspace = torch.empty(lib().evamx_w4_linear_workspace_bytes(rows, weight.n_in), dtype=torch.uint8, device=x.device)
-    _dev(workspace, "workspace", torch.uint8, 1)
-    for t, name in ((weight, "weight"), (bias, "bias"), (out, "out"), (workspace, "workspace")):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    with torch.cuda.device(x.device):
-        check(lib().evamx_w4_linear(ptr(x), _DTYPES[x.dtype], x_stride, rows, ctypes.byref(weight.desc), ptr(bias), ptr(out),
-                                    out_stride, ptr(workspace), workspace.numel(), stream_handle(x.device)),
-              "evamx_w4_linear")
+        workspace = torch.empty(lib().evamx_w4_linear_workspace_bytes(rows, weight.n_in), dtype=torch.uint8, device=device)
+    else:
+        _dev(workspace, "workspace", torch.uint8, 1)
+    if weight.device != device or workspace.device != device:
+        raise ValueError(f"x is on {device}, the weight on {weight.device}, the workspace on {workspace.device}")
+    _launch(lib().evamx_w4_linear, "evamx_w4_linear", device, ptr(x), _DTYPES[x.dtype], x_stride, rows, ctypes.byref(weight.desc),
+            ptr(bias), ptr(out), out_stride, ptr(workspace), workspace.numel())
     return out
 
 
@@ -277,10 +286,8 @@ def balance_stats(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "s
     counts = torch.empty(n, experts, dtype=torch.int32, device=dev)
     tokens = torch.empty(n, dtype=torch.int32, device=dev)
     ws = torch.empty(lib().evamx_balance_workspace_bytes(rows, experts, n), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        check(lib().evamx_balance_loss(ptr(logits), _LOGIT_DTYPES[logits.dtype], stride, rows, experts, ptr(sel), sel.shape[1],
-                                       SCORE_FNS[score_fn], ptr(seq_starts), n, ptr(token_mask), ptr(loss), ptr(counts), ptr(tokens),
-                                       ptr(ws), ws.numel(), stream_handle(dev)), "evamx_balance_loss")
+    _launch(lib().evamx_balance_loss, "evamx_balance_loss", dev, ptr(logits), _LOGIT_DTYPES[logits.dtype], stride, rows, experts, ptr(sel),
+            sel.shape[1], SCORE_FNS[score_fn], ptr(seq_starts), n, ptr(token_mask), ptr(loss), ptr(counts), ptr(tokens), ptr(ws), ws.numel())
     return loss, counts, tokens
 
 
@@ -297,10 +304,8 @@ def balance_loss_grad(grad_loss: torch.Tensor, logits: torch.Tensor, counts: tor
         if tuple(t.shape) != shape or t.device != logits.device:
             raise ValueError(f"{name} must be {shape} on {logits.device}, got {tuple(t.shape)} on {t.device}")
     grad = torch.empty(rows, experts, dtype=logits.dtype, device=logits.device)
-    with torch.cuda.device(logits.device):
-        check(lib().evamx_balance_grad(ptr(grad_loss), ptr(logits), _LOGIT_DTYPES[logits.dtype], stride, rows, experts, topk,
-                                       SCORE_FNS[score_fn], ptr(seq_starts), n, ptr(token_mask), ptr(counts), ptr(tokens), ptr(grad),
-                                       stream_handle(logits.device)), "evamx_balance_grad")
+    _launch(lib().evamx_balance_grad, "evamx_balance_grad", logits.device, ptr(grad_loss), ptr(logits), _LOGIT_DTYPES[logits.dtype],
+            stride, rows, experts, topk, SCORE_FNS[score_fn], ptr(seq_starts), n, ptr(token_mask), ptr(counts), ptr(tokens), ptr(grad))
     return grad
 
 
@@ -648,8 +653,7 @@ def w4_moe_forward(x: torch.Tensor, gate: W4Weight, up: W4Weight, down: W4Weight
     a = W4MoeArgs(ptr(x), ptr(sel), ptr(weights), ctypes.pointer(gate.desc), ctypes.pointer(up.desc), ctypes.pointer(down.desc), ptr(out),
                   ptr(workspace), workspace.numel(), x_stride, out_stride, first_expert, _DTYPES[x.dtype], rows, sel.shape[1], n_shared,
                   float(limit))
-    with torch.cuda.device(x.device):
-        check(lib().evamx_w4_moe_forward(ctypes.byref(a), stream_handle(x.device)), "evamx_w4_moe_forward")
+    _launch(lib().evamx_w4_moe_forward, "evamx_w4_moe_forward", x.device, ctypes.byref(a))
     return out
 
 

@@ -21,6 +21,8 @@ class W4Linear:
         self.in_features, self.out_features = weight.n_in, weight.n_out
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.ndim == 2 and 0 < x.shape[0] <= MAX_CALL_ROWS and x.is_contiguous():
+            return ops.w4_linear(x, self.weight, self.bias)
         if x.shape[-1] != self.in_features:
             raise ValueError(f"x has {x.shape[-1]} features, the weight {self.in_features}")
         flat = x.reshape(-1, self.in_features)
