@@ -71,7 +71,7 @@ __global__ __launch_bounds__(512) void w4_linear_few_kernel(W4LinearParams p, W4
 template <int SG, bool ZERO, int NB, int MB>
 __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat m)
 {
-    constexpr int RING = MB == 1 ? 1 : 2;
+    constexpr int RING = 1;
     extern __shared__ w4_f32x4 part[];                       // [parts][NB][MB][64]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, parts = blockDim.x >> 6;
     const int k0 = w4_part_begin(m.kt, parts, wave), k1 = w4_part_begin(m.kt, parts, wave + 1), r0 = 16 * MB * blockIdx.y;
@@ -106,8 +106,6 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat 
         w4_linear_store(p, m, r, n, v, p.row_scale ? p.row_scale[r] : 1.0f);
     }
 }
-
-constexpr int W4G_MIN_TILES = 200;
 
 // Long calls: 64 rows by 256 columns a workgroup (w4_gemm.hpp). Consecutive workgroups go to the eight XCDs in turn, so each XCD
 // takes a contiguous run of tiles, eight row tiles by all columns at a time: its rows' tiles stay in its L2 while it passes over
@@ -189,7 +187,7 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
     if (workspace_bytes < need) { set_error("evamx_w4_linear: workspace %zu bytes < %zu", workspace_bytes, need); return EVAMX_ENOSPACE; }
     const hipStream_t s = (hipStream_t)stream;
     const W4Mat m = w4_mat(*w);
-    const int parts = w4_parts(m.kt);
+    const int parts = w4_parts(m.kt, m.nt);
     W4LinearParams p;
     p.x = x; p.x_stride = (size_t)x_stride; p.rows = rows; p.bf16 = x_dtype == EVAMX_DTYPE_BF16;
     p.aligned = (((uintptr_t)x | (uintptr_t)(2 * x_stride)) & 15) == 0;
@@ -209,17 +207,25 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
         p.xh = xh;
         p.row_scale = rs;
     }
-    // fewer than two workgroups a CU otherwise: 16 columns each (5001 -> 2303 at 13 rows: 12.3 us against 14.9 with 32), else
-    // 32 on the same rows (7168 -> 18432 at 5 rows: 21.8 us against 25.8 with 16)
-    if (rows <= 16 && m.nt < 1024) w4_launch_linear<1, 1>(p, m, *w, parts, s);
-    else if (rows <= 16) w4_launch_linear<2, 1>(p, m, *w, parts, s);
-    else if ((long)w4_ceil(rows, W4G_ROWS) * w4_ceil(m.n_out, W4G_COLS) >= W4G_MIN_TILES) {
-        const int rt = w4_ceil(rows, W4G_ROWS), ct = w4_ceil(m.n_out, W4G_COLS);
+    const long row_tiles = w4_ceil(rows, W4G_ROWS), col_tiles = w4_ceil(m.n_out, W4G_COLS), wide = (long)w4_ceil(m.nt, 4) * w4_ceil(rows, 32);
+    if (rows <= 16) {
+        // 16 columns a workgroup where 32 would leave CUs without one (5001 -> 2303 at 13 rows: 12.3 us against 14.9 with 32),
+        // else 32 on the same rows (7168 -> 18432 at 5 rows: 21.8 us against 25.8 with 16)
+        if (m.nt < 1024) w4_launch_linear<1, 1>(p, m, *w, parts, s);
+        else w4_launch_linear<2, 1>(p, m, *w, parts, s);
+    } else if (row_tiles * col_tiles * m.kt >= 104l * m.kt + 600) {
+        // The 64 x 256 tiles take about 1.5 us a k-tile and 5 for all of a round, the kernel below 0.014 us a tile and k-tile
+        // (7168 -> 2048 at 200 rows: 80 us against 22; at 1024: 83 against 89; 2048 -> 7168 at 400: 38 and 36)
         w4_dispatch(*w, [&](auto sg, auto zero) {
-            w4_linear_gemm_kernel<decltype(sg)::value, decltype(zero)::value><<<8 * w4_ceil(rt * ct, 8), 256, 0, s>>>(p, m, rt, ct);
+            w4_linear_gemm_kernel<decltype(sg)::value, decltype(zero)::value>
+                <<<8 * w4_ceil((int)(row_tiles * col_tiles), 8), 256, 0, s>>>(p, m, (int)row_tiles, (int)col_tiles);
         });
+    } else if (wide < 160) {
+        // 32 columns by 32 rows where 64 columns would leave CUs without a workgroup (7168 -> 2048 at 17 rows: 12.4 us against
+        // 17.7, at 128: 18.6 against 20.4), else 64 (at 200: 34 against 22)
+        w4_launch_linear<2, 2>(p, m, *w, m.kt >= 8 ? 8 : parts, s);
+    } else {
+        w4_launch_linear<4, 2>(p, m, *w, parts < 4 ? parts : 4, s);
     }
-    else if (rows <= 32) w4_launch_linear<2, 2>(p, m, *w, parts, s);
-    else w4_launch_linear<2, 4>(p, m, *w, parts < 4 ? parts : 4, s);
     return launched("w4_linear");
 }
