@@ -479,16 +479,12 @@ struct W4Stage {
 };
 
 // A result of x's type, to nearest even; NaN stays.
-__device__ __forceinline__ void w4_store(void* y, size_t at, float v, int bf16)
+__device__ __forceinline__ uint16_t w4_bits(float v, int bf16)
 {
-    if (bf16) {
-        uint32_t b = __builtin_bit_cast(uint32_t, v);
-        b = (b & 0x7fffffffu) > 0x7f800000u ? 0x7fc00000u : b + 0x7fffu + ((b >> 16) & 1);
-        ((uint16_t*)y)[at] = (uint16_t)(b >> 16);
-    } else {
-        ((w4_half*)y)[at] = (w4_half)v;
-    }
+    return bf16 ? __builtin_bit_cast(uint16_t, (__bf16)v) : __builtin_bit_cast(uint16_t, (w4_half)v);
 }
+
+__device__ __forceinline__ void w4_store(void* y, size_t at, float v, int bf16) { ((uint16_t*)y)[at] = w4_bits(v, bf16); }
 
 // f(groups per k-tile, zero points or none) with both as types, for the kernels built for them.
 template <class F>

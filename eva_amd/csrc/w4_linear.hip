@@ -1,4 +1,5 @@
 // y = x W^T (+ bias) on 4-bit weights with group scales (w4.hpp).
+#include "evamx_gemv.hpp"
 #include "evamx_internal.hpp"
 #include "w4_gemm.hpp"
 
@@ -9,7 +10,7 @@ struct W4LinearParams {
     size_t x_stride;
     const w4_half* xh;           // made ready: rows of kt * 128
     const float* row_scale;      // NULL: 1
-    int rows, aligned, bf16;
+    int rows, aligned, y_aligned, bf16;          // x's and y's rows start at 16-byte addresses
     const void* bias;
     void* y;
     size_t y_stride;
@@ -123,7 +124,34 @@ __device__ __forceinline__ void w4_linear_gemm(const W4LinearParams& p, const W4
     for (int i = 0; i < MB; ++i) rows.at[i] = (w4g_row<MB>(i) < have ? w4g_row<MB>(i) : have - 1) * ld + w4g_chunk<MB>(i);
     w4_f32x4 acc[W4G_NB][MB] = {};
     w4g_run<SG, ZERO, false, MB>(acc, st, rows, lds, m.kt, m.bf16);
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();                                         // no wave reads the rows' tiles any more
+    if (16 * (nt0 + W4G_NB) <= m.n_out && p.y_aligned) {
+        // whole columns: through LDS (a piece of its own a wave, rows 144 bytes apart: no two of a store's rows in the same banks)
+        // into 16-byte pieces of the rows
+        constexpr int ROW = 144;
+        char* mine = lds + wave * (W4G_ROWS * ROW);
+        float bias[W4G_NB];
+#pragma unroll
+        for (int b = 0; b < W4G_NB; ++b) bias[b] = p.bias ? w4_bias(p.bias, 16 * (nt0 + b) + (lane & 15), p.bf16) : 0.0f;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 16 * mb + 4 * (lane >> 4) + i;
+                const float f = p.row_scale ? p.row_scale[r0 + (r < have ? r : have - 1)] : 1.0f;
+#pragma unroll
+                for (int b = 0; b < W4G_NB; ++b)
+                    *(uint16_t*)(mine + r * ROW + 2 * (16 * b + (lane & 15))) = w4_bits(p.bias ? acc[b][mb][i] * f + bias[b] : acc[b][mb][i] * f, p.bf16);
+            }
+        wave_lds_fence();
+#pragma unroll
+        for (int k = 0; k < 2 * MB; ++k) {
+            const int r = 8 * k + (lane >> 3);
+            if (r < have) *(w4_u32x4*)((uint16_t*)p.y + (size_t)(r0 + r) * p.y_stride + 16 * nt0 + 8 * (lane & 7)) = *(const w4_u32x4*)(mine + r * ROW + 16 * (lane & 7));
+        }
+        return;
+    }
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -191,6 +219,7 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
     W4LinearParams p;
     p.x = x; p.x_stride = (size_t)x_stride; p.rows = rows; p.bf16 = x_dtype == EVAMX_DTYPE_BF16;
     p.aligned = (((uintptr_t)x | (uintptr_t)(2 * x_stride)) & 15) == 0;
+    p.y_aligned = (((uintptr_t)y | (uintptr_t)(2 * y_stride)) & 15) == 0;
     p.bias = bias; p.y = y; p.y_stride = (size_t)y_stride; p.xh = nullptr; p.row_scale = nullptr;
     if (w4_stage_fits(rows, m.kt, parts)) {
         w4_dispatch(*w, [&](auto sg, auto zero) {

@@ -517,7 +517,7 @@ __global__ __launch_bounds__(256) void w4_combine_kernel(W4MoeParams p)
 {
     __shared__ float w[64];
     __shared__ int use[64];
-    const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const int t = blockIdx.x, n = (blockIdx.y * 256 + threadIdx.x) * 4;
     if ((int)threadIdx.x < p.kt_slots) {
         const int k = threadIdx.x;
         use[k] = w4_slot_expert(p, t * p.kt_slots + k) >= 0;
@@ -570,7 +570,8 @@ static W4MoeLayout w4_moe_layout(int rows, int topk, int n_shared, int hidden, i
     l.n_units = take(8);
     l.units = take(slots * sizeof(W4Unit));
     l.big = take(w4_max_big(slots) * sizeof(W4Unit));
-    l.order = take((rows <= W4_FEW_ROWS ? slots * slots : slots) * 4);
+    const size_t few = slots < W4_FEW_SLOTS ? slots : W4_FEW_SLOTS;   // units of few tokens have a list each; bytes grow with the rows
+    l.order = take((few * few > slots ? few * few : slots) * 4);
     l.xs = take((size_t)rows * 4);
     l.x = take(rows * kx * 2);
     l.h = take(slots * kh * 4);
@@ -619,8 +620,8 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
                   u.n_out, u.n_in, d.count, d.n_out, d.n_in);
         return EVAMX_EINVAL;
     }
-    if (g.group != u.group || (g.zeros == nullptr) != (u.zeros == nullptr)) {
-        set_error("%s: gate and up differ in their group size or zero points", who);
+    if (g.group != u.group || g.scale_dtype != u.scale_dtype || (g.zeros == nullptr) != (u.zeros == nullptr)) {
+        set_error("%s: gate and up differ in their group size, scale type or zero points", who);
         return EVAMX_EINVAL;
     }
     if (!w4_moe_shape_ok(a->rows, a->topk, a->n_shared, g.n_in, g.n_out, who)) return EVAMX_EINVAL;
@@ -703,6 +704,6 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
             w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, true><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
         }
     });
-    w4_combine_kernel<<<dim3(w4_ceil(p.hidden, 1024), p.rows), 256, 0, s>>>(p);
+    w4_combine_kernel<<<dim3(p.rows, w4_ceil(p.hidden, 1024)), 256, 0, s>>>(p);
     return launched("w4_moe_forward");
 }

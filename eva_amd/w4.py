@@ -45,8 +45,8 @@ class W4Experts:
         shape = (gate.count, gate.n_out, gate.n_in)
         if (up.count, up.n_out, up.n_in) != shape or (down.count, down.n_in, down.n_out) != shape:
             raise ValueError("gate and up must be stacks [inter, hidden], down [hidden, inter], of as many matrices")
-        if up.desc.group != gate.desc.group or (up.zeros is None) != (gate.zeros is None):
-            raise ValueError("gate and up must agree in their group size and in having zero points")
+        if (up.desc.group, up.scales.dtype, up.zeros is None) != (gate.desc.group, gate.scales.dtype, gate.zeros is None):
+            raise ValueError("gate and up must agree in their group size, their scales' type and in having zero points")
         if not 0 <= n_shared <= gate.count:
             raise ValueError(f"{n_shared} shared experts of {gate.count}")
         self.gate, self.up, self.down = gate, up, down

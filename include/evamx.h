@@ -297,7 +297,7 @@ typedef struct evamx_w4_moe_args {
     const int64_t* sel;           /* device [rows][topk] */
     const float* weights;         /* device [rows][topk] */
     const evamx_w4_weight* gate;  /* HOST: stacks of `count` [inter][hidden], [inter][hidden], [hidden][inter]; gate */
-    const evamx_w4_weight* up;    /* and up alike in group size and in having zero points */
+    const evamx_w4_weight* up;    /* and up alike in group size, scale type, zero points */
     const evamx_w4_weight* down;
     void* out;                    /* device, x's type, [rows][out_stride]; must not overlap x */
     void* workspace;              /* device, evamx_w4_moe_workspace_bytes bytes, 16-byte aligned; needs no clearing */

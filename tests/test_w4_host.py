@@ -57,7 +57,7 @@ def test_linear_is_checked():
         assert call(**bad) == _lib.EVAMX_EINVAL, bad
         assert L.evamx_last_error()
     assert call(nb=16) == _lib.EVAMX_ENOSPACE
-    sizes = [L.evamx_w4_linear_workspace_bytes(r, 512) for r in (1, 2, 16, 17, 65536)]
+    sizes = [L.evamx_w4_linear_workspace_bytes(r, 512) for r in (*range(1, 70), 65536)]
     assert all(a <= b for a, b in zip(sizes, sizes[1:])) and sizes[0] > 0
     assert L.evamx_w4_linear_workspace_bytes(0, 512) == 0 and L.evamx_w4_linear_workspace_bytes(65537, 512) == 0
 
@@ -79,7 +79,7 @@ def _moe(**kw):
     dict(x=0), dict(sel=0), dict(weights=0), dict(out=0), dict(workspace=0), dict(workspace=FAKE + 4), dict(x_stride=511), dict(out_stride=511),
     dict(x_dtype=2), dict(rows=0), dict(rows=21846), dict(topk=0), dict(topk=33), dict(n_shared=-1), dict(n_shared=10), dict(limit=-1.0),
     dict(limit=float("inf")), dict(limit=float("nan")), dict(gate=dict(codes=0)), dict(up=dict(group=48)), dict(down=dict(n_out=500)),
-    dict(up=dict(n_out=255)), dict(down=dict(count=8)), dict(up=dict(group=64)), dict(up=dict(zeros=FAKE)), dict(down=dict(scale_dtype=5)),
+    dict(up=dict(n_out=255)), dict(down=dict(count=8)), dict(up=dict(group=64)), dict(up=dict(zeros=FAKE)), dict(up=dict(scale_dtype=1)), dict(down=dict(scale_dtype=5)),
 ])
 def test_moe_is_checked(bad):
     assert _moe(**bad) == _lib.EVAMX_EINVAL
@@ -92,6 +92,9 @@ def test_moe_workspace():
     assert L.evamx_w4_moe_forward(None, None) == _lib.EVAMX_EINVAL
     sizes = [L.evamx_w4_moe_workspace_bytes(r, 8, 1, 7168, 2048) for r in (1, 2, 16, 17, 512, 7281)]
     assert sizes[0] > 0 and all(a <= b for a, b in zip(sizes, sizes[1:]))
+    for shape in ((8, 1, 64, 64), (32, 32, 64, 32), (1, 0, 7168, 2048), (32, 0, 128, 4096)):       # a larger call's serves a smaller one
+        need = [L.evamx_w4_moe_workspace_bytes(r, *shape) for r in (*range(1, 40), 64, 100, 500, 1000)]
+        assert all(0 < a <= b for a, b in zip(need, need[1:])), shape
     for bad in ((0, 8, 1, 64, 64), (7282, 8, 1, 64, 64), (1, 0, 0, 64, 64), (1, 8, 33, 64, 64), (1, 8, 0, 0, 64), (1, 8, 0, 64, 1 << 19)):
         assert L.evamx_w4_moe_workspace_bytes(*bad) == 0, bad
 
