@@ -273,15 +273,13 @@ def _balance_args(logits, score_fn, seq_starts, token_mask):
     return stride, n
 
 
-def balance_stats(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "sigmoid", seq_starts: torch.Tensor | None = None,
-                  token_mask: torch.Tensor | None = None):
-    """``(loss fp32 [S], counts int32 [S, E], tokens int32 [S])`` of ``balance_loss``, outside autograd."""
-    stride, n = _balance_args(logits, score_fn, seq_starts, token_mask)
+def _balance_forward(logits, sel, score_fn, stride, n, seq_starts, token_mask):
+    """(loss, counts, tokens) for checked arguments."""
     rows, experts = logits.shape
-    _dev(sel, "sel", torch.int64, 2)
-    if sel.shape[0] != rows or sel.device != logits.device:
-        raise ValueError(f"sel must be [{rows}, topk] on {logits.device}, got {tuple(sel.shape)} on {sel.device}")
     dev = logits.device
+    _dev(sel, "sel", torch.int64, 2)
+    if sel.shape[0] != rows or sel.device != dev:
+        raise ValueError(f"sel must be [{rows}, topk] on {dev}, got {tuple(sel.shape)} on {sel.device}")
     loss = torch.empty(n, dtype=torch.float32, device=dev)
     counts = torch.empty(n, experts, dtype=torch.int32, device=dev)
     tokens = torch.empty(n, dtype=torch.int32, device=dev)
@@ -291,40 +289,55 @@ def balance_stats(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "s
     return loss, counts, tokens
 
 
-def balance_loss_grad(grad_loss: torch.Tensor, logits: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor, topk: int, *,
-                      score_fn: str = "sigmoid", seq_starts: torch.Tensor | None = None,
-                      token_mask: torch.Tensor | None = None) -> torch.Tensor:
-    """The gradient of ``(grad_loss * loss).sum()`` with respect to the logits, for the ``counts`` and
-    ``tokens`` that ``balance_stats`` gave for the same arguments; zero for rows that do not count."""
-    stride, n = _balance_args(logits, score_fn, seq_starts, token_mask)
+def _balance_backward(grad_loss, logits, counts, tokens, topk, score_fn, stride, n, seq_starts, token_mask):
+    """The logits' gradient for checked arguments."""
     rows, experts = logits.shape
-    for t, name, dtype, shape in ((grad_loss, "grad_loss", torch.float32, (n,)), (counts, "counts", torch.int32, (n, experts)),
-                                  (tokens, "tokens", torch.int32, (n,))):
-        _dev(t, name, dtype)
-        if tuple(t.shape) != shape or t.device != logits.device:
-            raise ValueError(f"{name} must be {shape} on {logits.device}, got {tuple(t.shape)} on {t.device}")
     grad = torch.empty(rows, experts, dtype=logits.dtype, device=logits.device)
     _launch(lib().evamx_balance_grad, "evamx_balance_grad", logits.device, ptr(grad_loss), ptr(logits), _LOGIT_DTYPES[logits.dtype],
             stride, rows, experts, topk, SCORE_FNS[score_fn], ptr(seq_starts), n, ptr(token_mask), ptr(counts), ptr(tokens), ptr(grad))
     return grad
 
 
+def balance_stats(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "sigmoid", seq_starts: torch.Tensor | None = None,
+                  token_mask: torch.Tensor | None = None):
+    """``(loss fp32 [S], counts int32 [S, E], tokens int32 [S])`` of ``balance_loss``, outside autograd."""
+    stride, n = _balance_args(logits, score_fn, seq_starts, token_mask)
+    return _balance_forward(logits, sel, score_fn, stride, n, seq_starts, token_mask)
+
+
+def balance_loss_grad(grad_loss: torch.Tensor, logits: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor, topk: int, *,
+                      score_fn: str = "sigmoid", seq_starts: torch.Tensor | None = None,
+                      token_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of ``(grad_loss * loss).sum()`` with respect to the logits, for the ``counts`` and
+    ``tokens`` that ``balance_stats`` gave for the same arguments; zero for rows that do not count."""
+    stride, n = _balance_args(logits, score_fn, seq_starts, token_mask)
+    for t, name, dtype, shape in ((grad_loss, "grad_loss", torch.float32, (n,)), (counts, "counts", torch.int32, (n, logits.shape[1])),
+                                  (tokens, "tokens", torch.int32, (n,))):
+        _dev(t, name, dtype)
+        if tuple(t.shape) != shape or t.device != logits.device:
+            raise ValueError(f"{name} must be {shape} on {logits.device}, got {tuple(t.shape)} on {t.device}")
+    return _balance_backward(grad_loss, logits, counts, tokens, topk, score_fn, stride, n, seq_starts, token_mask)
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, sel, score_fn, seq_starts, token_mask):
-        loss, counts, tokens = balance_stats(logits, sel, score_fn=score_fn, seq_starts=seq_starts, token_mask=token_mask)
+        stride, n = _balance_args(logits, score_fn, seq_starts, token_mask)
+        loss, counts, tokens = _balance_forward(logits, sel, score_fn, stride, n, seq_starts, token_mask)
         ctx.save_for_backward(logits, counts, tokens, seq_starts, token_mask)
-        ctx.topk, ctx.score_fn = sel.shape[1], score_fn
+        ctx.args = sel.shape[1], score_fn, stride, n
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)                 # no zeros for the counts, which have no gradient
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss, _):
+        if grad_loss is None:
+            return None, None, None, None, None
+        if torch.is_grad_enabled():                      # create_graph=True
+            raise RuntimeError("balance_loss is differentiable once")
         logits, counts, tokens, seq_starts, token_mask = ctx.saved_tensors
-        grad = balance_loss_grad(grad_loss.contiguous(), logits, counts, tokens, ctx.topk, score_fn=ctx.score_fn,
-                                 seq_starts=seq_starts, token_mask=token_mask)
-        return grad, None, None, None, None
+        return _balance_backward(grad_loss.contiguous(), logits, counts, tokens, *ctx.args, seq_starts, token_mask), None, None, None, None
 
 
 def balance_loss(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "sigmoid", seq_starts: torch.Tensor | None = None,

@@ -214,6 +214,8 @@ def test_refusals(dev):
     with pytest.raises(ops._lib.EvamxError):
         ops.balance_loss(z, torch.zeros(4, 33, dtype=torch.int64, device=dev))
     leaf = z.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(ops.balance_loss(leaf, sel)[0].sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="captured"):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
