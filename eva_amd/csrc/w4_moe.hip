@@ -517,7 +517,7 @@ __global__ __launch_bounds__(256) void w4_combine_kernel(W4MoeParams p)
 {
     __shared__ float w[64];
     __shared__ int use[64];
-    const int t = blockIdx.x, n = (blockIdx.y * 256 + threadIdx.x) * 4;
+    const int cols = (p.hidden + 1023) / 1024, t = blockIdx.x / cols, n = ((blockIdx.x - t * cols) * 256 + threadIdx.x) * 4;
     if ((int)threadIdx.x < p.kt_slots) {
         const int k = threadIdx.x;
         use[k] = w4_slot_expert(p, t * p.kt_slots + k) >= 0;
@@ -704,6 +704,6 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
             w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, true><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
         }
     });
-    w4_combine_kernel<<<dim3(p.rows, w4_ceil(p.hidden, 1024)), 256, 0, s>>>(p);
+    w4_combine_kernel<<<p.rows * w4_ceil(p.hidden, 1024), 256, 0, s>>>(p);
     return launched("w4_moe_forward");
 }

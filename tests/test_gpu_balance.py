@@ -103,6 +103,16 @@ def test_sequences_and_masks(dev, starts, score):
     assert torch.equal(again, grad) and (again.cpu()[~mask] == 0).all()
 
 
+@pytest.mark.parametrize("rows,sequences", [(5000, 700), (16385, 3), (40000, 64), (300, 4000)])
+def test_many_sequences(dev, rows, sequences):
+    """Sequences of one token, many to a chunk of rows and many chunks to a sequence."""
+    g = _gen(sequences)
+    z = torch.randn(rows, 70, generator=g)
+    cuts = torch.randint(0, rows + 1, (sequences - 1,), generator=g).sort().values.tolist()
+    mask = torch.rand(rows, generator=g) < 0.9
+    _check(dev, z, z.topk(3, 1).indices, "sigmoid", [0, *cuts, rows], mask)
+
+
 @pytest.mark.parametrize("score", SCORES)
 def test_far_logits(dev, score):
     """Scores that underflow for a whole row keep their shares; -inf has none; a row of -inf alone has only picks."""

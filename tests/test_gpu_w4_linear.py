@@ -41,6 +41,51 @@ def test_linear(dev, n_out, n_in, group, rows):
         check_linear(ops.w4_linear(x, m.pack(dev), b), x, m.w, b)
 
 
+@pytest.mark.parametrize("n_out,n_in,group,zeros,dtype", [(4096, 512, 128, False, torch.bfloat16), (4100, 517, 64, True, torch.float16),
+                                                          (4351, 900, 32, False, torch.float16), (12000, 128, 128, True, torch.bfloat16)])
+@pytest.mark.parametrize("rows", [1024, 1025, 1041, 1070, 1087])
+def test_many_rows(dev, n_out, n_in, group, zeros, dtype, rows):
+    """The tiles of 64 rows by 256 columns: last tiles of every kind (1, 17, 33 rows and more; columns that end inside
+    a wave's), one to eight k-tiles, results at any address."""
+    g = _gen(rows + n_in)
+    m = Matrix(g, n_out, n_in, group, zeros=zeros, dtype=dtype)
+    w, w64 = m.pack(dev), m.w.to(dev)
+    x = torch.randn(rows, n_in, generator=g).to(dtype).to(dev)
+    b = torch.randn(n_out, generator=g).to(dtype).to(dev)
+    y = ops.w4_linear(x, w, b)
+    check_linear(y, x, w64, b)
+    out = torch.full((rows, n_out + 9), 7.0, dtype=dtype, device=dev)
+    ops.w4_linear(x, w, b, out=out[:, 3:n_out + 3])
+    assert torch.equal(out[:, 3:n_out + 3], y) and (out[:, :3] == 7).all() and (out[:, n_out + 3:] == 7).all()
+    if n_in % 128 == 0 and dtype == torch.bfloat16:      # fp16 rows at whole tiles are read as they lie
+        half = x.half()
+        check_linear(ops.w4_linear(half, w), half, w64)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 9, 40, 300])
+def test_workspace_holds_anything(dev, rows):
+    """What a workspace held before does not matter, nor that it is larger than needed, or was used by another call."""
+    g = _gen(rows)
+    m = Matrix(g, 300, 650, 64, dtype=torch.bfloat16)
+    w = m.pack(dev)
+    x = torch.randn(rows, 650, generator=g).bfloat16().to(dev)
+    ref = ops.w4_linear(x, w)
+    ws = torch.empty(ops.lib().evamx_w4_linear_workspace_bytes(2 * rows, 650) + 100, dtype=torch.uint8, device=dev)
+    for fill in (0, 255, 0x7f):
+        ws.fill_(fill)
+        assert torch.equal(ops.w4_linear(x, w, workspace=ws), ref)
+    assert torch.equal(ops.w4_linear(x[:1], w, workspace=ws), ops.w4_linear(x[:1], w))
+
+
+def test_fp16_denormals(dev):
+    """fp16 values below 2^-14 keep their bits in the products."""
+    g = _gen(4)
+    m = Matrix(g, 64, 256, 128, scale=64.0)
+    for rows in (1, 5, 40):
+        x = (torch.randn(rows, 256, generator=g) * 2.0 ** -18).half().to(dev)
+        check_linear(ops.w4_linear(x, m.pack(dev)), x, m.w)
+
+
 @pytest.mark.parametrize("rows", [1, 3, 16, 40, 200])
 def test_strides_and_alignment(dev, rows):
     """Rows that start at odd elements, strides that are no multiple of anything, results into a slice: the same

@@ -172,6 +172,48 @@ def test_strides_graph_and_streams(dev, rows):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype,group,zeros", [(torch.bfloat16, 128, False), (torch.float16, 64, True), (torch.bfloat16, 32, True),
+                                               (torch.float16, 128, False)])
+def test_expert_loads_at_the_units_edges(dev, dtype, group, zeros):
+    """Experts of every number of rows at which the kernels or their units change, in one call: none, 1, 16, 17, up to 257."""
+    loads = [0, 1, 16, 17, 31, 0, 32, 33, 48, 49, 63, 64, 65, 80, 81, 96, 97, 127, 128, 129, 0, 257, 15]
+    g = _gen(group)
+    ex = Experts(g, 320, 200, len(loads), group, zeros=zeros, dtype=dtype)
+    sel = torch.cat([torch.full((n,), e) for e, n in enumerate(loads)])
+    sel = sel[torch.randperm(len(sel), generator=g)].reshape(-1, 1)
+    x = (1.5 * torch.randn(len(sel), 320, generator=g)).to(dtype)
+    w = torch.randn(len(sel), 1, generator=g)
+    _check(dev, ex, x, sel, w, limit=2.0)
+
+
+@pytest.mark.parametrize("experts", [200, 1000])
+def test_many_experts_few_rows_each(dev, experts):
+    """As many units as a call can have: every expert with one more row than a unit holds, or with one."""
+    g = _gen(experts)
+    ex = Experts(g, 64, 48, experts, 32)
+    for per in (1, 16, 17):
+        if per * experts > 8000:
+            continue
+        sel = torch.arange(experts).repeat(per)[torch.randperm(per * experts, generator=g)].reshape(-1, 1)
+        x = torch.randn(len(sel), 64, generator=g).bfloat16()
+        _check(dev, ex, x, sel, torch.ones(len(sel), 1))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 12, 100])
+def test_workspace_holds_anything(dev, rows):
+    g = _gen(rows)
+    ex = Experts(g, 256, 160, 9, 64, zeros=True)
+    m = ex.module(dev, n_shared=1)
+    x = torch.randn(rows, 256, generator=g).bfloat16().to(dev)
+    sel, w = (t.to(dev) for t in _routes(g, rows, 8, 3))
+    sel[0, 0] = 50                                        # a slot that nobody computes
+    ref = m(x, sel, w)
+    ws = torch.empty(ops.lib().evamx_w4_moe_workspace_bytes(2 * rows, 3, 1, 256, 160), dtype=torch.uint8, device=dev)
+    for fill in (0, 255, 0x7f):
+        ws.fill_(fill)
+        assert torch.equal(ops.w4_moe_forward(x, m.gate, m.up, m.down, sel, w, n_shared=1, workspace=ws), ref)
+
+
 def test_router_statistics_and_experts_together(dev):
     """A layer as it is used: the router's logits and routes, its balance, the experts' products."""
     g = _gen(2)
@@ -224,5 +266,7 @@ def test_refusals(dev):
             call(**kw)
     with pytest.raises(ops._lib.EvamxError, match="fit"):
         ops.w4_moe_forward(x, m.gate, m.up, m.gate, sel, w)
+    with pytest.raises(ops._lib.EvamxError, match="scale type"):
+        ops.w4_moe_forward(x, m.gate, Experts(g, 64, 32, 3, 32, dtype=torch.float16).up.pack(dev), m.down, sel, w)
     with pytest.raises(ops._lib.EvamxError, match="group size"):
         ops.w4_moe_forward(x, m.gate, Experts(g, 64, 32, 3, 64).up.pack(dev), m.down, sel, w)

@@ -40,15 +40,17 @@ def sum_error(n_in):
 
 
 def check_linear(y, x, w, bias=None, input_error=0.0):
-    """y against x W^T + bias in 64 bits: half a step of y's type, the sums' error, and inputs off by input_error."""
-    x64 = x.double().cpu()
+    """y against x W^T + bias in 64 bits, where w is: half a step of y's type, the sums' error, and inputs off by
+    input_error."""
+    x64 = x.double().to(w.device)
     ref = x64 @ w.t()
     mag = x64.abs() @ w.abs().t()
     if bias is not None:
-        ref, mag = ref + bias.double().cpu(), mag + bias.double().cpu().abs()
+        b = bias.double().to(w.device)
+        ref, mag = ref + b, mag + b.abs()
     tol = mag * (sum_error(x.shape[-1]) + input_error)
     tol = tol + half_step(y.dtype) * (ref.abs() + tol) + torch.finfo(y.dtype).smallest_normal * half_step(y.dtype)
-    off = (y.double().cpu() - ref).abs()
+    off = (y.double().to(w.device) - ref).abs()
     assert (off <= tol).all(), float((off / tol).max())
 
 
