@@ -30,7 +30,8 @@ __device__ __forceinline__ void w4_linear_store(const W4LinearParams& p, const W
 
 // Up to four rows: one launch. A workgroup takes 16 NB columns, a wave one part of the k-tiles; the rows are made ready in LDS
 // while the first tiles are on their way, and each stands in four of the 16 rows of a matrix operand, so that one of the four
-// accumulators of a lane is all there is to scale.
+// accumulators of a lane is all there is to scale. 2048 -> 7168 at one row: 4.9 us in a graph, of which an empty launch is 1.6;
+// the rest is the loads' one round trip and the join.
 template <int SG, bool ZERO, int NB>
 __global__ __launch_bounds__(512) void w4_linear_few_kernel(W4LinearParams p, W4Mat m)
 {
@@ -68,7 +69,9 @@ __global__ __launch_bounds__(512) void w4_linear_few_kernel(W4LinearParams p, W4
     w4_linear_store(p, m, r, n, v, scale[r]);
 }
 
-// 16 MB rows by 16 NB columns a workgroup, a wave one part of the k-tiles; the rows come ready from memory with the tiles.
+// 16 MB rows by 16 NB columns a workgroup, a wave one part of the k-tiles; the rows come ready from memory (L2) with the tiles.
+// 7168 -> 18432 with groups of 64 and zero points at 5 rows: 17.4 us, 4.2 TB/s; 7168 -> 2048 at 200 rows: 21.5 us, 273 TFLOP/s,
+// bound by the rows' operands, 8 KiB a k-tile and wave beside 4 of codes.
 template <int SG, bool ZERO, int NB, int MB>
 __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat m)
 {
@@ -110,7 +113,7 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat 
 
 // Long calls: 64 rows by 256 columns a workgroup (w4_gemm.hpp). Consecutive workgroups go to the eight XCDs in turn, so each XCD
 // takes a contiguous run of tiles, eight row tiles by all columns at a time: its rows' tiles stay in its L2 while it passes over
-// the columns.
+// the columns. 8192 rows of 2048 -> 7168: about 225 us, 1070 TFLOP/s, and 13 to make the bf16 rows ready.
 template <int SG, bool ZERO, int MB>
 __device__ __forceinline__ void w4_linear_gemm(const W4LinearParams& p, const W4Mat& m, int r0, int have, int nt0, char* lds)
 {

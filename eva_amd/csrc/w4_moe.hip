@@ -168,7 +168,8 @@ constexpr int W4_GU_CT = 2, W4_DOWN_NB = 4;
 
 // Up to W4_FEW_ROWS tokens, without a launch before it: 16 columns of gate and up of one expert a column group, the tokens' rows
 // in LDS (w4_linear_few_kernel's scheme). Unit u is the expert of slot u, if no slot before it has that expert; with one token
-// every slot is a unit.
+// every slot is a unit. One token of a 7168 x 2048 layer with eight experts and a shared one: 28.6 us for 136 MB, 4.8 TB/s; reading
+// as much with no decode takes 26.
 constexpr int W4_FEW_ROWS = 4, W4_FEW_SLOTS = W4_FEW_ROWS * 64;
 
 template <int SG, bool ZERO>
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_few_kernel(W4MoePara
     for (int r0 = 4; r0 < rows; r0 += 4) block(r0, [] {});          // only where a token repeats an expert
 }
 
-// 16 CT columns of gate and up a column group, by a unit of up to 16 MB rows.
+// 16 CT columns of gate and up a column group, by a unit of up to 16 MB rows. 16 tokens of that layer, 83 experts: 235 us, 5.3 TB/s.
 template <int RING, int SG, bool ZERO, int CT, int MB>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_kernel(W4MoeParams p, W4Mat gate, W4Mat up, int parts)
 {
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(256) void w4_hidden_kernel(W4MoeParams p, int n_pad
     if (threadIdx.x == 0) p.hs[s] = f;
 }
 
-// 16 NB columns of the output a column group, by a unit of up to 16 MB rows.
+// 16 NB columns of the output a column group, by a unit of up to 16 MB rows. 16 tokens as above: 127 us, 4.9 TB/s.
 template <int RING, int SG, bool ZERO, int NB, int MB, bool HL>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W4Mat down, int parts)
 {
@@ -357,7 +358,9 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W
     }
 }
 
-// 128 columns of gate and up by a unit of up to 64 rows: the streams of a wave are gate and up of two column tiles.
+// 128 columns of gate and up by a unit of up to 64 rows: the streams of a wave are gate and up of two column tiles. 2000 tokens of
+// a 7168 x 2048 layer with groups of 32 and Zipf loads: 1409 us here and 382 in the small experts' kernel; with groups of 128 and
+// even loads the whole layer runs at 650 TFLOP/s, of 8 slots a token.
 template <int SG, bool ZERO, int MB>
 __device__ __forceinline__ void w4_gate_up_gemm(const W4MoeParams& p, const W4Mat& gate, const W4Mat& up, const W4Unit& u, char* lds)
 {
@@ -454,7 +457,8 @@ __global__ __launch_bounds__(64 * W4G_WAVES, HL ? 1 : 2) void w4_down_gemm_kerne
 }
 
 // One token: 16 NB columns of the output, a wave a slot (up to 16, then the next ones), its parts of the k-tiles one after the
-// other; the slots' sums meet in LDS, so that no launch follows.
+// other; the slots' sums meet in LDS, so that no launch follows. The layer above: 20.3 us for 68 MB, 3.3 TB/s; a wave's 32 KiB of
+// codes are too few to make up for its start (with 16 columns a wave 24.6 us).
 constexpr int W4_ONE_WAVES = 16, W4_ONE_NB = 2;
 
 template <int SG, bool ZERO, bool HL>

@@ -24,6 +24,8 @@
  *                            plus the shared expert added by Block.experts (model.py:418-452,498)
  *   evamx_moe_workspace_bytes  WorkspaceLayout.scratch_bytes / exl3_moe_coop_ctr_len
  *                            (moe_coop3072.py:120-152; exl3_moe_coop.cuh:154-159)
+ * evamx_w4_* (4-bit weights with group scales) and evamx_balance_* (a router's balance loss) have
+ * no counterpart in the reference.
  */
 #ifndef EVAMX_H
 #define EVAMX_H
