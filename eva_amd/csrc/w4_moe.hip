@@ -459,15 +459,15 @@ __global__ __launch_bounds__(64 * W4G_WAVES, HL ? 1 : 2) void w4_down_gemm_kerne
 // One token: 16 NB columns of the output, a wave a slot (up to 16, then the next ones), its parts of the k-tiles one after the
 // other; the slots' sums meet in LDS, so that no launch follows. The layer above: 20.3 us for 68 MB, 3.3 TB/s; a wave's 32 KiB of
 // codes are too few to make up for its start (with 16 columns a wave 24.6 us).
-constexpr int W4_ONE_WAVES = 16, W4_ONE_NB = 2;
+constexpr int W4_ONE_WAVES = 16, W4_ONE_NB = 2, W4_ONE_LDS = 128 * 1024;
 
 template <int SG, bool ZERO, bool HL>
 __global__ __launch_bounds__(64 * W4_ONE_WAVES) void w4_down_one_kernel(W4MoeParams p, W4Mat down, int parts)
 {
-    extern __shared__ w4_half hs[];                          // per wave, its slot's activations
-    __shared__ float y[64][W4_ONE_NB][16];
+    extern __shared__ w4_half hs[];                          // per wave, its slot's activations; then y[kt_slots][W4_ONE_NB][16]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, n_pad = down.kt * W4_TILE_K;
     w4_half* mine = hs + wave * (HL ? 2 * n_pad : n_pad);
+    float (*y)[W4_ONE_NB][16] = (float (*)[W4_ONE_NB][16])(hs + waves * (HL ? 2 * n_pad : n_pad));
     const w4_half* a = mine + 8 * (lane >> 4);
     for (int s = wave; s < p.kt_slots; s += waves) {
         const int e = __builtin_amdgcn_readfirstlane(w4_slot_expert(p, s));
@@ -666,8 +666,8 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
                 <<<dim3(w4_ceil(gm.nt, W4_WAVES / gp), units), 64 * W4_WAVES, w4_stage_bytes(p.rows, gm.kt), s>>>(p, gm, um, gp);
         });
         const int one_waves = p.kt_slots < W4_ONE_WAVES ? p.kt_slots : W4_ONE_WAVES;
-        const size_t one_bytes = (size_t)one_waves * h_pad * (p.bf16 ? 2 : 4);
-        if (p.rows == 1 && one_bytes <= 56 * 1024) {
+        const size_t one_bytes = (size_t)one_waves * h_pad * (p.bf16 ? 2 : 4) + (size_t)p.kt_slots * W4_ONE_NB * 16 * 4;
+        if (p.rows == 1 && one_bytes <= W4_ONE_LDS) {
             w4_dispatch(d, [&](auto sg, auto zero) {
                 constexpr int SG = decltype(sg)::value;
                 constexpr bool ZERO = decltype(zero)::value;

@@ -51,6 +51,17 @@ def test_layer(dev, config, rows):
     _check(dev, ex, x, sel, w, n_shared=shared, limit=0.0 if rows % 3 else 0.5)
 
 
+@pytest.mark.parametrize("inter", [700, 2100, 5000])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_one_token_of_wide_experts(dev, inter, dtype):
+    """One token whose slots' hidden activations take little of the workgroup's LDS, most of it, or do not fit."""
+    g = _gen(inter)
+    ex = Experts(g, 192, inter, 11, 64, zeros=True, dtype=dtype)
+    x = (1.5 * torch.randn(1, 192, generator=g)).to(dtype)
+    sel, w = _routes(g, 1, 10, 9)
+    _check(dev, ex, x, sel, w, n_shared=1, limit=3.0)
+
+
 @pytest.mark.parametrize("rows", [1, 5, 16, 70, 200])
 def test_a_rank_of_the_experts(dev, rows):
     """An expert range: slots of other experts add nothing, a token with none of them gets zeros whatever its
