@@ -9,6 +9,13 @@ from . import ops
 MAX_CALL_ROWS = 65536       # rows per evamx_w4_linear call
 
 
+def _moe_call_rows(slots: int, hidden: int, inter: int) -> int:
+    """Rows of ``slots`` experts each that one evamx_w4_moe_forward call takes (its limits of slots, of x's and of the
+    hidden activations' padded values)."""
+    pad_hidden, pad_inter, slots = -(-hidden // 128) * 128, -(-inter // 128) * 128, max(slots, 1)
+    return max(min(ops._lib.W4_MOE_MAX_SLOTS // slots, (2 ** 31 - 1) // pad_hidden, (2 ** 30 - 1) // (slots * pad_inter)), 1)
+
+
 class W4Linear:
     """``y = x W^T (+ bias)`` for one packed matrix; x fp16 or bf16 with any leading dimensions."""
 
@@ -64,7 +71,7 @@ class W4Experts:
         sel = sel.reshape(rows, topk).to(torch.int64).contiguous()
         weights = weights.reshape(rows, topk).to(torch.float32).contiguous()
         out = torch.empty(rows, self.hidden, dtype=x.dtype, device=x.device)
-        step = ops._lib.W4_MOE_MAX_SLOTS // (topk + self.n_shared)
+        step = _moe_call_rows(topk + self.n_shared, self.hidden, self.inter)
         for r0 in range(0, rows, step):
             part = slice(r0, r0 + step)
             ops.w4_moe_forward(flat[part], self.gate, self.up, self.down, sel[part], weights[part], n_shared=self.n_shared,

@@ -99,6 +99,15 @@ def test_moe_workspace():
         assert L.evamx_w4_moe_workspace_bytes(*bad) == 0, bad
 
 
+@pytest.mark.parametrize("hidden, inter", [(7168, 2048), (100, 16384), (4096, 16300), (64, 1 << 18), (1 << 18, 128), (1 << 18, 1 << 18)])
+@pytest.mark.parametrize("topk, shared", [(1, 0), (8, 1), (32, 32)])
+def test_the_module_splits_by_every_limit(hidden, inter, topk, shared):
+    """The rows of a call that W4Experts makes are within its limits, and no more would be."""
+    from eva_amd.w4 import _moe_call_rows
+    need, n = _lib.lib().evamx_w4_moe_workspace_bytes, _moe_call_rows(topk + shared, hidden, inter)
+    assert n >= 1 and need(n, topk, shared, hidden, inter) > 0 and need(n + 1, topk, shared, hidden, inter) == 0
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     import os
     import subprocess
