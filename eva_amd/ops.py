@@ -88,8 +88,8 @@ class W4Weight:
         if nbytes == 0:
             raise ValueError(f"{count} matrices [{n_out}, {n_in}] outside 1..{_lib.W4_MAX_COUNT} and 1..{_lib.W4_MAX_DIM}")
         self.count, self.n_out, self.n_in, self.group = count, n_out, n_in, group
-        self.device = torch.device(device)
         self.codes = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.device = self.codes.device                      # with its index, whatever `device` names
         self.scales = torch.empty(groups, dtype=scale_dtype, device=device)
         self.zeros = torch.empty(groups, dtype=torch.uint8, device=device) if zeros else None
         self.desc = W4Desc(ptr(self.codes), ptr(self.scales), ptr(self.zeros), count, n_out, n_in, stored,

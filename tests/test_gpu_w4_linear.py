@@ -188,6 +188,19 @@ def test_module_graph_and_streams(dev, rows):
         torch.cuda.synchronize()
 
 
+def test_a_weight_filled_by_its_owner(dev):
+    """A weight made without w4_pack (its buffers read from a file, say), on a device named without an index."""
+    g = torch.Generator().manual_seed(5)
+    m = Matrix(g, 48, 160, 32, zeros=True)
+    packed = m.pack(dev)
+    w = ops.W4Weight(1, 48, 160, 32, torch.float16, True, "cuda")
+    for a, b in ((w.codes, packed.codes), (w.scales, packed.scales), (w.zeros, packed.zeros)):
+        a.copy_(b)
+    x = torch.randn(3, 160, generator=g).half().to(dev)
+    assert torch.equal(ops.w4_dequant(w), ops.w4_dequant(packed))
+    assert torch.equal(ops.w4_linear(x, w), ops.w4_linear(x, packed))
+
+
 def test_refusals(dev):
     g = _gen(1)
     m = Matrix(g, 32, 64, 32)
