@@ -330,7 +330,10 @@ struct W4ReadyRow {
         for (int e = 0; e < 8; ++e) {
             const float x = o[e] * down;
             h[e] = (w4_half)x;
-            if constexpr (HL) l[e] = (w4_half)(x - (float)h[e]);
+            if constexpr (HL) {
+                const float left = x - (float)h[e];
+                l[e] = (w4_half)(left == left ? left : 0.0f);    // of an infinity nothing is left
+            }
         }
         *(w4_half8*)dst = h;
         if constexpr (HL) *(w4_half8*)(dst + lo_off) = l;

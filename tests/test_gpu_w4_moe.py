@@ -129,6 +129,23 @@ def test_inf_and_nan_stay_in_their_rows(dev, rows):
     assert y[0].isnan().all()
 
 
+@pytest.mark.parametrize("rows", [1, 2, 9, 40])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_one_infinite_hidden_activation(dev, rows, dtype):
+    """One hidden activation overflows fp32: the outputs are infinities of its weights' signs, not NaN."""
+    g = _gen(rows)
+    ex = Experts(g, 128, 256, 2, 128)
+    for m in (ex.gate, ex.up):
+        m.q[0, 17] = 15
+        m.codes[0, 17] = 255
+    ex.up.scales[0, 17] = 3e38
+    ex.down.q[0, :, 17] = torch.randint(0, 2, (128,), generator=g, dtype=torch.uint8) * 15
+    ex.down.codes[0, :, 8] = ex.down.q[0, :, 16] | ex.down.q[0, :, 17] << 4
+    x = torch.ones(rows, 128, dtype=dtype)
+    y = ex.module(dev)(x.to(dev), torch.zeros(rows, 1, dtype=torch.int64, device=dev), torch.ones(rows, 1, device=dev)).cpu()
+    assert torch.equal(y.float(), torch.where(ex.down.q[0, :, 17] == 15, torch.inf, -torch.inf).expand(rows, 128))
+
+
 def test_rows_do_not_depend_on_their_batch(dev):
     """Up to 16 rows a token's bits are those it has alone."""
     g = _gen(8)
