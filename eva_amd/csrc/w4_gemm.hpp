@@ -13,7 +13,7 @@
 
 namespace evamx {
 
-// A tile of at most 32 or 16 rows is run as one of 2 or 1 blocks of 16 (MB): it brings, reads and multiplies no more.
+// A tile of fewer rows is run as one of fewer blocks of 16 (MB): it brings, reads and multiplies no more.
 constexpr int W4G_ROWS = 64, W4G_NB = 4, W4G_WAVES = 4;
 constexpr int W4G_COLS = 16 * W4G_NB * W4G_WAVES;                   // 256
 constexpr int W4G_STAGE = W4G_ROWS * W4_TILE_K * 2;                 // bytes of the rows' k-tile
