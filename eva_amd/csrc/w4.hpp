@@ -261,8 +261,8 @@ __device__ __forceinline__ int w4_exponent(uint32_t top)
 // A row of activations made ready by THREADS threads (a wave or a workgroup) for w4_tile: load() requests it, 8 values a thread
 // and chunk, finish() writes fp16 values times 2^-e and returns 2^e, e the exponent that takes the row's largest finite
 // magnitude into [2^14, 2^15) (0 for fp16 rows, which need none). The factor is a power of two, so bf16 values down to 2^-28
-// of the largest are exact and none overflows. fp32 rows (hidden activations) are rounded to fp16's 11 bits; with HL what that
-// leaves goes into a second half lo_off values on. Zeros from n_in to n_pad. Rows longer than NC chunks are read twice.
+// of the largest are exact and none overflows. Of fp32 rows (hidden activations) the values are fp16's 11 bits and, with HL, what
+// that leaves in a second half lo_off values on. Zeros from n_in to n_pad. Rows longer than NC chunks are read twice.
 constexpr int W4_SRC_F32 = 2;
 
 template <int SRC, int THREADS, bool HL>

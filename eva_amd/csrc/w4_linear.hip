@@ -173,7 +173,7 @@ __device__ __forceinline__ void w4_linear_gemm(const W4LinearParams& p, const W4
 template <int SG, bool ZERO>
 __global__ __launch_bounds__(256, 2) void w4_linear_gemm_kernel(W4LinearParams p, W4Mat m, int row_tiles, int col_tiles)
 {
-    __shared__ __attribute__((aligned(128))) char lds[W4G_STAGES * W4G_STAGE];
+    __shared__ __attribute__((aligned(128))) char lds[w4g_lds<false>()];
     const int total = row_tiles * col_tiles, per = w4_ceil(total, 8), t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || t >= total) return;
     const int band = t / (8 * col_tiles), in_band = t - band * 8 * col_tiles, deep = row_tiles - 8 * band < 8 ? row_tiles - 8 * band : 8;

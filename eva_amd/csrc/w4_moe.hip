@@ -297,23 +297,23 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_kernel(W4MoeParams p
     }
 }
 
-// The hidden activations of the slots there are, ready for the down products. HL, for fp16 calls: what rounding them to 11 bits
-// leaves is kept in a second half, since their results' own rounding is no coarser (relative error of a layer 2.9e-4 with one
-// half, 2.1e-4 being the results' rounding; of bf16 results 1.7e-3 with one half or two).
-template <bool HL>
+// The hidden activations of the slots there are, ready for the down products, each as the sum of two halves: their first 11 bits,
+// and what that rounding leaves, so that some 22 bits of them reach the results (relative error of an fp16 layer 2.9e-4 with one
+// half, 2.1e-4 being the results' own rounding; bf16 results then differed by 9e-4 from those of fp32 arithmetic, now by 1e-5).
 __global__ __launch_bounds__(256) void w4_hidden_kernel(W4MoeParams p, int n_pad)
 {
     __shared__ uint32_t part[4];
     const int s = blockIdx.x;
     if (w4_slot_expert(p, s) < 0) return;
-    W4ReadyRow<W4_SRC_F32, 256, HL> row{(const char*)(p.h + (size_t)s * p.h_ld), p.inter, n_pad, true, (int)threadIdx.x};
+    W4ReadyRow<W4_SRC_F32, 256, true> row{(const char*)(p.h + (size_t)s * p.h_ld), p.inter, n_pad, true, (int)threadIdx.x};
     row.load();
-    const float f = row.finish(p.hh + s * (size_t)(HL ? 2 * n_pad : n_pad), n_pad, part);
+    const float f = row.finish(p.hh + s * (size_t)(2 * n_pad), n_pad, part);
     if (threadIdx.x == 0) p.hs[s] = f;
 }
 
-// 16 NB columns of the output a column group, by a unit of up to 16 MB rows. 16 tokens as above: 127 us, 4.9 TB/s.
-template <int RING, int SG, bool ZERO, int NB, int MB, bool HL>
+// 16 NB columns of the output a column group, by a unit of up to 16 MB rows. 16 tokens as above: 146 us, 4.3 TB/s (127 with one half
+// a value).
+template <int RING, int SG, bool ZERO, int NB, int MB>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W4Mat down, int parts)
 {
     __shared__ w4_f32x4 part[W4_WAVES][NB][MB][64];
@@ -326,8 +326,8 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W
     W4Stream st[NB];
 #pragma unroll
     for (int c = 0; c < NB; ++c) st[c] = w4_stream<SG, ZERO>(down, u.expert, nt + c < down.nt ? nt + c : down.nt - 1, k1);
-    W4GlobalRows<RING, MB, HL> rows;
-    const uint32_t ld = (HL ? 4 : 2) * n_pad;
+    W4GlobalRows<RING, MB, true> rows;
+    const uint32_t ld = 4 * n_pad;
     rows.src = w4_rsrc(p.hh, (uint32_t)p.slots * ld);
     rows.lo_off = 2 * n_pad;
     for (int r0 = 0; r0 < u.rows; r0 += 16 * MB) {           // once, but for few tokens that repeat an expert
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W
             rows.at[mb] = (uint32_t)s * ld + 16 * (lane >> 4);
         }
         w4_f32x4 acc[NB][MB] = {};
-        w4_run<RING, SG, ZERO, NB, MB, 4, HL>(
+        w4_run<RING, SG, ZERO, NB, MB, 4, true>(
             acc, st, k0, k1, down.bf16, [&](int d, int kt) { rows.request(d, kt); },
             [&](int d, int, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) { rows.take(d, x, lo); }, [] {});
 #pragma unroll
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W
 // 128 columns of gate and up by a unit of up to 64 rows: the streams of a wave are gate and up of two column tiles. 2000 tokens of
 // a 7168 x 2048 layer with groups of 32 and Zipf loads: 1409 us here and 382 in the small experts' kernel; with groups of 128 and
 // even loads the whole layer runs at 650 TFLOP/s, of 8 slots a token. Three blocks of rows have a path of their own: 1250 tokens,
-// 39 rows an expert, 1622 us against 1698 with four blocks; fp16 with groups of 64 and zero points 2390 against 2605.
+// 39 rows an expert, 1810 us against 1970 with four blocks; fp16 with groups of 64 and zero points 2100 against 2430.
 template <int SG, bool ZERO, int MB>
 __device__ __forceinline__ void w4_gate_up_gemm(const W4MoeParams& p, const W4Mat& gate, const W4Mat& up, const W4Unit& u, char* lds)
 {
@@ -403,7 +403,7 @@ __device__ __forceinline__ void w4_gate_up_gemm(const W4MoeParams& p, const W4Ma
 template <int SG, bool ZERO>
 __global__ __launch_bounds__(64 * W4G_WAVES, 2) void w4_gate_up_gemm_kernel(W4MoeParams p, W4Mat gate, W4Mat up)
 {
-    __shared__ __attribute__((aligned(128))) char lds[W4G_STAGES * W4G_STAGE];
+    __shared__ __attribute__((aligned(128))) char lds[w4g_lds<false>()];
     if ((int)blockIdx.y >= p.n_units[1]) return;
     const W4Unit u = p.big[blockIdx.y];
     if (u.rows > 48) w4_gate_up_gemm<SG, ZERO, 4>(p, gate, up, u, lds);
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(64 * W4G_WAVES, 2) void w4_gate_up_gemm_kernel(W4Mo
 }
 
 // 256 columns of the output by a unit of up to 64 rows.
-template <int SG, bool ZERO, bool HL, int MB>
+template <int SG, bool ZERO, int MB>
 __device__ __forceinline__ void w4_down_gemm(const W4MoeParams& p, const W4Mat& down, const W4Unit& u, char* lds)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = (blockIdx.x * W4G_WAVES + wave) * W4G_NB;
@@ -421,7 +421,7 @@ __device__ __forceinline__ void w4_down_gemm(const W4MoeParams& p, const W4Mat& 
 #pragma unroll
     for (int b = 0; b < W4G_NB; ++b) st[b] = w4_stream<SG, ZERO>(down, u.expert, nt + b < down.nt ? nt + b : down.nt - 1, down.kt);
     W4GemmRows<MB> rows;
-    const uint32_t half = down.kt * (W4_TILE_K * 2), ld = HL ? 2 * half : half;
+    const uint32_t half = down.kt * (W4_TILE_K * 2), ld = 2 * half;
     rows.src = w4_rsrc(p.hh, p.slots * ld);
     rows.lo_off = half;
 #pragma unroll
@@ -430,7 +430,7 @@ __device__ __forceinline__ void w4_down_gemm(const W4MoeParams& p, const W4Mat& 
         rows.at[i] = p.order[u.r0 + (r < u.rows ? r : u.rows - 1)] * ld + w4g_chunk<MB>(i);
     }
     w4_f32x4 acc[W4G_NB][MB] = {};
-    w4g_run<SG, ZERO, HL, MB>(acc, st, rows, lds, down.kt, down.bf16);
+    w4g_run<SG, ZERO, true, MB>(acc, st, rows, lds, down.kt, down.bf16);
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -447,36 +447,37 @@ __device__ __forceinline__ void w4_down_gemm(const W4MoeParams& p, const W4Mat& 
         }
 }
 
-template <int SG, bool ZERO, bool HL>
-__global__ __launch_bounds__(64 * W4G_WAVES, HL ? 1 : 2) void w4_down_gemm_kernel(W4MoeParams p, W4Mat down)
+template <int SG, bool ZERO>
+__global__ __launch_bounds__(64 * W4G_WAVES, 2) void w4_down_gemm_kernel(W4MoeParams p, W4Mat down)
 {
-    __shared__ __attribute__((aligned(128))) char lds[W4G_STAGES * W4G_STAGE * (HL ? 2 : 1)];
+    __shared__ __attribute__((aligned(128))) char lds[w4g_lds<true>()];
     if ((int)blockIdx.y >= p.n_units[1]) return;
     const W4Unit u = p.big[blockIdx.y];
-    if (u.rows > 48) w4_down_gemm<SG, ZERO, HL, 4>(p, down, u, lds);
-    else if (u.rows > 32) w4_down_gemm<SG, ZERO, HL, 3>(p, down, u, lds);
-    else if (u.rows > 16) w4_down_gemm<SG, ZERO, HL, 2>(p, down, u, lds);
-    else w4_down_gemm<SG, ZERO, HL, 1>(p, down, u, lds);
+    if (u.rows > 48) w4_down_gemm<SG, ZERO, 4>(p, down, u, lds);
+    else if (u.rows > 32) w4_down_gemm<SG, ZERO, 3>(p, down, u, lds);
+    else if (u.rows > 16) w4_down_gemm<SG, ZERO, 2>(p, down, u, lds);
+    else w4_down_gemm<SG, ZERO, 1>(p, down, u, lds);
 }
 
 // One token: 16 NB columns of the output, a wave a slot (up to 16, then the next ones), its parts of the k-tiles one after the
-// other; the slots' sums meet in LDS, so that no launch follows. The layer above: 20.3 us for 68 MB, 3.3 TB/s; a wave's 32 KiB of
-// codes are too few to make up for its start (with 16 columns a wave 24.6 us). Calls whose slots' activations do not fit W4_ONE_LDS
-// take the general path: at nine slots of fp16 (two halves a value) with groups of 64 and zero points 74.1 us, here 60.2.
+// other; the slots' sums meet in LDS, so that no launch follows. The layer above: 25.0 us for 68 MB, 2.7 TB/s; a wave's 32 KiB of
+// codes are too few to make up for its start, and every value is read from LDS as two halves (20.3 with one; then 24.6 with 16
+// columns a wave). Calls whose slots' activations do not fit W4_ONE_LDS take the general path: at nine slots of fp16 with groups of
+// 64 and zero points 74.1 us, here 60.2.
 constexpr int W4_ONE_WAVES = 16, W4_ONE_NB = 2, W4_ONE_LDS = 128 * 1024;
 
-template <int SG, bool ZERO, bool HL>
+template <int SG, bool ZERO>
 __global__ __launch_bounds__(64 * W4_ONE_WAVES) void w4_down_one_kernel(W4MoeParams p, W4Mat down, int parts)
 {
     extern __shared__ w4_half hs[];                          // per wave, its slot's activations; then y[kt_slots][W4_ONE_NB][16]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, n_pad = down.kt * W4_TILE_K;
-    w4_half* mine = hs + wave * (HL ? 2 * n_pad : n_pad);
-    float (*y)[W4_ONE_NB][16] = (float (*)[W4_ONE_NB][16])(hs + waves * (HL ? 2 * n_pad : n_pad));
+    w4_half* mine = hs + wave * (2 * n_pad);
+    float (*y)[W4_ONE_NB][16] = (float (*)[W4_ONE_NB][16])(hs + waves * (2 * n_pad));
     const w4_half* a = mine + 8 * (lane >> 4);
     for (int s = wave; s < p.kt_slots; s += waves) {
         const int e = __builtin_amdgcn_readfirstlane(w4_slot_expert(p, s));
         if (e < 0) continue;
-        W4ReadyRow<W4_SRC_F32, 64, HL> row{(const char*)(p.h + (size_t)s * p.h_ld), p.inter, n_pad, true, lane};
+        W4ReadyRow<W4_SRC_F32, 64, true> row{(const char*)(p.h + (size_t)s * p.h_ld), p.inter, n_pad, true, lane};
         row.load();
         W4Stream st[W4_ONE_NB];
 #pragma unroll
@@ -487,13 +488,13 @@ __global__ __launch_bounds__(64 * W4_ONE_WAVES) void w4_down_one_kernel(W4MoePar
         float f = 0, v[W4_ONE_NB] = {};
         auto part = [&](int q, auto begin) {
             w4_f32x4 acc[W4_ONE_NB][1] = {};
-            w4_run<2, SG, ZERO, W4_ONE_NB, 1, 1, HL>(
+            w4_run<2, SG, ZERO, W4_ONE_NB, 1, 1, true>(
                 acc, st, w4_part_begin(down.kt, parts, q), w4_part_begin(down.kt, parts, q + 1), down.bf16, [](int, int) {},
                 [&](int, int kt, w4_half8 (&x)[1][4], w4_half8 (&lo)[1][4]) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         x[0][j] = *(const w4_half8*)(a + kt * W4_TILE_K + 32 * j);
-                        if constexpr (HL) lo[0][j] = *(const w4_half8*)(a + n_pad + kt * W4_TILE_K + 32 * j);
+                        lo[0][j] = *(const w4_half8*)(a + n_pad + kt * W4_TILE_K + 32 * j);
                     }
                 },
                 begin);
@@ -584,7 +585,7 @@ static W4MoeLayout w4_moe_layout(int rows, int topk, int n_shared, int hidden, i
     l.x = take(rows * kx * 2);
     l.h = take(slots * kh * 4);
     l.hs = take(slots * 4);
-    l.hh = take(slots * kh * 4);                             // fp16 calls keep two halves a value
+    l.hh = take(slots * kh * 4);                             // two halves a value
     l.y = take(slots * hidden * 4);
     l.total = at;
     return l;
@@ -670,14 +671,11 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
                 <<<dim3(w4_ceil(gm.nt, W4_WAVES / gp), units), 64 * W4_WAVES, w4_stage_bytes(p.rows, gm.kt), s>>>(p, gm, um, gp);
         });
         const int one_waves = p.kt_slots < W4_ONE_WAVES ? p.kt_slots : W4_ONE_WAVES;
-        const size_t one_bytes = (size_t)one_waves * h_pad * (p.bf16 ? 2 : 4) + (size_t)p.kt_slots * W4_ONE_NB * 16 * 4;
+        const size_t one_bytes = (size_t)one_waves * h_pad * 4 + (size_t)p.kt_slots * W4_ONE_NB * 16 * 4;
         if (p.rows == 1 && one_bytes <= W4_ONE_LDS) {
             w4_dispatch(d, [&](auto sg, auto zero) {
-                constexpr int SG = decltype(sg)::value;
-                constexpr bool ZERO = decltype(zero)::value;
-                const int blocks = w4_ceil(dm.nt, W4_ONE_NB);
-                if (p.bf16) w4_down_one_kernel<SG, ZERO, false><<<blocks, 64 * one_waves, one_bytes, s>>>(p, dm, dp);
-                else w4_down_one_kernel<SG, ZERO, true><<<blocks, 64 * one_waves, one_bytes, s>>>(p, dm, dp);
+                w4_down_one_kernel<decltype(sg)::value, decltype(zero)::value>
+                    <<<w4_ceil(dm.nt, W4_ONE_NB), 64 * one_waves, one_bytes, s>>>(p, dm, dp);
             });
             return launched("w4_moe_forward");
         }
@@ -698,19 +696,13 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
                 <<<dim3(w4_ceil(gm.nt, W4_GU_CT * (W4_WAVES / gp)), units), 64 * W4_WAVES, 0, s>>>(p, gm, um, gp);
         });
     }
-    if (p.bf16) w4_hidden_kernel<false><<<p.slots, 256, 0, s>>>(p, h_pad);
-    else w4_hidden_kernel<true><<<p.slots, 256, 0, s>>>(p, h_pad);
+    w4_hidden_kernel<<<p.slots, 256, 0, s>>>(p, h_pad);
     w4_dispatch(d, [&](auto sg, auto zero) {
         constexpr int SG = decltype(sg)::value;
         constexpr bool ZERO = decltype(zero)::value;
         const dim3 grid(w4_ceil(dm.nt, W4_DOWN_NB * (W4_WAVES / dp)), units), big_grid(w4_ceil(dm.nt, W4G_WAVES * W4G_NB), bigs);
-        if (p.bf16) {
-            if (bigs) w4_down_gemm_kernel<SG, ZERO, false><<<big_grid, 64 * W4G_WAVES, 0, s>>>(p, dm);
-            w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, false><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
-        } else {
-            if (bigs) w4_down_gemm_kernel<SG, ZERO, true><<<big_grid, 64 * W4G_WAVES, 0, s>>>(p, dm);
-            w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1, true><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
-        }
+        if (bigs) w4_down_gemm_kernel<SG, ZERO><<<big_grid, 64 * W4G_WAVES, 0, s>>>(p, dm);
+        w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
     });
     w4_combine_kernel<<<p.rows * w4_ceil(p.hidden, 1024), 256, 0, s>>>(p);
     return launched("w4_moe_forward");

@@ -290,9 +290,9 @@ const void* evamx_moe_rotated_ptr(const evamx_moe_shape* shape, void* workspace)
  * with e in [0, n_local), n_local = count - n_shared; other slots (another rank's experts) add 0. The
  * last n_shared matrices of the stacks are shared experts: every token takes each with weight 1.
  * act = min(silu(g), limit) * clamp(u, -limit, limit), the shared experts' min(g, limit) before SiLU
- * (limit 0: no clamping; a NaN stays NaN). fp32 sums, fp16 hidden activations with a power-of-two
- * factor per row (they neither overflow nor vanish), routing weights as given, slots added in slot
- * order, one rounding to x's type. */
+ * (limit 0: no clamping; a NaN stays NaN). fp32 sums, hidden activations as the sum of two fp16 halves
+ * (22 bits) with a power-of-two factor per row (they neither overflow nor vanish), routing weights as
+ * given, slots added in slot order, one rounding to x's type. */
 enum { EVAMX_W4_MOE_MAX_SLOTS = 65536 };   /* rows * (topk + n_shared) of a call */
 typedef struct evamx_w4_moe_args {
     const void* x;                /* device fp16/bf16 [rows][x_stride] */
