@@ -19,7 +19,7 @@ EVAMX_OK, EVAMX_EINVAL, EVAMX_ELAUNCH, EVAMX_ENOSPACE = 0, -1, -2, -3
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 SCORE_SIGMOID, SCORE_SQRT_SOFTPLUS = 0, 1
 ERR_EXPERT_RANGE, ERR_RATE = 1, 2
-W4_MAX_DIM, W4_MAX_COUNT = 1 << 18, 1024         # EVAMX_W4_MAX_DIM, matrices of a stack
+W4_MAX_DIM, W4_MAX_COUNT, W4_MAX_ZERO = 1 << 18, 1024, 31   # EVAMX_W4_MAX_DIM, matrices of a stack, zero points
 W4_MOE_MAX_SLOTS = 65536                         # EVAMX_W4_MOE_MAX_SLOTS
 STRICT_MAX_ROWS, STRICT_MAX_SLOTS = 64, 256      # EVAMX_STRICT_MAX_ROWS / EVAMX_STRICT_MAX_SLOTS
 

@@ -1,5 +1,5 @@
-// 4-bit weights with group scales on gfx950: W[n][k] = scale[n][k/G] * (code[n][k] - zero[n][k/G]), codes 0..15, zero 8
-// where a matrix has no zero points.
+// 4-bit weights with group scales on gfx950: W[n][k] = scale[n][k/G] * (code[n][k] - zero[n][k/G]), codes 0..15, zero
+// points 0..31, or 8 where a matrix has none.
 //
 // Layout (evamx_w4_pack), per matrix [n_out][n_in]:
 //   - codes: tiles of 16 rows of W (the output columns of a product) by 128 k, [n_out/16][n_in/128] tiles of 1 KiB, both
@@ -27,6 +27,7 @@ typedef float w4_f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t w4_u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int W4_TILE_N = 16, W4_TILE_K = 128, W4_TILE_DWORDS = 256;
+constexpr uint32_t W4_ZERO_MAX = 31;         // zero points are the low five bits of their bytes, here and in evamx_w4_dequant
 
 // A stack of matrices as the kernels take it.
 struct W4Mat {
@@ -154,7 +155,7 @@ __device__ __forceinline__ void w4_tile(w4_f32x4 (&acc)[MB], const W4Raw<SG>& r,
 {
 #pragma unroll
     for (int g = 0; g < SG; ++g) {
-        const W4Zero z = w4_zero(ZERO ? (r.z >> (8 * g)) & 15 : 8);
+        const W4Zero z = w4_zero(ZERO ? (r.z >> (8 * g)) & W4_ZERO_MAX : 8);
         w4_f32x4 part[MB];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) part[mb] = w4_f32x4{0, 0, 0, 0};

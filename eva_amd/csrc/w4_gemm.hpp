@@ -83,7 +83,7 @@ __device__ __forceinline__ void w4g_run(w4_f32x4 (&acc)[NB][MB], const W4Stream 
     auto decode = [&](int j, const W4Raw<SG> (&r)[NB], int b0, int b1) {   // the weights of streams b0 .. b1 - 1 at the 32 k of j
 #pragma unroll
         for (int b = b0; b < b1; ++b)
-            w[j & 1][b] = w4_operand(r[b].c[j], w4_zero(ZERO ? (r[b].z >> (8 * (j * SG / 4))) & 15 : 8), consts);
+            w[j & 1][b] = w4_operand(r[b].c[j], w4_zero(ZERO ? (r[b].z >> (8 * (j * SG / 4))) & W4_ZERO_MAX : 8), consts);
     };
     auto products = [&](int q, const W4Raw<SG> (&r)[NB]) {
         constexpr int PER = PHASES / SG;                               // phases of a group

@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void w4_pack_groups_kernel(const uint16_t* __r
         const bool in = n < (size_t)m.n_out && k < m.n_in;
         const size_t at = in ? (mat * m.n_out + n) * src_n + k / src_group : 0;
         out_s[i] = in ? scales[at] : 0;
-        if (zeros) out_z[i] = in ? zeros[at] & 15 : 0;
+        if (zeros) out_z[i] = in ? zeros[at] : 0;
     }
 }
 
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void w4_dequant_kernel(W4Mat m, int sg, float*
         const uint32_t w = m.codes[(mat * m.tiles + tile) * W4_TILE_DWORDS + (col + 16 * g) * 4 + j];
         const int q = (w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15;
         const size_t at = mat * m.groups + (tile * W4_TILE_N + col) * sg + in_tile * sg / W4_TILE_K;
-        out[i] = w4_scale(m.scales[at], m.bf16) * (float)(q - (m.zeros ? (int)m.zeros[at] : 8));
+        out[i] = w4_scale(m.scales[at], m.bf16) * (float)(q - (m.zeros ? (int)(m.zeros[at] & W4_ZERO_MAX) : 8));
     }
 }
 

@@ -102,8 +102,9 @@ _DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 def w4_pack(codes: torch.Tensor, scales: torch.Tensor, *, n_in: int, group: int, zeros: torch.Tensor | None = None) -> W4Weight:
     """Lay 4-bit weights out for ``w4_linear`` / ``w4_moe_forward``. ``codes`` uint8 ``[(count,) n_out,
     ceil(n_in / 2)]``, two codes of a row to a byte, the even one in the lower half; ``scales`` fp16 or
-    bf16 ``[(count,) n_out, ceil(n_in / group)]``; ``zeros`` uint8 like the scales, the codes that stand
-    for zero (0..15; without them 8). ``group``: a multiple of 32 input features that share a scale."""
+    bf16 ``[(count,) n_out, ceil(n_in / group)]``; ``zeros`` uint8 like the scales, the values that stand
+    for zero (0..31, so also the 16 of formats that hold them less one; without them 8), read back to be checked
+    unless in a graph capture. ``group``: a multiple of 32 input features that share a scale."""
     _dev(codes, "codes", torch.uint8)
     if codes.ndim not in (2, 3):
         raise ValueError("codes must be [n_out, ceil(n_in / 2)] or a stack of such")
@@ -118,6 +119,8 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, *, n_in: int, group: int,
         _dev(zeros, "zeros", torch.uint8, codes.ndim)
         if tuple(zeros.shape) != groups:
             raise ValueError(f"zeros must have the scales' shape {groups}, got {tuple(zeros.shape)}")
+        if zeros.numel() and not torch.cuda.is_current_stream_capturing() and int(zeros.max()) > _lib.W4_MAX_ZERO:
+            raise ValueError(f"zero points up to {int(zeros.max())}: a weight takes 0..{_lib.W4_MAX_ZERO}")
     for t, name in ((scales, "scales"), (zeros, "zeros")):
         if t is not None and t.device != codes.device:
             raise ValueError(f"{name} is on {t.device}, the codes on {codes.device}")

@@ -76,7 +76,8 @@ int evamx_exl3_linear(const void* x_fp16, int rows, int in_features, int out_fea
 
 /* ---- linear on 4-bit weights with group scales --------------------------------------------- */
 
-/* W[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), codes 0..15; without zero
+/* W[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), codes 0..15, zero
+ * points 0..31 (the low five bits of their bytes; 16 where a format holds zero - 1); without zero
  * points zero is 8. A stack of `count` matrices [n_out][n_in] in the layout the kernels read,
  * made by evamx_w4_pack; all pointers device, 16-byte aligned. */
 enum { EVAMX_W4_MAX_DIM = 1 << 18 };
@@ -96,8 +97,8 @@ int evamx_w4_stored_group(int group);
 size_t evamx_w4_code_bytes(int count, int n_out, int n_in);
 size_t evamx_w4_group_count(int count, int n_out, int n_in, int group);
 /* Lay a stack out: codes uint8 [count][n_out][ceil(n_in / 2)] (the lower half of a byte is the even
- * k), scales [count][n_out][ceil(n_in / group)] of w->scale_dtype, zeros likewise uint8 (codes
- * 0..15) or NULL, written to the buffers of w. */
+ * k), scales [count][n_out][ceil(n_in / group)] of w->scale_dtype, zeros likewise uint8
+ * (0..31) or NULL, written to the buffers of w. */
 int evamx_w4_pack(const uint8_t* codes, const void* scales, const uint8_t* zeros, int group,
                   const evamx_w4_weight* w, evamx_stream_t stream);
 /* fp32 W[count][n_out][n_in] of a packed stack. */
