@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import MoeArgs, MoeShape, W4Desc, W4MoeArgs, check, lib, ptr, stream_handle
@@ -158,10 +159,15 @@ def _row_stride(t: torch.Tensor, name: str, dtype=None) -> int:
 
 
 def _no_grad(name, *tensors):
+    """Refuses tensors whose derivatives autograd would expect ``name`` to carry on, backward or forward."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} has no backward: call it under torch.no_grad() or with detached tensors")
+    if forward_ad._current_level >= 0 and not torch.is_inference_mode_enabled():      # no_grad does not switch forward mode off
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivative: call it with the primal of {forward_ad.__name__}.unpack_dual")
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
