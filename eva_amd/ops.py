@@ -328,6 +328,9 @@ def balance_loss_grad(grad_loss: torch.Tensor, logits: torch.Tensor, counts: tor
     return _balance_backward(grad_loss, logits, counts, tokens, topk, score_fn, stride, n, seq_starts, token_mask)
 
 
+_NO_CAPTURE = "balance_loss is not captured with a backward pass: call balance_stats and balance_loss_grad"
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, sel, score_fn, seq_starts, token_mask):
@@ -343,8 +346,10 @@ class _BalanceLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _):
         if grad_loss is None:
             return None, None, None, None, None
-        if torch.is_grad_enabled():                      # create_graph=True
+        if torch.is_grad_enabled():                      # create_graph=True: a gradient without a graph would pass for a constant
             raise RuntimeError("balance_loss is differentiable once")
+        if torch.cuda.is_current_stream_capturing():     # of a forward pass that was not
+            raise RuntimeError(_NO_CAPTURE)
         logits, counts, tokens, seq_starts, token_mask = ctx.saved_tensors
         return _balance_backward(grad_loss.contiguous(), logits, counts, tokens, *ctx.args, seq_starts, token_mask), None, None, None, None
 
@@ -363,10 +368,11 @@ def balance_loss(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "si
     Picks outside ``[0, E)`` are not counted.
 
     The backward pass is not for a graph capture (autograd's own streams and accumulators are not): there call
-    ``balance_stats`` and ``balance_loss_grad``."""
+    ``balance_stats`` and ``balance_loss_grad``. It is refused there and with ``create_graph=True``: there is no
+    second derivative."""
     if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad and logits.is_cuda and \
             torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("balance_loss is not captured with a backward pass: call balance_stats and balance_loss_grad")
+        raise RuntimeError(_NO_CAPTURE)
     return _BalanceLoss.apply(logits, sel, score_fn, seq_starts, token_mask)
 
 
