@@ -361,8 +361,9 @@ def balance_loss(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "si
 
     With ``p = score / score.sum(1)``, ``n`` tokens and ``c_e`` picks of expert e in a sequence, the loss is
     ``sum_e (E c_e / (topk n)) (sum_t p_te / n)``: 1 where picks and shares are even, larger where the experts
-    that are picked often also have large scores. It is differentiable in the logits; the counts (which serve
-    a selection bias as well as the loss) are constants. ``seq_starts`` int32 ``[S + 1]`` ascending: sequence
+    that are picked often also have large scores. It is differentiable in the logits, for a program whose own
+    product makes them (``router_logits`` and ``route`` have no backward pass: behind them ``balance_stats`` gives
+    the same numbers); the counts (which serve a selection bias as well as the loss) are constants. ``seq_starts`` int32 ``[S + 1]`` ascending: sequence
     s is rows ``seq_starts[s]`` to ``seq_starts[s + 1]``, and rows of none count nowhere; without it all rows
     are one sequence. ``token_mask`` bool ``[T]``: rows that count. A sequence without such rows has loss 0.
     Picks outside ``[0, E)`` are not counted.
