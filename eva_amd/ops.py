@@ -652,8 +652,8 @@ def w4_moe_forward(x: torch.Tensor, gate: W4Weight, up: W4Weight, down: W4Weight
     ``[rows, hidden]``, ``sel`` int64 and ``weights`` fp32 ``[rows, topk]`` (``route`` / ``route_topk``), the
     result of x's dtype. ``gate`` and ``up`` are stacks ``[inter, hidden]``, ``down`` ``[hidden, inter]``: the
     experts ``first_expert`` and up, then ``n_shared`` shared experts that every token takes with weight 1.
-    Slots of other experts add nothing (expert parallelism). ``limit`` clamps as in ``moe_forward``. ``out``
-    must not overlap ``x``. At most 65536 slots, 2^31 padded values of ``x`` and 2^30 hidden activations a
+    Slots of other experts add nothing (expert parallelism). ``limit`` clamps as in ``moe_forward``, but a
+    NaN stays NaN (a routed expert there takes it to the limit). ``out`` must not overlap ``x``. At most 65536 slots, 2^31 padded values of ``x`` and 2^30 hidden activations a
     call (``W4Experts`` splits larger ones)."""
     x_stride = _row_stride(x, "x")
     if x.dtype not in _DTYPES:

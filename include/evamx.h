@@ -108,7 +108,8 @@ size_t evamx_w4_linear_workspace_bytes(int rows, int n_in);
 /* y[r][n] = sum_k x[r][k] W[n][k] + bias[n] for one matrix, summed in fp32 and rounded once. x and y
  * fp16 or bf16 (x_dtype; the bias too), rows of x_stride and y_stride elements of any alignment;
  * bias [n_out] or NULL; rows in 1..65536. A row's values are scaled by a power of two into fp16's
- * range for the products, so bf16 values keep their bits down to 2^-28 of the row's largest. */
+ * range for the products, so bf16 values keep their bits down to 2^-28 of the row's largest; the sums
+ * are fp32's before that is undone, so group scales of 2^90 and more can overflow them. */
 int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int rows, const evamx_w4_weight* w,
                     const void* bias, void* y, int64_t y_stride, void* workspace, size_t workspace_bytes,
                     evamx_stream_t stream);
