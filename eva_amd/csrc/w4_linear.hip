@@ -184,6 +184,8 @@ __global__ __launch_bounds__(256, 2) void w4_linear_gemm_kernel(W4LinearParams p
     else w4_linear_gemm<SG, ZERO, 1>(p, m, r0, have, nt0, lds);
 }
 
+constexpr int W4_CUS = 256;
+
 template <int NB, int MB>
 static void w4_launch_linear(const W4LinearParams& p, const W4Mat& m, const evamx_w4_weight& w, int parts, hipStream_t s)
 {
@@ -239,11 +241,13 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
         p.xh = xh;
         p.row_scale = rs;
     }
-    const long row_tiles = w4_ceil(rows, W4G_ROWS), col_tiles = w4_ceil(m.n_out, W4G_COLS), wide = (long)w4_ceil(m.nt, 4) * w4_ceil(rows, 32);
+    const long row_tiles = w4_ceil(rows, W4G_ROWS), col_tiles = w4_ceil(m.n_out, W4G_COLS);
     if (rows <= 16) {
-        // 16 columns a workgroup where 32 would leave CUs without one (5001 -> 2303 at 13 rows: 12.3 us against 14.9 with 32),
-        // else 32 on the same rows (7168 -> 18432 at 5 rows: 21.8 us against 25.8 with 16)
-        if (m.nt < 1024) w4_launch_linear<1, 1>(p, m, *w, parts, s);
+        // 16 columns a workgroup while that gives a CU at most one (7168 -> 4096 at 5 and 16 rows: 10.9 and 14.5 us against 11.9 and
+        // 15.2 with 32), else 32 on the same rows (7168 -> 5120: 12.0 and 15.3 against 14.4 and 22.3 with 16; 7168 -> 8192, whose
+        // k-tiles are cut into four parts instead of eight: 16.4 and 18.0 against 14.5 and 21.3; 7168 -> 18432: 21.3 and 31 against
+        // 26 and 42)
+        if (m.nt <= W4_CUS) w4_launch_linear<1, 1>(p, m, *w, parts, s);
         else w4_launch_linear<2, 1>(p, m, *w, parts, s);
     } else if (row_tiles * col_tiles * m.kt >= 104l * m.kt + 600) {
         // The 64 x 256 tiles take about 1.5 us a k-tile and 5 for all of a round, the kernel below 0.014 us a tile and k-tile
@@ -252,9 +256,9 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
             w4_linear_gemm_kernel<decltype(sg)::value, decltype(zero)::value>
                 <<<8 * w4_ceil((int)(row_tiles * col_tiles), 8), 256, 0, s>>>(p, m, (int)row_tiles, (int)col_tiles);
         });
-    } else if (wide < 160) {
-        // 32 columns by 32 rows where 64 columns would leave CUs without a workgroup (7168 -> 2048 at 17 rows: 12.4 us against
-        // 17.7, at 128: 18.6 against 20.4), else 64 (at 200: 34 against 22)
+    } else if ((long)w4_ceil(m.nt, 2) * w4_ceil(rows, 32) <= W4_CUS) {
+        // 32 columns by 32 rows while that gives a CU at most one workgroup (7168 -> 2048 at 17 rows: 12.6 us against 18.4, at 128:
+        // 18.6 against 21.1), else 64 (7168 -> 2112 at 128: 33.4 against 21.4; 7168 -> 2048 at 200: 33.6 against 21.2)
         w4_launch_linear<2, 2>(p, m, *w, m.kt >= 8 ? 8 : parts, s);
     } else {
         w4_launch_linear<4, 2>(p, m, *w, parts < 4 ? parts : 4, s);
