@@ -185,9 +185,9 @@ __host__ __device__ inline int w4_part_begin(int kt, int parts, int i) { return 
 inline int w4_parts(int kt, int nt) { return kt >= 32 && nt < 512 ? 8 : kt >= 8 ? 4 : kt >= 2 ? 2 : 1; }
 constexpr int W4_MAX_PARTS = 8;
 
-// acc[b][mb] += rows times the k-tiles [k0, k1) of NB streams, RING tiles of each in flight. `rows(kt, x, lo)` gives the lane's activations of a tile at
-// the time its products are due; `ahead(d, kt)` is called with each request for tile kt into place d of the ring,
-// `begin()` once the first are under way.
+// acc[b][mb] += rows times the k-tiles [k0, k1) of NB streams, RING tiles of each in flight. `rows(d, kt, x, lo)` gives the lane's
+// activations of a tile at the time its products are due; `ahead(d, kt)` is called with each request for tile kt into place d of
+// the ring, `begin()` once the first are under way.
 template <int RING, int SG, bool ZERO, int NB, int MB, int NR, bool HL, class Ahead, class Rows, class Begin>
 __device__ __forceinline__ void w4_run(w4_f32x4 (&acc)[NB][MB], const W4Stream (&st)[NB], int k0, int k1, int bf16, Ahead&& ahead, Rows&& rows,
                                        Begin&& begin)
@@ -222,32 +222,32 @@ __device__ __forceinline__ void w4_run(w4_f32x4 (&acc)[NB][MB], const W4Stream (
 // Activations in global memory, made ready by w4_launch_rows: requested with the tiles they multiply (from a descriptor, as
 // the weights: plain loads would be sunk to their use). at[mb]: byte offset of the lane's row at its k offset 8 (lane >> 4);
 // a low half lies lo_off bytes behind. Offsets are below 2^32 (the entry points see to it).
-template <int RING, int MB, bool HL>
+template <int MB, bool HL>
 struct W4GlobalRows {
     __amdgpu_buffer_rsrc_t src;
     uint32_t at[MB], lo_off;
-    w4_half8 buf[RING][MB][4], low[HL ? RING : 1][MB][4];
+    w4_half8 buf[MB][4], low[HL ? MB : 1][4];
 
-    __device__ __forceinline__ void request(int d, int kt)
+    __device__ __forceinline__ void request(int kt)
     {
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t o = at[mb] + (uint32_t)kt * (W4_TILE_K * 2) + 64 * j;
-                buf[d][mb][j] = __builtin_bit_cast(w4_half8, __builtin_amdgcn_raw_buffer_load_b128(src, o, 0, 0));
-                if constexpr (HL) low[d][mb][j] = __builtin_bit_cast(w4_half8, __builtin_amdgcn_raw_buffer_load_b128(src, o + lo_off, 0, 0));
+                buf[mb][j] = __builtin_bit_cast(w4_half8, __builtin_amdgcn_raw_buffer_load_b128(src, o, 0, 0));
+                if constexpr (HL) low[mb][j] = __builtin_bit_cast(w4_half8, __builtin_amdgcn_raw_buffer_load_b128(src, o + lo_off, 0, 0));
             }
     }
 
-    __device__ __forceinline__ void take(int d, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) const
+    __device__ __forceinline__ void take(w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) const
     {
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                x[mb][j] = buf[d][mb][j];
-                if constexpr (HL) lo[mb][j] = low[d][mb][j];
+                x[mb][j] = buf[mb][j];
+                if constexpr (HL) lo[mb][j] = low[mb][j];
             }
     }
 };

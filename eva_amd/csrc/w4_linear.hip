@@ -28,44 +28,38 @@ __device__ __forceinline__ void w4_linear_store(const W4LinearParams& p, const W
     w4_store(p.y, (size_t)row * p.y_stride + n, v, p.bf16);
 }
 
-// Up to four rows: one launch. A workgroup takes 16 NB columns, a wave one part of the k-tiles; the rows are made ready in LDS
+// Up to four rows: one launch. A workgroup takes 16 columns, a wave one part of the k-tiles; the rows are made ready in LDS
 // while the first tiles are on their way, and each stands in four of the 16 rows of a matrix operand, so that one of the four
 // accumulators of a lane is all there is to scale. 2048 -> 7168 at one row: 4.9 us in a graph, of which an empty launch is 1.6;
 // the rest is the loads' one round trip and the join.
-template <int SG, bool ZERO, int NB>
+template <int SG, bool ZERO>
 __global__ __launch_bounds__(512) void w4_linear_few_kernel(W4LinearParams p, W4Mat m)
 {
     extern __shared__ w4_half xs[];
     __shared__ uint32_t top[W4_MAX_PARTS][4];
-    __shared__ float scale[4], part[W4_MAX_PARTS][NB][64];
+    __shared__ float scale[4], part[W4_MAX_PARTS][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, parts = blockDim.x >> 6, ld = m.kt * W4_TILE_K + W4_STAGE_PAD;
     const int k0 = w4_part_begin(m.kt, parts, wave), k1 = w4_part_begin(m.kt, parts, wave + 1);
     W4Stage stage{(const uint16_t*)p.x, p.x_stride, p.rows, m.n_in, m.kt, p.bf16, p.aligned};
     stage.load();
-    W4Stream st[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int nt = NB * blockIdx.x + b;
-        st[b] = w4_stream<SG, ZERO>(m, 0, nt < m.nt ? nt : m.nt - 1, k1);
-    }
+    const W4Stream st[1] = {w4_stream<SG, ZERO>(m, 0, blockIdx.x, k1)};
     const int row = (lane & 15) >> 2;
     const w4_half* a = xs + (row < p.rows ? row : p.rows - 1) * ld + 8 * (lane >> 4);
-    w4_f32x4 acc[NB][1] = {};
-    w4_run<2, SG, ZERO, NB, 1, 1, false>(
+    w4_f32x4 acc[1][1] = {};
+    w4_run<2, SG, ZERO, 1, 1, 1, false>(
         acc, st, k0, k1, m.bf16, [](int, int) {},
         [&](int, int kt, w4_half8 (&x)[1][4], w4_half8 (&)[1][4]) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[0][j] = *(const w4_half8*)(a + kt * W4_TILE_K + 32 * j);
         },
         [&] { stage.finish(xs, top, scale); });
-#pragma unroll
-    for (int b = 0; b < NB; ++b) part[wave][b][lane] = acc[b][0][0];
+    part[wave][lane] = acc[0][0][0];
     __syncthreads();
-    if (threadIdx.x >= 64 * NB) return;
-    const int r = lane >> 4, n = 16 * (NB * blockIdx.x + wave) + (lane & 15);
+    if (wave) return;
+    const int r = lane >> 4, n = 16 * blockIdx.x + (lane & 15);
     if (r >= p.rows || n >= m.n_out) return;
     float v = 0;
-    for (int w = 0; w < parts; ++w) v += part[w][wave][lane];
+    for (int w = 0; w < parts; ++w) v += part[w][lane];
     w4_linear_store(p, m, r, n, v, scale[r]);
 }
 
@@ -75,7 +69,6 @@ __global__ __launch_bounds__(512) void w4_linear_few_kernel(W4LinearParams p, W4
 template <int SG, bool ZERO, int NB, int MB>
 __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat m)
 {
-    constexpr int RING = 1;
     extern __shared__ w4_f32x4 part[];                       // [parts][NB][MB][64]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, parts = blockDim.x >> 6;
     const int k0 = w4_part_begin(m.kt, parts, wave), k1 = w4_part_begin(m.kt, parts, wave + 1), r0 = 16 * MB * blockIdx.y;
@@ -85,7 +78,7 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat 
         const int nt = NB * blockIdx.x + b;
         st[b] = w4_stream<SG, ZERO>(m, 0, nt < m.nt ? nt : m.nt - 1, k1);
     }
-    W4GlobalRows<RING, MB, false> rows;
+    W4GlobalRows<MB, false> rows;
     rows.src = w4_rsrc(p.xh + (size_t)r0 * m.kt * W4_TILE_K, (uint32_t)(p.rows - r0 < 16 * MB ? p.rows - r0 : 16 * MB) * m.kt * (W4_TILE_K * 2));
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
@@ -93,9 +86,9 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat 
         rows.at[mb] = (uint32_t)(r0 + r < p.rows ? r : p.rows - 1 - r0) * m.kt * (W4_TILE_K * 2) + 16 * (lane >> 4);
     }
     w4_f32x4 acc[NB][MB] = {};
-    w4_run<RING, SG, ZERO, NB, MB, 4, false>(
-        acc, st, k0, k1, m.bf16, [&](int d, int kt) { rows.request(d, kt); },
-        [&](int d, int, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) { rows.take(d, x, lo); }, [] {});
+    w4_run<1, SG, ZERO, NB, MB, 4, false>(
+        acc, st, k0, k1, m.bf16, [&](int, int kt) { rows.request(kt); },
+        [&](int, int, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) { rows.take(x, lo); }, [] {});
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -228,7 +221,7 @@ extern "C" int evamx_w4_linear(const void* x, int x_dtype, int64_t x_stride, int
     p.bias = bias; p.y = y; p.y_stride = (size_t)y_stride; p.xh = nullptr; p.row_scale = nullptr;
     if (w4_stage_fits(rows, m.kt, parts)) {
         w4_dispatch(*w, [&](auto sg, auto zero) {
-            w4_linear_few_kernel<decltype(sg)::value, decltype(zero)::value, 1><<<m.nt, 64 * parts, w4_stage_bytes(rows, m.kt), s>>>(p, m);
+            w4_linear_few_kernel<decltype(sg)::value, decltype(zero)::value><<<m.nt, 64 * parts, w4_stage_bytes(rows, m.kt), s>>>(p, m);
         });
         return launched("w4_linear");
     }

@@ -250,11 +250,12 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_few_kernel(W4MoePara
     for (int r0 = 4; r0 < rows; r0 += 4) block(r0, [] {});          // only where a token repeats an expert
 }
 
-// 16 CT columns of gate and up a column group, by a unit of up to 16 MB rows. 16 tokens of that layer, 83 experts: 235 us, 5.3 TB/s.
-template <int RING, int SG, bool ZERO, int CT, int MB>
+// 16 W4_GU_CT columns of gate and up a column group, by a unit of up to 16 rows. 16 tokens of that layer, 83 experts: 235 us, 5.3 TB/s.
+template <int SG, bool ZERO>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_kernel(W4MoeParams p, W4Mat gate, W4Mat up, int parts)
 {
-    __shared__ w4_f32x4 part[W4_WAVES][2 * CT][MB][64];
+    constexpr int CT = W4_GU_CT;
+    __shared__ w4_f32x4 part[W4_WAVES][2 * CT][64];
     if ((int)blockIdx.y >= *p.units_in_use) return;
     const W4Unit u = p.units[blockIdx.y];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = W4_WAVES / parts;
@@ -267,29 +268,24 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_kernel(W4MoeParams p
         st[2 * c] = w4_stream<SG, ZERO>(gate, u.expert, t, k1);
         st[2 * c + 1] = w4_stream<SG, ZERO>(up, u.expert, t, k1);
     }
-    W4GlobalRows<RING, MB, false> rows;
+    W4GlobalRows<1, false> rows;
     rows.src = w4_rsrc(p.x, (uint32_t)p.rows * gate.kt * (W4_TILE_K * 2));
+    const int mine = lane & 15, token = w4_token(p, p.order[u.r0 + (mine < u.rows ? mine : u.rows - 1)]);
+    rows.at[0] = (uint32_t)token * gate.kt * (W4_TILE_K * 2) + 16 * (lane >> 4);
+    w4_f32x4 acc[2 * CT][1] = {};
+    w4_run<1, SG, ZERO, 2 * CT, 1, 4, false>(
+        acc, st, k0, k1, gate.bf16, [&](int, int kt) { rows.request(kt); },
+        [&](int, int, w4_half8 (&x)[1][4], w4_half8 (&lo)[1][4]) { rows.take(x, lo); }, [] {});
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-        const int r = 16 * mb + (lane & 15), t = w4_token(p, p.order[u.r0 + (r < u.rows ? r : u.rows - 1)]);
-        rows.at[mb] = (uint32_t)t * gate.kt * (W4_TILE_K * 2) + 16 * (lane >> 4);
-    }
-    w4_f32x4 acc[2 * CT][MB] = {};
-    w4_run<RING, SG, ZERO, 2 * CT, MB, 4, false>(
-        acc, st, k0, k1, gate.bf16, [&](int d, int kt) { rows.request(d, kt); },
-        [&](int d, int, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) { rows.take(d, x, lo); }, [] {});
-#pragma unroll
-    for (int b = 0; b < 2 * CT; ++b)
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) part[wave][b][mb][lane] = acc[b][mb];
+    for (int b = 0; b < 2 * CT; ++b) part[wave][b][lane] = acc[b][0];
     __syncthreads();
-    for (int t = q; t < CT * MB * 4; t += parts) {           // the parts share the values of their column group
-        const int i = t & 3, mb = (t >> 2) % MB, c = (t >> 2) / MB, r = 16 * mb + 4 * (lane >> 4) + i, n = 16 * (nt + c) + (lane & 15);
+    for (int t = q; t < CT * 4; t += parts) {                // the parts share the values of their column group
+        const int i = t & 3, c = t >> 2, r = 4 * (lane >> 4) + i, n = 16 * (nt + c) + (lane & 15);
         if (r >= u.rows || n >= p.inter) continue;
         float g = 0, v = 0;
         for (int w = wave - q; w < wave - q + parts; ++w) {
-            g += part[w][2 * c][mb][lane][i];
-            v += part[w][2 * c + 1][mb][lane][i];
+            g += part[w][2 * c][lane][i];
+            v += part[w][2 * c + 1][lane][i];
         }
         const int s = p.order[u.r0 + r];
         const float f = p.xs ? p.xs[w4_token(p, s)] : 1.0f;
@@ -311,12 +307,13 @@ __global__ __launch_bounds__(256) void w4_hidden_kernel(W4MoeParams p, int n_pad
     if (threadIdx.x == 0) p.hs[s] = f;
 }
 
-// 16 NB columns of the output a column group, by a unit of up to 16 MB rows. 16 tokens as above: 146 us, 4.3 TB/s (127 with one half
+// 16 W4_DOWN_NB columns of the output a column group, by a unit of up to 16 rows. 16 tokens as above: 146 us, 4.3 TB/s (127 with one half
 // a value).
-template <int RING, int SG, bool ZERO, int NB, int MB>
+template <int SG, bool ZERO>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W4Mat down, int parts)
 {
-    __shared__ w4_f32x4 part[W4_WAVES][NB][MB][64];
+    constexpr int NB = W4_DOWN_NB;
+    __shared__ w4_f32x4 part[W4_WAVES][NB][64];
     if (p.units_in_use && (int)blockIdx.y >= *p.units_in_use) return;
     const W4Unit u = p.units[blockIdx.y];
     if (u.expert < 0) return;
@@ -326,31 +323,25 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W
     W4Stream st[NB];
 #pragma unroll
     for (int c = 0; c < NB; ++c) st[c] = w4_stream<SG, ZERO>(down, u.expert, nt + c < down.nt ? nt + c : down.nt - 1, k1);
-    W4GlobalRows<RING, MB, true> rows;
+    W4GlobalRows<1, true> rows;
     const uint32_t ld = 4 * n_pad;
     rows.src = w4_rsrc(p.hh, (uint32_t)p.slots * ld);
     rows.lo_off = 2 * n_pad;
-    for (int r0 = 0; r0 < u.rows; r0 += 16 * MB) {           // once, but for few tokens that repeat an expert
+    for (int r0 = 0; r0 < u.rows; r0 += W4_UNIT_ROWS) {           // once, but for few tokens that repeat an expert
+        const int mine = r0 + (lane & 15);
+        rows.at[0] = (uint32_t)p.order[u.r0 + (mine < u.rows ? mine : u.rows - 1)] * ld + 16 * (lane >> 4);
+        w4_f32x4 acc[NB][1] = {};
+        w4_run<1, SG, ZERO, NB, 1, 4, true>(
+            acc, st, k0, k1, down.bf16, [&](int, int kt) { rows.request(kt); },
+            [&](int, int, w4_half8 (&x)[1][4], w4_half8 (&lo)[1][4]) { rows.take(x, lo); }, [] {});
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-            const int r = r0 + 16 * mb + (lane & 15), s = p.order[u.r0 + (r < u.rows ? r : u.rows - 1)];
-            rows.at[mb] = (uint32_t)s * ld + 16 * (lane >> 4);
-        }
-        w4_f32x4 acc[NB][MB] = {};
-        w4_run<RING, SG, ZERO, NB, MB, 4, true>(
-            acc, st, k0, k1, down.bf16, [&](int d, int kt) { rows.request(d, kt); },
-            [&](int d, int, w4_half8 (&x)[MB][4], w4_half8 (&lo)[MB][4]) { rows.take(d, x, lo); }, [] {});
-#pragma unroll
-        for (int c = 0; c < NB; ++c)
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb) part[wave][c][mb][lane] = acc[c][mb];
+        for (int c = 0; c < NB; ++c) part[wave][c][lane] = acc[c][0];
         __syncthreads();
-        for (int t = q; t < NB * MB * 4; t += parts) {
-            const int i = t & 3, mb = (t >> 2) % MB, b = (t >> 2) / MB;
-            const int r = r0 + 16 * mb + 4 * (lane >> 4) + i, n = 16 * (nt + b) + (lane & 15);
+        for (int t = q; t < NB * 4; t += parts) {
+            const int i = t & 3, b = t >> 2, r = r0 + 4 * (lane >> 4) + i, n = 16 * (nt + b) + (lane & 15);
             if (r >= u.rows || n >= p.hidden) continue;
             float v = 0;
-            for (int w = wave - q; w < wave - q + parts; ++w) v += part[w][b][mb][lane][i];
+            for (int w = wave - q; w < wave - q + parts; ++w) v += part[w][b][lane][i];
             const int s = p.order[u.r0 + r];
             p.y[(size_t)s * p.hidden + n] = v * p.hs[s];
         }
@@ -692,7 +683,7 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
             constexpr int SG = decltype(sg)::value;
             constexpr bool ZERO = decltype(zero)::value;
             if (bigs) w4_gate_up_gemm_kernel<SG, ZERO><<<dim3(w4_ceil(gm.nt, W4G_WAVES * W4G_NB / 2), bigs), 64 * W4G_WAVES, 0, s>>>(p, gm, um);
-            w4_gate_up_kernel<1, SG, ZERO, W4_GU_CT, 1>
+            w4_gate_up_kernel<SG, ZERO>
                 <<<dim3(w4_ceil(gm.nt, W4_GU_CT * (W4_WAVES / gp)), units), 64 * W4_WAVES, 0, s>>>(p, gm, um, gp);
         });
     }
@@ -702,7 +693,7 @@ extern "C" int evamx_w4_moe_forward(const evamx_w4_moe_args* a, evamx_stream_t s
         constexpr bool ZERO = decltype(zero)::value;
         const dim3 grid(w4_ceil(dm.nt, W4_DOWN_NB * (W4_WAVES / dp)), units), big_grid(w4_ceil(dm.nt, W4G_WAVES * W4G_NB), bigs);
         if (bigs) w4_down_gemm_kernel<SG, ZERO><<<big_grid, 64 * W4G_WAVES, 0, s>>>(p, dm);
-        w4_down_kernel<1, SG, ZERO, W4_DOWN_NB, 1><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
+        w4_down_kernel<SG, ZERO><<<grid, 64 * W4_WAVES, 0, s>>>(p, dm, dp);
     });
     w4_combine_kernel<<<p.rows * w4_ceil(p.hidden, 1024), 256, 0, s>>>(p);
     return launched("w4_moe_forward");
