@@ -64,8 +64,8 @@ __global__ __launch_bounds__(512) void w4_linear_few_kernel(W4LinearParams p, W4
 }
 
 // 16 MB rows by 16 NB columns a workgroup, a wave one part of the k-tiles; the rows come ready from memory (L2) with the tiles.
-// 7168 -> 18432 with groups of 64 and zero points at 5 rows: 17.4 us, 4.2 TB/s; 7168 -> 2048 at 200 rows: 21.5 us, 273 TFLOP/s,
-// bound by the rows' operands, 8 KiB a k-tile and wave beside 4 of codes.
+// 7168 -> 18432 with groups of 64 and zero points at 5 rows: 19.6 us, 3.7 TB/s; 7168 -> 2048 at 200 rows: 21.5 us, 273 TFLOP/s,
+// bound by the rows' operands, 8 KiB a k-tile and wave beside 4 of codes, which no wave shares with another.
 template <int SG, bool ZERO, int NB, int MB>
 __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat m)
 {
@@ -106,7 +106,8 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4LinearParams p, W4Mat 
 
 // Long calls: 64 rows by 256 columns a workgroup (w4_gemm.hpp). Consecutive workgroups go to the eight XCDs in turn, so each XCD
 // takes a contiguous run of tiles, eight row tiles by all columns at a time: its rows' tiles stay in its L2 while it passes over
-// the columns. 8192 rows of 2048 -> 7168: about 225 us, 1070 TFLOP/s, and 13 to make the bf16 rows ready.
+// the columns. 8192 rows of 2048 -> 7168: about 225 us, 1070 TFLOP/s, in a graph (242 and more in a trace), and 13 to make the bf16
+// rows ready.
 template <int SG, bool ZERO, int MB>
 __device__ __forceinline__ void w4_linear_gemm(const W4LinearParams& p, const W4Mat& m, int r0, int have, int nt0, char* lds)
 {

@@ -166,8 +166,8 @@ inline int w4_moe_parts(int kt) { return kt >= 48 ? 4 : kt >= 24 ? 2 : 1; }
 // registers of waves that hide more (with two tiles in flight a stream instead of one: 374 us, with four 442).
 constexpr int W4_GU_CT = 2, W4_DOWN_NB = 4;
 
-// Up to W4_FEW_ROWS tokens, without a launch before it: 16 columns of gate and up of one expert a column group, the tokens' rows
-// in LDS (w4_linear_few_kernel's scheme). Unit u is the expert of slot u, if no slot before it has that expert; with one token
+// Up to W4_FEW_ROWS tokens whose rows a workgroup can stage (w4_stage_fits: 2 tokens of 7168 features), without a launch before it:
+// 16 columns of gate and up of one expert a column group, the rows in LDS (w4_linear_few_kernel's scheme). Unit u is the expert of slot u, if no slot before it has that expert; with one token
 // every slot is a unit. One token of a 7168 x 2048 layer with eight experts and a shared one: 28.6 us for 136 MB, 4.8 TB/s; reading
 // as much with no decode takes 26.
 constexpr int W4_FEW_ROWS = 4, W4_FEW_SLOTS = W4_FEW_ROWS * 64;
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_few_kernel(W4MoePara
     for (int r0 = 4; r0 < rows; r0 += 4) block(r0, [] {});          // only where a token repeats an expert
 }
 
-// 16 W4_GU_CT columns of gate and up a column group, by a unit of up to 16 rows. 16 tokens of that layer, 83 experts: 235 us, 5.3 TB/s.
+// 16 W4_GU_CT columns of gate and up a column group, by a unit of up to 16 rows. 16 tokens of that layer, 82 experts: 237 us, 5.2 TB/s.
 template <int SG, bool ZERO>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_kernel(W4MoeParams p, W4Mat gate, W4Mat up, int parts)
 {

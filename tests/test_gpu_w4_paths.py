@@ -152,3 +152,14 @@ def test_a_linear_of_more_than_4_gib(dev):
     some = _some(rows, 2 ** 31 // n_in).to(dev)
     check_linear(y[some], x[some], m.w)
     assert y.isfinite().all()
+
+
+@pytest.mark.parametrize("inter", [3968, 3970])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_one_token_at_the_most_lds(dev, inter, dtype):
+    """Eight slots' hidden activations that just fit one workgroup's LDS, and that just do not."""
+    g = _gen(inter)
+    ex = Experts(g, 200, inter, 9, 64, dtype=dtype)
+    x = torch.randn(1, 200, generator=g).to(dtype)
+    sel, w = _routes(g, 1, 9, 8)
+    _check(dev, ex, x, sel, w, limit=5.0)
