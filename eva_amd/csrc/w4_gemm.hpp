@@ -6,8 +6,8 @@
 // row r lies at c ^ (r & 15)), so that the 16 rows of an operand are read from 16 different banks' quads. The direct load
 // writes its lanes' pieces one after the other, so the swap is made in the addresses it reads.
 //
-// Per k-tile and wave: 64 matrix instructions (1024 cycles; 128 for rows of two halves), 144 to decode, 64 to add the groups' sums times their scales (256
-// with groups of 32), 16 reads of 1 KiB from LDS (32).
+// Per k-tile and wave: 64 matrix instructions (1024 cycles; 128 for rows of two halves), 144 to decode, 64 to add the groups' sums
+// times their scales (256 with groups of 32), 16 reads of 1 KiB from LDS (32).
 #pragma once
 #include "w4.hpp"
 

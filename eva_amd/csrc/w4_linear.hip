@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256, 2) void w4_linear_gemm_kernel(W4LinearParams p
     else w4_linear_gemm<SG, ZERO, 1>(p, m, r0, have, nt0, lds);
 }
 
-constexpr int W4_CUS = 256;
+constexpr int W4_CUS = 256;                                  // of an MI355X
 
 template <int NB, int MB>
 static void w4_launch_linear(const W4LinearParams& p, const W4Mat& m, const evamx_w4_weight& w, int parts, hipStream_t s)

@@ -167,9 +167,9 @@ inline int w4_moe_parts(int kt) { return kt >= 48 ? 4 : kt >= 24 ? 2 : 1; }
 constexpr int W4_GU_CT = 2, W4_DOWN_NB = 4;
 
 // Up to W4_FEW_ROWS tokens whose rows a workgroup can stage (w4_stage_fits: 2 tokens of 7168 features), without a launch before it:
-// 16 columns of gate and up of one expert a column group, the rows in LDS (w4_linear_few_kernel's scheme). Unit u is the expert of slot u, if no slot before it has that expert; with one token
-// every slot is a unit. One token of a 7168 x 2048 layer with eight experts and a shared one: 28.6 us for 136 MB, 4.8 TB/s; reading
-// as much with no decode takes 26.
+// 16 columns of gate and up of one expert a column group, the rows in LDS (w4_linear_few_kernel's scheme). Unit u is the expert of
+// slot u, if no slot before it has that expert; with one token every slot is a unit. One token of a 7168 x 2048 layer with eight
+// experts and a shared one: 28.6 us for 136 MB, 4.8 TB/s; reading as much with no decode takes 26.
 constexpr int W4_FEW_ROWS = 4, W4_FEW_SLOTS = W4_FEW_ROWS * 64;
 
 template <int SG, bool ZERO>
@@ -250,7 +250,8 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_few_kernel(W4MoePara
     for (int r0 = 4; r0 < rows; r0 += 4) block(r0, [] {});          // only where a token repeats an expert
 }
 
-// 16 W4_GU_CT columns of gate and up a column group, by a unit of up to 16 rows. 16 tokens of that layer, 82 experts: 237 us, 5.2 TB/s.
+// 16 W4_GU_CT columns of gate and up a column group, by a unit of up to 16 rows. 16 tokens of that layer, 82 experts: 237 us,
+// 5.2 TB/s.
 template <int SG, bool ZERO>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_gate_up_kernel(W4MoeParams p, W4Mat gate, W4Mat up, int parts)
 {
@@ -307,8 +308,8 @@ __global__ __launch_bounds__(256) void w4_hidden_kernel(W4MoeParams p, int n_pad
     if (threadIdx.x == 0) p.hs[s] = f;
 }
 
-// 16 W4_DOWN_NB columns of the output a column group, by a unit of up to 16 rows. 16 tokens as above: 146 us, 4.3 TB/s (127 with one half
-// a value).
+// 16 W4_DOWN_NB columns of the output a column group, by a unit of up to 16 rows. 16 tokens as above: 146 us, 4.3 TB/s (127 with
+// one half a value).
 template <int SG, bool ZERO>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W4Mat down, int parts)
 {
@@ -327,7 +328,7 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_down_kernel(W4MoeParams p, W
     const uint32_t ld = 4 * n_pad;
     rows.src = w4_rsrc(p.hh, (uint32_t)p.slots * ld);
     rows.lo_off = 2 * n_pad;
-    for (int r0 = 0; r0 < u.rows; r0 += W4_UNIT_ROWS) {           // once, but for few tokens that repeat an expert
+    for (int r0 = 0; r0 < u.rows; r0 += W4_UNIT_ROWS) {      // once, but for few tokens that repeat an expert
         const int mine = r0 + (lane & 15);
         rows.at[0] = (uint32_t)p.order[u.r0 + (mine < u.rows ? mine : u.rows - 1)] * ld + 16 * (lane >> 4);
         w4_f32x4 acc[NB][1] = {};
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(64 * W4G_WAVES, 2) void w4_down_gemm_kernel(W4MoePa
 // other; the slots' sums meet in LDS, so that no launch follows. The layer above: 25.0 us for 68 MB, 2.7 TB/s; a wave's 32 KiB of
 // codes are too few to make up for its start, and every value is read from LDS as two halves (20.3 with one; then 24.6 with 16
 // columns a wave). Calls whose slots' activations do not fit W4_ONE_LDS take the general path: at nine slots of fp16 with groups of
-// 64 and zero points 74.1 us, here 60.2.
+// 64 and zero points 74.1 us, here 60.2; two slots of bf16 and 14336 105 here, of 16384 91 there.
 constexpr int W4_ONE_WAVES = 16, W4_ONE_NB = 2, W4_ONE_LDS = 128 * 1024;
 
 template <int SG, bool ZERO>
