@@ -2,9 +2,9 @@
 //
 // Each of the four waves owns 64 columns (four streams of 16) for all 64 rows, so a weight is decoded once per 64 rows and by
 // one wave only: codes go from memory to registers, two k-tiles ahead, and from there to the matrix cores (w4.hpp's layout). The
-// rows' k-tile (16 KiB, of two halves 32) comes to LDS directly, into w4g_stages places in turn; its 16-byte chunks are swapped by the row's low bits (chunk c of
-// row r lies at c ^ (r & 15)), so that the 16 rows of an operand are read from 16 different banks' quads. The direct load
-// writes its lanes' pieces one after the other, so the swap is made in the addresses it reads.
+// rows' k-tile (16 KiB, of two halves 32) comes to LDS directly, into w4g_stages places in turn; its 16-byte chunks are swapped by
+// the row's low bits (chunk c of row r lies at c ^ (r & 15)), so that the 16 rows of an operand are read from 16 different banks'
+// quads. The direct load writes its lanes' pieces one after the other, so the swap is made in the addresses it reads.
 //
 // Per k-tile and wave: 64 matrix instructions (1024 cycles; 128 for rows of two halves), 144 to decode, 64 to add the groups' sums
 // times their scales (256 with groups of 32), 16 reads of 1 KiB from LDS (32).
