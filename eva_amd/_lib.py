@@ -21,10 +21,12 @@ SCORE_SIGMOID, SCORE_SQRT_SOFTPLUS = 0, 1
 ERR_EXPERT_RANGE, ERR_RATE = 1, 2
 W4_MAX_DIM, W4_MAX_COUNT, W4_MAX_ZERO = 1 << 18, 1024, 31   # EVAMX_W4_MAX_DIM, matrices of a stack, zero points
 W4_MOE_MAX_SLOTS = 65536                         # EVAMX_W4_MOE_MAX_SLOTS
+TOKENS_MAX_EXPERTS, TOKENS_MAX_TOPK, TOKENS_MAX_SLOTS = 1024, 32, 1 << 26    # of evamx_expert_order, evamx_sort_tokens, ..
 STRICT_MAX_ROWS, STRICT_MAX_SLOTS = 64, 256      # EVAMX_STRICT_MAX_ROWS / EVAMX_STRICT_MAX_SLOTS
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
 _f32 = ctypes.c_float
 
 
@@ -104,6 +106,14 @@ _SIGNATURES = {
     "evamx_moe_rotated_ptr": (_vp, [ctypes.POINTER(MoeShape), _vp]),
     "evamx_w4_moe_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 5),
     "evamx_w4_moe_forward": (ctypes.c_int, [ctypes.POINTER(W4MoeArgs), _vp]),
+    "evamx_expert_order_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
+    "evamx_expert_order": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, _i64, ctypes.c_int, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "evamx_sort_tokens": (ctypes.c_int, [_vp, ctypes.c_int, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp,
+                                         _i64, _i64, _vp]),
+    "evamx_combine_tokens": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _i64,
+                                            _vp, _i64, _vp]),
+    "evamx_combine_tokens_grad": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _vp, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp,
+                                                 _vp, ctypes.c_int, _vp, _vp, _i64, _vp, _vp]),
     "evamx_bench_decode": (ctypes.c_int, [_f32, ctypes.c_int, ctypes.c_int, _vp, _vp]),
     "evamx_bench_read": (ctypes.c_int, [_vp, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]),
 }

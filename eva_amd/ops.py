@@ -6,6 +6,7 @@ computes on the CPU.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
@@ -164,6 +165,11 @@ def _no_grad(name, *tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} has no backward: call it under torch.no_grad() or with detached tensors")
+    _no_tangent(name, *tensors)
+
+
+def _no_tangent(name, *tensors):
+    """Refuses tensors whose forward-mode derivative ``name`` would drop."""
     if forward_ad._current_level >= 0 and not torch.is_inference_mode_enabled():      # no_grad does not switch forward mode off
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
@@ -375,6 +381,179 @@ def balance_loss(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "si
             torch.cuda.is_current_stream_capturing():
         raise RuntimeError(_NO_CAPTURE)
     return _BalanceLoss.apply(logits, sel, score_fn, seq_starts, token_mask)
+
+
+def _wants_grad(name: str, instead: str, *tensors) -> bool:
+    """Whether autograd is to follow a call; refused in a graph capture, where its own streams and accumulators are not."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name} is not captured with a backward pass: call it under torch.no_grad(), and {instead}")
+    return True
+
+
+def _check_backward(name: str, instead: str) -> None:
+    if torch.is_grad_enabled():                          # create_graph=True: a gradient without a graph would pass for a constant
+        raise RuntimeError(f"{name} is differentiable once")
+    if torch.cuda.is_current_stream_capturing():         # of a forward pass that was not
+        raise RuntimeError(f"the backward pass of {name} is not captured: call {instead}")
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself if its rows are contiguous and do not overlap, or a copy (a gradient may come expanded)."""
+    rows, cols = t.shape
+    return t.contiguous() if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols) else t
+
+
+class ExpertOrder(NamedTuple):
+    """Slots sorted by expert (``expert_order``): expert e's take the sorted rows ``starts[e]`` to
+    ``starts[e + 1]`` (int32 ``[n_experts + 1]``), and a slot's row is ``position`` (int32 ``[T, topk]``, -1
+    for a slot of none of the experts)."""
+    starts: torch.Tensor
+    position: torch.Tensor
+
+
+def expert_order(sel: torch.Tensor, n_experts: int, *, first_expert: int = 0) -> ExpertOrder:
+    """The order in which ``sort_tokens`` lays out the tokens of routes ``sel`` int64 ``[T, topk]`` (``route_topk``) for the
+    experts ``first_expert`` to ``first_expert + n_experts - 1``: by expert, an expert's in the order of the slots.
+    Slots of other numbers (another rank's experts; -1 for padding) have no row. Up to 1024 experts, 32 a token, 2^26 slots."""
+    _dev(sel, "sel", torch.int64, 2)
+    rows, topk = sel.shape
+    dev = sel.device
+    need = lib().evamx_expert_order_workspace_bytes(rows, topk, n_experts)
+    if need == 0:
+        raise ValueError(lib().evamx_last_error().decode())
+    starts = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
+    position = torch.empty(rows, topk, dtype=torch.int32, device=dev)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    _launch(lib().evamx_expert_order, "evamx_expert_order", dev, ptr(sel), rows, topk, first_expert, n_experts, ptr(starts), ptr(position),
+            ptr(workspace), need)
+    return ExpertOrder(starts, position)
+
+
+def _order_args(order: ExpertOrder, device: torch.device):
+    """(rows, topk, experts) of a checked order."""
+    starts, position = order
+    _dev(starts, "order.starts", torch.int32, 1)
+    _dev(position, "order.position", torch.int32, 2)
+    if starts.device != device or position.device != device:
+        raise ValueError(f"the order is on {starts.device} and {position.device}, the rows on {device}")
+    return *position.shape, starts.numel() - 1
+
+
+def _token_rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None, shape=(None, None)) -> int:
+    """Row stride of fp16, bf16 or fp32 rows (of ``like``'s type and device)."""
+    stride = _row_stride(t, name, None if like is None else like.dtype)
+    if like is None and t.dtype not in _LOGIT_DTYPES:
+        raise ValueError(f"{name} must be fp16, bf16 or fp32")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+    if any(want is not None and want != have for want, have in zip(shape, t.shape)):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    return stride
+
+
+def _sort_rows(x, order, out_rows):
+    """``x``'s rows at their positions of ``out_rows`` sorted ones."""
+    rows, topk, experts = _order_args(order, x.device)
+    stride = _token_rows(x, "x", None, (rows, None))
+    out = torch.empty(out_rows, x.shape[1], dtype=x.dtype, device=x.device)
+    _launch(lib().evamx_sort_tokens, "evamx_sort_tokens", x.device, ptr(x), _LOGIT_DTYPES[x.dtype], stride, rows, x.shape[1], topk,
+            ptr(order.position), ptr(order.starts), experts, ptr(out), x.shape[1], out_rows)
+    return out
+
+
+def _combine(y, order, weights, residual):
+    """The weighted sums of ``combine_tokens``."""
+    rows, topk, _ = _order_args(order, y.device)
+    stride, hidden = _token_rows(y, "y"), y.shape[1]
+    residual_stride = 0 if residual is None else _token_rows(residual, "residual", y, (rows, hidden))
+    if weights is not None:
+        _dev(weights, "weights", torch.float32, 2)
+        if tuple(weights.shape) != (rows, topk) or weights.device != y.device:
+            raise ValueError(f"weights must be [{rows}, {topk}] on {y.device}, got {list(weights.shape)} on {weights.device}")
+    out = torch.empty(rows, hidden, dtype=y.dtype, device=y.device)
+    _launch(lib().evamx_combine_tokens, "evamx_combine_tokens", y.device, ptr(y), _LOGIT_DTYPES[y.dtype], stride, y.shape[0], rows, hidden,
+            topk, ptr(order.position), ptr(weights), ptr(residual), residual_stride, ptr(out), hidden)
+    return out
+
+
+_SORT_GRAD, _COMBINE_GRAD = "sort_tokens_grad", "combine_tokens_grad"
+
+
+class _SortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, starts, position):
+        ctx.save_for_backward(starts, position)
+        return _sort_rows(x, ExpertOrder(starts, position), position.numel())
+
+    @staticmethod
+    def backward(ctx, grad):
+        _check_backward("sort_tokens", _SORT_GRAD)
+        return sort_tokens_grad(_rows_of(grad), ExpertOrder(*ctx.saved_tensors)), None, None
+
+
+def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
+    """The tokens ``x [T, hidden]`` (fp16, bf16 or fp32) sorted by expert, ``[T * topk, hidden]``: row ``order.position[t, k]``
+    is ``x[t]``. The rows behind ``order.starts[-1]``, where slots have no row, are zeros. Differentiable in x (once, and not in a
+    graph capture: there call it under ``torch.no_grad()``, and ``sort_tokens_grad``)."""
+    _no_tangent("sort_tokens", x)
+    if _wants_grad("sort_tokens", _SORT_GRAD, x):
+        return _SortTokens.apply(x, *order)
+    return _sort_rows(x, order, order.position.numel())
+
+
+def sort_tokens_grad(grad: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
+    """The gradient of ``sort_tokens`` in its tokens: each one's rows of ``grad`` added up (in fp32, rounded once)."""
+    return _combine(grad, order, None, None)
+
+
+class _CombineTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, starts, position, weights, residual):
+        ctx.save_for_backward(y if weights is not None else None, starts, position, weights)
+        ctx.y_rows = y.shape[0]
+        return _combine(y, ExpertOrder(starts, position), weights, residual)
+
+    @staticmethod
+    def backward(ctx, grad):
+        _check_backward("combine_tokens", _COMBINE_GRAD)
+        y, starts, position, weights = ctx.saved_tensors
+        grad, order, dy, dweights = _rows_of(grad), ExpertOrder(starts, position), None, None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[3]:
+            if weights is None:
+                dy = _sort_rows(grad, order, ctx.y_rows)
+            else:
+                dy, dweights = combine_tokens_grad(grad, y, order, weights)
+        return dy, None, None, dweights, grad if ctx.needs_input_grad[4] else None
+
+
+def combine_tokens(y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor | None = None, *,
+                   residual: torch.Tensor | None = None) -> torch.Tensor:
+    """Sorted rows back to their tokens: ``out[t] = sum_k weights[t, k] * y[order.position[t, k]] + residual[t]``, for ``y [rows,
+    hidden]`` (fp16, bf16 or fp32), ``weights`` fp32 ``[T, topk]`` (1 without) and ``residual`` of y's type; slots without a row add
+    nothing. fp32 sums in slot order, rounded once. Differentiable in y, weights and residual (once, and not in a graph capture:
+    there call it under ``torch.no_grad()``, and ``combine_tokens_grad``)."""
+    _no_tangent("combine_tokens", y, weights, residual)
+    if _wants_grad("combine_tokens", _COMBINE_GRAD, y, weights, residual):
+        return _CombineTokens.apply(y, *order, weights, residual)
+    return _combine(y, order, weights, residual)
+
+
+def combine_tokens_grad(grad: torch.Tensor, y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor):
+    """``(y's gradient, weights' gradient fp32 [T, topk])`` of ``combine_tokens`` for ``grad [T, hidden]``; zeros in y's rows behind
+    the last one that a slot has."""
+    rows, topk, experts = _order_args(order, y.device)
+    y_stride, hidden = _token_rows(y, "y"), y.shape[1]
+    stride = _token_rows(grad, "grad", y, (rows, hidden))
+    _dev(weights, "weights", torch.float32, 2)
+    if tuple(weights.shape) != (rows, topk) or weights.device != y.device:
+        raise ValueError(f"weights must be [{rows}, {topk}] on {y.device}, got {list(weights.shape)} on {weights.device}")
+    dy = torch.empty(y.shape[0], hidden, dtype=y.dtype, device=y.device)
+    dweights = torch.empty(rows, topk, dtype=torch.float32, device=y.device)
+    _launch(lib().evamx_combine_tokens_grad, "evamx_combine_tokens_grad", y.device, ptr(grad), _LOGIT_DTYPES[y.dtype], stride, ptr(y), y_stride,
+            y.shape[0], rows, hidden, topk, ptr(order.position), ptr(order.starts), experts, ptr(weights), ptr(dy), hidden, ptr(dweights))
+    return dy, dweights
 
 
 def prepare_routes_workspace_bytes(capacity: int, topk: int) -> int:

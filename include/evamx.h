@@ -24,8 +24,9 @@
  *                            plus the shared expert added by Block.experts (model.py:418-452,498)
  *   evamx_moe_workspace_bytes  WorkspaceLayout.scratch_bytes / exl3_moe_coop_ctr_len
  *                            (moe_coop3072.py:120-152; exl3_moe_coop.cuh:154-159)
- * evamx_w4_* (4-bit weights with group scales) and evamx_balance_* (a router's balance loss) have
- * no counterpart in the reference.
+ * evamx_w4_* (4-bit weights with group scales), evamx_balance_* (a router's balance loss) and
+ * evamx_expert_order, evamx_sort_tokens, evamx_combine_tokens* (tokens sorted by expert and back)
+ * have no counterpart in the reference.
  */
 #ifndef EVAMX_H
 #define EVAMX_H
@@ -312,6 +313,42 @@ typedef struct evamx_w4_moe_args {
 } evamx_w4_moe_args;
 size_t evamx_w4_moe_workspace_bytes(int rows, int topk, int n_shared, int hidden, int inter);
 int evamx_w4_moe_forward(const evamx_w4_moe_args* args, evamx_stream_t stream);
+
+/* ---- tokens sorted by expert, and back ------------------------------------------------------ */
+
+/* No counterpart in the reference: the dispatch around experts whose products are the caller's own
+ * (evamx_dense.h), with its gradients. A slot is one of a token's topk picks; rows * topk <= 2^26
+ * slots, topk 1..32, 1..1024 local experts, hidden 1..EVAMX_W4_MAX_DIM. Rows of fp16, bf16 or fp32
+ * (dtype), of any alignment and strides of at least the row length, in elements. Results repeat bit
+ * for bit; sums are fp32's, rounded once. Nothing an array holds makes a call read or write outside of
+ * the given rows. */
+
+/* The order: sel device int64 [rows][topk], of which the experts first_expert .. first_expert +
+ * n_local - 1 are local and every other number is none. starts device int32 [n_local + 1]: expert e's
+ * slots take the sorted rows starts[e] .. starts[e + 1] - 1, in the order of the slots (the same expert
+ * twice takes two rows); position device int32 [rows][topk]: a slot's row, or -1. The workspace
+ * (4-byte aligned) needs no clearing; calls that share one must not overlap. */
+size_t evamx_expert_order_workspace_bytes(int rows, int topk, int n_local);
+int evamx_expert_order(const int64_t* sel, int rows, int topk, int64_t first_expert, int n_local, int32_t* starts,
+                       int32_t* position, void* workspace, size_t workspace_bytes, evamx_stream_t stream);
+/* out[position[t][k]] = x[t]; the rows of out [out_rows][out_stride] from starts[n_local] on are zeros (out_rows =
+ * rows * topk holds every slot; a row outside of out is not written). */
+int evamx_sort_tokens(const void* x, int dtype, int64_t x_stride, int rows, int hidden, int topk, const int32_t* position,
+                      const int32_t* starts, int n_local, void* out, int64_t out_stride, int64_t out_rows,
+                      evamx_stream_t stream);
+/* out[t] = sum_k weights[t][k] * y[position[t][k]] + residual[t], added in slot order; y
+ * [y_rows][y_stride]; a position outside of it adds nothing. weights fp32 [rows][topk], or NULL for 1
+ * (the gradient of evamx_sort_tokens); residual of dtype, or NULL. out may be the residual. */
+int evamx_combine_tokens(const void* y, int dtype, int64_t y_stride, int64_t y_rows, int rows, int hidden, int topk,
+                         const int32_t* position, const float* weights, const void* residual, int64_t residual_stride,
+                         void* out, int64_t out_stride, evamx_stream_t stream);
+/* Of the gradient grad [rows][grad_stride] of that sum: grad_y[position[t][k]] = weights[t][k] * grad[t]
+ * (zeros in its rows from starts[n_local] on; all y_rows are written) and grad_weights[t][k] =
+ * <grad[t], y[position[t][k]]>, fp32 (0 for a slot without a row). */
+int evamx_combine_tokens_grad(const void* grad, int dtype, int64_t grad_stride, const void* y, int64_t y_stride, int64_t y_rows,
+                              int rows, int hidden, int topk, const int32_t* position, const int32_t* starts, int n_local,
+                              const float* weights, void* grad_y, int64_t grad_y_stride, float* grad_weights,
+                              evamx_stream_t stream);
 
 /* ---- measurement --------------------------------------------------------------------------- */
 
