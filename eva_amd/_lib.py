@@ -13,7 +13,9 @@ import torch  # noqa: F401  (loads the HIP runtime the library resolves against)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libevamx.so")
+DENSE_LIB_PATH = os.path.join(HERE, "libevamx_dense.so")
 ABI_VERSION = 5
+DENSE_VERSION = 1
 
 EVAMX_OK, EVAMX_EINVAL, EVAMX_ELAUNCH, EVAMX_ENOSPACE = 0, -1, -2, -3
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
@@ -61,11 +63,27 @@ class W4MoeArgs(ctypes.Structure):
                 ("x_dtype", _i32), ("rows", _i32), ("topk", _i32), ("n_shared", _i32), ("limit", _f32)]
 
 
+class LinearArgs(ctypes.Structure):
+    """evamx_linear_args."""
+    _fields_ = [("x", _vp), ("w", _vp), ("bias", _vp), ("residual", _vp), ("y", _vp), ("pre", _vp), ("starts", _vp), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t), ("x_stride", _i64), ("w_stride", _i64), ("w_expert_stride", _i64),
+                ("residual_stride", _i64), ("y_stride", _i64), ("dtype", _i32), ("rows", _i32), ("n_in", _i32), ("n_out", _i32),
+                ("experts", _i32), ("act", _i32), ("limit", _f32)]
+
+
+class LinearGradArgs(ctypes.Structure):
+    """evamx_linear_grad_args."""
+    _fields_ = [("grad", _vp), ("x", _vp), ("w", _vp), ("pre", _vp), ("starts", _vp), ("grad_x", _vp), ("grad_w", _vp), ("grad_bias", _vp),
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("grad_stride", _i64), ("x_stride", _i64), ("w_stride", _i64),
+                ("w_expert_stride", _i64), ("grad_x_stride", _i64), ("dtype", _i32), ("rows", _i32), ("n_in", _i32), ("n_out", _i32),
+                ("experts", _i32), ("act", _i32), ("limit", _f32)]
+
+
 class EvamxError(RuntimeError):
     pass
 
 
-_lib = None
+_lib = _dense_lib = None
 
 # name -> (restype, argtypes)
 _SIGNATURES = {
@@ -118,30 +136,56 @@ _SIGNATURES = {
     "evamx_bench_read": (ctypes.c_int, [_vp, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]),
 }
 
+# of libevamx_dense.so (include/evamx_dense.h)
+_DENSE_SIGNATURES = {
+    "evamx_dense_last_error": (ctypes.c_char_p, []),
+    "evamx_dense_version": (ctypes.c_int, []),
+    "evamx_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "evamx_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), _vp]),
+    "evamx_linear_grad_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "evamx_linear_grad": (ctypes.c_int, [ctypes.POINTER(LinearGradArgs), _vp]),
+}
+
 EXPORTS = tuple(_SIGNATURES)
+DENSE_EXPORTS = tuple(_DENSE_SIGNATURES)
+
+
+def _load(path, signatures):
+    if not os.path.exists(path):
+        raise EvamxError(f"{path} is missing: build it with `python -m eva_amd.build` (or __graft_entry__.build())")
+    handle = ctypes.CDLL(path)
+    for name, (res, args) in signatures.items():
+        fn = getattr(handle, name)
+        fn.restype = res
+        fn.argtypes = args
+    return handle
 
 
 def lib():
     """The loaded library (raises if it has not been built)."""
     global _lib
     if _lib is None:
-        if not os.path.exists(LIB_PATH):
-            raise EvamxError(f"{LIB_PATH} is missing: build it with `python -m eva_amd.build` "
-                             "(or __graft_entry__.build())")
-        handle = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in _SIGNATURES.items():
-            fn = getattr(handle, name)
-            fn.restype = res
-            fn.argtypes = args
+        handle = _load(LIB_PATH, _SIGNATURES)
         if handle.evamx_abi_version() != ABI_VERSION:
             raise EvamxError("libevamx ABI version mismatch; rebuild the library")
         _lib = handle
     return _lib
 
 
-def check(rc: int, what: str):
+def dense_lib():
+    """The loaded library of the products on 16-bit weights (raises if it has not been built)."""
+    global _dense_lib
+    if _dense_lib is None:
+        handle = _load(DENSE_LIB_PATH, _DENSE_SIGNATURES)
+        if handle.evamx_dense_version() != DENSE_VERSION:
+            raise EvamxError("libevamx_dense version mismatch; rebuild the library")
+        _dense_lib = handle
+    return _dense_lib
+
+
+def check(rc: int, what: str, last_error=None):
     if rc != EVAMX_OK:
-        msg = lib().evamx_last_error().decode(errors="replace")
+        msg = (last_error or lib().evamx_last_error)().decode(errors="replace")
         raise EvamxError(f"{what} failed ({rc}): {msg}")
 
 

@@ -1,9 +1,9 @@
-"""Build libevamx.so (the C-ABI HIP library) in-tree for gfx950 with hipcc.
+"""Build the C-ABI HIP libraries in-tree for gfx950 with hipcc.
 
-    python -m eva_amd.build            # compile every csrc/*.hip and link eva_amd/libevamx.so
+    python -m eva_amd.build            # csrc/*.hip -> eva_amd/libevamx.so, csrc/dense/*.hip -> eva_amd/libevamx_dense.so
 
-Objects go to eva_amd/_build/ (git-ignored); the .so sits next to this file so that it travels
-with the source tree to the GPU box.
+Objects go to eva_amd/_build/ (git-ignored); the .so files sit next to this file so that they travel
+with the source tree.
 """
 from __future__ import annotations
 
@@ -16,6 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libevamx.so")
+DENSE_CSRC = os.path.join(CSRC, "dense")
+DENSE_LIB = os.path.join(HERE, "libevamx_dense.so")
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
@@ -25,12 +27,12 @@ FLAGS = [
 ]
 
 
-def sources():
-    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
+def sources(folder: str = CSRC):
+    return sorted(os.path.join(folder, f) for f in os.listdir(folder) if f.endswith(".hip"))
 
 
 def _compile(src):
-    obj = os.path.join(OBJ, os.path.basename(src)[:-4] + ".o")
+    obj = os.path.join(OBJ, os.path.relpath(src, CSRC)[:-4].replace(os.sep, "_") + ".o")
     cmd = [HIPCC, *FLAGS, "-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     msgs = "\n".join(l for l in (r.stdout + r.stderr).splitlines()
@@ -40,21 +42,27 @@ def _compile(src):
     return obj, msgs
 
 
+def _link(lib, objs):
+    tmp = lib + ".tmp"
+    r = subprocess.run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs,
+                        "-Wl,-rpath,/opt/rocm/lib"], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stdout}{r.stderr}")
+    os.replace(tmp, lib)
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
+    main, dense = sources(), sources(DENSE_CSRC)
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
-        results = list(ex.map(_compile, sources()))
+        results = list(ex.map(_compile, main + dense))
     if verbose:
         for _, m in results:
             if m.strip():
                 print(m, file=sys.stderr)
     objs = [o for o, _ in results]
-    tmp = LIB + ".tmp"
-    r = subprocess.run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs,
-                        "-Wl,-rpath,/opt/rocm/lib"], capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stdout}{r.stderr}")
-    os.replace(tmp, LIB)
+    _link(LIB, objs[:len(main)])
+    _link(DENSE_LIB, objs[len(main):])
     return LIB
 
 

@@ -1,0 +1,200 @@
+// Products on 16-bit weights, one matrix for all rows or one for each expert's rows: what their kernels share.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "../../../include/evamx_dense.h"
+
+namespace evamx_dense {
+
+void set_error(const char* fmt, ...);
+int launched(const char* what);
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef u16x8 u16x8_loose __attribute__((aligned(2)));      // 16 bytes at any value's address: the hardware takes them, only slower
+typedef u16x4 u16x4_loose __attribute__((aligned(2)));
+
+constexpr int MAX_EXPERTS = 1024, CUS = 256;
+
+struct Bf16 {
+    static __device__ __forceinline__ float get(uint16_t v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
+    static __device__ __forceinline__ uint16_t put(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+    static __device__ __forceinline__ f32x4 mfma(u16x8 a, u16x8 b, f32x4 c)
+    {
+#ifdef __HIP_DEVICE_COMPILE__
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+#else
+        return c;
+#endif
+    }
+};
+struct F16 {
+    static __device__ __forceinline__ float get(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
+    static __device__ __forceinline__ uint16_t put(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+    static __device__ __forceinline__ f32x4 mfma(u16x8 a, u16x8 b, f32x4 c)
+    {
+#ifdef __HIP_DEVICE_COMPILE__
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+#else
+        return c;
+#endif
+    }
+};
+
+// ---- activations ------------------------------------------------------------------------------
+
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+
+// Clamps that leave a NaN as it is.
+__device__ __forceinline__ float at_most(float v, float m) { return v > m ? m : v; }
+__device__ __forceinline__ float within(float v, float m) { return v > m ? m : v < -m ? -m : v; }
+
+__device__ __forceinline__ float swiglu(float gate, float up, float limit)
+{
+    const float a = gate * sigmoid(gate);
+    return limit > 0 ? at_most(a, limit) * within(up, limit) : a * up;
+}
+
+__device__ __forceinline__ float activate(float v, int act)
+{
+    if (act == EVAMX_ACT_SILU) return v * sigmoid(v);
+    if (act == EVAMX_ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+    if (act == EVAMX_ACT_RELU) return v < 0 ? 0.0f : v;
+    return v;
+}
+
+// d activate(v) / dv
+__device__ __forceinline__ float slope(float v, int act)
+{
+    if (act == EVAMX_ACT_SILU) {
+        const float s = sigmoid(v);
+        return s * (1.0f + v * (1.0f - s));
+    }
+    if (act == EVAMX_ACT_GELU) return 0.5f * (1.0f + erff(v * 0.70710678f)) + v * 0.39894228f * __expf(-0.5f * v * v);
+    return v > 0 ? 1.0f : v == v ? 0.0f : v;                     // ReLU; a NaN stays one
+}
+
+// ---- which rows a workgroup takes ---------------------------------------------------------------
+
+// Rows of expert e are [starts[e], starts[e + 1]), cut to the rows there are, whatever the table holds; without a table all rows
+// are one expert's.
+struct Groups {
+    const int32_t* starts;
+    int experts, rows;
+
+    __device__ __forceinline__ int start(int e) const
+    {
+        const int v = starts[e];
+        return v < 0 ? 0 : v > rows ? rows : v;
+    }
+    __device__ __forceinline__ int end() const { return starts ? start(experts) : rows; }
+};
+
+struct Tile {
+    int expert, row, have, col;   // rows row .. row + have - 1 (of a tile of at most TQ), column tile col
+};
+
+// The work's tile t (row tiles of each expert by cols column tiles); false: none. Tiles go expert by expert, within one
+// eight row tiles by all columns at a time, so that neighbours share their rows and weights in the L2. All threads call it;
+// s: 2 + threads / 64 ints of LDS.
+template <int THREADS>
+__device__ __forceinline__ bool find_tile(const Groups& g, int tq, int cols, int t, int* s, Tile& tile, int& expert_tiles)
+{
+    int e = 0, first = 0, begin = 0, count = g.rows;
+    if (g.starts) {
+        constexpr int PER = (MAX_EXPERTS + THREADS - 1) / THREADS;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (g.experts + THREADS - 1) / THREADS;
+        int a[PER + 1], mine = 0;
+#pragma unroll
+        for (int i = 0; i <= PER; ++i) {
+            const int at = (int)threadIdx.x * per + i;
+            a[i] = i <= per && at <= g.experts ? g.start(at) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (i < per && (int)threadIdx.x * per + i < g.experts && a[i + 1] > a[i]) mine += (a[i + 1] - a[i] + tq - 1) / tq;
+        int upto = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int n = __shfl_up(upto, d);
+            if (lane >= d) upto += n;
+        }
+        if (lane == 63) s[2 + wave] = upto;
+        if (threadIdx.x == 0) s[0] = -1;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) upto += s[2 + w];
+        int total = 0;
+        for (int w = 0; w < THREADS / 64; ++w) total += s[2 + w];
+        // consecutive workgroups go to the eight XCDs in turn: each XCD gets a contiguous run of tiles
+        const long all = (long)total * cols;
+        const int per_xcd = (int)((all + 7) / 8);
+        const bool any = t / 8 < per_xcd && (long)(t & 7) * per_xcd + t / 8 < all;
+        const long at = (long)(t & 7) * per_xcd + t / 8;
+        const int row_tile = any ? (int)(at / cols) : -1;
+        if (row_tile >= upto - mine && row_tile < upto) {            // one thread's
+            int before = upto - mine;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (i < per && (int)threadIdx.x * per + i < g.experts && a[i + 1] > a[i]) {
+                    const int n = (a[i + 1] - a[i] + tq - 1) / tq;
+                    if (row_tile >= before && row_tile < before + n) {
+                        s[0] = (int)threadIdx.x * per + i;
+                        s[1] = before;
+                    }
+                    before += n;
+                }
+        }
+        __syncthreads();
+        e = __builtin_amdgcn_readfirstlane(s[0]);
+        if (e < 0) return false;
+        first = __builtin_amdgcn_readfirstlane(s[1]);
+        begin = g.start(e);
+        count = g.start(e + 1) - begin;
+        t = (int)(at - (long)first * cols);
+    } else {
+        const long all = (long)((g.rows + tq - 1) / tq) * cols;
+        const int per_xcd = (int)((all + 7) / 8);
+        const long at = (long)(t & 7) * per_xcd + t / 8;
+        if (t / 8 >= per_xcd || at >= all) return false;
+        t = (int)at;
+    }
+    const int row_tiles = (count + tq - 1) / tq, band = t / (8 * cols), in_band = t - band * 8 * cols;
+    const int deep = row_tiles - 8 * band < 8 ? row_tiles - 8 * band : 8;
+    const int r = tq * (8 * band + in_band % deep);
+    tile.expert = e;
+    tile.row = begin + r;
+    tile.have = count - r < tq ? count - r : tq;
+    tile.col = in_band / deep;
+    expert_tiles = row_tiles;
+    return true;
+}
+
+// Zeros in rows [from, rows) of out; workgroup b of n.
+__device__ __forceinline__ void zero_rows(uint16_t* out, size_t stride, int cols, int64_t from, int64_t rows, int b, int n)
+{
+    for (int64_t r = from + b; r < rows; r += n) {
+        uint16_t* at = out + (size_t)r * stride;
+        for (int c = threadIdx.x * 8; c < cols; c += blockDim.x * 8) {
+            if (c + 8 <= cols) {
+                *(u16x8_loose*)(at + c) = (u16x8)(uint16_t)0;
+            } else {
+                for (int i = c; i < cols; ++i) at[i] = 0;
+            }
+        }
+    }
+}
+
+static inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+// Row tiles that the experts' rows can make at most.
+static inline int64_t most_row_tiles(int rows, int experts, bool grouped, int tq)
+{
+    return grouped ? rows / tq + (rows < experts ? rows : experts) : ceil_div(rows, tq);
+}
+
+}  // namespace evamx_dense

@@ -12,7 +12,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from ._lib import MoeArgs, MoeShape, W4Desc, W4MoeArgs, check, lib, ptr, stream_handle
+from ._lib import LinearArgs, LinearGradArgs, MoeArgs, MoeShape, W4Desc, W4MoeArgs, check, dense_lib, lib, ptr, stream_handle
 
 SCORE_FNS = {"sigmoid": _lib.SCORE_SIGMOID, "sqrt_softplus": _lib.SCORE_SQRT_SOFTPLUS}
 RATES = (2.0, 3.0, 4.0, 5.0)
@@ -138,13 +138,13 @@ def w4_dequant(weight: W4Weight) -> torch.Tensor:
     return out
 
 
-def _launch(fn, what: str, device: torch.device, *args):
+def _launch(fn, what: str, device: torch.device, *args, last_error=None):
     """One library call on the current stream of ``device``, which is made current if it is not."""
     if device.index == torch.cuda.current_device():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what)
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what, last_error)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what)
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what, last_error)
 
 
 def _row_stride(t: torch.Tensor, name: str, dtype=None) -> int:
@@ -554,6 +554,155 @@ def combine_tokens_grad(grad: torch.Tensor, y: torch.Tensor, order: ExpertOrder,
     _launch(lib().evamx_combine_tokens_grad, "evamx_combine_tokens_grad", y.device, ptr(grad), _LOGIT_DTYPES[y.dtype], stride, ptr(y), y_stride,
             y.shape[0], rows, hidden, topk, ptr(order.position), ptr(order.starts), experts, ptr(weights), ptr(dy), hidden, ptr(dweights))
     return dy, dweights
+
+
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3, "swiglu": 4}      # EVAMX_ACT_*
+
+
+def _matrix(w: torch.Tensor, like: torch.Tensor, ndim: int):
+    """(experts, n_out, n_in, row stride, expert stride) of checked weights ``[n_out, n_in]`` or ``[experts, n_out, n_in]``."""
+    if not isinstance(w, torch.Tensor) or not w.is_cuda or w.ndim != ndim:
+        raise ValueError(f"w must be a {ndim}-dim device tensor")
+    if w.dtype != like.dtype or w.device != like.device:
+        raise ValueError(f"w is {w.dtype} on {w.device}, x {like.dtype} on {like.device}")
+    experts, (n_out, n_in) = 1 if ndim == 2 else w.shape[0], w.shape[-2:]
+    row = w.stride(-2) if n_out > 1 else n_in
+    whole = w.stride(0) if experts > 1 else 0
+    if (n_in > 1 and w.stride(-1) != 1) or row < n_in or (experts > 1 and whole < row * (n_out - 1) + n_in):
+        raise ValueError("w must have unit column stride and rows and matrices that do not overlap")
+    return experts, n_out, n_in, row, whole
+
+
+def _linear_setup(name, x, w, starts, activation, limit):
+    """(x's row stride, experts, n_out, n_in, w's strides, activation number, result columns), checked."""
+    stride = _row_stride(x, "x")
+    if x.dtype not in _DTYPES:
+        raise ValueError("x must be fp16 or bf16")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation {activation!r} not in {list(ACTIVATIONS)}")
+    if not limit >= 0 or (limit and activation != "swiglu"):
+        raise ValueError(f"limit {limit}: 0 or more, and of swiglu alone")
+    experts, n_out, n_in, row, whole = _matrix(w, x, 2 if starts is None else 3)
+    if x.shape[1] != n_in:
+        raise ValueError(f"x has {x.shape[1]} features, w {n_in}")
+    if activation == "swiglu" and n_out % 2:
+        raise ValueError(f"swiglu needs gate and up rows in w, got {n_out}")
+    if starts is not None:
+        _dev(starts, "starts", torch.int32, 1)
+        if starts.numel() != experts + 1 or starts.device != x.device:
+            raise ValueError(f"starts must be [{experts + 1}] on {x.device}, got {list(starts.shape)} on {starts.device}")
+    return stride, experts, n_out, n_in, row, whole, ACTIVATIONS[activation], n_out // 2 if activation == "swiglu" else n_out
+
+
+def _linear_forward(name, x, w, starts, bias, activation, limit, residual, keep):
+    """(result, fp32 input of the activation or None)."""
+    stride, experts, n_out, n_in, row, whole, act, cols = _linear_setup(name, x, w, starts, activation, limit)
+    rows, dev = x.shape[0], x.device
+    if bias is not None:
+        _dev(bias, "bias", x.dtype)
+        if tuple(bias.shape) != ((n_out,) if starts is None else (experts, n_out)) or bias.device != dev:
+            raise ValueError(f"bias {list(bias.shape)} on {bias.device} does not go with w {list(w.shape)} on {dev}")
+    residual_stride = 0 if residual is None else _token_rows(residual, "residual", x, (rows, cols))
+    y = torch.empty(rows, cols, dtype=x.dtype, device=dev)
+    pre = torch.empty(rows, n_out, dtype=torch.float32, device=dev) if keep and act else None
+    need = dense_lib().evamx_linear_workspace_bytes(rows, n_in, n_out, experts, starts is not None)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    a = LinearArgs(ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(y), ptr(pre), ptr(starts), ptr(workspace), need, stride, row, whole,
+                   residual_stride, cols, _DTYPES[x.dtype], rows, n_in, n_out, experts, act, limit)
+    _launch(dense_lib().evamx_linear, name, dev, ctypes.byref(a), last_error=dense_lib().evamx_dense_last_error)
+    return y, pre
+
+
+def _linear_backward(name, grad, x, w, starts, pre, activation, limit, want_x, want_w, want_bias):
+    """The wanted ones of (x's, w's, bias's) gradients."""
+    stride, experts, n_out, n_in, row, whole, act, cols = _linear_setup(name, x, w, starts, activation, limit)
+    rows, dev = x.shape[0], x.device
+    grad_stride = _token_rows(grad, "grad", x, (rows, cols))
+    if act:
+        if pre is None:
+            raise ValueError("the gradient of an activation needs pre, what the forward call gave with return_pre=True")
+        _dev(pre, "pre", torch.float32, 2)
+        if tuple(pre.shape) != (rows, n_out) or pre.device != dev:
+            raise ValueError(f"pre must be [{rows}, {n_out}] on {dev}, got {list(pre.shape)} on {pre.device}")
+    dx = torch.empty(rows, n_in, dtype=x.dtype, device=dev) if want_x else None
+    dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_w else None
+    db = torch.empty(w.shape[:-1], dtype=x.dtype, device=dev) if want_bias else None
+    need = dense_lib().evamx_linear_grad_workspace_bytes(rows, n_in, n_out, experts, starts is not None, act)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    a = LinearGradArgs(ptr(grad), ptr(x), ptr(w), ptr(pre) if act else None, ptr(starts), ptr(dx), ptr(dw), ptr(db), ptr(workspace), need,
+                       grad_stride, stride, row, whole, n_in, _DTYPES[x.dtype], rows, n_in, n_out, experts, act, limit)
+    _launch(dense_lib().evamx_linear_grad, name, dev, ctypes.byref(a), last_error=dense_lib().evamx_dense_last_error)
+    return dx, dw, db
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, starts, bias, activation, limit, residual):
+        y, pre = _linear_forward(_linear_name(starts), x, w, starts, bias, activation, limit, residual, True)
+        ctx.save_for_backward(x, w, starts, pre)
+        ctx.args = activation, limit
+        return y
+
+    @staticmethod
+    def backward(ctx, grad):
+        x, w, starts, pre = ctx.saved_tensors
+        name, need = _linear_name(starts), ctx.needs_input_grad
+        _check_backward(name, name + "_grad")
+        dx = dw = db = None
+        if need[0] or need[1] or need[3]:
+            dx, dw, db = _linear_backward(name + "_grad", _rows_of(grad), x, w, starts, pre, *ctx.args, need[0], need[1], need[3])
+        return dx, dw, None, db, None, None, grad if need[6] else None
+
+
+def _linear_name(starts):
+    return "linear" if starts is None else "expert_linear"
+
+
+def _linear_call(x, w, starts, bias, activation, limit, residual, return_pre):
+    name = _linear_name(starts)
+    _no_tangent(name, x, w, bias, residual)
+    if not return_pre and _wants_grad(name, f"{name}_grad", x, w, bias, residual):
+        return _Linear.apply(x, w, starts, bias, activation, float(limit), residual)
+    y, pre = _linear_forward(name, x, w, starts, bias, activation, float(limit), residual, return_pre)
+    return (y, pre) if return_pre else y
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None, limit: float = 0.0,
+           residual: torch.Tensor | None = None, return_pre: bool = False):
+    """``activation(x @ w.T + bias) + residual`` on 16-bit weights: ``x`` fp16 or bf16 ``[rows, n_in]``, ``w [n_out, n_in]``, ``bias
+    [n_out]`` and ``residual [rows, n_out]`` of its type. ``activation``: None, "silu", "gelu" (x times the normal distribution
+    function), "relu" or "swiglu", whose ``w`` holds the gate's rows and then the up product's: ``min(silu(g), limit) * clamp(u, -limit,
+    limit)`` of half as many columns, as the routed experts of ``moe_forward`` (``limit`` 0: not clamped; a NaN stays NaN). fp32
+    sums, rounded once, at the end.
+
+    Differentiable in x, w, bias and residual: a call that autograd follows keeps what the activation takes, in fp32. Once, and not
+    in a graph capture: there, ``return_pre=True`` gives ``(y, pre)`` outside autograd, for ``linear_grad``."""
+    if not isinstance(w, torch.Tensor) or w.ndim != 2:
+        raise ValueError("w must be a 2-dim device tensor")
+    return _linear_call(x, w, None, bias, activation, limit, residual, return_pre)
+
+
+def expert_linear(x: torch.Tensor, w: torch.Tensor, starts: torch.Tensor, bias: torch.Tensor | None = None, *,
+                  activation: str | None = None, limit: float = 0.0, return_pre: bool = False):
+    """``linear`` on rows sorted by expert (``sort_tokens``), each expert's with its own matrix: ``w [experts, n_out, n_in]``, ``bias
+    [experts, n_out]``, ``starts`` int32 ``[experts + 1]`` (``expert_order``). Rows behind ``starts[-1]`` are not read, and are zeros in
+    the result and in x's gradient; an expert without rows has gradients of zero."""
+    _dev(starts, "starts", torch.int32, 1)
+    return _linear_call(x, w, starts, bias, activation, limit, None, return_pre)
+
+
+def linear_grad(grad: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: torch.Tensor | None = None, *, activation: str | None = None,
+                limit: float = 0.0):
+    """``(x's, w's, bias's)`` gradients of ``linear`` for ``grad [rows, n_out]``; ``pre`` from the forward call where there is an
+    activation (its gradient is rounded to x's type before the products). The residual's is ``grad``."""
+    return _linear_backward("linear_grad", grad, x, w, None, pre, activation, float(limit), True, True, True)
+
+
+def expert_linear_grad(grad: torch.Tensor, x: torch.Tensor, w: torch.Tensor, starts: torch.Tensor, pre: torch.Tensor | None = None, *,
+                       activation: str | None = None, limit: float = 0.0):
+    """``(x's, w's, bias's)`` gradients of ``expert_linear``, as ``linear_grad``."""
+    _dev(starts, "starts", torch.int32, 1)
+    return _linear_backward("expert_linear_grad", grad, x, w, starts, pre, activation, float(limit), True, True, True)
 
 
 def prepare_routes_workspace_bytes(capacity: int, topk: int) -> int:
