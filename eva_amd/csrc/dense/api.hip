@@ -106,7 +106,7 @@ static bool space_ok(const char* who, const void* ws, size_t have, size_t need)
 // Rows that the direct loads take: 16-byte addresses and lengths, 32-bit offsets.
 static bool direct(const void* p, int64_t stride, int64_t rows, int len)
 {
-    return (((uintptr_t)p | (uintptr_t)(2 * stride)) & 15) == 0 && len % 8 == 0 && (rows + 512) * stride * 2 < 0xffffff00ll;
+    return (((uintptr_t)p | (uintptr_t)(2 * stride)) & 15) == 0 && len % 8 == 0 && (rows + 512) * stride * 2 < 0xf0000000ll;
 }
 
 }  // namespace evamx_dense

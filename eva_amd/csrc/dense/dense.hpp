@@ -21,6 +21,40 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef u16x8 u16x8_loose __attribute__((aligned(2)));      // 16 bytes at any value's address: the hardware takes them, only slower
 typedef u16x4 u16x4_loose __attribute__((aligned(2)));
 
+typedef f32x4 f32x4_loose __attribute__((aligned(4)));
+
+// N (4 or 8) floats in a row, or as many as there are.
+template <int N>
+__device__ __forceinline__ void store_floats(float* p, const float (&v)[N], int have)
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        if (have >= i + 4) {
+            *(f32x4_loose*)(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+        } else {
+#pragma unroll
+            for (int j = i; j < i + 3; ++j)
+                if (j < have) p[j] = v[j];
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void add_floats(float (&v)[N], const float* p, int have)
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        if (have >= i + 4) {
+            const f32x4 x = *(const f32x4_loose*)(p + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i + j] += x[j];
+        } else {
+#pragma unroll
+            for (int j = i; j < i + 3; ++j)
+                if (j < have) v[j] += p[j];
+        }
+    }
+}
+
 constexpr int MAX_EXPERTS = 1024, CUS = 256;
 
 struct Bf16 {
@@ -105,7 +139,7 @@ struct Tile {
 // eight row tiles by all columns at a time, so that neighbours share their rows and weights in the L2. All threads call it;
 // s: 2 + threads / 64 ints of LDS.
 template <int THREADS>
-__device__ __forceinline__ bool find_tile(const Groups& g, int tq, int cols, int t, int* s, Tile& tile, int& expert_tiles)
+__device__ __forceinline__ bool find_tile(const Groups& g, int tq, int cols, int t, int* s, Tile& tile)
 {
     int e = 0, first = 0, begin = 0, count = g.rows;
     if (g.starts) {
@@ -171,11 +205,10 @@ __device__ __forceinline__ bool find_tile(const Groups& g, int tq, int cols, int
     tile.row = begin + r;
     tile.have = count - r < tq ? count - r : tq;
     tile.col = in_band / deep;
-    expert_tiles = row_tiles;
     return true;
 }
 
-// Zeros in rows [from, rows) of out; workgroup b of n.
+// Zeros in rows [from, rows) of out: those of workgroup b of n.
 __device__ __forceinline__ void zero_rows(uint16_t* out, size_t stride, int cols, int64_t from, int64_t rows, int b, int n)
 {
     for (int64_t r = from + b; r < rows; r += n) {

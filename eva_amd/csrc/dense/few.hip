@@ -81,16 +81,13 @@ __device__ __forceinline__ void few_product(const LinearParams& p, const Tile& t
 }
 
 template <class T, bool GATED, bool LOOSE>
-__global__ __launch_bounds__(FEW_THREADS) void few_kernel(LinearParams p, int cols, int work)
+__global__ __launch_bounds__(FEW_THREADS) void few_kernel(LinearParams p, int cols)
 {
     extern __shared__ f32x4 part[];
-    if ((int)blockIdx.x >= work) {
-        if (p.g.starts) zero_rows(p.y, p.y_stride, GATED ? p.inter : p.n_out, p.g.end(), p.g.rows, blockIdx.x - work, gridDim.x - work);
-        return;
-    }
     Tile t;
-    int row_tiles;
-    if (!find_tile<FEW_THREADS>(p.g, FEW_ROWS, cols, blockIdx.x, (int*)part, t, row_tiles)) return;
+    const bool any = find_tile<FEW_THREADS>(p.g, FEW_ROWS, cols, blockIdx.x, (int*)part, t);
+    if (p.g.starts) zero_rows(p.y, p.y_stride, GATED ? p.inter : p.n_out, p.g.end(), p.g.rows, blockIdx.x, gridDim.x);
+    if (!any) return;
     __syncthreads();
     if (t.have > 32) few_product<T, GATED, LOOSE, 4>(p, t, part);
     else if (t.have > 16) few_product<T, GATED, LOOSE, 2>(p, t, part);
@@ -101,9 +98,8 @@ template <class T, bool GATED, bool LOOSE>
 static void launch_few_as(const LinearParams& p, hipStream_t s)
 {
     const int cols = ceil_div(GATED ? p.inter : p.n_out, 16), most = p.g.rows > 32 ? 4 : p.g.rows > 16 ? 2 : 1;
-    const int64_t work = 8 * (int64_t)ceil_div(most_row_tiles(p.g.rows, p.g.experts, p.g.starts, FEW_ROWS) * cols, 8);
-    const int tail = p.g.starts ? (p.g.rows < 64 ? p.g.rows : 64) : 0;
-    few_kernel<T, GATED, LOOSE><<<(unsigned)(work + tail), FEW_THREADS, (GATED ? 2 : 1) * FEW_WAVES * most * 1024, s>>>(p, cols, (int)work);
+    const int64_t work = most_row_tiles(p.g.rows, p.g.experts, p.g.starts, FEW_ROWS) * cols;
+    few_kernel<T, GATED, LOOSE><<<(unsigned)(8 * ceil_div(work, 8)), FEW_THREADS, (GATED ? 2 : 1) * FEW_WAVES * most * 1024, s>>>(p, cols);
 }
 
 int launch_few(const LinearParams& p, int dtype, bool loose, hipStream_t s)

@@ -1,6 +1,6 @@
 // The tiles of the larger products: acc[p][q] += sum_k P[p][k] Q[q][k] on v_mfma_f32_16x16x32.
 //
-// p runs along a row of the result (so that a lane ends up with eight values in a row), q over its rows. A matrix comes either
+// p runs along a row of the result (so that a lane ends up with four values in a row), q over its rows. A matrix comes either
 // with k along its rows in memory, or (TR) with k over its rows: then LDS holds it as it lies in memory and ds_read_b64_tr_b16
 // turns it on the way to the registers. k-tiles of 64 come to LDS directly, two stages in turn.
 #pragma once
@@ -18,12 +18,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, uint3
                                              0x00027000);
 }
 
+// The rows that one turning read takes together (four of every eight, of sixteen) in eight places.
+__device__ __forceinline__ int turn(int row) { return (row & 3) | (row >> 1 & 4); }
+
 // One matrix of a workgroup's product: N values of p or q, by k.
 //   k along the rows:  value n is row map(n) of base, cut to `rows` rows, of `len` = K values.
 //   TR:                k is the row, cut to `rows` = K rows; value n is column n of base, cut to `len` columns.
 // In LDS in chunks of 16 bytes, in the order in which the direct loads write them; the chunks of a row are swapped by the row's low
 // bits (in the addresses that are loaded), so that what an instruction reads together lies in different banks.
-template <bool TR, int N, int WAVES, bool PERM, bool LOOSE>
+template <bool TR, int N, int WAVES, bool LOOSE>
 struct Side {
     static constexpr int BYTES = N * TILE_K * 2, LOADS = BYTES / 1024 / WAVES, ROW_CHUNKS = TR ? N / 8 : TILE_K / 8;
     static_assert(LOADS >= 1 && LOADS * WAVES * 1024 == BYTES);
@@ -31,8 +34,9 @@ struct Side {
     size_t stride;
     int rows, len;
     uint32_t at[LOADS];           // byte offsets of a lane's chunks (LOOSE: their row and first value, row << 8 | chunk)
+    __amdgpu_buffer_rsrc_t all;   // the whole of the matrix with k along its rows
 
-    static __device__ __forceinline__ int swap(int row) { return TR ? (row & 3) << (PERM ? 2 : 1) : row & 7; }
+    static __device__ __forceinline__ int swap(int row) { return TR ? turn(row) * 2 : row & 7; }
 
     template <class Map>
     __device__ __forceinline__ void init(const uint16_t* b, size_t s, int r, int l, Map map)
@@ -45,9 +49,13 @@ struct Side {
             const int from = TR ? row : map(row);
             at[i] = LOOSE ? (uint32_t)from << 8 | chunk : (uint32_t)from * (uint32_t)stride * 2 + chunk * 16;
         }
+        if constexpr (!TR && !LOOSE) all = buffer(base, rows <= 0 ? 0u : (uint32_t)((rows - 1) * stride + len) * 2);
     }
+    // k-tiles before this one end within the rows (TR: a descriptor a k-tile sees to that)
+    __device__ __forceinline__ int whole() const { return TR ? 1 << 30 : len / TILE_K; }
     // k-tile kt to LDS at `to`. Rows, columns and k that are not there become zeros; with TR, columns behind the last may hold the
     // next row's values, which end in results that are not stored.
+    template <bool WHOLE>         // the k-tile ends within the rows
     __device__ __forceinline__ void bring(char* to, int kt) const
     {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -77,40 +85,50 @@ struct Side {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)(to + (i * WAVES + wave) * 1024), 16, at[i],
                                                          0, 0, 0);
         } else {
-            const __amdgpu_buffer_rsrc_t src = buffer(base, rows <= 0 ? 0u : (uint32_t)((rows - 1) * stride + len) * 2);
-            const int left = len - k0;                                  // chunks behind the row's end: no address
+            const int left = len - k0;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int chunk = ((i * WAVES + wave) * 64 + lane) % ROW_CHUNKS ^ swap(((i * WAVES + wave) * 64 + lane) / ROW_CHUNKS);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)(to + (i * WAVES + wave) * 1024), 16,
-                                                         chunk * 8 < left ? at[i] + (uint32_t)k0 * 2 : 0xfffffff0u, 0, 0, 0);
+                // chunks behind the row's end: no address
+                const uint32_t from = WHOLE ? at[i] : chunk * 8 < left ? at[i] : 0xfffffff0u - (uint32_t)k0 * 2;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(all, (__attribute__((address_space(3))) void*)(to + (i * WAVES + wave) * 1024), 16, from,
+                                                         k0 * 2, 0, 0);
             }
         }
 #endif
     }
 };
 
+// Four rows of 16 values of LDS, of which lane l of 16 names the four values 4 (l % 4) of row l / 4, to four rows' values of
+// column l. restrict tells the compiler's count of open loads that what is under way to LDS goes elsewhere; without it each read
+// waits for all of them (x's gradient of 8192 rows, 4096 -> 7168: 529 us).
+__device__ __forceinline__ s16x4 turned(const char* __restrict__ p)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+#else
+    return s16x4{};
+#endif
+}
+
 // What a lane of a wave reads of a side: BLOCKS blocks of 16 values from block `first` on, lane c + 16 g the k 8 g .. 8 g + 7 of
-// each 32. With PERM blocks come in pairs: value c of block b of a pair is p = 8 (c / 4) + 4 b + c % 4 of its 32 (k along the rows: the
-// caller's map has put it there).
-template <bool TR, int N, int BLOCKS, bool PERM>
+// each 32.
+template <bool TR, int N, int BLOCKS>
 struct Reader {
-    static constexpr int BASES = !TR ? 2 : PERM ? BLOCKS / 2 : BLOCKS < 4 ? BLOCKS : 4;
+    static constexpr int BASES = TR ? BLOCKS : 2;
     uint32_t at[BASES];
 
-    __device__ __forceinline__ void init(int first)
+    // step: the half of a k-tile that read()'s step 0 is
+    __device__ __forceinline__ void init(int first, int step)
     {
         const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
         if constexpr (!TR) {
-            at[0] = (16 * first + c) * (TILE_K * 2) + ((g ^ (c & 7)) * 16);
+            at[0] = (16 * first + c) * (TILE_K * 2) + (((g + 4 * step) ^ (c & 7)) * 16);
             at[1] = at[0] ^ 64;
         } else {
-            const int row = 8 * g + (c >> 2), low = row & 3;
+            const int row = 32 * step + 8 * g + (c >> 2);
 #pragma unroll
-            for (int j = 0; j < BASES; ++j) {
-                const int chunk = PERM ? 4 * ((first / 2 + j) ^ low) + (c & 3) : 2 * ((first + j) ^ low) + ((c & 3) >> 1);
-                at[j] = row * (N * 2) + chunk * 16 + (PERM ? 0 : 8 * (c & 1));
-            }
+            for (int j = 0; j < BASES; ++j) at[j] = row * (N * 2) + ((first + j) ^ turn(row)) * 32 + 8 * (c & 3);
         }
     }
     __device__ __forceinline__ u16x8 read(const char* lds, int step, int b) const
@@ -119,10 +137,8 @@ struct Reader {
         if constexpr (!TR) {
             return *(const u16x8*)(lds + at[step] + b * (16 * TILE_K * 2));
         } else {
-            const char* p = lds + (PERM ? at[b >> 1] + 8 * (b & 1) : at[b & 3] + (b >> 2) * 128) + step * (32 * N * 2);
-            typedef __attribute__((address_space(3))) s16x4* lds4;
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * N * 2));
-            return __builtin_bit_cast(u16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            const char* p = lds + at[b] + step * (32 * N * 2);
+            return __builtin_bit_cast(u16x8, __builtin_shufflevector(turned(p), turned(p + 4 * N * 2), 0, 1, 2, 3, 4, 5, 6, 7));
         }
 #else
         return u16x8{};
@@ -142,62 +158,175 @@ __device__ __forceinline__ void arrive()                                // all w
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// WP by WQ waves of PB by QB blocks each.
-template <class T, bool PTR, bool QTR, int WP, int WQ, int PB, int QB, bool LOOSE>
+// WP by WQ waves of PB by QB blocks each, KW times: with KW = 2 each half of a k-tile is another wave's, and the two's sums meet in
+// LDS at the end. STAGES k-tiles in LDS.
+template <class T, bool PTR, bool QTR, int WP, int WQ, int PB, int QB, int KW, int STAGES, bool LOOSE>
 struct Gemm {
-    static constexpr int TP = 16 * PB * WP, TQ = 16 * QB * WQ, WAVES = WP * WQ;
-    typedef Side<PTR, TP, WAVES, true, LOOSE> P;
-    typedef Side<QTR, TQ, WAVES, false, LOOSE> Q;
-    static constexpr int STAGE = P::BYTES + Q::BYTES, LDS = 2 * STAGE;
+    static constexpr int TP = 16 * PB * WP, TQ = 16 * QB * WQ, WAVES = WP * WQ * KW, THREADS = 64 * WAVES;
+    typedef Side<PTR, TP, WAVES, LOOSE> P;
+    typedef Side<QTR, TQ, WAVES, LOOSE> Q;
+    static constexpr int STAGE = P::BYTES + Q::BYTES, JOIN = KW == 1 ? 0 : WP * WQ * PB * QB * 1024;
+    static constexpr int OUT = WP * WQ * (64 * 68 * 4);
+    static constexpr int LDS = STAGES * STAGE > JOIN ? STAGES * STAGE > OUT ? STAGES * STAGE : OUT : JOIN > OUT ? JOIN : OUT;
 
-    // Lane c + 16 g: acc[2 j + b][q][i] belongs to p = 32 j + 8 g + 4 b + i of the wave's 16 PB and row 16 q + c of its 16 QB.
-    // A k-tile is two phases of 32 k: while one's products run, the next one's operands are read; the barrier lies before the second,
-    // when a wave has read all it needs of the k-tile, whose place the k-tile after the next then takes.
-    static __device__ __forceinline__ void run(f32x4 (&acc)[PB][QB], const P& p, const Q& q, char* lds, int kt0, int kt1)
+    static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+    static __device__ __forceinline__ int wp() { return wave() % WP; }
+    static __device__ __forceinline__ int wq() { return wave() / WP % WQ; }
+    static __device__ __forceinline__ int kw() { return wave() / (WP * WQ); }
+
+    // Lane c + 16 g: acc[b][q][i] belongs to p = 16 b + 4 g + i of the wave's 16 PB and row 16 q + c of its 16 QB.
+    // With KW = 2 the sums are those of the waves with kw() = 0; the others return false.
+    //
+    // The barrier of a k-tile lies where a wave has read all it needs of it: its place then takes the k-tile STAGES further, and the
+    // next one's first operands are read while the last products of this one run.
+    static __device__ __forceinline__ bool run(f32x4 (&acc)[PB][QB], const P& p, const Q& q, char* lds, int kt0, int kt1)
     {
 #ifdef __HIP_DEVICE_COMPILE__
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        Reader<PTR, TP, PB, true> rp;
-        Reader<QTR, TQ, QB, false> rq;
-        rp.init(PB * (wave % WP));
-        rq.init(QB * (wave / WP));
+        const int half = KW == 2 ? kw() : 0;
+        Reader<PTR, TP, PB> rp;
+        Reader<QTR, TQ, QB> rq;
+        rp.init(PB * wp(), half);
+        rq.init(QB * wq(), half);
         u16x8 a[2][PB], b[2][QB];
-        auto read = [&](int slot, int step) {
+        auto read = [&](int set, const char* from, int step) {
 #pragma unroll
-            for (int i = 0; i < PB; ++i) a[step][i] = rp.read(lds + slot, step, i);
+            for (int i = 0; i < PB; ++i) a[set][i] = rp.read(from, step, i);
 #pragma unroll
-            for (int i = 0; i < QB; ++i) b[step][i] = rq.read(lds + slot + P::BYTES, step, i);
+            for (int i = 0; i < QB; ++i) b[set][i] = rq.read(from + P::BYTES, step, i);
         };
-        auto products = [&](int step) {
+        auto products = [&](int set) {
 #pragma unroll
             for (int j = 0; j < QB; ++j)
 #pragma unroll
-                for (int i = 0; i < PB; ++i) acc[i][j] = T::mfma(a[step][i], b[step][j], acc[i][j]);
+                for (int i = 0; i < PB; ++i) acc[i][j] = T::mfma(a[set][i], b[set][j], acc[i][j]);
         };
-        auto bring = [&](int slot, int kt) {
-            p.bring(lds + slot, kt);
-            q.bring(lds + slot + P::BYTES, kt);
+        auto bring = [&](int slot, int kt, auto whole) {
+            p.template bring<decltype(whole)::value>(lds + slot, kt);
+            q.template bring<decltype(whole)::value>(lds + slot + P::BYTES, kt);
         };
-        if (kt0 >= kt1) return;
-        bring(0, kt0);
-        if (kt0 + 1 < kt1) bring(STAGE, kt0 + 1);
-        if (kt0 + 1 < kt1) wait_loads<LOOSE ? 0 : P::LOADS + Q::LOADS>();
-        else wait_loads<0>();
-        arrive();
-        read(0, 0);
-        int now = 0;
-        for (int kt = kt0; kt < kt1; ++kt) {
-            read(now, 1);
-            products(0);
-            wait_loads<0>();
+        constexpr int LOADS = P::LOADS + Q::LOADS;
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+        // operands of the next products between these: the reads spread over the first of them
+        auto mix = [&] {
+            constexpr int READS = (PTR ? 2 : 1) * PB + (QTR ? 2 : 1) * QB, EACH = PB * QB / READS > 1 ? 2 : 1;
+#pragma unroll
+            for (int i = 0; i < READS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, PB * QB - EACH * READS, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // k-tile kt has come for all waves, of which later ones are under way
+        auto come = [&](auto later) {
+            wait_loads<LOOSE ? 0 : decltype(later)::value * LOADS>();
             arrive();
-            if (kt + 2 < kt1) bring(now, kt + 2);
-            now ^= STAGE;
-            if (kt + 1 < kt1) read(now, 0);
-            products(1);
+        };
+        if (kt0 < kt1) {
+#pragma unroll
+            for (int i = 0; i < STAGES; ++i)
+                if (kt0 + i < kt1) bring(i * STAGE, kt0 + i, no);
+            if (kt0 + STAGES - 1 < kt1) come(std::integral_constant<int, STAGES - 1>());
+            else come(std::integral_constant<int, 0>());
+            int now = 0, kt = kt0;
+            auto next = [&] { return now == (STAGES - 1) * STAGE ? 0 : now + STAGE; };
+            // MORE: this k-tile's place takes another, which is whole
+            auto arrive_next = [&](auto more) {
+                if constexpr (decltype(more)::value) {
+                    come(std::integral_constant<int, STAGES - 2>());
+                    bring(now, kt + STAGES, yes);
+                } else {
+                    come(std::integral_constant<int, 0>());
+                    if (kt + STAGES < kt1) bring(now, kt + STAGES, no);
+                }
+                now = next();
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            const int whole = (p.whole() < q.whole() ? p.whole() : q.whole()) < kt1 ? (p.whole() < q.whole() ? p.whole() : q.whole()) : kt1;
+            if constexpr (KW == 1) {
+                auto step = [&](auto more) {
+                    read(1, lds + now, 1);
+                    products(0);
+                    mix();
+                    arrive_next(more);
+                    read(0, lds + now, 0);              // behind the last k-tile: what is there, for no product
+                    products(1);
+                    mix();
+                    ++kt;
+                };
+                read(0, lds, 0);
+                while (kt + STAGES < whole) step(yes);
+                while (kt < kt1) step(no);
+            } else {
+                auto step = [&](int set, auto more) {
+                    arrive_next(more);
+                    read(set ^ 1, lds + now, 0);
+                    products(set);
+                    mix();
+                    ++kt;
+                };
+                read(0, lds, 0);
+                while (kt + 1 + STAGES < whole) {
+                    step(0, yes);
+                    step(1, yes);
+                }
+                while (kt + 1 < kt1) {
+                    step(0, no);
+                    step(1, no);
+                }
+                if (kt < kt1) step(0, no);
+            }
+        }
+        __syncthreads();
+        if constexpr (KW == 2) {
+            f32x4* join = (f32x4*)lds + (wave() % (WP * WQ)) * (PB * QB * 64) + (threadIdx.x & 63);
+            if (half) {
+#pragma unroll
+                for (int i = 0; i < PB; ++i)
+#pragma unroll
+                    for (int j = 0; j < QB; ++j) join[(i * QB + j) * 64] = acc[i][j];
+            }
+            __syncthreads();
+            if (!half) {
+#pragma unroll
+                for (int i = 0; i < PB; ++i)
+#pragma unroll
+                    for (int j = 0; j < QB; ++j) acc[i][j] += join[(i * QB + j) * 64];
+            }
+            __syncthreads();
+            return !half;
         }
 #endif
+        return true;
     }
 };
+
+// A wave's results by way of LDS: 16 PB columns of 64 rows at a time, rows ROW floats apart, so that a lane gets eight values
+// in a row, neighbours the next eight, and the code that takes them is there once. f(row of the wave's 16 QB, eight columns, values).
+constexpr int OUT_ROW = 68, OUT_ROWS = 64, OUT_BYTES = OUT_ROWS * OUT_ROW * 4;
+
+template <int PB, int QB, class F>
+__device__ __forceinline__ void rows_of(const f32x4 (&acc)[PB][QB], char* lds, int slot, F f)
+{
+    static_assert(PB == 4);
+    constexpr int QH = QB < 4 ? QB : 4;
+    float* mine = (float*)(lds + slot * OUT_BYTES);
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int half = 0; half < QB / QH; ++half) {
+#pragma unroll
+        for (int j = 0; j < QH; ++j)
+#pragma unroll
+            for (int i = 0; i < PB; ++i) *(f32x4*)(mine + (16 * j + c) * OUT_ROW + 16 * i + 4 * g) = acc[i][half * QH + j];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        f(mine, half * QH * 16, QH * 16);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
 
 }  // namespace evamx_dense

@@ -1,5 +1,7 @@
 // The gradients of act(x W^T + b): D = act'(pre) grad, W's D^T x, the bias's column sums of D. x's, D W, is a product as the
 // forward one (tiles.hip).
+#include <stdlib.h>
+
 #include "grads.hpp"
 
 namespace evamx_dense {
@@ -18,10 +20,9 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p)
     load8(gr, p.grad + (size_t)row * p.grad_stride + n, have, BF);
     const float* pre = p.pre + (size_t)row * p.n_out + n;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = i < have ? pre[i] : 0.0f;
-        if (GATED) u[i] = i < have ? pre[cols + i] : 0.0f;
-    }
+    for (int i = 0; i < 8; ++i) v[i] = u[i] = 0;
+    add_floats(v, pre, have);
+    if (GATED) add_floats(u, pre + cols, have);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         if (GATED) {
@@ -51,11 +52,11 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p)
 }
 
 // W's gradient: result rows q = n of W, p = k. The sum runs over the expert's rows, in tiles of 64.
-template <class T, bool LOOSE, int WP, int WQ, int QB>
-__global__ __launch_bounds__(64 * WP * WQ, 2) void weight_grad_kernel(WeightGradParams p)
+template <class T, bool LOOSE, int WP, int WQ, int QB, int KW>
+__global__ __launch_bounds__(64 * WP * WQ * KW, 2) void weight_grad_kernel(WeightGradParams p)
 {
     constexpr int PB = 4;
-    typedef Gemm<T, true, true, WP, WQ, PB, QB, LOOSE> G;
+    typedef Gemm<T, true, true, WP, WQ, PB, QB, KW, 2, LOOSE> G;
     __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
     const int pt = (p.n_in + G::TP - 1) / G::TP, qt = (p.n_out + G::TQ - 1) / G::TQ, tiles = pt * qt;
     // an XCD takes a contiguous run of tiles, eight tiles of n by all of k at a time
@@ -70,38 +71,33 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void weight_grad_kernel(WeightGrad
     b.init(p.d + (size_t)begin * p.d_stride + q0, p.d_stride, count, p.n_out - q0, [](int n) { return n; });
     f32x4 acc[PB][QB] = {};
     const int kt = (count + TILE_K - 1) / TILE_K, k0 = (int)((long)kt * blockIdx.z / p.splits), k1 = (int)((long)kt * (blockIdx.z + 1) / p.splits);
-    G::run(acc, a, b, lds, k0, k1);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    const int wp = wave % WP, wq = wave / WP;
+    if (!G::run(acc, a, b, lds, k0, k1)) return;
+    const int lane = threadIdx.x & 63, wp = G::wp(), wq = G::wq(), k = p0 + 64 * wp + 8 * (lane & 7), have = p.n_in - k;
+    rows_of<PB, QB>(acc, lds, wq * WP + wp, [&](const float* mine, int first, int count) {
+        if (have <= 0) return;
+        for (int r = lane >> 3; r < count; r += 8) {
+            const int q = q0 + 16 * QB * wq + first + r;
+            if (q >= p.n_out) break;
+            float v[8];
 #pragma unroll
-    for (int j = 0; j < QB; ++j) {
-        const int q = q0 + 16 * (QB * wq + j) + c;
-        if (q >= p.n_out) continue;
-        const size_t row = (size_t)e * p.n_out + q;
-#pragma unroll
-        for (int h = 0; h < PB / 2; ++h) {
-            const int k = p0 + 64 * wp + 32 * h + 8 * g, have = p.n_in - k;
-            if (have <= 0) continue;
+            for (int i = 0; i < 8; ++i) v[i] = mine[r * OUT_ROW + 8 * (lane & 7) + i];
             if (p.splits > 1) {
-                float* part = p.part + ((size_t)blockIdx.z * p.n_out + q) * p.n_in + k;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < have) part[i] = acc[2 * h + i / 4][j][i % 4];
+                store_floats(p.part + ((size_t)blockIdx.z * p.n_out + q) * p.n_in + k, v, have);
                 continue;
             }
-            uint16_t* out = p.out + row * p.n_in + k;
+            uint16_t* out = p.out + ((size_t)e * p.n_out + q) * p.n_in + k;
             if (have >= 8) {
                 u16x8 o;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = T::put(acc[2 * h + i / 4][j][i % 4]);
+                for (int i = 0; i < 8; ++i) o[i] = T::put(v[i]);
                 *(u16x8_loose*)out = o;
             } else {
 #pragma unroll
                 for (int i = 0; i < 7; ++i)
-                    if (i < have) out[i] = T::put(acc[2 * h + i / 4][j][i % 4]);
+                    if (i < have) out[i] = T::put(v[i]);
             }
         }
-    }
+    });
 }
 
 // Sums of `count` arrays of n values each, rounded; array s of value i of matrix y: part[(y * count + s) * n + i].
@@ -165,11 +161,11 @@ int launch_act_grad(const ActGradParams& p, int dtype, hipStream_t s)
     return launched("linear_grad");
 }
 
-template <class T, bool LOOSE, int WP, int WQ, int QB>
+template <class T, bool LOOSE, int WP, int WQ, int QB, int KW>
 static void launch_weight_grad_as(const WeightGradParams& p, hipStream_t s)
 {
     const int64_t tiles = (int64_t)ceil_div(p.n_in, 64 * WP) * ceil_div(p.n_out, 16 * QB * WQ);
-    weight_grad_kernel<T, LOOSE, WP, WQ, QB><<<dim3((unsigned)(8 * ceil_div(tiles, 8)), p.g.experts, p.splits), 64 * WP * WQ, 0, s>>>(p);
+    weight_grad_kernel<T, LOOSE, WP, WQ, QB, KW><<<dim3((unsigned)(8 * ceil_div(tiles, 8)), p.g.experts, p.splits), 64 * WP * WQ * KW, 0, s>>>(p);
 }
 
 int launch_weight_grad(const WeightGradParams& p, int dtype, bool loose, hipStream_t s)
@@ -177,9 +173,12 @@ int launch_weight_grad(const WeightGradParams& p, int dtype, bool loose, hipStre
     by_type(dtype, [&](auto type) {
         typedef decltype(type) T;
         const int64_t big = (int64_t)ceil_div(p.n_in, 256) * ceil_div(p.n_out, 256) * p.g.experts;
-        if (loose) launch_weight_grad_as<T, true, 2, 2, 4>(p, s);
-        else if (p.splits == 1 && big >= CUS / 2 && p.g.rows / p.g.experts >= 1024) launch_weight_grad_as<T, false, 4, 2, 8>(p, s);
-        else launch_weight_grad_as<T, false, 2, 2, 4>(p, s);
+        static const char* force = getenv("DW_SIZE");
+        const int size = force ? atoi(force) : p.splits == 1 && big >= 200 ? 2 : 0;
+        if (loose) launch_weight_grad_as<T, true, 2, 1, 8, 2>(p, s);
+        else if (size == 2) launch_weight_grad_as<T, false, 4, 2, 8, 1>(p, s);
+        else if (size == 1) launch_weight_grad_as<T, false, 2, 2, 4, 1>(p, s);
+        else launch_weight_grad_as<T, false, 2, 1, 8, 2>(p, s);
         if (p.splits > 1) {
             const int64_t n = (int64_t)p.n_out * p.n_in;
             sum_parts_kernel<T><<<dim3((unsigned)ceil_div(n, 256), 1), 256, 0, s>>>(p.part, p.splits, n, p.out);

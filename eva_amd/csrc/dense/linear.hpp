@@ -71,12 +71,8 @@ __device__ __forceinline__ void finish(const LinearParams& p, int expert, int ro
     }
     if (p.pre) {
         float* at = p.pre + (size_t)row * p.n_out + n;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < have) {
-                at[i] = v[i];
-                if (GATED) at[p.inter + i] = u[i];
-            }
+        store_floats(at, v, have);
+        if (GATED) store_floats(at + p.inter, u, have);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = GATED ? swiglu(v[i], u[i], p.limit) : activate(v[i], p.act);
