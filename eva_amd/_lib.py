@@ -140,9 +140,9 @@ _SIGNATURES = {
 _DENSE_SIGNATURES = {
     "evamx_dense_last_error": (ctypes.c_char_p, []),
     "evamx_dense_version": (ctypes.c_int, []),
-    "evamx_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "evamx_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
     "evamx_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), _vp]),
-    "evamx_linear_grad_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "evamx_linear_grad_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 7),
     "evamx_linear_grad": (ctypes.c_int, [ctypes.POINTER(LinearGradArgs), _vp]),
 }
 

@@ -28,43 +28,79 @@ constexpr int MAX_ROWS = 1 << 24, MAX_SPLITS = 16;
 
 static size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Parts of a sum of `k_tiles` for a result of `tiles` tiles of 128 by 128, so that a GPU's worth of workgroups runs: each adds its
-// partial sums' way through memory, so it takes at least `least` k-tiles.
-static int splits_of(int64_t tiles, int k_tiles, int least)
+static Plan plan_with(int64_t rows, int64_t cols, int64_t k, double& least)
 {
-    if (tiles >= CUS || tiles == 0) return 1;
-    int64_t n = (2 * CUS + tiles - 1) / tiles;
-    if (n > k_tiles / least) n = k_tiles / least;
-    if (n > MAX_SPLITS) n = MAX_SPLITS;
-    return n < 1 ? 1 : (int)n;
+    const int64_t kt = (k + TILE_K - 1) / TILE_K;
+    Plan best = {TILES_256, 1};
+    least = 1e30;
+    for (int size = TILES_128; size <= TILES_256; size += TILES_256 - TILES_128)
+        for (int splits = 1; splits <= MAX_SPLITS && (splits == 1 || kt / splits >= 4); ++splits) {
+            const int64_t edge = size == TILES_256 ? 256 : 128, at_once = size == TILES_256 ? CUS : 2 * CUS;
+            const int64_t work = ((rows + edge - 1) / edge) * ((cols + edge - 1) / edge) * splits, rest = work % at_once;
+            const double each = (double)((kt + splits - 1) / splits);
+            auto round = [&](int64_t n) {
+                const double x = size == TILES_256 ? 1.2 + 0.35 * n / CUS : n <= CUS ? 0.7 : 0.7 + 0.35 * (n - CUS) / CUS;
+                return each * x + 6;
+            };
+            double time = (double)(work / at_once) * round(at_once) + (rest ? round(rest) : 0);
+            if (splits > 1) time += 4 + 2.0 * splits * rows * cols * 4 / 4.5e6;
+            if (time < least) {
+                least = time;
+                best = {size, splits};
+            }
+        }
+    return best;
 }
 
-static bool few_rows(int rows, int experts, bool grouped) { return grouped ? rows <= 32 * experts : rows <= 64; }
-
-static int forward_splits(int rows, int k, int n, bool grouped)
+Plan plan_of(int64_t rows, int64_t cols, int64_t k)
 {
-    return grouped ? 1 : splits_of((int64_t)ceil_div(rows, 128) * ceil_div(n, 128), ceil_div(k, TILE_K), 4);
+    double least;
+    return plan_with(rows, cols, k, least);
 }
-static size_t forward_part(int rows, int k, int n, bool grouped)
+
+// Whether few.hip takes a call: for one matrix where its time (5 us, the weights at 4.9 TB/s, and the rows of x, which each workgroup
+// reads, at 8.5) is below the tiles', up to 64 rows (measured, us, at 1, 16 and 64 rows: 7168 -> 2048: 12, 16, 35 against 19, 20, 21;
+// 7168 -> 18432: 53, 82, 188 against 56, 56, 62); for experts up to four rows for each, of which most may be another rank's (64 experts of
+// 4096 by 7168 at 4 rows: 742 against 662; 25 of them at one row: 294, all of it the weights).
+static bool few_rows(int rows, int k, int n, int experts, bool grouped)
 {
-    const int s = forward_splits(rows, k, n, grouped);
+    if (grouped) return rows <= 4 * (int64_t)experts;
+    if (rows > 64) return false;
+    double tiles;
+    plan_with(rows, n, k, tiles);
+    const double blocks = rows > 32 ? 4 : rows > 16 ? 2 : 1, x = ceil_div(n, rows > 8 && n >= 24 * CUS ? 32 : 16) * 16.0 * blocks * k * 2;
+    return 5 + (double)n * k * 2 / 4.9e6 + (rows > 2 ? x / 8.5e6 : 0) <= tiles;
+}
+
+// Experts' rows are known to the device alone: large tiles (which the kernel takes by halves and quarters where an expert ends), if
+// the most there can be fill the GPU.
+static Plan forward_plan(int rows, int k, int n, int experts, bool grouped)
+{
+    if (!grouped) return plan_of(rows, n, k);
+    return {most_row_tiles(rows, experts, true, 256) * ceil_div(n, 256) >= CUS * 3 / 4 ? TILES_256 : TILES_128, 1};
+}
+static size_t forward_part(int rows, int k, int n, int experts, bool grouped)
+{
+    const int s = forward_plan(rows, k, n, experts, grouped).splits;
     return s > 1 ? align256((size_t)s * rows * n * 4) : 0;
 }
-static int weight_splits(int rows, int n_in, int n_out, bool grouped)
+static Plan weight_plan(int rows, int n_in, int n_out, int experts, bool grouped)
 {
-    return grouped ? 1 : splits_of((int64_t)ceil_div(n_in, 128) * ceil_div(n_out, 128), ceil_div(rows, TILE_K), 4);
+    if (!grouped) return plan_of(n_out, n_in, rows);
+    return {(int64_t)ceil_div(n_out, 256) * ceil_div(n_in, 256) * experts >= CUS * 3 / 4 ? TILES_256 : TILES_128, 1};
 }
-static size_t weight_part(int rows, int n_in, int n_out, bool grouped)
+static size_t weight_part(int rows, int n_in, int n_out, int experts, bool grouped)
 {
-    const int s = weight_splits(rows, n_in, n_out, grouped);
+    const int s = weight_plan(rows, n_in, n_out, experts, grouped).splits;
     return s > 1 ? align256((size_t)s * n_in * n_out * 4) : 0;
 }
+// Runs of rows whose column sums are made apart: enough for the GPU, at least 32 rows each.
 static int column_parts(int rows, int n_out, int experts)
 {
     const int64_t groups = (int64_t)ceil_div(n_out, 512) * experts;
-    int64_t n = (4 * CUS + groups - 1) / groups;
+    int64_t n = (CUS + groups - 1) / groups;
     if (n > rows / 32) n = rows / 32;
-    if (n > 64) n = 64;
+    if (n > 32) n = 32;
     return n < 1 ? 1 : (int)n;
 }
 static size_t column_part(int rows, int n_out, int experts)
@@ -103,10 +139,33 @@ static bool space_ok(const char* who, const void* ws, size_t have, size_t need)
     return true;
 }
 
-// Rows that the direct loads take: 16-byte addresses and lengths, 32-bit offsets.
-static bool direct(const void* p, int64_t stride, int64_t rows, int len)
+// Rows that tiles take as they are: 16-byte addresses and lengths, and strides whose multiples in a tile stay 32-bit offsets.
+static bool direct(const void* p, int64_t stride, int len)
 {
-    return (((uintptr_t)p | (uintptr_t)(2 * stride)) & 15) == 0 && len % 8 == 0 && (rows + 512) * stride * 2 < 0xf0000000ll;
+    return (((uintptr_t)p | (uintptr_t)(2 * stride)) & 15) == 0 && len % 8 == 0 && stride <= 1 << 21;
+}
+
+static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+static size_t padded(int64_t rows, int n) { return align256((size_t)rows * pad8(n) * 2); }
+
+// Rows that tiles take: as they are, or copied to `at`, which moves on.
+struct Rows {
+    const uint16_t* p;
+    int64_t stride, matrix_stride;
+};
+static int ready(Rows& r, bool as_is, int64_t rows, int count, int n, char*& at, hipStream_t s)
+{
+    if (as_is) return EVAMX_OK;
+    uint16_t* to = (uint16_t*)at;
+    at += padded(rows * count, n);
+    const int rc = launch_pad(r.p, (size_t)r.stride, (size_t)r.matrix_stride, (int)rows, count, n, to, s);
+    r = Rows{to, pad8(n), rows * pad8(n)};
+    return rc;
+}
+static int lie_of(const void* p, int64_t stride, int64_t matrix_stride)
+{
+    const uint64_t all = (uint64_t)(uintptr_t)p | (uint64_t)(2 * stride) | (uint64_t)(2 * matrix_stride);
+    return all & 3 ? LIE_2 : all & 15 ? LIE_4 : LIE_16;
 }
 
 }  // namespace evamx_dense
@@ -116,11 +175,22 @@ using namespace evamx_dense;
 extern "C" const char* evamx_dense_last_error(void) { return g_error; }
 extern "C" int evamx_dense_version(void) { return EVAMX_DENSE_VERSION; }
 
-extern "C" size_t evamx_linear_workspace_bytes(int rows, int n_in, int n_out, int experts, int grouped)
+// What a call may copy of x and w: both, unless their sizes rule it out (their addresses and strides are the call's).
+static size_t forward_copies(int rows, int n_in, int n_out, int experts) { return padded(rows, n_in) + padded((int64_t)n_out * experts, n_in); }
+
+extern "C" size_t evamx_linear_workspace_bytes(int rows, int n_in, int n_out, int experts, int grouped, int direct)
 {
     set_error("%s", "");
     if (!sizes_ok("evamx_linear_workspace_bytes", rows, n_in, n_out, experts, grouped)) return 0;
-    return few_rows(rows, experts, grouped) ? 0 : forward_part(rows, n_in, n_out, grouped);
+    if (few_rows(rows, n_in, n_out, experts, grouped)) return 0;
+    return forward_part(rows, n_in, n_out, experts, grouped) + (direct ? 0 : forward_copies(rows, n_in, n_out, experts));
+}
+
+// Whether a forward call takes x and w as they are.
+static bool x_direct(const evamx_linear_args* a) { return direct(a->x, a->x_stride, a->n_in); }
+static bool w_direct(const void* w, int64_t stride, int64_t matrix, int experts, int n_in)
+{
+    return direct(w, stride, n_in) && (experts == 1 || matrix % 8 == 0);
 }
 
 extern "C" int evamx_linear(const evamx_linear_args* a, evamx_stream_t stream)
@@ -139,34 +209,55 @@ extern "C" int evamx_linear(const evamx_linear_args* a, evamx_stream_t stream)
     }
     if (a->rows == 0) return EVAMX_OK;
     if (!a->x || !a->w || !a->y) { set_error("%s: null pointer", who); return EVAMX_EINVAL; }
-    const size_t need = evamx_linear_workspace_bytes(a->rows, a->n_in, a->n_out, a->experts, grouped);
+    const bool xd = x_direct(a), wd = w_direct(a->w, a->w_stride, a->w_expert_stride, a->experts, a->n_in);
+    const size_t need = evamx_linear_workspace_bytes(a->rows, a->n_in, a->n_out, a->experts, grouped, xd && wd);
     if (!space_ok(who, a->workspace, a->workspace_bytes, need)) return need > a->workspace_bytes && a->workspace ? EVAMX_ENOSPACE : EVAMX_EINVAL;
     LinearParams p = {};
-    p.x = (const uint16_t*)a->x; p.w = (const uint16_t*)a->w; p.bias = (const uint16_t*)a->bias; p.residual = (const uint16_t*)a->residual;
+    Rows x = {(const uint16_t*)a->x, a->x_stride, 0}, w = {(const uint16_t*)a->w, a->w_stride, a->experts > 1 ? a->w_expert_stride : 0};
+    p.bias = (const uint16_t*)a->bias; p.residual = (const uint16_t*)a->residual;
     p.y = (uint16_t*)a->y; p.pre = a->pre;
-    p.x_stride = (size_t)a->x_stride; p.w_stride = (size_t)a->w_stride; p.w_expert_stride = (size_t)a->w_expert_stride;
     p.residual_stride = (size_t)a->residual_stride; p.y_stride = (size_t)a->y_stride;
     p.g = Groups{a->starts, a->experts, a->rows};
     p.n_in = a->n_in; p.n_out = a->n_out; p.inter = a->act == EVAMX_ACT_SWIGLU ? cols : 0;
     p.act = a->act; p.limit = a->limit;
     p.splits = 1;
-    const bool loose = !direct(a->x, a->x_stride, 256, a->n_in) || !direct(a->w, a->w_stride, a->n_out, a->n_in) ||
-                       (a->experts > 1 && a->w_expert_stride % 8);
-    if (few_rows(a->rows, a->experts, grouped)) return launch_few(p, a->dtype, loose, (hipStream_t)stream);
-    p.splits = forward_splits(a->rows, a->n_in, a->n_out, grouped);
-    p.part = (float*)a->workspace;
-    return launch_tiles(p, a->dtype, false, loose, (hipStream_t)stream);
+    const hipStream_t s = (hipStream_t)stream;
+    const bool few = few_rows(a->rows, a->n_in, a->n_out, a->experts, grouped);
+    if (!few) {
+        char* at = (char*)a->workspace;
+        int rc = ready(x, xd, a->rows, 1, a->n_in, at, s);
+        if (rc == EVAMX_OK) rc = ready(w, wd, a->n_out, a->experts, a->n_in, at, s);
+        if (rc != EVAMX_OK) return rc;
+        const Plan plan = forward_plan(a->rows, a->n_in, a->n_out, a->experts, grouped);
+        p.size = plan.size; p.splits = plan.splits; p.part = (float*)at;
+        p.x_cols = p.w_cols = (int)pad8(a->n_in);
+        if (p.inter && (a->n_out + 512) * w.stride * 2 >= 0xf0000000ll) {    // one descriptor spans the gate's and the up product's rows
+            set_error("%s: a SwiGLU matrix of %d rows %lld apart", who, a->n_out, (long long)w.stride);
+            return EVAMX_EINVAL;
+        }
+    }
+    p.x = x.p; p.x_stride = (size_t)x.stride; p.w = w.p; p.w_stride = (size_t)w.stride; p.w_expert_stride = (size_t)w.matrix_stride;
+    if (!few) return launch_tiles(p, a->dtype, false, s);
+    const int lx = lie_of(a->x, a->x_stride, 0), lw = lie_of(a->w, a->w_stride, a->experts > 1 ? a->w_expert_stride : 0);
+    const int lie = lx > lw ? lx : lw;
+    return launch_few(p, a->dtype, lie == LIE_16 && a->n_in % 8 ? LIE_4 : lie, s);
 }
 
-extern "C" size_t evamx_linear_grad_workspace_bytes(int rows, int n_in, int n_out, int experts, int grouped, int act)
+// What a gradient call may copy: D (where there is no activation to write it anew), x and w.
+static size_t grad_copies(int rows, int n_in, int n_out, int experts)
+{
+    return padded(rows, n_out) + padded(rows, n_in) + padded((int64_t)n_out * experts, n_in);
+}
+
+extern "C" size_t evamx_linear_grad_workspace_bytes(int rows, int n_in, int n_out, int experts, int grouped, int act, int direct)
 {
     set_error("%s", "");
     if (!sizes_ok("evamx_linear_grad_workspace_bytes", rows, n_in, n_out, experts, grouped)) return 0;
-    size_t part = forward_part(rows, n_out, n_in, grouped);
-    const size_t w = weight_part(rows, n_in, n_out, grouped), c = column_part(rows, n_out, experts);
+    size_t part = forward_part(rows, n_out, n_in, experts, grouped);
+    const size_t w = weight_part(rows, n_in, n_out, experts, grouped), c = column_part(rows, n_out, experts);
     if (w > part) part = w;
     if (c > part) part = c;
-    return part + (act != EVAMX_ACT_NONE ? align256((size_t)rows * ((n_out + 7) / 8 * 8) * 2) : 0);
+    return part + (direct ? act != EVAMX_ACT_NONE ? padded(rows, n_out) : 0 : grad_copies(rows, n_in, n_out, experts));
 }
 
 extern "C" int evamx_linear_grad(const evamx_linear_grad_args* a, evamx_stream_t stream)
@@ -187,44 +278,49 @@ extern "C" int evamx_linear_grad(const evamx_linear_grad_args* a, evamx_stream_t
         set_error("%s: null pointer", who);
         return EVAMX_EINVAL;
     }
-    const size_t need = evamx_linear_grad_workspace_bytes(a->rows, a->n_in, a->n_out, a->experts, grouped, a->act);
+    const bool act = a->act != EVAMX_ACT_NONE;
+    const bool dd = act || direct(a->grad, a->grad_stride, a->n_out), xd = direct(a->x, a->x_stride, a->n_in);
+    const bool wd = w_direct(a->w, a->w_stride, a->w_expert_stride, a->experts, a->n_in);
+    const bool all = dd && (!a->grad_w || xd) && (!a->grad_x || wd);
+    const size_t need = evamx_linear_grad_workspace_bytes(a->rows, a->n_in, a->n_out, a->experts, grouped, a->act, all);
     if (!space_ok(who, a->workspace, a->workspace_bytes, need)) return need > a->workspace_bytes && a->workspace ? EVAMX_ENOSPACE : EVAMX_EINVAL;
     const hipStream_t s = (hipStream_t)stream;
     const Groups g{a->starts, a->experts, a->rows};
-    const uint16_t* d = (const uint16_t*)a->grad;
-    size_t d_stride = (size_t)a->grad_stride;
-    char* ws = (char*)a->workspace;
-    if (a->act != EVAMX_ACT_NONE) {
-        d_stride = (size_t)(a->n_out + 7) / 8 * 8;
-        uint16_t* out = (uint16_t*)ws;
-        ws += align256((size_t)a->rows * d_stride * 2);
-        d = out;
-        if (a->rows) {
-            const int rc = launch_act_grad(ActGradParams{(const uint16_t*)a->grad, (size_t)a->grad_stride, a->pre, out, d_stride, g, a->n_out,
-                                                         a->act, a->limit}, a->dtype, s);
-            if (rc != EVAMX_OK) return rc;
-        }
+    char* at = (char*)a->workspace;
+    Rows d = {(const uint16_t*)a->grad, a->grad_stride, 0}, x = {(const uint16_t*)a->x, a->x_stride, 0};
+    Rows w = {(const uint16_t*)a->w, a->w_stride, a->experts > 1 ? a->w_expert_stride : 0};
+    int rc = EVAMX_OK;
+    if (act) {
+        uint16_t* out = (uint16_t*)at;
+        at += padded(a->rows, a->n_out);
+        d = Rows{out, pad8(a->n_out), 0};
+        if (a->rows)
+            rc = launch_act_grad(ActGradParams{(const uint16_t*)a->grad, (size_t)a->grad_stride, a->pre, out, (size_t)d.stride, g, a->n_out, a->act,
+                                               a->limit}, a->dtype, s);
+    } else if (a->rows && (a->grad_x || a->grad_w)) {
+        rc = ready(d, dd, a->rows, 1, a->n_out, at, s);
     }
-    const bool loose_d = !direct(d, (int64_t)d_stride, 256, a->n_out);
+    if (rc == EVAMX_OK && a->grad_w && a->rows) rc = ready(x, xd, a->rows, 1, a->n_in, at, s);
+    if (rc == EVAMX_OK && a->grad_x && a->rows) rc = ready(w, wd, a->n_out, a->experts, a->n_in, at, s);
+    if (rc != EVAMX_OK) return rc;
     if (a->grad_x && a->rows) {
         LinearParams p = {};
-        p.x = d; p.x_stride = d_stride; p.w = (const uint16_t*)a->w; p.w_stride = (size_t)a->w_stride; p.w_expert_stride = (size_t)a->w_expert_stride;
+        p.x = d.p; p.x_stride = (size_t)d.stride; p.w = w.p; p.w_stride = (size_t)w.stride; p.w_expert_stride = (size_t)w.matrix_stride;
         p.y = (uint16_t*)a->grad_x; p.y_stride = (size_t)a->grad_x_stride;
-        p.g = g; p.n_in = a->n_out; p.n_out = a->n_in;
-        p.splits = forward_splits(a->rows, a->n_out, a->n_in, grouped);
-        p.part = (float*)ws;
-        const bool loose = loose_d || !direct(a->w, a->w_stride, TILE_K, a->n_in) || (a->experts > 1 && a->w_expert_stride % 8);
-        const int rc = launch_tiles(p, a->dtype, true, loose, s);
+        p.g = g; p.n_in = a->n_out; p.n_out = a->n_in; p.x_cols = (int)pad8(a->n_out); p.w_cols = (int)pad8(a->n_in);
+        const Plan plan = forward_plan(a->rows, a->n_out, a->n_in, a->experts, grouped);
+        p.size = plan.size; p.splits = plan.splits; p.part = (float*)at;
+        rc = launch_tiles(p, a->dtype, true, s);
         if (rc != EVAMX_OK) return rc;
     }
     if (a->grad_w) {
-        WeightGradParams p = {(const uint16_t*)a->x, d, (size_t)a->x_stride, d_stride, (uint16_t*)a->grad_w, g, a->n_in, a->n_out, (float*)ws,
-                              weight_splits(a->rows, a->n_in, a->n_out, grouped)};
-        const int rc = launch_weight_grad(p, a->dtype, loose_d || !direct(a->x, a->x_stride, TILE_K, a->n_in), s);
+        WeightGradParams p = {x.p, d.p, (size_t)x.stride, (size_t)d.stride, (uint16_t*)a->grad_w, g, a->n_in, a->n_out, (int)pad8(a->n_in),
+                              (int)pad8(a->n_out), (float*)at, weight_plan(a->rows, a->n_in, a->n_out, a->experts, grouped)};
+        rc = launch_weight_grad(p, a->dtype, s);
         if (rc != EVAMX_OK) return rc;
     }
     if (a->grad_bias) {
-        ColumnSumParams p = {d, d_stride, (uint16_t*)a->grad_bias, g, a->n_out, (float*)ws, column_parts(a->rows, a->n_out, a->experts)};
+        ColumnSumParams p = {d.p, (size_t)d.stride, (uint16_t*)a->grad_bias, g, a->n_out, (float*)at, column_parts(a->rows, a->n_out, a->experts)};
         return launch_column_sums(p, a->dtype, s);
     }
     return EVAMX_OK;

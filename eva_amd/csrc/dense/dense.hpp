@@ -82,6 +82,24 @@ struct F16 {
     }
 };
 
+// Eight values from p on where no row starts at more than a value's address: whole 4-byte words and a shift (a load whose words straddle
+// takes about three times as long: 13 rows, 5001 -> 2304, 24 us against 10 for 5000). Reads one value in front of p and two behind the eight.
+__device__ __forceinline__ u16x8 load8_shifted(const uint16_t* p)
+{
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef u32x4 words __attribute__((aligned(4)));
+    const uint32_t* at = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
+    const int shift = (int)((uintptr_t)p & 2) * 8;
+    const u32x4 v = *(const words*)at;
+    const uint32_t end = at[4];
+    u32x4 o;
+    o[0] = __builtin_amdgcn_alignbit(v[1], v[0], shift);
+    o[1] = __builtin_amdgcn_alignbit(v[2], v[1], shift);
+    o[2] = __builtin_amdgcn_alignbit(v[3], v[2], shift);
+    o[3] = __builtin_amdgcn_alignbit(end, v[3], shift);
+    return __builtin_bit_cast(u16x8, o);
+}
+
 // ---- activations ------------------------------------------------------------------------------
 
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }

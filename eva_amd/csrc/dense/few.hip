@@ -7,32 +7,36 @@ namespace evamx_dense {
 // A workgroup takes 16 columns (SwiGLU: of the gate and of the up product) of up to 64 rows; its waves split the sum and meet in LDS.
 constexpr int FEW_WAVES = 8, FEW_THREADS = 64 * FEW_WAVES, FEW_ROWS = 64;
 
-// 16 bytes at k of a row of n values; values behind the row's end are zeros.
-template <bool LOOSE>
+// 16 bytes at k of a row of n values. TAIL: the row may begin or end there; values behind its end are zeros.
+template <int LIE, bool TAIL>
 __device__ __forceinline__ u16x8 few_load(const uint16_t* row, int k, int n)
 {
-    if (!LOOSE || k + 8 <= n) {
-        if (!LOOSE && k >= n) return (u16x8)(uint16_t)0;
-        return *(const typename std::conditional<LOOSE, u16x8_loose, u16x8>::type*)(row + k);
-    }
+    if (LIE == LIE_2 && !TAIL) return load8_shifted(row + k);
+    if (!TAIL || k + 8 <= n) return *(const typename std::conditional<LIE != LIE_16, u16x8_loose, u16x8>::type*)(row + k);
     u16x8 x = (u16x8)(uint16_t)0;
+    if (LIE != LIE_16) {
 #pragma unroll
-    for (int i = 0; i < 7; ++i)
-        if (k + i < n) x[i] = row[k + i];
+        for (int i = 0; i < 7; ++i)
+            if (k + i < n) x[i] = row[k + i];
+    }
     return x;
 }
 
-template <class T, bool GATED, bool LOOSE, int MB>
+template <class T, bool GATED, int LIE, int MB, int CB>
 __device__ __forceinline__ void few_product(const LinearParams& p, const Tile& t, f32x4* part)
 {
-    constexpr int NB = GATED ? 2 : 1, AHEAD = MB == 1 ? 8 : MB == 2 ? 4 : 2;
+    constexpr int NB = GATED ? 2 * CB : CB, AHEAD = (NB + MB) <= 2 ? 8 : NB + MB <= 5 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const uint16_t* w = p.w + (size_t)t.expert * p.w_expert_stride;
-    const uint16_t* a[NB];
+    const uint16_t* a[NB];                                               // the up product's blocks behind the gate's
     const uint16_t* x[MB];
-    const int n = 16 * t.col + c, cols = GATED ? p.inter : p.n_out, nn = n < cols ? n : cols - 1;
-    a[0] = w + (size_t)nn * p.w_stride;
-    if (GATED) a[NB - 1] = w + (size_t)(p.inter + nn) * p.w_stride;
+    const int cols = GATED ? p.inter : p.n_out;
+#pragma unroll
+    for (int b = 0; b < CB; ++b) {
+        const int n = 16 * (CB * t.col + b) + c, nn = n < cols ? n : cols - 1;
+        a[b] = w + (size_t)nn * p.w_stride;
+        if (GATED) a[NB - CB + b] = w + (size_t)(p.inter + nn) * p.w_stride;
+    }
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
         const int r = 16 * m + c;
@@ -41,16 +45,17 @@ __device__ __forceinline__ void few_product(const LinearParams& p, const Tile& t
     f32x4 acc[NB][MB] = {};
     const int steps = (p.n_in + 31) / 32, s1 = (int)((long)steps * (wave + 1) / FEW_WAVES);
     int s = (int)((long)steps * wave / FEW_WAVES);
-    auto some = [&](auto count) {
+    auto some = [&](auto count, auto tail) {
         constexpr int C = decltype(count)::value;
+        constexpr bool TAIL = decltype(tail)::value;
         u16x8 wv[C][NB], xv[C][MB];
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             const int k = 32 * (s + i) + 8 * g;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) wv[i][b] = few_load<LOOSE>(a[b], k, p.n_in);
+            for (int b = 0; b < NB; ++b) wv[i][b] = few_load<LIE, TAIL>(a[b], k, p.n_in);
 #pragma unroll
-            for (int m = 0; m < MB; ++m) xv[i][m] = few_load<LOOSE>(x[m], k, p.n_in);
+            for (int m = 0; m < MB; ++m) xv[i][m] = few_load<LIE, TAIL>(x[m], k, p.n_in);
         }
 #pragma unroll
         for (int i = 0; i < C; ++i)
@@ -60,59 +65,74 @@ __device__ __forceinline__ void few_product(const LinearParams& p, const Tile& t
                 for (int m = 0; m < MB; ++m) acc[b][m] = T::mfma(wv[i][b], xv[i][m], acc[b][m]);
         s += C;
     };
-    while (s + AHEAD <= s1) some(std::integral_constant<int, AHEAD>());
-    while (s < s1) some(std::integral_constant<int, 1>());
+    // steps that end within the rows; loads of shifted words also begin there, and reach two values further
+    const int inside = (LIE == LIE_2 ? p.n_in - 2 : p.n_in) / 32, whole = inside < s1 ? inside : s1;
+    if (LIE == LIE_2 && s == 0 && s < s1) some(std::integral_constant<int, 1>(), std::true_type());
+    while (s + AHEAD <= whole) some(std::integral_constant<int, AHEAD>(), std::false_type());
+    if (s + AHEAD / 2 <= whole) some(std::integral_constant<int, AHEAD / 2>(), std::false_type());
+    while (s < whole) some(std::integral_constant<int, 1>(), std::false_type());
+    while (s < s1) some(std::integral_constant<int, 1>(), std::true_type());
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int m = 0; m < MB; ++m) part[((wave * NB + b) * MB + m) * 64 + lane] = acc[b][m];
     __syncthreads();
-    for (int m = wave; m < MB; m += FEW_WAVES) {
-        const int r = 16 * m + c;
+    for (int block = wave; block < CB * MB; block += FEW_WAVES) {
+        const int m = block % MB, b = block / MB, r = 16 * m + c;
         if (r >= t.have) continue;
-        float v[NB][4] = {};
-        for (int q = 0; q < FEW_WAVES; ++q)
+        float v[4] = {}, u[4] = {};
+        for (int q = 0; q < FEW_WAVES; ++q) {
+            const f32x4 s = part[((q * NB + b) * MB + m) * 64 + lane], s2 = part[((q * NB + NB - CB + b) * MB + m) * 64 + lane];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[b][i] += part[((q * NB + b) * MB + m) * 64 + lane][i];
-        finish<T, GATED, 4>(p, t.expert, t.row + r, 16 * t.col + 4 * g, v[0], v[NB - 1]);
+            for (int i = 0; i < 4; ++i) {
+                v[i] += s[i];
+                if (GATED) u[i] += s2[i];
+            }
+        }
+        finish<T, GATED, 4>(p, t.expert, t.row + r, 16 * (CB * t.col + b) + 4 * g, v, u);
     }
 }
 
-template <class T, bool GATED, bool LOOSE>
+template <class T, bool GATED, int LIE, int CB>
 __global__ __launch_bounds__(FEW_THREADS) void few_kernel(LinearParams p, int cols)
 {
     extern __shared__ f32x4 part[];
-    Tile t;
-    const bool any = find_tile<FEW_THREADS>(p.g, FEW_ROWS, cols, blockIdx.x, (int*)part, t);
+    Tile t = {0, 0, p.g.rows, (int)blockIdx.x};
+    bool any = (int)blockIdx.x < cols;
+    if (p.g.starts || p.g.rows > FEW_ROWS) any = find_tile<FEW_THREADS>(p.g, FEW_ROWS, cols, blockIdx.x, (int*)part, t);
     if (p.g.starts) zero_rows(p.y, p.y_stride, GATED ? p.inter : p.n_out, p.g.end(), p.g.rows, blockIdx.x, gridDim.x);
     if (!any) return;
     __syncthreads();
-    if (t.have > 32) few_product<T, GATED, LOOSE, 4>(p, t, part);
-    else if (t.have > 16) few_product<T, GATED, LOOSE, 2>(p, t, part);
-    else few_product<T, GATED, LOOSE, 1>(p, t, part);
+    if (t.have > 32) few_product<T, GATED, LIE, 4, CB>(p, t, part);
+    else if (t.have > 16) few_product<T, GATED, LIE, 2, CB>(p, t, part);
+    else few_product<T, GATED, LIE, 1, CB>(p, t, part);
 }
 
-template <class T, bool GATED, bool LOOSE>
+template <class T, bool GATED, int LIE, int CB>
 static void launch_few_as(const LinearParams& p, hipStream_t s)
 {
-    const int cols = ceil_div(GATED ? p.inter : p.n_out, 16), most = p.g.rows > 32 ? 4 : p.g.rows > 16 ? 2 : 1;
+    const int cols = ceil_div(GATED ? p.inter : p.n_out, 16 * CB), most = p.g.rows > 32 ? 4 : p.g.rows > 16 ? 2 : 1;
     const int64_t work = most_row_tiles(p.g.rows, p.g.experts, p.g.starts, FEW_ROWS) * cols;
-    few_kernel<T, GATED, LOOSE><<<(unsigned)(8 * ceil_div(work, 8)), FEW_THREADS, (GATED ? 2 : 1) * FEW_WAVES * most * 1024, s>>>(p, cols);
+    few_kernel<T, GATED, LIE, CB><<<(unsigned)(8 * ceil_div(work, 8)), FEW_THREADS, (GATED ? 2 : 1) * CB * FEW_WAVES * most * 1024, s>>>(p, cols);
 }
 
-int launch_few(const LinearParams& p, int dtype, bool loose, hipStream_t s)
+int launch_few(const LinearParams& p, int dtype, int lie, hipStream_t s)
 {
-    auto go = [&](auto type) {
+    // 32 columns a workgroup, which read the rows once for twice the weights, where that leaves a workgroup for most CUs (16 rows of
+    // 2048 -> 7168: 9.6 us against 11.1, 64: 14.3 against 21; 7168 -> 2048: 21 and 40 against 16 and 35)
+    const bool wide = !p.inter && p.g.rows > 8 && p.n_out >= 32 * CUS * 3 / 4;
+    auto as = [&](auto type, auto gated, auto cb) {
         typedef decltype(type) T;
-        if (p.inter) {
-            if (loose) launch_few_as<T, true, true>(p, s);
-            else launch_few_as<T, true, false>(p, s);
-        } else {
-            if (loose) launch_few_as<T, false, true>(p, s);
-            else launch_few_as<T, false, false>(p, s);
-        }
+        constexpr bool G = decltype(gated)::value;
+        constexpr int CB = decltype(cb)::value;
+        if (lie == LIE_16) launch_few_as<T, G, LIE_16, CB>(p, s);
+        else if (lie == LIE_4) launch_few_as<T, G, LIE_4, CB>(p, s);
+        else launch_few_as<T, G, LIE_2, CB>(p, s);
+    };
+    auto go = [&](auto type) {
+        if (p.inter) as(type, std::true_type(), std::integral_constant<int, 1>());
+        else if (wide) as(type, std::false_type(), std::integral_constant<int, 2>());
+        else as(type, std::false_type(), std::integral_constant<int, 1>());
     };
     if (dtype == EVAMX_DTYPE_BF16) go(Bf16());
     else go(F16());

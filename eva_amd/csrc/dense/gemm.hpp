@@ -24,16 +24,17 @@ __device__ __forceinline__ int turn(int row) { return (row & 3) | (row >> 1 & 4)
 // One matrix of a workgroup's product: N values of p or q, by k.
 //   k along the rows:  value n is row map(n) of base, cut to `rows` rows, of `len` = K values.
 //   TR:                k is the row, cut to `rows` = K rows; value n is column n of base, cut to `len` columns.
+// Addresses and lengths are multiples of 16 bytes (what comes otherwise is copied first).
 // In LDS in chunks of 16 bytes, in the order in which the direct loads write them; the chunks of a row are swapped by the row's low
 // bits (in the addresses that are loaded), so that what an instruction reads together lies in different banks.
-template <bool TR, int N, int WAVES, bool LOOSE>
+template <bool TR, int N, int WAVES>
 struct Side {
     static constexpr int BYTES = N * TILE_K * 2, LOADS = BYTES / 1024 / WAVES, ROW_CHUNKS = TR ? N / 8 : TILE_K / 8;
     static_assert(LOADS >= 1 && LOADS * WAVES * 1024 == BYTES);
     const uint16_t* base;
     size_t stride;
     int rows, len;
-    uint32_t at[LOADS];           // byte offsets of a lane's chunks (LOOSE: their row and first value, row << 8 | chunk)
+    uint32_t at[LOADS];           // byte offsets of a lane's chunks
     __amdgpu_buffer_rsrc_t all;   // the whole of the matrix with k along its rows
 
     static __device__ __forceinline__ int swap(int row) { return TR ? turn(row) * 2 : row & 7; }
@@ -47,9 +48,9 @@ struct Side {
         for (int i = 0; i < LOADS; ++i) {
             const int slot = (i * WAVES + wave) * 64 + lane, row = slot / ROW_CHUNKS, chunk = (slot % ROW_CHUNKS) ^ swap(row);
             const int from = TR ? row : map(row);
-            at[i] = LOOSE ? (uint32_t)from << 8 | chunk : (uint32_t)from * (uint32_t)stride * 2 + chunk * 16;
+            at[i] = (uint32_t)from * (uint32_t)stride * 2 + chunk * 16;
         }
-        if constexpr (!TR && !LOOSE) all = buffer(base, rows <= 0 ? 0u : (uint32_t)((rows - 1) * stride + len) * 2);
+        if constexpr (!TR) all = buffer(base, rows <= 0 ? 0u : (uint32_t)((rows - 1) * stride + len) * 2);
     }
     // k-tiles before this one end within the rows (TR: a descriptor a k-tile sees to that)
     __device__ __forceinline__ int whole() const { return TR ? 1 << 30 : len / TILE_K; }
@@ -60,24 +61,7 @@ struct Side {
     {
 #ifdef __HIP_DEVICE_COMPILE__
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k0 = kt * TILE_K;
-        if constexpr (LOOSE) {
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int row = (int)(at[i] >> 8) + (TR ? k0 : 0), v = (int)(at[i] & 255) * 8 + (TR ? 0 : k0);
-                u16x8 x = (u16x8)(uint16_t)0;
-                if (row < rows && v < len) {
-                    const uint16_t* p = base + (size_t)row * stride + v;
-                    if (v + 8 <= len) {
-                        x = *(const u16x8_loose*)p;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 7; ++j)
-                            if (v + j < len) x[j] = p[j];
-                    }
-                }
-                *(u16x8*)(to + (i * WAVES + wave) * 1024 + lane * 16) = x;
-            }
-        } else if constexpr (TR) {
+        if constexpr (TR) {
             const int left = rows - k0 < TILE_K ? rows - k0 : TILE_K;
             const __amdgpu_buffer_rsrc_t src = buffer(base + (size_t)k0 * stride, left <= 0 ? 0u : (uint32_t)((left - 1) * stride + len) * 2);
 #pragma unroll
@@ -160,11 +144,11 @@ __device__ __forceinline__ void arrive()                                // all w
 
 // WP by WQ waves of PB by QB blocks each, KW times: with KW = 2 each half of a k-tile is another wave's, and the two's sums meet in
 // LDS at the end. STAGES k-tiles in LDS.
-template <class T, bool PTR, bool QTR, int WP, int WQ, int PB, int QB, int KW, int STAGES, bool LOOSE>
+template <class T, bool PTR, bool QTR, int WP, int WQ, int PB, int QB, int KW, int STAGES>
 struct Gemm {
     static constexpr int TP = 16 * PB * WP, TQ = 16 * QB * WQ, WAVES = WP * WQ * KW, THREADS = 64 * WAVES;
-    typedef Side<PTR, TP, WAVES, LOOSE> P;
-    typedef Side<QTR, TQ, WAVES, LOOSE> Q;
+    typedef Side<PTR, TP, WAVES> P;
+    typedef Side<QTR, TQ, WAVES> Q;
     static constexpr int STAGE = P::BYTES + Q::BYTES, JOIN = KW == 1 ? 0 : WP * WQ * PB * QB * 1024;
     static constexpr int OUT = WP * WQ * (64 * 68 * 4);
     static constexpr int LDS = STAGES * STAGE > JOIN ? STAGES * STAGE > OUT ? STAGES * STAGE : OUT : JOIN > OUT ? JOIN : OUT;
@@ -179,7 +163,19 @@ struct Gemm {
     //
     // The barrier of a k-tile lies where a wave has read all it needs of it: its place then takes the k-tile STAGES further, and the
     // next one's first operands are read while the last products of this one run.
-    static __device__ __forceinline__ bool run(f32x4 (&acc)[PB][QB], const P& p, const Q& q, char* lds, int kt0, int kt1)
+    // begin() asks for the first k-tiles, run() does the rest. under: each wave has made UNDER other requests between the two, which
+    // need not be waited for (requests end in their order).
+    static __device__ __forceinline__ void begin(const P& p, const Q& q, char* lds, int kt0, int kt1)
+    {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i)
+            if (kt0 + i < kt1) {
+                p.template bring<false>(lds + i * STAGE, kt0 + i);
+                q.template bring<false>(lds + i * STAGE + P::BYTES, kt0 + i);
+            }
+    }
+    template <int UNDER = 0>
+    static __device__ __forceinline__ bool run(f32x4 (&acc)[PB][QB], const P& p, const Q& q, char* lds, int kt0, int kt1, bool under = false)
     {
 #ifdef __HIP_DEVICE_COMPILE__
         const int half = KW == 2 ? kw() : 0;
@@ -219,14 +215,14 @@ struct Gemm {
             __builtin_amdgcn_sched_barrier(0);
         };
         // k-tile kt has come for all waves, of which later ones are under way
+        bool early = under;                             // nothing has been asked for since
         auto come = [&](auto later) {
-            wait_loads<LOOSE ? 0 : decltype(later)::value * LOADS>();
+            constexpr int OPEN = decltype(later)::value * LOADS;
+            if (UNDER && early) wait_loads<OPEN + UNDER>();
+            else wait_loads<OPEN>();
             arrive();
         };
         if (kt0 < kt1) {
-#pragma unroll
-            for (int i = 0; i < STAGES; ++i)
-                if (kt0 + i < kt1) bring(i * STAGE, kt0 + i, no);
             if (kt0 + STAGES - 1 < kt1) come(std::integral_constant<int, STAGES - 1>());
             else come(std::integral_constant<int, 0>());
             int now = 0, kt = kt0;
@@ -240,6 +236,7 @@ struct Gemm {
                     come(std::integral_constant<int, 0>());
                     if (kt + STAGES < kt1) bring(now, kt + STAGES, no);
                 }
+                early = early && kt + STAGES >= kt1;
                 now = next();
                 __builtin_amdgcn_sched_barrier(0);
             };
@@ -301,6 +298,25 @@ struct Gemm {
         return true;
     }
 };
+
+// Two blocks of 16 values of a row, four a lane, to eight in a row a lane: lanes 16 apart exchange halves. Lane c + 16 g gets values
+// 16 (g & 1) + 8 (g >> 1) .. + 7 of the 32.
+template <class T>
+__device__ __forceinline__ u16x8 paired(f32x4 a, f32x4 b)
+{
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 o = {};
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t x = T::put(a[2 * i]) | (uint32_t)T::put(a[2 * i + 1]) << 16, y = T::put(b[2 * i]) | (uint32_t)T::put(b[2 * i + 1]) << 16;
+        const auto s = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+        o[i] = s[0];
+        o[2 + i] = s[1];
+    }
+#endif
+    return __builtin_bit_cast(u16x8, o);
+}
 
 // A wave's results by way of LDS: 16 PB columns of 64 rows at a time, rows ROW floats apart, so that a lane gets eight values
 // in a row, neighbours the next eight, and the code that takes them is there once. f(row of the wave's 16 QB, eight columns, values).

@@ -1,7 +1,5 @@
 // The gradients of act(x W^T + b): D = act'(pre) grad, W's D^T x, the bias's column sums of D. x's, D W, is a product as the
 // forward one (tiles.hip).
-#include <stdlib.h>
-
 #include "grads.hpp"
 
 namespace evamx_dense {
@@ -49,55 +47,116 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p)
     };
     store(out, dv);
     if (GATED) store(out + cols, du);
+    if (have <= 8) {                                                    // the row's end: zeros up to the stride
+        for (int i = p.n_out; i < (int)p.out_stride; ++i) p.out[(size_t)row * p.out_stride + i] = 0;
+    }
 }
 
-// W's gradient: result rows q = n of W, p = k. The sum runs over the expert's rows, in tiles of 64.
-template <class T, bool LOOSE, int WP, int WQ, int QB, int KW>
-__global__ __launch_bounds__(64 * WP * WQ * KW, 2) void weight_grad_kernel(WeightGradParams p)
+// Tiles of n that a run of tiles takes together for all of k: eight share more of what they read; with the experts' shorter sums,
+// whose results are most of the traffic, one, so that rows are written whole (32 experts of 128 rows, 4096 by 7168: 665 us against
+// 708; one of 8192 rows: 411 against 389).
+__device__ __forceinline__ int deep_of(const WeightGradParams& p) { return p.g.starts ? 1 : 8; }
+
+// W's gradient: result rows q = n of W, p = k. The sum runs over the expert's rows, in tiles of 64. A workgroup takes one tile after
+// another: the next one's first k-tiles are asked for before this one's results are stored, so that with few rows an expert, where
+// the stores are most of the work, they go on without a pause.
+template <class T, int WP, int WQ, int QB, int KW>
+__global__ __launch_bounds__(64 * WP * WQ * KW, 2) void weight_grad_kernel(WeightGradParams p, int tiles)
 {
     constexpr int PB = 4;
-    typedef Gemm<T, true, true, WP, WQ, PB, QB, KW, 2, LOOSE> G;
+    typedef Gemm<T, true, true, WP, WQ, PB, QB, KW, 2> G;
     __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
-    const int pt = (p.n_in + G::TP - 1) / G::TP, qt = (p.n_out + G::TQ - 1) / G::TQ, tiles = pt * qt;
-    // an XCD takes a contiguous run of tiles, eight tiles of n by all of k at a time
-    const int per = (tiles + 7) / 8, at = (blockIdx.x & 7) * per + blockIdx.x / 8;
-    if ((int)blockIdx.x / 8 >= per || at >= tiles) return;
-    const int band = at / (8 * pt), in_band = at - band * 8 * pt, deep = qt - 8 * band < 8 ? qt - 8 * band : 8;
-    const int q0 = G::TQ * (8 * band + in_band % deep), p0 = G::TP * (in_band / deep), e = blockIdx.y;
-    const int begin = p.g.starts ? p.g.start(e) : 0, end = p.g.starts ? p.g.start(e + 1) : p.g.rows, count = end > begin ? end - begin : 0;
+    const int pt = (p.n_in + G::TP - 1) / G::TP, qt = (p.n_out + G::TQ - 1) / G::TQ;
     typename G::P a;
     typename G::Q b;
-    a.init(p.x + (size_t)begin * p.x_stride + p0, p.x_stride, count, p.n_in - p0, [](int n) { return n; });
-    b.init(p.d + (size_t)begin * p.d_stride + q0, p.d_stride, count, p.n_out - q0, [](int n) { return n; });
-    f32x4 acc[PB][QB] = {};
-    const int kt = (count + TILE_K - 1) / TILE_K, k0 = (int)((long)kt * blockIdx.z / p.splits), k1 = (int)((long)kt * (blockIdx.z + 1) / p.splits);
-    if (!G::run(acc, a, b, lds, k0, k1)) return;
-    const int lane = threadIdx.x & 63, wp = G::wp(), wq = G::wq(), k = p0 + 64 * wp + 8 * (lane & 7), have = p.n_in - k;
-    rows_of<PB, QB>(acc, lds, wq * WP + wp, [&](const float* mine, int first, int count) {
-        if (have <= 0) return;
-        for (int r = lane >> 3; r < count; r += 8) {
-            const int q = q0 + 16 * QB * wq + first + r;
-            if (q >= p.n_out) break;
-            float v[8];
+    int e, p0, q0, k0, k1;
+    // work item u: tile by tile of an expert (and split), each XCD a contiguous run of them, eight tiles of n by all of k at a time
+    auto take = [&](int u) {
+        const int per = (tiles + 7) / 8, unit = u / (8 * per), in = u - unit * 8 * per, at = (in & 7) * per + in / 8;
+        if (at >= tiles) return false;
+        const int split = unit % p.plan.splits;
+        e = unit / p.plan.splits;
+        const int band = at / (deep_of(p) * pt), in_band = at - band * deep_of(p) * pt, deep = qt - deep_of(p) * band < deep_of(p) ? qt - deep_of(p) * band : deep_of(p);
+        q0 = G::TQ * (deep_of(p) * band + in_band % deep);
+        p0 = G::TP * (in_band / deep);
+        const int begin = p.g.starts ? p.g.start(e) : 0, end = p.g.starts ? p.g.start(e + 1) : p.g.rows, count = end > begin ? end - begin : 0;
+        a.init(p.x + (size_t)begin * p.x_stride + p0, p.x_stride, count, p.x_cols - p0, [](int n) { return n; });
+        b.init(p.d + (size_t)begin * p.d_stride + q0, p.d_stride, count, p.d_cols - q0, [](int n) { return n; });
+        const int kt = (count + TILE_K - 1) / TILE_K;
+        k0 = (int)((long)kt * split / p.plan.splits);
+        k1 = (int)((long)kt * (split + 1) / p.plan.splits);
+        return true;
+    };
+    const int units = 8 * ((tiles + 7) / 8) * p.g.experts * p.plan.splits, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    int u = blockIdx.x;
+    while (u < units && !take(u)) u += gridDim.x;
+    if (u >= units) return;
+    G::begin(a, b, lds, k0, k1);
+    bool stored = false;                                               // PB / 2 * QB stores of the last tile's results are under way
+    for (;;) {
+        f32x4 acc[PB][QB] = {};
+        const int split = u / (8 * ((tiles + 7) / 8)) % p.plan.splits;
+        const size_t row0 = p.plan.splits > 1 ? (size_t)split * p.n_out : (size_t)e * p.n_out;
+        const int to_p = p0 + 64 * G::wp(), to_q = q0 + 16 * QB * G::wq();
+        const bool whole = p0 + G::TP <= p.n_in && q0 + G::TQ <= p.n_out && p.plan.splits == 1;
+        const bool mine = G::template run<PB / 2 * QB>(acc, a, b, lds, k0, k1, stored);
+        stored = mine && whole;
+        do u += gridDim.x;
+        while (u < units && !take(u));
+        if (u < units) G::begin(a, b, lds, k0, k1);
+        if (mine) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = mine[r * OUT_ROW + 8 * (lane & 7) + i];
-            if (p.splits > 1) {
-                store_floats(p.part + ((size_t)blockIdx.z * p.n_out + q) * p.n_in + k, v, have);
-                continue;
-            }
-            uint16_t* out = p.out + ((size_t)e * p.n_out + q) * p.n_in + k;
-            if (have >= 8) {
-                u16x8 o;
+            for (int j = 0; j < QB; ++j) {
+                const int q = to_q + 16 * j + c;
+                if (whole) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = T::put(v[i]);
-                *(u16x8_loose*)out = o;
-            } else {
+                    for (int i = 0; i < PB; i += 2)
+                        *(u16x8_loose*)(p.out + (row0 + q) * p.n_in + to_p + 16 * i + 16 * (g & 1) + 8 * (g >> 1)) = paired<T>(acc[i][j], acc[i + 1][j]);
+                } else if (q < p.n_out) {
 #pragma unroll
-                for (int i = 0; i < 7; ++i)
-                    if (i < have) out[i] = T::put(v[i]);
+                    for (int i = 0; i < PB; ++i) {
+                        const int k = to_p + 16 * i + 4 * g;
+                        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                        if (p.plan.splits > 1) {
+                            store_floats(p.part + (row0 + q) * p.n_in + k, v, p.n_in - k);
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < 4; ++h)
+                                if (k + h < p.n_in) p.out[(row0 + q) * p.n_in + k + h] = T::put(v[h]);
+                        }
+                    }
+                }
             }
         }
-    });
+        if (u >= units) return;
+    }
+}
+
+__global__ __launch_bounds__(256) void pad_kernel(const uint16_t* from, size_t stride, size_t matrix_stride, int rows, int64_t all, int n, uint16_t* to)
+{
+    const int per = (n + 7) / 8;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / per;
+    const int v = (int)(at % per) * 8;
+    if (row >= all) return;
+    const uint16_t* p = from + (size_t)(row / rows) * matrix_stride + (size_t)(row % rows) * stride + v;
+    u16x8 x = (u16x8)(uint16_t)0;
+    if (v > 0 && v + 10 <= n) {
+        x = load8_shifted(p);
+    } else if (v + 8 <= n) {
+        x = *(const u16x8_loose*)p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (v + i < n) x[i] = p[i];
+    }
+    *(u16x8*)(to + (size_t)row * (8 * per) + v) = x;
+}
+
+int launch_pad(const uint16_t* from, size_t stride, size_t matrix_stride, int rows, int count, int n, uint16_t* to, hipStream_t s)
+{
+    const int64_t all = (int64_t)rows * count;
+    pad_kernel<<<(unsigned)ceil_div(all * ((n + 7) / 8), 256), 256, 0, s>>>(from, stride, matrix_stride, rows, all, n, to);
+    return launched("linear");
 }
 
 // Sums of `count` arrays of n values each, rounded; array s of value i of matrix y: part[(y * count + s) * n + i].
@@ -161,27 +220,23 @@ int launch_act_grad(const ActGradParams& p, int dtype, hipStream_t s)
     return launched("linear_grad");
 }
 
-template <class T, bool LOOSE, int WP, int WQ, int QB, int KW>
+template <class T, int WP, int WQ, int QB, int KW>
 static void launch_weight_grad_as(const WeightGradParams& p, hipStream_t s)
 {
     const int64_t tiles = (int64_t)ceil_div(p.n_in, 64 * WP) * ceil_div(p.n_out, 16 * QB * WQ);
-    weight_grad_kernel<T, LOOSE, WP, WQ, QB, KW><<<dim3((unsigned)(8 * ceil_div(tiles, 8)), p.g.experts, p.splits), 64 * WP * WQ * KW, 0, s>>>(p);
+    const int64_t units = 8 * ceil_div(tiles, 8) * (int64_t)p.g.experts * p.plan.splits, at_once = WP * WQ * KW == 8 ? CUS : 2 * CUS;
+    weight_grad_kernel<T, WP, WQ, QB, KW><<<(unsigned)(units < at_once ? units : at_once), 64 * WP * WQ * KW, 0, s>>>(p, (int)tiles);
 }
 
-int launch_weight_grad(const WeightGradParams& p, int dtype, bool loose, hipStream_t s)
+int launch_weight_grad(const WeightGradParams& p, int dtype, hipStream_t s)
 {
     by_type(dtype, [&](auto type) {
         typedef decltype(type) T;
-        const int64_t big = (int64_t)ceil_div(p.n_in, 256) * ceil_div(p.n_out, 256) * p.g.experts;
-        static const char* force = getenv("DW_SIZE");
-        const int size = force ? atoi(force) : p.splits == 1 && big >= 200 ? 2 : 0;
-        if (loose) launch_weight_grad_as<T, true, 2, 1, 8, 2>(p, s);
-        else if (size == 2) launch_weight_grad_as<T, false, 4, 2, 8, 1>(p, s);
-        else if (size == 1) launch_weight_grad_as<T, false, 2, 2, 4, 1>(p, s);
-        else launch_weight_grad_as<T, false, 2, 1, 8, 2>(p, s);
-        if (p.splits > 1) {
+        if (p.plan.size == TILES_256) launch_weight_grad_as<T, 4, 2, 8, 1>(p, s);
+        else launch_weight_grad_as<T, 2, 2, 4, 1>(p, s);
+        if (p.plan.splits > 1) {
             const int64_t n = (int64_t)p.n_out * p.n_in;
-            sum_parts_kernel<T><<<dim3((unsigned)ceil_div(n, 256), 1), 256, 0, s>>>(p.part, p.splits, n, p.out);
+            sum_parts_kernel<T><<<dim3((unsigned)ceil_div(n, 256), 1), 256, 0, s>>>(p.part, p.plan.splits, n, p.out);
         }
     });
     return launched("linear_grad");

@@ -22,8 +22,9 @@ struct WeightGradParams {
     uint16_t* out;               // [experts][n_out][n_in]
     Groups g;
     int n_in, n_out;
+    int x_cols, d_cols;          // values in a row of x and d: multiples of 8, zeros behind the last
     float* part;                 // [splits][n_out][n_in] (one expert)
-    int splits;
+    Plan plan;
 };
 
 struct ColumnSumParams {
@@ -37,7 +38,7 @@ struct ColumnSumParams {
 };
 
 int launch_act_grad(const ActGradParams& p, int dtype, hipStream_t s);
-int launch_weight_grad(const WeightGradParams& p, int dtype, bool loose, hipStream_t s);
+int launch_weight_grad(const WeightGradParams& p, int dtype, hipStream_t s);
 int launch_column_sums(const ColumnSumParams& p, int dtype, hipStream_t s);
 
 }  // namespace evamx_dense

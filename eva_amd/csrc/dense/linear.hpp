@@ -14,12 +14,23 @@ struct LinearParams {
     size_t x_stride, w_stride, w_expert_stride, residual_stride, y_stride;
     Groups g;
     int n_in, n_out;             // of the product: k is 0 .. n_in - 1
+    int x_cols, w_cols;          // values in a row of x and w in tiles: multiples of 8, zeros behind the last
     int inter;                   // SwiGLU: n_out / 2, else 0
     int act;
     float limit;
     float* part;                 // [splits][rows][n_out] partial sums, or NULL
-    int splits, aligned_y;
+    int size, splits;            // of the tiles (plan_of)
 };
+
+// Tiles of 256 by 256, one workgroup a CU, or of 128 by 128, two a CU, and the parts a sum is cut into.
+enum { TILES_128 = 0, TILES_256 = 2 };
+struct Plan {
+    int size, splits;
+};
+// For a result of rows by cols that sums k values: the plan of the least time as measured for both kinds of tiles, a k-tile of 64 in
+// 1.2 us for a lone 256 by 256 tile to 1.55 with all CUs at work (128 by 128: 0.7 to one a CU, 1.05 with two), 6 us for a tile's
+// begin and end, and for a cut sum its way through memory at 4.5 TB/s and 4 us for the join.
+Plan plan_of(int64_t rows, int64_t cols, int64_t k);
 
 // Eight values at p of a row, or as many as there are.
 __device__ __forceinline__ void load8(float (&v)[8], const uint16_t* p, int have, bool bf16)
@@ -101,8 +112,12 @@ __device__ __forceinline__ void finish(const LinearParams& p, int expert, int ro
     }
 }
 
-int launch_tiles(const LinearParams& p, int dtype, bool transposed, bool loose, hipStream_t s);
-int launch_few(const LinearParams& p, int dtype, bool loose, hipStream_t s);
+int launch_tiles(const LinearParams& p, int dtype, bool transposed, hipStream_t s);
+// How x and w lie: 16-byte addresses and rows, whole words, or single values.
+enum { LIE_16 = 0, LIE_4 = 1, LIE_2 = 2 };
+int launch_few(const LinearParams& p, int dtype, int lie, hipStream_t s);
+// Rows of n values (rows of each of `count` matrices) to rows of a multiple of 8, zeros behind the last.
+int launch_pad(const uint16_t* from, size_t stride, size_t matrix_stride, int rows, int count, int n, uint16_t* to, hipStream_t s);
 int launch_join(const LinearParams& p, int dtype, hipStream_t s);
 
 }  // namespace evamx_dense

@@ -1,32 +1,35 @@
 // y = act(x W^T + b) + residual in tiles, and x's gradient D W, whose matrix has k over its rows.
-#include <stdlib.h>
-
 #include "linear.hpp"
 
 namespace evamx_dense {
 
 // WP by WQ by KW waves of 64 columns by 16 QB rows each.
-template <class T, bool GATED, bool PTR, bool LOOSE, int WP, int WQ, int QB, int KW, int STAGES>
+template <class T, bool GATED, bool PTR, int WP, int WQ, int QB, int KW, int STAGES>
 __device__ __forceinline__ void tile_product(const LinearParams& p, const Tile& t, char* lds)
 {
     constexpr int PB = 4;
-    typedef Gemm<T, PTR, false, WP, WQ, PB, QB, KW, STAGES, LOOSE> G;
+    typedef Gemm<T, PTR, false, WP, WQ, PB, QB, KW, STAGES> G;
     constexpr int COLS = GATED ? G::TP / 2 : G::TP;
     const uint16_t* w = p.w + (size_t)t.expert * p.w_expert_stride;
     typename G::P a;
     typename G::Q b;
     if constexpr (PTR) {
-        a.init(w + t.col * COLS, p.w_stride, p.n_in, p.n_out - t.col * COLS, [](int n) { return n; });
+        a.init(w + t.col * COLS, p.w_stride, p.n_in, p.w_cols - t.col * COLS, [](int n) { return n; });
     } else {
-        a.init(w, p.w_stride, p.n_out, p.n_in, [&](int n) {
-            if constexpr (!GATED) return COLS * t.col + n;
-            const int j = COLS * t.col + 32 * (n >> 6) + (n & 31);
-            return (n & 32) ? p.inter + j : j;                           // a wave's first 32 values are of the gate
-        });
+        if constexpr (GATED) {
+            a.init(w, p.w_stride, p.n_out, p.w_cols, [&](int n) {           // a wave's first 32 values are of the gate
+                const int j = COLS * t.col + 32 * (n >> 6) + (n & 31);
+                return (n & 32) ? p.inter + j : j;
+            });
+        } else {
+            const int n0 = COLS * t.col;
+            a.init(w + (size_t)n0 * p.w_stride, p.w_stride, p.n_out - n0 < COLS ? p.n_out - n0 : COLS, p.w_cols, [](int n) { return n; });
+        }
     }
-    b.init(p.x + (size_t)t.row * p.x_stride, p.x_stride, t.have, p.n_in, [](int n) { return n; });
+    b.init(p.x + (size_t)t.row * p.x_stride, p.x_stride, t.have, p.x_cols, [](int n) { return n; });
     f32x4 acc[PB][QB] = {};
     const int kt = (p.n_in + TILE_K - 1) / TILE_K, k0 = (int)((long)kt * blockIdx.y / p.splits), k1 = (int)((long)kt * (blockIdx.y + 1) / p.splits);
+    G::begin(a, b, lds, k0, k1);
     if (!G::run(acc, a, b, lds, k0, k1)) return;
     const int lane = threadIdx.x & 63, wp = G::wp(), wq = G::wq();
     constexpr int CHUNKS = GATED ? 4 : 8, PASS = 64 / CHUNKS;            // eights of a row (SwiGLU: of the gate's half), rows a pass
@@ -53,19 +56,19 @@ __device__ __forceinline__ void tile_product(const LinearParams& p, const Tile& 
     });
 }
 
-// SIZE: columns by rows of a workgroup's tile, 2: 256 by 256, 1: 256 by 128, 0: 128 by 128.
+// A workgroup's tile: 256 columns by 256 rows, or 128 by 128, whose waves take half a k-tile each.
 template <int SIZE>
 struct TileShape {
-    static constexpr int WP = SIZE ? 4 : 2, WQ = SIZE == 2 ? 2 : 1, KW = SIZE == 2 ? 1 : 2, STAGES = SIZE == 1 ? 3 : 2;
-    static constexpr int TQ = 128 * WQ, THREADS = 64 * WP * WQ * KW;
+    static constexpr bool BIG = SIZE == TILES_256;
+    static constexpr int WP = BIG ? 4 : 2, WQ = BIG ? 2 : 1, KW = BIG ? 1 : 2, TQ = 128 * WQ, THREADS = 64 * WP * WQ * KW;
 };
 
-template <class T, bool GATED, bool PTR, bool LOOSE, int SIZE>
+template <class T, bool GATED, bool PTR, int SIZE>
 __global__ __launch_bounds__(TileShape<SIZE>::THREADS, 2) void tiles_kernel(LinearParams p, int cols)
 {
     typedef TileShape<SIZE> S;
-    constexpr int WIDE = Gemm<T, PTR, false, S::WP, S::WQ, 4, 8, S::KW, S::STAGES, LOOSE>::LDS;
-    constexpr int HALF = SIZE == 2 ? Gemm<T, PTR, false, 4, 1, 4, 8, 2, 3, LOOSE>::LDS : 0;
+    constexpr int WIDE = Gemm<T, PTR, false, S::WP, S::WQ, 4, 8, S::KW, 2>::LDS;
+    constexpr int HALF = S::BIG ? Gemm<T, PTR, false, 4, 1, 4, 8, 2, 3>::LDS : 0;
     __shared__ __attribute__((aligned(1024))) char lds[WIDE > HALF ? WIDE : HALF];
     Tile t;
     const bool any = find_tile<S::THREADS>(p.g, S::TQ, cols, blockIdx.x, (int*)lds, t);
@@ -73,14 +76,13 @@ __global__ __launch_bounds__(TileShape<SIZE>::THREADS, 2) void tiles_kernel(Line
     if (p.g.starts) zero_rows(p.y, p.y_stride, GATED ? p.inter : p.n_out, p.g.end(), p.g.rows, blockIdx.x, gridDim.x);
     if (!any) return;
     __syncthreads();
-    if constexpr (SIZE == 2) {
-        if (t.have <= 64) return tile_product<T, GATED, PTR, LOOSE, 4, 1, 4, 2, 3>(p, t, lds);
-        if (t.have <= 128) return tile_product<T, GATED, PTR, LOOSE, 4, 1, 8, 2, 3>(p, t, lds);
+    if constexpr (S::BIG) {
+        // an expert's last rows: waves of half a k-tile, three k-tiles in LDS (32 experts of 128 rows, 7168 -> 4096: 438 us against 530
+        // with the waves of the whole tile)
+        if (t.have <= 64) return tile_product<T, GATED, PTR, 4, 1, 4, 2, 3>(p, t, lds);
+        if (t.have <= 128) return tile_product<T, GATED, PTR, 4, 1, 8, 2, 3>(p, t, lds);
     }
-    if constexpr (SIZE == 1) {
-        if (t.have <= 64) return tile_product<T, GATED, PTR, LOOSE, 4, 1, 4, 2, 3>(p, t, lds);
-    }
-    tile_product<T, GATED, PTR, LOOSE, S::WP, S::WQ, 8, S::KW, S::STAGES>(p, t, lds);
+    tile_product<T, GATED, PTR, S::WP, S::WQ, 8, S::KW, 2>(p, t, lds);
 }
 
 // Sums of the splits, and what follows a sum.
@@ -100,48 +102,34 @@ __global__ __launch_bounds__(256) void join_kernel(LinearParams p)
     finish<T, GATED, 8>(p, 0, row, n, v, u);
 }
 
-template <class T, bool GATED, bool PTR, bool LOOSE, int SIZE>
+template <class T, bool GATED, bool PTR, int SIZE>
 static void launch_size(const LinearParams& p, hipStream_t s)
 {
     typedef TileShape<SIZE> S;
     const int cols = ceil_div(GATED ? p.inter : p.n_out, GATED ? 32 * S::WP : 64 * S::WP);
     const int64_t work = most_row_tiles(p.g.rows, p.g.experts, p.g.starts, S::TQ) * cols;
-    tiles_kernel<T, GATED, PTR, LOOSE, SIZE><<<dim3((unsigned)(8 * ceil_div(work, 8)), p.splits), S::THREADS, 0, s>>>(p, cols);
+    tiles_kernel<T, GATED, PTR, SIZE><<<dim3((unsigned)(8 * ceil_div(work, 8)), p.splits), S::THREADS, 0, s>>>(p, cols);
 }
 
-template <class T, bool GATED, bool PTR, bool LOOSE>
+template <class T, bool GATED, bool PTR>
 static void launch_by_size(const LinearParams& p, hipStream_t s)
 {
-    if (p.splits > 1 || LOOSE) return launch_size<T, GATED, PTR, LOOSE, 0>(p, s);
-    if constexpr (!LOOSE) {
-        const int64_t tiles = most_row_tiles(p.g.rows, p.g.experts, p.g.starts, 256) * ceil_div(p.n_out, 256);
-        static const char* force = getenv("TILE_SIZE");
-        const int size = force ? atoi(force) : p.g.starts ? 2 : tiles >= 200 ? 2 : tiles >= 100 ? 1 : 0;
-        if (size == 2) launch_size<T, GATED, PTR, LOOSE, 2>(p, s);
-        else if (size == 1) launch_size<T, GATED, PTR, LOOSE, 1>(p, s);
-        else launch_size<T, GATED, PTR, LOOSE, 0>(p, s);
-    }
+    if (p.size == TILES_256) launch_size<T, GATED, PTR, TILES_256>(p, s);
+    else launch_size<T, GATED, PTR, TILES_128>(p, s);
 }
 
 template <class T>
-static void launch_typed(const LinearParams& p, bool transposed, bool loose, hipStream_t s)
+static void launch_typed(const LinearParams& p, bool transposed, hipStream_t s)
 {
-    if (transposed) {
-        if (loose) launch_by_size<T, false, true, true>(p, s);
-        else launch_by_size<T, false, true, false>(p, s);
-    } else if (p.inter) {
-        if (loose) launch_by_size<T, true, false, true>(p, s);
-        else launch_by_size<T, true, false, false>(p, s);
-    } else {
-        if (loose) launch_by_size<T, false, false, true>(p, s);
-        else launch_by_size<T, false, false, false>(p, s);
-    }
+    if (transposed) launch_by_size<T, false, true>(p, s);
+    else if (p.inter) launch_by_size<T, true, false>(p, s);
+    else launch_by_size<T, false, false>(p, s);
 }
 
-int launch_tiles(const LinearParams& p, int dtype, bool transposed, bool loose, hipStream_t s)
+int launch_tiles(const LinearParams& p, int dtype, bool transposed, hipStream_t s)
 {
-    if (dtype == EVAMX_DTYPE_BF16) launch_typed<Bf16>(p, transposed, loose, s);
-    else launch_typed<F16>(p, transposed, loose, s);
+    if (dtype == EVAMX_DTYPE_BF16) launch_typed<Bf16>(p, transposed, s);
+    else launch_typed<F16>(p, transposed, s);
     if (p.splits > 1) return launch_join(p, dtype, s);
     return launched("linear");
 }

@@ -605,7 +605,8 @@ def _linear_forward(name, x, w, starts, bias, activation, limit, residual, keep)
     residual_stride = 0 if residual is None else _token_rows(residual, "residual", x, (rows, cols))
     y = torch.empty(rows, cols, dtype=x.dtype, device=dev)
     pre = torch.empty(rows, n_out, dtype=torch.float32, device=dev) if keep and act else None
-    need = dense_lib().evamx_linear_workspace_bytes(rows, n_in, n_out, experts, starts is not None)
+    direct = not ((x.data_ptr() | w.data_ptr()) & 15 or (stride | row | whole | n_in) & 7 or max(stride, row) > 1 << 21)
+    need = dense_lib().evamx_linear_workspace_bytes(rows, n_in, n_out, experts, starts is not None, direct)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     a = LinearArgs(ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(y), ptr(pre), ptr(starts), ptr(workspace), need, stride, row, whole,
                    residual_stride, cols, _DTYPES[x.dtype], rows, n_in, n_out, experts, act, limit)
@@ -627,7 +628,9 @@ def _linear_backward(name, grad, x, w, starts, pre, activation, limit, want_x, w
     dx = torch.empty(rows, n_in, dtype=x.dtype, device=dev) if want_x else None
     dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_w else None
     db = torch.empty(w.shape[:-1], dtype=x.dtype, device=dev) if want_bias else None
-    need = dense_lib().evamx_linear_grad_workspace_bytes(rows, n_in, n_out, experts, starts is not None, act)
+    direct = not ((grad.data_ptr() | x.data_ptr() | w.data_ptr()) & 15 or (grad_stride | stride | row | whole | n_in | n_out) & 7 or
+                  max(grad_stride, stride, row) > 1 << 21)
+    need = dense_lib().evamx_linear_grad_workspace_bytes(rows, n_in, n_out, experts, starts is not None, act, direct)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     a = LinearGradArgs(ptr(grad), ptr(x), ptr(w), ptr(pre) if act else None, ptr(starts), ptr(dx), ptr(dw), ptr(db), ptr(workspace), need,
                        grad_stride, stride, row, whole, n_in, _DTYPES[x.dtype], rows, n_in, n_out, experts, act, limit)

@@ -71,11 +71,11 @@ def test_null_and_sizes():
     wide = dict(rows=100, n_in=4096, x_stride=4096, w_stride=4096)
     assert _call(_lib.LinearArgs, L.evamx_linear, workspace_bytes=64, **wide) == _lib.EVAMX_ENOSPACE
     assert _call(_lib.LinearGradArgs, L.evamx_linear_grad, act=1, pre=FAKE, workspace_bytes=64) == _lib.EVAMX_ENOSPACE
-    assert L.evamx_linear_workspace_bytes(100, 4096, 32, 1, 0) > 0 and L.evamx_linear_workspace_bytes(100, 0, 32, 1, 0) == 0
+    assert L.evamx_linear_workspace_bytes(100, 4096, 32, 1, 0, 1) > 0 and L.evamx_linear_workspace_bytes(100, 0, 32, 1, 0, 1) == 0
     # what a larger call's workspace serves stays within what was asked for, at any size
     for rows in (0, 1, 64, 65, 1000, 1 << 24):
         for n in (1, 520, 1 << 18):
-            assert L.evamx_linear_grad_workspace_bytes(rows, n, 64, 1, 0, 1) < (1 << 40)
+            assert L.evamx_linear_grad_workspace_bytes(rows, n, 64, 1, 0, 1, 0) < (1 << 45)
 
 
 def test_built_library_keeps_the_wait_states(tmp_path, monkeypatch):
