@@ -360,7 +360,8 @@ extern "C" size_t evamx_expert_order_workspace_bytes(int rows, int topk, int n_l
 {
     set_error("%s", "");
     if (!tok_sizes_ok("evamx_expert_order_workspace_bytes", rows, topk, n_local)) return 0;
-    return ((size_t)ord_chunks((int64_t)rows * topk, nullptr) * n_local + 1) * sizeof(int32_t);
+    const int chunks = ord_chunks((int64_t)rows * topk, nullptr);
+    return chunks <= 1 ? 0 : (size_t)chunks * n_local * sizeof(int32_t);
 }
 
 extern "C" int evamx_expert_order(const int64_t* sel, int rows, int topk, int64_t first_expert, int n_local, int32_t* starts,
@@ -368,8 +369,8 @@ extern "C" int evamx_expert_order(const int64_t* sel, int rows, int topk, int64_
 {
     set_error("%s", "");
     if (!tok_sizes_ok("evamx_expert_order", rows, topk, n_local)) return EVAMX_EINVAL;
-    if (!starts || (rows && (!sel || !position)) || !workspace) { set_error("evamx_expert_order: null pointer"); return EVAMX_EINVAL; }
     const size_t need = evamx_expert_order_workspace_bytes(rows, topk, n_local);
+    if (!starts || (rows && (!sel || !position)) || (need && !workspace)) { set_error("evamx_expert_order: null pointer"); return EVAMX_EINVAL; }
     if (workspace_bytes < need) { set_error("evamx_expert_order: workspace %zu bytes < %zu", workspace_bytes, need); return EVAMX_ENOSPACE; }
     if ((uintptr_t)workspace & 3) { set_error("evamx_expert_order: the workspace must be 4-byte aligned"); return EVAMX_EINVAL; }
     OrderParams p;

@@ -6,6 +6,7 @@ computes on the CPU.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -140,11 +141,14 @@ def w4_dequant(weight: W4Weight) -> torch.Tensor:
 
 def _launch(fn, what: str, device: torch.device, *args, last_error=None):
     """One library call on the current stream of ``device``, which is made current if it is not."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what, last_error)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what, last_error)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what, last_error)
 
 
 def _row_stride(t: torch.Tensor, name: str, dtype=None) -> int:
@@ -385,11 +389,13 @@ def balance_loss(logits: torch.Tensor, sel: torch.Tensor, *, score_fn: str = "si
 
 def _wants_grad(name: str, instead: str, *tensors) -> bool:
     """Whether autograd is to follow a call; refused in a graph capture, where its own streams and accumulators are not."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
-        return False
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{name} is not captured with a backward pass: call it under torch.no_grad(), and {instead}")
-    return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(f"{name} is not captured with a backward pass: call it under torch.no_grad(), and {instead}")
+                return True
+    return False
 
 
 def _check_backward(name: str, instead: str) -> None:
@@ -413,6 +419,11 @@ class ExpertOrder(NamedTuple):
     position: torch.Tensor
 
 
+@functools.lru_cache(maxsize=1024)
+def _order_workspace(*sizes):
+    return lib().evamx_expert_order_workspace_bytes(*sizes)
+
+
 def expert_order(sel: torch.Tensor, n_experts: int, *, first_expert: int = 0) -> ExpertOrder:
     """The order in which ``sort_tokens`` lays out the tokens of routes ``sel`` int64 ``[T, topk]`` (``route_topk``) for the
     experts ``first_expert`` to ``first_expert + n_experts - 1``: by expert, an expert's in the order of the slots.
@@ -420,12 +431,13 @@ def expert_order(sel: torch.Tensor, n_experts: int, *, first_expert: int = 0) ->
     _dev(sel, "sel", torch.int64, 2)
     rows, topk = sel.shape
     dev = sel.device
-    need = lib().evamx_expert_order_workspace_bytes(rows, topk, n_experts)
-    if need == 0:
-        raise ValueError(lib().evamx_last_error().decode())
+    if not (1 <= topk <= _lib.TOKENS_MAX_TOPK and rows * topk <= _lib.TOKENS_MAX_SLOTS and 1 <= n_experts <= _lib.TOKENS_MAX_EXPERTS):
+        raise ValueError(f"sel {list(sel.shape)} and {n_experts} experts: up to {_lib.TOKENS_MAX_TOPK} experts a token, 2^26 slots and "
+                         f"{_lib.TOKENS_MAX_EXPERTS} experts")
+    need = _order_workspace(rows, topk, n_experts)
     starts = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
     position = torch.empty(rows, topk, dtype=torch.int32, device=dev)
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _launch(lib().evamx_expert_order, "evamx_expert_order", dev, ptr(sel), rows, topk, first_expert, n_experts, ptr(starts), ptr(position),
             ptr(workspace), need)
     return ExpertOrder(starts, position)
@@ -573,7 +585,12 @@ def _matrix(w: torch.Tensor, like: torch.Tensor, ndim: int):
     return experts, n_out, n_in, row, whole
 
 
-def _linear_setup(name, x, w, starts, activation, limit):
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(*sizes):
+    return dense_lib().evamx_linear_workspace_bytes(*sizes)
+
+
+def _linear_setup(x, w, starts, activation, limit):
     """(x's row stride, experts, n_out, n_in, w's strides, activation number, result columns), checked."""
     stride = _row_stride(x, "x")
     if x.dtype not in _DTYPES:
@@ -596,7 +613,7 @@ def _linear_setup(name, x, w, starts, activation, limit):
 
 def _linear_forward(name, x, w, starts, bias, activation, limit, residual, keep):
     """(result, fp32 input of the activation or None)."""
-    stride, experts, n_out, n_in, row, whole, act, cols = _linear_setup(name, x, w, starts, activation, limit)
+    stride, experts, n_out, n_in, row, whole, act, cols = _linear_setup(x, w, starts, activation, limit)
     rows, dev = x.shape[0], x.device
     if bias is not None:
         _dev(bias, "bias", x.dtype)
@@ -606,7 +623,7 @@ def _linear_forward(name, x, w, starts, bias, activation, limit, residual, keep)
     y = torch.empty(rows, cols, dtype=x.dtype, device=dev)
     pre = torch.empty(rows, n_out, dtype=torch.float32, device=dev) if keep and act else None
     direct = not ((x.data_ptr() | w.data_ptr()) & 15 or (stride | row | whole | n_in) & 7 or max(stride, row) > 1 << 21)
-    need = dense_lib().evamx_linear_workspace_bytes(rows, n_in, n_out, experts, starts is not None, direct)
+    need = _linear_workspace(rows, n_in, n_out, experts, starts is not None, direct)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     a = LinearArgs(ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(y), ptr(pre), ptr(starts), ptr(workspace), need, stride, row, whole,
                    residual_stride, cols, _DTYPES[x.dtype], rows, n_in, n_out, experts, act, limit)
@@ -616,7 +633,7 @@ def _linear_forward(name, x, w, starts, bias, activation, limit, residual, keep)
 
 def _linear_backward(name, grad, x, w, starts, pre, activation, limit, want_x, want_w, want_bias):
     """The wanted ones of (x's, w's, bias's) gradients."""
-    stride, experts, n_out, n_in, row, whole, act, cols = _linear_setup(name, x, w, starts, activation, limit)
+    stride, experts, n_out, n_in, row, whole, act, cols = _linear_setup(x, w, starts, activation, limit)
     rows, dev = x.shape[0], x.device
     grad_stride = _token_rows(grad, "grad", x, (rows, cols))
     if act:
@@ -664,9 +681,9 @@ def _linear_name(starts):
 def _linear_call(x, w, starts, bias, activation, limit, residual, return_pre):
     name = _linear_name(starts)
     _no_tangent(name, x, w, bias, residual)
-    if not return_pre and _wants_grad(name, f"{name}_grad", x, w, bias, residual):
-        return _Linear.apply(x, w, starts, bias, activation, float(limit), residual)
-    y, pre = _linear_forward(name, x, w, starts, bias, activation, float(limit), residual, return_pre)
+    if not return_pre and _wants_grad(name, name + "_grad", x, w, bias, residual):
+        return _Linear.apply(x, w, starts, bias, activation, limit, residual)
+    y, pre = _linear_forward(name, x, w, starts, bias, activation, limit, residual, return_pre)
     return (y, pre) if return_pre else y
 
 
@@ -698,14 +715,14 @@ def linear_grad(grad: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: torch
                 limit: float = 0.0):
     """``(x's, w's, bias's)`` gradients of ``linear`` for ``grad [rows, n_out]``; ``pre`` from the forward call where there is an
     activation (its gradient is rounded to x's type before the products). The residual's is ``grad``."""
-    return _linear_backward("linear_grad", grad, x, w, None, pre, activation, float(limit), True, True, True)
+    return _linear_backward("linear_grad", grad, x, w, None, pre, activation, limit, True, True, True)
 
 
 def expert_linear_grad(grad: torch.Tensor, x: torch.Tensor, w: torch.Tensor, starts: torch.Tensor, pre: torch.Tensor | None = None, *,
                        activation: str | None = None, limit: float = 0.0):
     """``(x's, w's, bias's)`` gradients of ``expert_linear``, as ``linear_grad``."""
     _dev(starts, "starts", torch.int32, 1)
-    return _linear_backward("expert_linear_grad", grad, x, w, starts, pre, activation, float(limit), True, True, True)
+    return _linear_backward("expert_linear_grad", grad, x, w, starts, pre, activation, limit, True, True, True)
 
 
 def prepare_routes_workspace_bytes(capacity: int, topk: int) -> int:

@@ -327,7 +327,8 @@ int evamx_w4_moe_forward(const evamx_w4_moe_args* args, evamx_stream_t stream);
  * n_local - 1 are local and every other number is none. starts device int32 [n_local + 1]: expert e's
  * slots take the sorted rows starts[e] .. starts[e + 1] - 1, in the order of the slots (the same expert
  * twice takes two rows); position device int32 [rows][topk]: a slot's row, or -1. The workspace
- * (4-byte aligned) needs no clearing; calls that share one must not overlap. */
+ * (4-byte aligned; calls of up to 2048 slots need none) needs no clearing; calls that share one must not
+ * overlap. */
 size_t evamx_expert_order_workspace_bytes(int rows, int topk, int n_local);
 int evamx_expert_order(const int64_t* sel, int rows, int topk, int64_t first_expert, int n_local, int32_t* starts,
                        int32_t* position, void* workspace, size_t workspace_bytes, evamx_stream_t stream);

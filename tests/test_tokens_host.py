@@ -39,7 +39,7 @@ EXPERTS = [dict(n=0), dict(n=1025)]
 
 
 @pytest.mark.parametrize("call,bad", [
-    *((_order, b) for b in SIZES + EXPERTS + [dict(sel=0), dict(starts=0), dict(pos=0), dict(ws=0), dict(ws=FAKE + 2)]),
+    *((_order, b) for b in SIZES + EXPERTS + [dict(sel=0), dict(starts=0), dict(pos=0), dict(rows=1000, ws=0), dict(rows=1000, ws=FAKE + 2)]),
     *((_sort, b) for b in ROWS + EXPERTS + [dict(x=0), dict(pos=0), dict(starts=0), dict(out=0), dict(st=63), dict(ost=63), dict(orows=-1)]),
     *((_combine, b) for b in ROWS + [dict(y=0), dict(pos=0), dict(out=0), dict(st=63), dict(ost=63), dict(yrows=-1), dict(res=FAKE, rst=63)]),
     *((_grad, b) for b in ROWS + EXPERTS + [dict(g=0), dict(y=0), dict(pos=0), dict(starts=0), dict(w=0), dict(dy=0), dict(dw=0),
@@ -51,9 +51,9 @@ def test_refused(call, bad):
 
 def test_sizes():
     L = _lib.lib()
-    assert L.evamx_expert_order_workspace_bytes(0, 8, 256) > 0
-    assert L.evamx_expert_order_workspace_bytes(1 << 23, 8, 1024) <= (256 * 1024 + 1) * 4
+    assert L.evamx_expert_order_workspace_bytes(256, 8, 256) == 0                                      # one workgroup's work
+    assert 0 < L.evamx_expert_order_workspace_bytes(1 << 23, 8, 1024) <= 256 * 1024 * 4
     assert L.evamx_expert_order_workspace_bytes(8, 8, 1025) == 0
-    assert _order(nb=0) == _lib.EVAMX_ENOSPACE
+    assert _order(rows=1000, nb=0) == _lib.EVAMX_ENOSPACE
     assert _combine(rows=0, pos=None, out=None) == _lib.EVAMX_OK             # nothing to do, nothing launched
     assert _sort(orows=0, out=None) == _lib.EVAMX_OK
