@@ -58,8 +58,8 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t k)
     return plan_with(rows, cols, k, least);
 }
 
-// Whether few.hip takes a call: for one matrix where its time (5 us, the weights at 4.9 TB/s, and the rows of x, which each workgroup
-// reads, at 8.5) is below the tiles', up to 64 rows (measured, us, at 1, 16 and 64 rows: 7168 -> 2048: 12, 16, 35 against 19, 20, 21;
+// Whether few.hip takes a call: for one matrix where its time (6 us, the weights at 5.6 TB/s, and the rows of x, which each workgroup
+// reads, at 8.9) is below the tiles', up to 64 rows (measured, us, at 1, 16 and 64 rows: 7168 -> 2048: 12, 16, 35 against 19, 20, 21;
 // 7168 -> 18432: 53, 82, 188 against 56, 56, 62); for experts up to four rows for each, of which most may be another rank's (64 experts of
 // 4096 by 7168 at 4 rows: 742 against 662; 25 of them at one row: 294, all of it the weights).
 static bool few_rows(int rows, int k, int n, int experts, bool grouped)
@@ -68,8 +68,8 @@ static bool few_rows(int rows, int k, int n, int experts, bool grouped)
     if (rows > 64) return false;
     double tiles;
     plan_with(rows, n, k, tiles);
-    const double blocks = rows > 32 ? 4 : rows > 16 ? 2 : 1, x = ceil_div(n, rows > 8 && n >= 24 * CUS ? 32 : 16) * 16.0 * blocks * k * 2;
-    return 5 + (double)n * k * 2 / 4.9e6 + (rows > 2 ? x / 8.5e6 : 0) <= tiles;
+    const double x = ceil_div(n, rows > 8 && n >= 24 * CUS ? 32 : 16) * (double)rows * k * 2;
+    return 6 + (double)n * k * 2 / 5.6e6 + x / 8.9e6 <= tiles;
 }
 
 // Experts' rows are known to the device alone: large tiles (which the kernel takes by halves and quarters where an expert ends), if

@@ -10,45 +10,47 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p)
 {
     constexpr bool BF = std::is_same<T, Bf16>::value;
     const int cols = GATED ? p.n_out / 2 : p.n_out, per = (cols + 7) / 8;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = at / per;
-    const int n = (int)(at % per) * 8, have = cols - n;
-    if (row >= p.g.end()) return;
-    float gr[8], v[8], u[8], dv[8], du[8];
-    load8(gr, p.grad + (size_t)row * p.grad_stride + n, have, BF);
-    const float* pre = p.pre + (size_t)row * p.n_out + n;
+    // rows of the experts alone, whose number the host does not know: each workgroup goes on to the next 2048 values
+    const int64_t all = (int64_t)p.g.end() * per;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
+        const int64_t row = at / per;
+        const int n = (int)(at - row * per) * 8, have = cols - n;
+        float gr[8], v[8], u[8], dv[8], du[8];
+        load8(gr, p.grad + (size_t)row * p.grad_stride + n, have, BF);
+        const float* pre = p.pre + (size_t)row * p.n_out + n;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = u[i] = 0;
-    add_floats(v, pre, have);
-    if (GATED) add_floats(u, pre + cols, have);
+        for (int i = 0; i < 8; ++i) v[i] = u[i] = 0;
+        add_floats(v, pre, have);
+        if (GATED) add_floats(u, pre + cols, have);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (GATED) {
-            const float sg = sigmoid(v[i]), a = v[i] * sg, s = sg * (1.0f + v[i] * (1.0f - sg));
-            const bool cut = p.limit > 0, whole_a = !cut || !(a > p.limit), whole_u = !cut || !(fabsf(u[i]) > p.limit);
-            dv[i] = whole_a ? gr[i] * (cut ? within(u[i], p.limit) : u[i]) * s : 0.0f;
-            du[i] = whole_u ? gr[i] * (cut ? at_most(a, p.limit) : a) : 0.0f;
-        } else {
-            dv[i] = gr[i] * slope(v[i], p.act);
+        for (int i = 0; i < 8; ++i) {
+            if (GATED) {
+                const float sg = sigmoid(v[i]), a = v[i] * sg, s = sg * (1.0f + v[i] * (1.0f - sg));
+                const bool cut = p.limit > 0, whole_a = !cut || !(a > p.limit), whole_u = !cut || !(fabsf(u[i]) > p.limit);
+                dv[i] = whole_a ? gr[i] * (cut ? within(u[i], p.limit) : u[i]) * s : 0.0f;
+                du[i] = whole_u ? gr[i] * (cut ? at_most(a, p.limit) : a) : 0.0f;
+            } else {
+                dv[i] = gr[i] * slope(v[i], p.act);
+            }
         }
-    }
-    uint16_t* out = p.out + (size_t)row * p.out_stride + n;
-    auto store = [&](uint16_t* to, const float (&d)[8]) {
-        if (have >= 8) {
-            u16x8 o;
+        uint16_t* out = p.out + (size_t)row * p.out_stride + n;
+        auto store = [&](uint16_t* to, const float (&d)[8]) {
+            if (have >= 8) {
+                u16x8 o;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = T::put(d[i]);
-            *(u16x8_loose*)to = o;
-        } else {
+                for (int i = 0; i < 8; ++i) o[i] = T::put(d[i]);
+                *(u16x8_loose*)to = o;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 7; ++i)
-                if (i < have) to[i] = T::put(d[i]);
+                for (int i = 0; i < 7; ++i)
+                    if (i < have) to[i] = T::put(d[i]);
+            }
+        };
+        store(out, dv);
+        if (GATED) store(out + cols, du);
+        if (have <= 8) {                                                    // the row's end: zeros up to the stride
+            for (int i = p.n_out; i < (int)p.out_stride; ++i) p.out[(size_t)row * p.out_stride + i] = 0;
         }
-    };
-    store(out, dv);
-    if (GATED) store(out + cols, du);
-    if (have <= 8) {                                                    // the row's end: zeros up to the stride
-        for (int i = p.n_out; i < (int)p.out_stride; ++i) p.out[(size_t)row * p.out_stride + i] = 0;
     }
 }
 
@@ -166,6 +168,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int c
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     float v = 0;
+#pragma unroll 8
     for (int s = 0; s < count; ++s) v += part[((size_t)blockIdx.y * count + s) * n + i];
     out[(size_t)blockIdx.y * n + i] = T::put(v);
 }
@@ -211,7 +214,8 @@ static void by_type(int dtype, F f)
 int launch_act_grad(const ActGradParams& p, int dtype, hipStream_t s)
 {
     const int cols = p.act == EVAMX_ACT_SWIGLU ? p.n_out / 2 : p.n_out;
-    const unsigned grid = (unsigned)ceil_div((int64_t)p.g.rows * ceil_div(cols, 8), 256);
+    const int64_t most = ceil_div((int64_t)p.g.rows * ceil_div(cols, 8), 256);
+    const unsigned grid = (unsigned)(most < 16 * CUS ? most : 16 * CUS);
     by_type(dtype, [&](auto type) {
         typedef decltype(type) T;
         if (p.act == EVAMX_ACT_SWIGLU) act_grad_kernel<T, true><<<grid, 256, 0, s>>>(p);

@@ -89,17 +89,26 @@ __global__ __launch_bounds__(TileShape<SIZE>::THREADS, 2) void tiles_kernel(Line
 template <class T, bool GATED>
 __global__ __launch_bounds__(256) void join_kernel(LinearParams p)
 {
-    const int cols = GATED ? p.inter : p.n_out, per = (cols + 7) / 8;
+    const int cols = GATED ? p.inter : p.n_out, per = (cols + 3) / 4;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int row = (int)(at / per), n = (int)(at % per) * 8;
+    const int row = (int)(at / per), n = (int)(at % per) * 4;
     if (row >= p.g.rows) return;
-    float v[8] = {}, u[8] = {};
-    for (int s = 0; s < p.splits; ++s) {
-        const float* part = p.part + ((size_t)s * p.g.rows + row) * p.n_out + n;
-        add_floats(v, part, cols - n);
-        if (GATED) add_floats(u, part + p.inter, cols - n);
+    float v[4] = {}, u[4] = {};
+    const float* part = p.part + (size_t)row * p.n_out + n;
+    const size_t next = (size_t)p.g.rows * p.n_out;
+    if (n + 4 <= cols) {
+#pragma unroll 8
+        for (int s = 0; s < p.splits; ++s) {
+            add_floats(v, part + s * next, 4);
+            if (GATED) add_floats(u, part + s * next + p.inter, 4);
+        }
+    } else {
+        for (int s = 0; s < p.splits; ++s) {
+            add_floats(v, part + s * next, cols - n);
+            if (GATED) add_floats(u, part + s * next + p.inter, cols - n);
+        }
     }
-    finish<T, GATED, 8>(p, 0, row, n, v, u);
+    finish<T, GATED, 4>(p, 0, row, n, v, u);
 }
 
 template <class T, bool GATED, bool PTR, int SIZE>
@@ -136,7 +145,7 @@ int launch_tiles(const LinearParams& p, int dtype, bool transposed, hipStream_t 
 
 int launch_join(const LinearParams& p, int dtype, hipStream_t s)
 {
-    const unsigned grid = (unsigned)ceil_div((int64_t)p.g.rows * ceil_div(p.inter ? p.inter : p.n_out, 8), 256);
+    const unsigned grid = (unsigned)ceil_div((int64_t)p.g.rows * ceil_div(p.inter ? p.inter : p.n_out, 4), 256);
     if (dtype == EVAMX_DTYPE_BF16) {
         if (p.inter) join_kernel<Bf16, true><<<grid, 256, 0, s>>>(p);
         else join_kernel<Bf16, false><<<grid, 256, 0, s>>>(p);
