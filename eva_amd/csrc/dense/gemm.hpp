@@ -150,8 +150,9 @@ struct Gemm {
     typedef Side<PTR, TP, WAVES> P;
     typedef Side<QTR, TQ, WAVES> Q;
     static constexpr int STAGE = P::BYTES + Q::BYTES, JOIN = KW == 1 ? 0 : WP * WQ * PB * QB * 1024;
+    static constexpr int STAGES_BYTES = STAGES * STAGE;
     static constexpr int OUT = WP * WQ * (64 * 68 * 4);
-    static constexpr int LDS = STAGES * STAGE > JOIN ? STAGES * STAGE > OUT ? STAGES * STAGE : OUT : JOIN > OUT ? JOIN : OUT;
+    static constexpr int LDS = STAGES_BYTES > JOIN ? STAGES_BYTES > OUT ? STAGES_BYTES : OUT : JOIN > OUT ? JOIN : OUT;
 
     static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
     static __device__ __forceinline__ int wp() { return wave() % WP; }
@@ -309,8 +310,31 @@ __device__ __forceinline__ u16x8 paired(f32x4 a, f32x4 b)
     return __builtin_bit_cast(u16x8, o);
 }
 
-// A wave's results by way of LDS: 16 PB columns of 64 rows at a time, rows ROW floats apart, so that a lane gets eight values
-// in a row, neighbours the next eight, and the code that takes them is there once. f(row of the wave's 16 QB, eight columns, values).
+// Four blocks of 16 values of a row to stores of whole lines: lanes 8 apart exchange what belongs to the first and the last 8 of the 16
+// rows. Lane c + 16 g gets values 32 (c / 8) + 16 (g & 1) + 8 (g / 2) .. + 7 of the 64, of row c % 8 (v[0]) and 8 + c % 8 (v[1]). Stores of
+// 64 bytes a row reach 3.7 TB/s, of 128 bytes 5.4.
+template <class T>
+__device__ __forceinline__ void lined(const f32x4 (&a)[4], u16x8 (&v)[2])
+{
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 x = __builtin_bit_cast(u32x4, paired<T>(a[0], a[1])), y = __builtin_bit_cast(u32x4, paired<T>(a[2], a[3]));
+    const bool first = (threadIdx.x & 8) == 0;
+    u32x4 p, q;
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t got = __builtin_amdgcn_update_dpp(0, first ? y[i] : x[i], 0x128, 0xf, 0xf, true);    // row_ror:8
+        p[i] = first ? x[i] : got;
+        q[i] = first ? got : y[i];
+    }
+#endif
+    v[0] = __builtin_bit_cast(u16x8, p);
+    v[1] = __builtin_bit_cast(u16x8, q);
+}
+
+// A wave's results by way of LDS: 16 PB columns of 64 rows at a time, rows OUT_ROW floats apart, so that neighbours get neighbouring
+// values of a row (whole lines are loaded and stored) and the code that takes them is there once. f(rows in LDS, the first one's
+// number in the wave's 16 QB, how many).
 constexpr int OUT_ROW = 68, OUT_ROWS = 64, OUT_BYTES = OUT_ROWS * OUT_ROW * 4;
 
 template <int PB, int QB, class F>

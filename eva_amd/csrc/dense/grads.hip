@@ -61,71 +61,75 @@ __device__ __forceinline__ int deep_of(const WeightGradParams& p) { return p.g.s
 
 // W's gradient: result rows q = n of W, p = k. The sum runs over the expert's rows, in tiles of 64. A workgroup takes one tile after
 // another: the next one's first k-tiles are asked for before this one's results are stored, so that with few rows an expert, where
-// the stores are most of the work, they go on without a pause.
-template <class T, int WP, int WQ, int QB, int KW>
-__global__ __launch_bounds__(64 * WP * WQ * KW, 2) void weight_grad_kernel(WeightGradParams p, int tiles)
+// the stores are most of the work, they need not be waited for.
+template <class T, int WP, int WQ, int QB>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void weight_grad_kernel(WeightGradParams p, int tiles)
 {
     constexpr int PB = 4;
-    typedef Gemm<T, true, true, WP, WQ, PB, QB, KW, 2> G;
-    __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
-    const int pt = (p.n_in + G::TP - 1) / G::TP, qt = (p.n_out + G::TQ - 1) / G::TQ;
+    typedef Gemm<T, true, true, WP, WQ, PB, QB, 1, 2> G;
+    __shared__ __attribute__((aligned(1024))) char lds[G::STAGES_BYTES];
+    const int pt = (p.n_in + G::TP - 1) / G::TP, qt = (p.n_out + G::TQ - 1) / G::TQ, splits = p.plan.splits;
     typename G::P a;
     typename G::Q b;
-    int e, p0, q0, k0, k1;
-    // work item u: tile by tile of an expert (and split), each XCD a contiguous run of them, eight tiles of n by all of k at a time
+    int e, p0, q0, k0, k1, split;
+    // work item u: tile by tile of an expert (and split), each XCD a contiguous run of them, deep_of tiles of n by all of k at a time
     auto take = [&](int u) {
         const int per = (tiles + 7) / 8, unit = u / (8 * per), in = u - unit * 8 * per, at = (in & 7) * per + in / 8;
         if (at >= tiles) return false;
-        const int split = unit % p.plan.splits;
-        e = unit / p.plan.splits;
-        const int band = at / (deep_of(p) * pt), in_band = at - band * deep_of(p) * pt, deep = qt - deep_of(p) * band < deep_of(p) ? qt - deep_of(p) * band : deep_of(p);
-        q0 = G::TQ * (deep_of(p) * band + in_band % deep);
+        split = unit % splits;
+        e = unit / splits;
+        const int most = deep_of(p), band = at / (most * pt), in_band = at - band * most * pt, deep = qt - most * band < most ? qt - most * band : most;
+        q0 = G::TQ * (most * band + in_band % deep);
         p0 = G::TP * (in_band / deep);
         const int begin = p.g.starts ? p.g.start(e) : 0, end = p.g.starts ? p.g.start(e + 1) : p.g.rows, count = end > begin ? end - begin : 0;
         a.init(p.x + (size_t)begin * p.x_stride + p0, p.x_stride, count, p.x_cols - p0, [](int n) { return n; });
         b.init(p.d + (size_t)begin * p.d_stride + q0, p.d_stride, count, p.d_cols - q0, [](int n) { return n; });
         const int kt = (count + TILE_K - 1) / TILE_K;
-        k0 = (int)((long)kt * split / p.plan.splits);
-        k1 = (int)((long)kt * (split + 1) / p.plan.splits);
+        k0 = splits > 1 ? (int)((long)kt * split / splits) : 0;
+        k1 = splits > 1 ? (int)((long)kt * (split + 1) / splits) : kt;
         return true;
     };
-    const int units = 8 * ((tiles + 7) / 8) * p.g.experts * p.plan.splits, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int units = 8 * ((tiles + 7) / 8) * p.g.experts * splits, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     int u = blockIdx.x;
     while (u < units && !take(u)) u += gridDim.x;
     if (u >= units) return;
     G::begin(a, b, lds, k0, k1);
-    bool stored = false;                                               // PB / 2 * QB stores of the last tile's results are under way
+    bool stored = false;                                               // 2 QB stores of the last tile's results are under way
     for (;;) {
         f32x4 acc[PB][QB] = {};
-        const int split = u / (8 * ((tiles + 7) / 8)) % p.plan.splits;
-        const size_t row0 = p.plan.splits > 1 ? (size_t)split * p.n_out : (size_t)e * p.n_out;
+        const size_t row0 = splits > 1 ? (size_t)split * p.n_out : (size_t)e * p.n_out;
         const int to_p = p0 + 64 * G::wp(), to_q = q0 + 16 * QB * G::wq();
-        const bool whole = p0 + G::TP <= p.n_in && q0 + G::TQ <= p.n_out && p.plan.splits == 1;
-        const bool mine = G::template run<PB / 2 * QB>(acc, a, b, lds, k0, k1, stored);
-        stored = mine && whole;
+        const bool whole = p0 + G::TP <= p.n_in && q0 + G::TQ <= p.n_out && splits == 1;
+        G::template run<2 * QB>(acc, a, b, lds, k0, k1, stored);
+        stored = whole;
         do u += gridDim.x;
         while (u < units && !take(u));
         if (u < units) G::begin(a, b, lds, k0, k1);
-        if (mine) {
+        if (whole) {
+            uint16_t* at = p.out + (row0 + to_q + (c & 7)) * p.n_in + to_p + 32 * (c >> 3) + 16 * (g & 1) + 8 * (g >> 1);
+#pragma unroll
+            for (int j = 0; j < QB; ++j) {
+                const f32x4 sums[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+                u16x8 v[2];
+                lined<T>(sums, v);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) *(u16x8_loose*)(at + (size_t)(2 * j + i) * 8 * p.n_in) = v[i];
+            }
+        } else {
 #pragma unroll
             for (int j = 0; j < QB; ++j) {
                 const int q = to_q + 16 * j + c;
-                if (whole) {
+                if (q >= p.n_out) continue;
 #pragma unroll
-                    for (int i = 0; i < PB; i += 2)
-                        *(u16x8_loose*)(p.out + (row0 + q) * p.n_in + to_p + 16 * i + 16 * (g & 1) + 8 * (g >> 1)) = paired<T>(acc[i][j], acc[i + 1][j]);
-                } else if (q < p.n_out) {
+                for (int i = 0; i < PB; ++i) {
+                    const int k = to_p + 16 * i + 4 * g;
+                    const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                    if (splits > 1) {
+                        store_floats(p.part + (row0 + q) * p.n_in + k, v, p.n_in - k);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < PB; ++i) {
-                        const int k = to_p + 16 * i + 4 * g;
-                        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                        if (p.plan.splits > 1) {
-                            store_floats(p.part + (row0 + q) * p.n_in + k, v, p.n_in - k);
-                        } else {
-#pragma unroll
-                            for (int h = 0; h < 4; ++h)
-                                if (k + h < p.n_in) p.out[(row0 + q) * p.n_in + k + h] = T::put(v[h]);
-                        }
+                        for (int h = 0; h < 4; ++h)
+                            if (k + h < p.n_in) p.out[(row0 + q) * p.n_in + k + h] = T::put(v[h]);
                     }
                 }
             }
@@ -224,20 +228,20 @@ int launch_act_grad(const ActGradParams& p, int dtype, hipStream_t s)
     return launched("linear_grad");
 }
 
-template <class T, int WP, int WQ, int QB, int KW>
+template <class T, int WP, int WQ, int QB>
 static void launch_weight_grad_as(const WeightGradParams& p, hipStream_t s)
 {
     const int64_t tiles = (int64_t)ceil_div(p.n_in, 64 * WP) * ceil_div(p.n_out, 16 * QB * WQ);
-    const int64_t units = 8 * ceil_div(tiles, 8) * (int64_t)p.g.experts * p.plan.splits, at_once = WP * WQ * KW == 8 ? CUS : 2 * CUS;
-    weight_grad_kernel<T, WP, WQ, QB, KW><<<(unsigned)(units < at_once ? units : at_once), 64 * WP * WQ * KW, 0, s>>>(p, (int)tiles);
+    const int64_t units = 8 * ceil_div(tiles, 8) * (int64_t)p.g.experts * p.plan.splits, at_once = WP * WQ == 8 ? CUS : 2 * CUS;
+    weight_grad_kernel<T, WP, WQ, QB><<<(unsigned)(units < at_once ? units : at_once), 64 * WP * WQ, 0, s>>>(p, (int)tiles);
 }
 
 int launch_weight_grad(const WeightGradParams& p, int dtype, hipStream_t s)
 {
     by_type(dtype, [&](auto type) {
         typedef decltype(type) T;
-        if (p.plan.size == TILES_256) launch_weight_grad_as<T, 4, 2, 8, 1>(p, s);
-        else launch_weight_grad_as<T, 2, 2, 4, 1>(p, s);
+        if (p.plan.size == TILES_256) launch_weight_grad_as<T, 4, 2, 8>(p, s);
+        else launch_weight_grad_as<T, 2, 2, 4>(p, s);
         if (p.plan.splits > 1) {
             const int64_t n = (int64_t)p.n_out * p.n_in;
             sum_parts_kernel<T><<<dim3((unsigned)ceil_div(n, 256), 1), 256, 0, s>>>(p.part, p.plan.splits, n, p.out);

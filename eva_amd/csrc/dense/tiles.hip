@@ -32,25 +32,21 @@ __device__ __forceinline__ void tile_product(const LinearParams& p, const Tile& 
     G::begin(a, b, lds, k0, k1);
     if (!G::run(acc, a, b, lds, k0, k1)) return;
     const int lane = threadIdx.x & 63, wp = G::wp(), wq = G::wq();
-    constexpr int CHUNKS = GATED ? 4 : 8, PASS = 64 / CHUNKS;            // eights of a row (SwiGLU: of the gate's half), rows a pass
-    const int n = (GATED ? COLS * t.col + 32 * wp : COLS * t.col + 64 * wp) + 8 * (lane % CHUNKS);
+    constexpr int FOURS = GATED ? 8 : 16, PASS = 64 / FOURS;              // fours of a row (SwiGLU: of the gate's half), rows a pass
+    const int in = 4 * (lane % FOURS), n = (GATED ? COLS * t.col + 32 * wp : COLS * t.col + 64 * wp) + in;
     rows_of<PB, QB>(acc, lds, wq * WP + wp, [&](const float* mine, int first, int count) {
-        for (int r0 = lane / CHUNKS; r0 < count; r0 += PASS) {
+        for (int r0 = lane / FOURS; r0 < count; r0 += PASS) {
             const int r = 16 * QB * wq + first + r0;
             if (r >= t.have) break;
-            float v[8], u[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[i] = mine[r0 * OUT_ROW + 8 * (lane % CHUNKS) + i];
-                u[i] = GATED ? mine[r0 * OUT_ROW + 32 + 8 * (lane % CHUNKS) + i] : 0.0f;
-            }
+            const f32x4 x = *(const f32x4*)(mine + r0 * OUT_ROW + in), y = *(const f32x4*)(mine + r0 * OUT_ROW + in + (GATED ? 32 : 0));
+            float v[4] = {x[0], x[1], x[2], x[3]}, u[4] = {y[0], y[1], y[2], y[3]};
             if (p.splits > 1) {
                 float* part = p.part + ((size_t)blockIdx.y * p.g.rows + t.row + r) * p.n_out + n;
                 const int have = (GATED ? p.inter : p.n_out) - n;
                 store_floats(part, v, have);
                 if (GATED) store_floats(part + p.inter, u, have);
             } else {
-                finish<T, GATED, 8>(p, t.expert, t.row + r, n, v, u);
+                finish<T, GATED, 4>(p, t.expert, t.row + r, n, v, u);
             }
         }
     });
