@@ -55,8 +55,8 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p)
 }
 
 // Tiles of n that a run of tiles takes together for all of k: eight share more of what they read; with the experts' shorter sums,
-// whose results are most of the traffic, one, so that rows are written whole (32 experts of 128 rows, 4096 by 7168: 665 us against
-// 708; one of 8192 rows: 411 against 389).
+// whose results are most of the traffic, one, so that rows are written whole (32 experts of 128 rows, 4096 by 7168: 655 us against
+// 700; one of 8192 rows: 411 against 389).
 __device__ __forceinline__ int deep_of(const WeightGradParams& p) { return p.g.starts ? 1 : 8; }
 
 // W's gradient: result rows q = n of W, p = k. The sum runs over the expert's rows, in tiles of 64. A workgroup takes one tile after

@@ -407,6 +407,8 @@ def _check_backward(name: str, instead: str) -> None:
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself if its rows are contiguous and do not overlap, or a copy (a gradient may come expanded)."""
+    if t.is_contiguous():
+        return t
     rows, cols = t.shape
     return t.contiguous() if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols) else t
 
@@ -444,13 +446,13 @@ def expert_order(sel: torch.Tensor, n_experts: int, *, first_expert: int = 0) ->
 
 
 def _order_args(order: ExpertOrder, device: torch.device):
-    """(rows, topk, experts) of a checked order."""
+    """(starts, position, rows, topk, experts) of a checked order."""
     starts, position = order
     _dev(starts, "order.starts", torch.int32, 1)
     _dev(position, "order.position", torch.int32, 2)
     if starts.device != device or position.device != device:
         raise ValueError(f"the order is on {starts.device} and {position.device}, the rows on {device}")
-    return *position.shape, starts.numel() - 1
+    return starts, position, *position.shape, starts.numel() - 1
 
 
 def _token_rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None, shape=(None, None)) -> int:
@@ -465,29 +467,44 @@ def _token_rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None, sh
     return stride
 
 
-def _sort_rows(x, order, out_rows):
-    """``x``'s rows at their positions of ``out_rows`` sorted ones."""
-    rows, topk, experts = _order_args(order, x.device)
-    stride = _token_rows(x, "x", None, (rows, None))
-    out = torch.empty(out_rows, x.shape[1], dtype=x.dtype, device=x.device)
-    _launch(lib().evamx_sort_tokens, "evamx_sort_tokens", x.device, ptr(x), _LOGIT_DTYPES[x.dtype], stride, rows, x.shape[1], topk,
-            ptr(order.position), ptr(order.starts), experts, ptr(out), x.shape[1], out_rows)
+def _weights_arg(weights, rows, topk, device):
+    _dev(weights, "weights", torch.float32, 2)
+    if tuple(weights.shape) != (rows, topk) or weights.device != device:
+        raise ValueError(f"weights must be [{rows}, {topk}] on {device}, got {list(weights.shape)} on {weights.device}")
+
+
+# The calls themselves, for checked arguments: autograd's backward passes, which get what their forward passes checked, go here.
+
+def _sort_call(x, stride, starts, position, experts, out_rows):
+    (rows, hidden), topk, dtype, dev = x.shape, position.shape[1], x.dtype, x.device
+    out = torch.empty(out_rows, hidden, dtype=dtype, device=dev)
+    _launch(lib().evamx_sort_tokens, "evamx_sort_tokens", dev, x.data_ptr(), _LOGIT_DTYPES[dtype], stride, rows, hidden, topk,
+            position.data_ptr(), starts.data_ptr(), experts, out.data_ptr(), hidden, out_rows)
     return out
 
 
-def _combine(y, order, weights, residual):
-    """The weighted sums of ``combine_tokens``."""
-    rows, topk, _ = _order_args(order, y.device)
-    stride, hidden = _token_rows(y, "y"), y.shape[1]
-    residual_stride = 0 if residual is None else _token_rows(residual, "residual", y, (rows, hidden))
-    if weights is not None:
-        _dev(weights, "weights", torch.float32, 2)
-        if tuple(weights.shape) != (rows, topk) or weights.device != y.device:
-            raise ValueError(f"weights must be [{rows}, {topk}] on {y.device}, got {list(weights.shape)} on {weights.device}")
-    out = torch.empty(rows, hidden, dtype=y.dtype, device=y.device)
-    _launch(lib().evamx_combine_tokens, "evamx_combine_tokens", y.device, ptr(y), _LOGIT_DTYPES[y.dtype], stride, y.shape[0], rows, hidden,
-            topk, ptr(order.position), ptr(weights), ptr(residual), residual_stride, ptr(out), hidden)
+def _combine_call(y, stride, position, weights, residual, residual_stride):
+    (rows, topk), (y_rows, hidden), dtype, dev = position.shape, y.shape, y.dtype, y.device
+    out = torch.empty(rows, hidden, dtype=dtype, device=dev)
+    _launch(lib().evamx_combine_tokens, "evamx_combine_tokens", dev, y.data_ptr(), _LOGIT_DTYPES[dtype], stride, y_rows, rows, hidden, topk,
+            position.data_ptr(), ptr(weights), ptr(residual), residual_stride, out.data_ptr(), hidden)
     return out
+
+
+def _combine_grad_call(grad, stride, y, y_stride, starts, position, experts, weights):
+    (rows, topk), (y_rows, hidden), dtype, dev = position.shape, y.shape, y.dtype, y.device
+    dy = torch.empty(y_rows, hidden, dtype=dtype, device=dev)
+    dweights = torch.empty(rows, topk, dtype=torch.float32, device=dev)
+    _launch(lib().evamx_combine_tokens_grad, "evamx_combine_tokens_grad", dev, grad.data_ptr(), _LOGIT_DTYPES[dtype], stride, y.data_ptr(),
+            y_stride, y_rows, rows, hidden, topk, position.data_ptr(), starts.data_ptr(), experts, weights.data_ptr(), dy.data_ptr(), hidden,
+            dweights.data_ptr())
+    return dy, dweights
+
+
+def _grad_rows(grad: torch.Tensor):
+    """A gradient as rows, and their stride."""
+    grad = _rows_of(grad)
+    return grad, grad.stride(0) if grad.shape[0] > 1 else grad.shape[1]
 
 
 _SORT_GRAD, _COMBINE_GRAD = "sort_tokens_grad", "combine_tokens_grad"
@@ -495,14 +512,16 @@ _SORT_GRAD, _COMBINE_GRAD = "sort_tokens_grad", "combine_tokens_grad"
 
 class _SortTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, starts, position):
-        ctx.save_for_backward(starts, position)
-        return _sort_rows(x, ExpertOrder(starts, position), position.numel())
+    def forward(ctx, x, stride, starts, position, experts):
+        ctx.save_for_backward(position)
+        return _sort_call(x, stride, starts, position, experts, position.numel())
 
     @staticmethod
     def backward(ctx, grad):
         _check_backward("sort_tokens", _SORT_GRAD)
-        return sort_tokens_grad(_rows_of(grad), ExpertOrder(*ctx.saved_tensors)), None, None
+        position, = ctx.saved_tensors
+        grad, stride = _grad_rows(grad)
+        return _combine_call(grad, stride, position, None, None, 0), None, None, None, None
 
 
 def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
@@ -510,34 +529,42 @@ def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     is ``x[t]``. The rows behind ``order.starts[-1]``, where slots have no row, are zeros. Differentiable in x (once, and not in a
     graph capture: there call it under ``torch.no_grad()``, and ``sort_tokens_grad``)."""
     _no_tangent("sort_tokens", x)
+    stride = _token_rows(x, "x")
+    starts, position, rows, _, experts = _order_args(order, x.device)
+    if x.shape[0] != rows:
+        raise ValueError(f"x has {x.shape[0]} rows, the order {rows}")
     if _wants_grad("sort_tokens", _SORT_GRAD, x):
-        return _SortTokens.apply(x, *order)
-    return _sort_rows(x, order, order.position.numel())
+        return _SortTokens.apply(x, stride, starts, position, experts)
+    return _sort_call(x, stride, starts, position, experts, position.numel())
 
 
 def sort_tokens_grad(grad: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """The gradient of ``sort_tokens`` in its tokens: each one's rows of ``grad`` added up (in fp32, rounded once)."""
-    return _combine(grad, order, None, None)
+    stride = _token_rows(grad, "grad")
+    return _combine_call(grad, stride, _order_args(order, grad.device)[1], None, None, 0)
 
 
 class _CombineTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, starts, position, weights, residual):
+    def forward(ctx, y, stride, starts, position, experts, weights, residual, residual_stride):
         ctx.save_for_backward(y if weights is not None else None, starts, position, weights)
-        ctx.y_rows = y.shape[0]
-        return _combine(y, ExpertOrder(starts, position), weights, residual)
+        ctx.sizes = y.shape[0], stride, experts
+        return _combine_call(y, stride, position, weights, residual, residual_stride)
 
     @staticmethod
     def backward(ctx, grad):
         _check_backward("combine_tokens", _COMBINE_GRAD)
-        y, starts, position, weights = ctx.saved_tensors
-        grad, order, dy, dweights = _rows_of(grad), ExpertOrder(starts, position), None, None
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[3]:
+        dy = dweights = None
+        need = ctx.needs_input_grad
+        if need[0] or need[5]:
+            y, starts, position, weights = ctx.saved_tensors
+            y_rows, y_stride, experts = ctx.sizes
+            rows, stride = _grad_rows(grad)
             if weights is None:
-                dy = _sort_rows(grad, order, ctx.y_rows)
+                dy = _sort_call(rows, stride, starts, position, experts, y_rows)
             else:
-                dy, dweights = combine_tokens_grad(grad, y, order, weights)
-        return dy, None, None, dweights, grad if ctx.needs_input_grad[4] else None
+                dy, dweights = _combine_grad_call(rows, stride, y, y_stride, starts, position, experts, weights)
+        return dy, None, None, None, None, dweights, grad if need[6] else None, None
 
 
 def combine_tokens(y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor | None = None, *,
@@ -547,25 +574,24 @@ def combine_tokens(y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor | 
     nothing. fp32 sums in slot order, rounded once. Differentiable in y, weights and residual (once, and not in a graph capture:
     there call it under ``torch.no_grad()``, and ``combine_tokens_grad``)."""
     _no_tangent("combine_tokens", y, weights, residual)
+    stride = _token_rows(y, "y")
+    starts, position, rows, topk, experts = _order_args(order, y.device)
+    residual_stride = 0 if residual is None else _token_rows(residual, "residual", y, (rows, y.shape[1]))
+    if weights is not None:
+        _weights_arg(weights, rows, topk, y.device)
     if _wants_grad("combine_tokens", _COMBINE_GRAD, y, weights, residual):
-        return _CombineTokens.apply(y, *order, weights, residual)
-    return _combine(y, order, weights, residual)
+        return _CombineTokens.apply(y, stride, starts, position, experts, weights, residual, residual_stride)
+    return _combine_call(y, stride, position, weights, residual, residual_stride)
 
 
 def combine_tokens_grad(grad: torch.Tensor, y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor):
     """``(y's gradient, weights' gradient fp32 [T, topk])`` of ``combine_tokens`` for ``grad [T, hidden]``; zeros in y's rows behind
     the last one that a slot has."""
-    rows, topk, experts = _order_args(order, y.device)
-    y_stride, hidden = _token_rows(y, "y"), y.shape[1]
-    stride = _token_rows(grad, "grad", y, (rows, hidden))
-    _dev(weights, "weights", torch.float32, 2)
-    if tuple(weights.shape) != (rows, topk) or weights.device != y.device:
-        raise ValueError(f"weights must be [{rows}, {topk}] on {y.device}, got {list(weights.shape)} on {weights.device}")
-    dy = torch.empty(y.shape[0], hidden, dtype=y.dtype, device=y.device)
-    dweights = torch.empty(rows, topk, dtype=torch.float32, device=y.device)
-    _launch(lib().evamx_combine_tokens_grad, "evamx_combine_tokens_grad", y.device, ptr(grad), _LOGIT_DTYPES[y.dtype], stride, ptr(y), y_stride,
-            y.shape[0], rows, hidden, topk, ptr(order.position), ptr(order.starts), experts, ptr(weights), ptr(dy), hidden, ptr(dweights))
-    return dy, dweights
+    starts, position, rows, topk, experts = _order_args(order, y.device)
+    y_stride = _token_rows(y, "y")
+    stride = _token_rows(grad, "grad", y, (rows, y.shape[1]))
+    _weights_arg(weights, rows, topk, y.device)
+    return _combine_grad_call(grad, stride, y, y_stride, starts, position, experts, weights)
 
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3, "swiglu": 4}      # EVAMX_ACT_*
@@ -590,6 +616,11 @@ def _linear_workspace(*sizes):
     return dense_lib().evamx_linear_workspace_bytes(*sizes)
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_grad_workspace(*sizes):
+    return dense_lib().evamx_linear_grad_workspace_bytes(*sizes)
+
+
 def _linear_setup(x, w, starts, activation, limit):
     """(x's row stride, experts, n_out, n_in, w's strides, activation number, result columns), checked."""
     stride = _row_stride(x, "x")
@@ -611,79 +642,97 @@ def _linear_setup(x, w, starts, activation, limit):
     return stride, experts, n_out, n_in, row, whole, ACTIVATIONS[activation], n_out // 2 if activation == "swiglu" else n_out
 
 
-def _linear_forward(name, x, w, starts, bias, activation, limit, residual, keep):
-    """(result, fp32 input of the activation or None)."""
+def _linear_args(x, w, starts, bias, activation, limit, residual):
+    """(sizes, residual's row stride) of a checked call, as _linear_call takes them."""
     stride, experts, n_out, n_in, row, whole, act, cols = _linear_setup(x, w, starts, activation, limit)
-    rows, dev = x.shape[0], x.device
     if bias is not None:
         _dev(bias, "bias", x.dtype)
-        if tuple(bias.shape) != ((n_out,) if starts is None else (experts, n_out)) or bias.device != dev:
-            raise ValueError(f"bias {list(bias.shape)} on {bias.device} does not go with w {list(w.shape)} on {dev}")
-    residual_stride = 0 if residual is None else _token_rows(residual, "residual", x, (rows, cols))
-    y = torch.empty(rows, cols, dtype=x.dtype, device=dev)
+        if tuple(bias.shape) != ((n_out,) if starts is None else (experts, n_out)) or bias.device != x.device:
+            raise ValueError(f"bias {list(bias.shape)} on {bias.device} does not go with w {list(w.shape)} on {x.device}")
+    residual_stride = 0 if residual is None else _token_rows(residual, "residual", x, (x.shape[0], cols))
+    return (stride, experts, n_out, n_in, row, whole, act, cols), residual_stride
+
+
+# The calls themselves, for checked arguments, as above.
+
+def _linear_call(x, w, starts, bias, residual, residual_stride, limit, keep, sizes):
+    """(result, fp32 input of the activation or None)."""
+    stride, experts, n_out, n_in, row, whole, act, cols = sizes
+    rows, dtype, dev, library = x.shape[0], x.dtype, x.device, dense_lib()
+    y = torch.empty(rows, cols, dtype=dtype, device=dev)
     pre = torch.empty(rows, n_out, dtype=torch.float32, device=dev) if keep and act else None
     direct = not ((x.data_ptr() | w.data_ptr()) & 15 or (stride | row | whole | n_in) & 7 or max(stride, row) > 1 << 21)
     need = _linear_workspace(rows, n_in, n_out, experts, starts is not None, direct)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    a = LinearArgs(ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(y), ptr(pre), ptr(starts), ptr(workspace), need, stride, row, whole,
-                   residual_stride, cols, _DTYPES[x.dtype], rows, n_in, n_out, experts, act, limit)
-    _launch(dense_lib().evamx_linear, name, dev, ctypes.byref(a), last_error=dense_lib().evamx_dense_last_error)
+    a = LinearArgs(x.data_ptr(), w.data_ptr(), ptr(bias), ptr(residual), y.data_ptr(), ptr(pre), ptr(starts), ptr(workspace), need, stride,
+                   row, whole, residual_stride, cols, _DTYPES[dtype], rows, n_in, n_out, experts, act, limit)
+    _launch(library.evamx_linear, "evamx_linear", dev, ctypes.byref(a), last_error=library.evamx_dense_last_error)
     return y, pre
 
 
-def _linear_backward(name, grad, x, w, starts, pre, activation, limit, want_x, want_w, want_bias):
+def _linear_grad_call(grad, grad_stride, x, w, starts, pre, limit, sizes, want_x, want_w, want_bias):
     """The wanted ones of (x's, w's, bias's) gradients."""
-    stride, experts, n_out, n_in, row, whole, act, cols = _linear_setup(x, w, starts, activation, limit)
-    rows, dev = x.shape[0], x.device
-    grad_stride = _token_rows(grad, "grad", x, (rows, cols))
+    stride, experts, n_out, n_in, row, whole, act, cols = sizes
+    rows, dtype, dev, library = x.shape[0], x.dtype, x.device, dense_lib()
+    dx = torch.empty(rows, n_in, dtype=dtype, device=dev) if want_x else None
+    dw = torch.empty(w.shape, dtype=dtype, device=dev) if want_w else None
+    db = torch.empty(w.shape[:-1], dtype=dtype, device=dev) if want_bias else None
+    direct = not ((grad.data_ptr() | x.data_ptr() | w.data_ptr()) & 15 or (grad_stride | stride | row | whole | n_in | n_out) & 7 or
+                  max(grad_stride, stride, row) > 1 << 21)
+    need = _linear_grad_workspace(rows, n_in, n_out, experts, starts is not None, act, direct)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    a = LinearGradArgs(grad.data_ptr(), x.data_ptr(), w.data_ptr(), ptr(pre), ptr(starts), ptr(dx), ptr(dw), ptr(db), ptr(workspace), need,
+                       grad_stride, stride, row, whole, n_in, _DTYPES[dtype], rows, n_in, n_out, experts, act, limit)
+    _launch(library.evamx_linear_grad, "evamx_linear_grad", dev, ctypes.byref(a), last_error=library.evamx_dense_last_error)
+    return dx, dw, db
+
+
+def _linear_backward(grad, x, w, starts, pre, activation, limit):
+    """All three gradients for arguments of a caller's own."""
+    sizes = _linear_setup(x, w, starts, activation, limit)
+    n_out, act, cols = sizes[2], sizes[6], sizes[7]
+    grad_stride = _token_rows(grad, "grad", x, (x.shape[0], cols))
     if act:
         if pre is None:
             raise ValueError("the gradient of an activation needs pre, what the forward call gave with return_pre=True")
         _dev(pre, "pre", torch.float32, 2)
-        if tuple(pre.shape) != (rows, n_out) or pre.device != dev:
-            raise ValueError(f"pre must be [{rows}, {n_out}] on {dev}, got {list(pre.shape)} on {pre.device}")
-    dx = torch.empty(rows, n_in, dtype=x.dtype, device=dev) if want_x else None
-    dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if want_w else None
-    db = torch.empty(w.shape[:-1], dtype=x.dtype, device=dev) if want_bias else None
-    direct = not ((grad.data_ptr() | x.data_ptr() | w.data_ptr()) & 15 or (grad_stride | stride | row | whole | n_in | n_out) & 7 or
-                  max(grad_stride, stride, row) > 1 << 21)
-    need = dense_lib().evamx_linear_grad_workspace_bytes(rows, n_in, n_out, experts, starts is not None, act, direct)
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    a = LinearGradArgs(ptr(grad), ptr(x), ptr(w), ptr(pre) if act else None, ptr(starts), ptr(dx), ptr(dw), ptr(db), ptr(workspace), need,
-                       grad_stride, stride, row, whole, n_in, _DTYPES[x.dtype], rows, n_in, n_out, experts, act, limit)
-    _launch(dense_lib().evamx_linear_grad, name, dev, ctypes.byref(a), last_error=dense_lib().evamx_dense_last_error)
-    return dx, dw, db
+        if tuple(pre.shape) != (x.shape[0], n_out) or pre.device != x.device:
+            raise ValueError(f"pre must be [{x.shape[0]}, {n_out}] on {x.device}, got {list(pre.shape)} on {pre.device}")
+    return _linear_grad_call(grad, grad_stride, x, w, starts, pre if act else None, limit, sizes, True, True, True)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, starts, bias, activation, limit, residual):
-        y, pre = _linear_forward(_linear_name(starts), x, w, starts, bias, activation, limit, residual, True)
+    def forward(ctx, x, w, starts, bias, residual, residual_stride, limit, sizes):
+        y, pre = _linear_call(x, w, starts, bias, residual, residual_stride, limit, True, sizes)
         ctx.save_for_backward(x, w, starts, pre)
-        ctx.args = activation, limit
+        ctx.args = limit, sizes
         return y
 
     @staticmethod
     def backward(ctx, grad):
+        need = ctx.needs_input_grad
         x, w, starts, pre = ctx.saved_tensors
-        name, need = _linear_name(starts), ctx.needs_input_grad
+        name = _linear_name(starts)
         _check_backward(name, name + "_grad")
         dx = dw = db = None
         if need[0] or need[1] or need[3]:
-            dx, dw, db = _linear_backward(name + "_grad", _rows_of(grad), x, w, starts, pre, *ctx.args, need[0], need[1], need[3])
-        return dx, dw, None, db, None, None, grad if need[6] else None
+            rows, stride = _grad_rows(grad)
+            dx, dw, db = _linear_grad_call(rows, stride, x, w, starts, pre, *ctx.args, need[0], need[1], need[3])
+        return dx, dw, None, db, grad if need[4] else None, None, None, None
 
 
 def _linear_name(starts):
     return "linear" if starts is None else "expert_linear"
 
 
-def _linear_call(x, w, starts, bias, activation, limit, residual, return_pre):
+def _linear(x, w, starts, bias, activation, limit, residual, return_pre):
     name = _linear_name(starts)
     _no_tangent(name, x, w, bias, residual)
+    sizes, residual_stride = _linear_args(x, w, starts, bias, activation, limit, residual)
     if not return_pre and _wants_grad(name, name + "_grad", x, w, bias, residual):
-        return _Linear.apply(x, w, starts, bias, activation, limit, residual)
-    y, pre = _linear_forward(name, x, w, starts, bias, activation, limit, residual, return_pre)
+        return _Linear.apply(x, w, starts, bias, residual, residual_stride, limit, sizes)
+    y, pre = _linear_call(x, w, starts, bias, residual, residual_stride, limit, return_pre, sizes)
     return (y, pre) if return_pre else y
 
 
@@ -699,7 +748,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *
     in a graph capture: there, ``return_pre=True`` gives ``(y, pre)`` outside autograd, for ``linear_grad``."""
     if not isinstance(w, torch.Tensor) or w.ndim != 2:
         raise ValueError("w must be a 2-dim device tensor")
-    return _linear_call(x, w, None, bias, activation, limit, residual, return_pre)
+    return _linear(x, w, None, bias, activation, limit, residual, return_pre)
 
 
 def expert_linear(x: torch.Tensor, w: torch.Tensor, starts: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -708,21 +757,21 @@ def expert_linear(x: torch.Tensor, w: torch.Tensor, starts: torch.Tensor, bias: 
     [experts, n_out]``, ``starts`` int32 ``[experts + 1]`` (``expert_order``). Rows behind ``starts[-1]`` are not read, and are zeros in
     the result and in x's gradient; an expert without rows has gradients of zero."""
     _dev(starts, "starts", torch.int32, 1)
-    return _linear_call(x, w, starts, bias, activation, limit, None, return_pre)
+    return _linear(x, w, starts, bias, activation, limit, None, return_pre)
 
 
 def linear_grad(grad: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: torch.Tensor | None = None, *, activation: str | None = None,
                 limit: float = 0.0):
     """``(x's, w's, bias's)`` gradients of ``linear`` for ``grad [rows, n_out]``; ``pre`` from the forward call where there is an
     activation (its gradient is rounded to x's type before the products). The residual's is ``grad``."""
-    return _linear_backward("linear_grad", grad, x, w, None, pre, activation, limit, True, True, True)
+    return _linear_backward(grad, x, w, None, pre, activation, limit)
 
 
 def expert_linear_grad(grad: torch.Tensor, x: torch.Tensor, w: torch.Tensor, starts: torch.Tensor, pre: torch.Tensor | None = None, *,
                        activation: str | None = None, limit: float = 0.0):
     """``(x's, w's, bias's)`` gradients of ``expert_linear``, as ``linear_grad``."""
     _dev(starts, "starts", torch.int32, 1)
-    return _linear_backward("expert_linear_grad", grad, x, w, starts, pre, activation, limit, True, True, True)
+    return _linear_backward(grad, x, w, starts, pre, activation, limit)
 
 
 def prepare_routes_workspace_bytes(capacity: int, topk: int) -> int:
