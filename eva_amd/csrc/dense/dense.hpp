@@ -153,78 +153,86 @@ struct Tile {
     int expert, row, have, col;   // rows row .. row + have - 1 (of a tile of at most TQ), column tile col
 };
 
-// The work's tile t (row tiles of each expert by cols column tiles); false: none. Tiles go expert by expert, within one
-// eight row tiles by all columns at a time, so that neighbours share their rows and weights in the L2. All threads call it;
-// s: 2 + threads / 64 ints of LDS.
-template <int THREADS>
-__device__ __forceinline__ bool find_tile(const Groups& g, int tq, int cols, int t, int* s, Tile& tile)
-{
-    int e = 0, first = 0, begin = 0, count = g.rows;
-    if (g.starts) {
-        constexpr int PER = (MAX_EXPERTS + THREADS - 1) / THREADS;
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (g.experts + THREADS - 1) / THREADS;
-        int a[PER + 1], mine = 0;
+// The work's tiles: row tiles of TQ of each expert by cols column tiles. They are numbered so that consecutive workgroups, which go to
+// the eight XCDs in turn, give each XCD a contiguous run of them: expert by expert, within one eight row tiles by all columns at a
+// time, so that neighbours share their rows and weights in the L2. All threads call init() and find(); s: 2 + THREADS / 64 ints of LDS
+// for them alone.
+template <int THREADS, int TQ>
+struct Tiles {
+    static constexpr int PER = (MAX_EXPERTS + THREADS - 1) / THREADS;
+    Groups g;
+    int* s;
+    int cols, all, each;          // tiles in all, and of an XCD
+    int upto, mine, per, count[PER];   // a thread's experts: row tiles up to and with them, theirs, and their rows
+
+    __device__ __forceinline__ void init(const Groups& groups, int columns, int* scratch)
+    {
+        g = groups; cols = columns; s = scratch;
+        int total;
+        if (g.starts) {
+            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+            per = (g.experts + THREADS - 1) / THREADS;
+            mine = 0;
 #pragma unroll
-        for (int i = 0; i <= PER; ++i) {
-            const int at = (int)threadIdx.x * per + i;
-            a[i] = i <= per && at <= g.experts ? g.start(at) : 0;
+            for (int i = 0; i < PER; ++i) {
+                const int e = (int)threadIdx.x * per + i;
+                count[i] = i < per && e < g.experts ? g.start(e + 1) - g.start(e) : 0;
+                if (count[i] > 0) mine += (count[i] + TQ - 1) / TQ;
+            }
+            upto = mine;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int n = __shfl_up(upto, d);
+                if (lane >= d) upto += n;
+            }
+            if (lane == 63) s[2 + wave] = upto;
+            __syncthreads();
+            total = 0;
+            for (int w = 0; w < THREADS / 64; ++w) {
+                if (w < wave) upto += s[2 + w];
+                total += s[2 + w];
+            }
+        } else {
+            total = (g.rows + TQ - 1) / TQ;
         }
+        all = __builtin_amdgcn_readfirstlane(total * cols);
+        each = (all + 7) / 8;
+    }
+    // Work item u < 8 * each; false: it has no tile.
+    __device__ __forceinline__ bool find(int u, Tile& tile)
+    {
+        int t = (u & 7) * each + u / 8, e = 0, begin = 0, rows = g.rows;
+        if (u / 8 >= each || t >= all) return false;
+        if (g.starts) {
+            const int row_tile = t / cols;
+            __syncthreads();                                           // the last call's answer has been read
+            if (row_tile >= upto - mine && row_tile < upto) {          // one thread's
+                int before = upto - mine;
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (i < per && (int)threadIdx.x * per + i < g.experts && a[i + 1] > a[i]) mine += (a[i + 1] - a[i] + tq - 1) / tq;
-        int upto = mine;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int n = __shfl_up(upto, d);
-            if (lane >= d) upto += n;
-        }
-        if (lane == 63) s[2 + wave] = upto;
-        if (threadIdx.x == 0) s[0] = -1;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) upto += s[2 + w];
-        int total = 0;
-        for (int w = 0; w < THREADS / 64; ++w) total += s[2 + w];
-        // consecutive workgroups go to the eight XCDs in turn: each XCD gets a contiguous run of tiles
-        const long all = (long)total * cols;
-        const int per_xcd = (int)((all + 7) / 8);
-        const bool any = t / 8 < per_xcd && (long)(t & 7) * per_xcd + t / 8 < all;
-        const long at = (long)(t & 7) * per_xcd + t / 8;
-        const int row_tile = any ? (int)(at / cols) : -1;
-        if (row_tile >= upto - mine && row_tile < upto) {            // one thread's
-            int before = upto - mine;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (i < per && (int)threadIdx.x * per + i < g.experts && a[i + 1] > a[i]) {
-                    const int n = (a[i + 1] - a[i] + tq - 1) / tq;
+                for (int i = 0; i < PER; ++i) {
+                    const int n = count[i] > 0 ? (count[i] + TQ - 1) / TQ : 0;
                     if (row_tile >= before && row_tile < before + n) {
                         s[0] = (int)threadIdx.x * per + i;
                         s[1] = before;
                     }
                     before += n;
                 }
+            }
+            __syncthreads();
+            e = __builtin_amdgcn_readfirstlane(s[0]);
+            t -= __builtin_amdgcn_readfirstlane(s[1]) * cols;
+            begin = g.start(e);
+            rows = g.start(e + 1) - begin;
         }
-        __syncthreads();
-        e = __builtin_amdgcn_readfirstlane(s[0]);
-        if (e < 0) return false;
-        first = __builtin_amdgcn_readfirstlane(s[1]);
-        begin = g.start(e);
-        count = g.start(e + 1) - begin;
-        t = (int)(at - (long)first * cols);
-    } else {
-        const long all = (long)((g.rows + tq - 1) / tq) * cols;
-        const int per_xcd = (int)((all + 7) / 8);
-        const long at = (long)(t & 7) * per_xcd + t / 8;
-        if (t / 8 >= per_xcd || at >= all) return false;
-        t = (int)at;
+        const int row_tiles = (rows + TQ - 1) / TQ, band = t / (8 * cols), in_band = t - band * 8 * cols;
+        const int deep = row_tiles - 8 * band < 8 ? row_tiles - 8 * band : 8;
+        const int r = TQ * (8 * band + in_band % deep);
+        tile.expert = e;
+        tile.row = begin + r;
+        tile.have = rows - r < TQ ? rows - r : TQ;
+        tile.col = in_band / deep;
+        return true;
     }
-    const int row_tiles = (count + tq - 1) / tq, band = t / (8 * cols), in_band = t - band * 8 * cols;
-    const int deep = row_tiles - 8 * band < 8 ? row_tiles - 8 * band : 8;
-    const int r = tq * (8 * band + in_band % deep);
-    tile.expert = e;
-    tile.row = begin + r;
-    tile.have = count - r < tq ? count - r : tq;
-    tile.col = in_band / deep;
-    return true;
-}
+};
 
 // Zeros in rows [from, rows) of out: those of workgroup b of n.
 __device__ __forceinline__ void zero_rows(uint16_t* out, size_t stride, int cols, int64_t from, int64_t rows, int b, int n)

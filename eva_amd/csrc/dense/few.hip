@@ -147,12 +147,16 @@ template <class T, bool GATED, int LIE, int CB>
 __global__ __launch_bounds__(FEW_THREADS) void few_kernel(LinearParams p, int cols)
 {
     extern __shared__ f32x4 part[];
+    __shared__ int scratch[2 + FEW_WAVES];
     Tile t = {0, 0, p.g.rows, (int)blockIdx.x};
     bool any = (int)blockIdx.x < cols;
-    if (p.g.starts || p.g.rows > FEW_ROWS) any = find_tile<FEW_THREADS>(p.g, FEW_ROWS, cols, blockIdx.x, (int*)part, t);
+    if (p.g.starts || p.g.rows > FEW_ROWS) {
+        Tiles<FEW_THREADS, FEW_ROWS> tiles;
+        tiles.init(p.g, cols, scratch);
+        any = tiles.find(blockIdx.x, t);
+    }
     if (p.g.starts) zero_rows(p.y, p.y_stride, GATED ? p.inter : p.n_out, p.g.end(), p.g.rows, blockIdx.x, gridDim.x);
     if (!any) return;
-    __syncthreads();
     if (t.have > 32) few_product<T, GATED, LIE, 4, CB>(p, t, part);
     else if (t.have > 16) few_product<T, GATED, LIE, 2, CB>(p, t, part);
     else few_product<T, GATED, LIE, 1, CB>(p, t, part);

@@ -5,18 +5,63 @@ namespace evamx_dense {
 
 // WP by WQ by KW waves of 64 columns by 16 QB rows each.
 template <class T, bool GATED, bool PTR, int WP, int WQ, int QB, int KW, int STAGES>
-__device__ __forceinline__ void tile_product(const LinearParams& p, const Tile& t, char* lds)
-{
-    constexpr int PB = 4;
+struct TileProduct {
+    static constexpr int PB = 4;
     typedef Gemm<T, PTR, false, WP, WQ, PB, QB, KW, STAGES> G;
-    constexpr int COLS = GATED ? G::TP / 2 : G::TP;
-    const uint16_t* w = p.w + (size_t)t.expert * p.w_expert_stride;
-    typename G::P a;
-    typename G::Q b;
-    if constexpr (PTR) {
-        a.init(w + t.col * COLS, p.w_stride, p.n_in, p.w_cols - t.col * COLS, [](int n) { return n; });
-    } else {
-        if constexpr (GATED) {
+    static constexpr int COLS = GATED ? G::TP / 2 : G::TP;
+
+    // Results that are the sums alone, of whole columns: from the registers to whole lines.
+    static __device__ __forceinline__ bool plain(const LinearParams& p, const Tile& t)
+    {
+        return !GATED && p.splits == 1 && !p.bias && !p.residual && !p.pre && p.act == EVAMX_ACT_NONE && COLS * (t.col + 1) <= p.n_out;
+    }
+    static __device__ __forceinline__ void store_plain(const LinearParams& p, const Tile& t, const f32x4 (&acc)[PB][QB])
+    {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, r0 = 16 * QB * G::wq() + (c & 7);
+        uint16_t* at = p.y + (size_t)(t.row + r0) * p.y_stride + COLS * t.col + 64 * G::wp() + 32 * (c >> 3) + 16 * (g & 1) + 8 * (g >> 1);
+        const bool all = t.have == G::TQ;
+#pragma unroll
+        for (int j = 0; j < QB; ++j) {
+            const f32x4 sums[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+            u16x8 v[2];
+            lined<T>(sums, v);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (all || r0 + 16 * j + 8 * i < t.have) *(u16x8_loose*)(at + (size_t)(16 * j + 8 * i) * p.y_stride) = v[i];
+        }
+    }
+    // All others, by way of LDS.
+    static __device__ __forceinline__ void store(const LinearParams& p, const Tile& t, const f32x4 (&acc)[PB][QB], char* lds)
+    {
+        const int lane = threadIdx.x & 63, wp = G::wp(), wq = G::wq();
+        constexpr int FOURS = GATED ? 8 : 16, PASS = 64 / FOURS;          // fours of a row (SwiGLU: of the gate's half), rows a pass
+        const int in = 4 * (lane % FOURS), n = (GATED ? COLS * t.col + 32 * wp : COLS * t.col + 64 * wp) + in;
+        rows_of<PB, QB>(acc, lds, wq * WP + wp, [&](const float* mine, int first, int count) {
+            for (int r0 = lane / FOURS; r0 < count; r0 += PASS) {
+                const int r = 16 * QB * wq + first + r0;
+                if (r >= t.have) break;
+                const f32x4 x = *(const f32x4*)(mine + r0 * OUT_ROW + in), y = *(const f32x4*)(mine + r0 * OUT_ROW + in + (GATED ? 32 : 0));
+                float v[4] = {x[0], x[1], x[2], x[3]}, u[4] = {y[0], y[1], y[2], y[3]};
+                if (p.splits > 1) {
+                    float* part = p.part + ((size_t)blockIdx.y * p.g.rows + t.row + r) * p.n_out + n;
+                    const int have = (GATED ? p.inter : p.n_out) - n;
+                    store_floats(part, v, have);
+                    if (GATED) store_floats(part + p.inter, u, have);
+                } else {
+                    finish<T, GATED, 4>(p, t.expert, t.row + r, n, v, u);
+                }
+            }
+        });
+    }
+
+    static __device__ __forceinline__ void take(const LinearParams& p, const Tile& t, char* lds)
+    {
+        const uint16_t* w = p.w + (size_t)t.expert * p.w_expert_stride;
+        typename G::P a;
+        typename G::Q b;
+        if constexpr (PTR) {
+            a.init(w + t.col * COLS, p.w_stride, p.n_in, p.w_cols - t.col * COLS, [](int n) { return n; });
+        } else if constexpr (GATED) {
             a.init(w, p.w_stride, p.n_out, p.w_cols, [&](int n) {           // a wave's first 32 values are of the gate
                 const int j = COLS * t.col + 32 * (n >> 6) + (n & 31);
                 return (n & 32) ? p.inter + j : j;
@@ -25,32 +70,16 @@ __device__ __forceinline__ void tile_product(const LinearParams& p, const Tile& 
             const int n0 = COLS * t.col;
             a.init(w + (size_t)n0 * p.w_stride, p.w_stride, p.n_out - n0 < COLS ? p.n_out - n0 : COLS, p.w_cols, [](int n) { return n; });
         }
+        b.init(p.x + (size_t)t.row * p.x_stride, p.x_stride, t.have, p.x_cols, [](int n) { return n; });
+        const int kt = (p.n_in + TILE_K - 1) / TILE_K;
+        const int k0 = p.splits > 1 ? (int)((long)kt * blockIdx.y / p.splits) : 0, k1 = p.splits > 1 ? (int)((long)kt * (blockIdx.y + 1) / p.splits) : kt;
+        f32x4 acc[PB][QB] = {};
+        G::begin(a, b, lds, k0, k1);
+        if (!G::run(acc, a, b, lds, k0, k1)) return;
+        if (plain(p, t)) store_plain(p, t, acc);
+        else store(p, t, acc, lds);
     }
-    b.init(p.x + (size_t)t.row * p.x_stride, p.x_stride, t.have, p.x_cols, [](int n) { return n; });
-    f32x4 acc[PB][QB] = {};
-    const int kt = (p.n_in + TILE_K - 1) / TILE_K, k0 = (int)((long)kt * blockIdx.y / p.splits), k1 = (int)((long)kt * (blockIdx.y + 1) / p.splits);
-    G::begin(a, b, lds, k0, k1);
-    if (!G::run(acc, a, b, lds, k0, k1)) return;
-    const int lane = threadIdx.x & 63, wp = G::wp(), wq = G::wq();
-    constexpr int FOURS = GATED ? 8 : 16, PASS = 64 / FOURS;              // fours of a row (SwiGLU: of the gate's half), rows a pass
-    const int in = 4 * (lane % FOURS), n = (GATED ? COLS * t.col + 32 * wp : COLS * t.col + 64 * wp) + in;
-    rows_of<PB, QB>(acc, lds, wq * WP + wp, [&](const float* mine, int first, int count) {
-        for (int r0 = lane / FOURS; r0 < count; r0 += PASS) {
-            const int r = 16 * QB * wq + first + r0;
-            if (r >= t.have) break;
-            const f32x4 x = *(const f32x4*)(mine + r0 * OUT_ROW + in), y = *(const f32x4*)(mine + r0 * OUT_ROW + in + (GATED ? 32 : 0));
-            float v[4] = {x[0], x[1], x[2], x[3]}, u[4] = {y[0], y[1], y[2], y[3]};
-            if (p.splits > 1) {
-                float* part = p.part + ((size_t)blockIdx.y * p.g.rows + t.row + r) * p.n_out + n;
-                const int have = (GATED ? p.inter : p.n_out) - n;
-                store_floats(part, v, have);
-                if (GATED) store_floats(part + p.inter, u, have);
-            } else {
-                finish<T, GATED, 4>(p, t.expert, t.row + r, n, v, u);
-            }
-        }
-    });
-}
+};
 
 // A workgroup's tile: 256 columns by 256 rows, or 128 by 128, whose waves take half a k-tile each.
 template <int SIZE>
@@ -63,22 +92,28 @@ template <class T, bool GATED, bool PTR, int SIZE>
 __global__ __launch_bounds__(TileShape<SIZE>::THREADS, 2) void tiles_kernel(LinearParams p, int cols)
 {
     typedef TileShape<SIZE> S;
-    constexpr int WIDE = Gemm<T, PTR, false, S::WP, S::WQ, 4, 8, S::KW, 2>::LDS;
-    constexpr int HALF = S::BIG ? Gemm<T, PTR, false, 4, 1, 4, 8, 2, 3>::LDS : 0;
-    __shared__ __attribute__((aligned(1024))) char lds[WIDE > HALF ? WIDE : HALF];
+    typedef TileProduct<T, GATED, PTR, S::WP, S::WQ, 8, S::KW, 2> Whole;
+    // an expert's last rows: waves of half a k-tile, three k-tiles in LDS (32 experts of 128 rows, 7168 -> 4096: 438 us against 530
+    // with the waves of the whole tile)
+    typedef TileProduct<T, GATED, PTR, 4, 1, 8, 2, 3> Half;
+    typedef TileProduct<T, GATED, PTR, 4, 1, 4, 2, 3> Quarter;
+    __shared__ __attribute__((aligned(1024))) char lds[S::BIG && Half::G::LDS > Whole::G::LDS ? Half::G::LDS : Whole::G::LDS];
     Tile t;
-    const bool any = find_tile<S::THREADS>(p.g, S::TQ, cols, blockIdx.x, (int*)lds, t);
+    bool any;
+    {
+        Tiles<S::THREADS, S::TQ> tiles;
+        tiles.init(p.g, cols, (int*)lds);
+        any = tiles.find(blockIdx.x, t);
+    }
     // each workgroup clears a share of the rows behind the last, beside the others' products
     if (p.g.starts) zero_rows(p.y, p.y_stride, GATED ? p.inter : p.n_out, p.g.end(), p.g.rows, blockIdx.x, gridDim.x);
     if (!any) return;
     __syncthreads();
     if constexpr (S::BIG) {
-        // an expert's last rows: waves of half a k-tile, three k-tiles in LDS (32 experts of 128 rows, 7168 -> 4096: 438 us against 530
-        // with the waves of the whole tile)
-        if (t.have <= 64) return tile_product<T, GATED, PTR, 4, 1, 4, 2, 3>(p, t, lds);
-        if (t.have <= 128) return tile_product<T, GATED, PTR, 4, 1, 8, 2, 3>(p, t, lds);
+        if (t.have <= 64) return Quarter::take(p, t, lds);
+        if (t.have <= 128) return Half::take(p, t, lds);
     }
-    tile_product<T, GATED, PTR, S::WP, S::WQ, 8, S::KW, 2>(p, t, lds);
+    Whole::take(p, t, lds);
 }
 
 // Sums of the splits, and what follows a sum.
@@ -112,8 +147,8 @@ static void launch_size(const LinearParams& p, hipStream_t s)
 {
     typedef TileShape<SIZE> S;
     const int cols = ceil_div(GATED ? p.inter : p.n_out, GATED ? 32 * S::WP : 64 * S::WP);
-    const int64_t work = most_row_tiles(p.g.rows, p.g.experts, p.g.starts, S::TQ) * cols;
-    tiles_kernel<T, GATED, PTR, SIZE><<<dim3((unsigned)(8 * ceil_div(work, 8)), p.splits), S::THREADS, 0, s>>>(p, cols);
+    const int64_t work = 8 * (int64_t)ceil_div(most_row_tiles(p.g.rows, p.g.experts, p.g.starts, S::TQ) * cols, 8);
+    tiles_kernel<T, GATED, PTR, SIZE><<<dim3((unsigned)work, p.splits), S::THREADS, 0, s>>>(p, cols);
 }
 
 template <class T, bool GATED, bool PTR>
