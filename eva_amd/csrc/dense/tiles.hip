@@ -10,24 +10,40 @@ struct TileProduct {
     typedef Gemm<T, PTR, false, WP, WQ, PB, QB, KW, STAGES> G;
     static constexpr int COLS = GATED ? G::TP / 2 : G::TP;
 
-    // Results that are the sums alone, of whole columns: from the registers to whole lines.
+    // Results that are the sums alone, or SwiGLU's of them, in whole columns: from the registers.
     static __device__ __forceinline__ bool plain(const LinearParams& p, const Tile& t)
     {
-        return !GATED && p.splits == 1 && !p.bias && !p.residual && !p.pre && p.act == EVAMX_ACT_NONE && COLS * (t.col + 1) <= p.n_out;
+        return p.splits == 1 && !p.bias && !p.residual && !p.pre && (GATED || p.act == EVAMX_ACT_NONE) && COLS * (t.col + 1) <= (GATED ? p.inter : p.n_out);
     }
     static __device__ __forceinline__ void store_plain(const LinearParams& p, const Tile& t, const f32x4 (&acc)[PB][QB])
     {
-        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, r0 = 16 * QB * G::wq() + (c & 7);
-        uint16_t* at = p.y + (size_t)(t.row + r0) * p.y_stride + COLS * t.col + 64 * G::wp() + 32 * (c >> 3) + 16 * (g & 1) + 8 * (g >> 1);
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
         const bool all = t.have == G::TQ;
+        if constexpr (GATED) {
+            const int r0 = 16 * QB * G::wq() + c;
+            uint16_t* at = p.y + (size_t)(t.row + r0) * p.y_stride + COLS * t.col + 32 * G::wp() + 16 * (g & 1) + 8 * (g >> 1);
 #pragma unroll
-        for (int j = 0; j < QB; ++j) {
-            const f32x4 sums[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
-            u16x8 v[2];
-            lined<T>(sums, v);
+            for (int j = 0; j < QB; ++j) {
+                f32x4 y[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (all || r0 + 16 * j + 8 * i < t.have) *(u16x8_loose*)(at + (size_t)(16 * j + 8 * i) * p.y_stride) = v[i];
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[b][i] = swiglu(acc[b][j][i], acc[2 + b][j][i], p.limit);
+                const u16x8 v = paired<T>(y[0], y[1]);
+                if (all || r0 + 16 * j < t.have) *(u16x8_loose*)(at + (size_t)(16 * j) * p.y_stride) = v;
+            }
+        } else {
+            const int r0 = 16 * QB * G::wq() + (c & 7);
+            uint16_t* at = p.y + (size_t)(t.row + r0) * p.y_stride + COLS * t.col + 64 * G::wp() + 32 * (c >> 3) + 16 * (g & 1) + 8 * (g >> 1);
+#pragma unroll
+            for (int j = 0; j < QB; ++j) {
+                const f32x4 sums[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+                u16x8 v[2];
+                lined<T>(sums, v);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (all || r0 + 16 * j + 8 * i < t.have) *(u16x8_loose*)(at + (size_t)(16 * j + 8 * i) * p.y_stride) = v[i];
+            }
         }
     }
     // All others, by way of LDS.
