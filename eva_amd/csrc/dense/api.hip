@@ -39,11 +39,15 @@ static Plan plan_with(int64_t rows, int64_t cols, int64_t k, double& least)
             const int64_t work = ((rows + edge - 1) / edge) * ((cols + edge - 1) / edge) * splits, rest = work % at_once;
             const double each = (double)((kt + splits - 1) / splits);
             auto round = [&](int64_t n) {
-                const double x = size == TILES_256 ? 1.2 + 0.35 * n / CUS : n <= CUS ? 0.7 : 0.7 + 0.35 * (n - CUS) / CUS;
-                return each * x + 6;
+                if (size == TILES_256) return each * (1.15 + (n > 160 ? 0.35 * (n - 160) / (CUS - 160) : 0)) + 5;
+                return each * (n <= CUS ? 0.58 + 0.04 * n / CUS : 0.62 + 0.23 * (n - CUS) / CUS) + 4;
             };
             double time = (double)(work / at_once) * round(at_once) + (rest ? round(rest) : 0);
-            if (splits > 1) time += 4 + 2.0 * splits * rows * cols * 4 / 4.5e6;
+            // what is read, at the rate that so many workgroups reach
+            const double many = (double)work / (size == TILES_256 ? 210 : 430), few = size == TILES_256 ? 0.2 : 0.4;
+            const double read = 2.0 * (rows + cols) * k / (4.9e6 * (few + (1 - few) * (many < 1 ? many : 1)));
+            if (time < read) time = read;
+            if (splits > 1) time += 7 + (double)splits * rows * cols * 4 / 2.9e6;
             if (time < least) {
                 least = time;
                 best = {size, splits};

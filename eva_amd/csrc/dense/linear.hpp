@@ -27,9 +27,11 @@ enum { TILES_128 = 0, TILES_256 = 2 };
 struct Plan {
     int size, splits;
 };
-// For a result of rows by cols that sums k values: the plan of the least time as measured for both kinds of tiles, a k-tile of 64 in
-// 1.2 us for a lone 256 by 256 tile to 1.55 with all CUs at work (128 by 128: 0.7 to one a CU, 1.05 with two), 6 us for a tile's
-// begin and end, and for a cut sum its way through memory at 4.5 TB/s and 4 us for the join.
+// For a result of rows by cols that sums k values: the plan of the least time as measured for both kinds of tiles: a k-tile of 64 takes
+// a 256 by 256 tile 1.15 us, 1.5 with all CUs at work, and a 128 by 128 one 0.58, with two on every CU 0.85; a tile's begin and end 5
+// and 4 us; no less than what is read at 4.9 TB/s (with 144 workgroups 2.6, 288 3.8); a cut sum 7 us more for the join and its way through memory at 2.9 TB/s. (us: 1024 rows
+// of 4096 -> 4096 in 128 by 128 tiles 43, cut in two 45, in four 58, in 256 by 256 tiles 79, 56 and 49; 128 rows 39, 29, 22 and 51,
+// 36, 26.)
 Plan plan_of(int64_t rows, int64_t cols, int64_t k);
 
 // Eight values at p of a row, or as many as there are.
