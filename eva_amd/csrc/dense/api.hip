@@ -33,7 +33,7 @@ static Plan plan_with(int64_t rows, int64_t cols, int64_t k, double& least)
     const int64_t kt = (k + TILE_K - 1) / TILE_K;
     Plan best = {TILES_256, 1};
     least = 1e30;
-    for (int size = TILES_128; size <= TILES_256; size += TILES_256 - TILES_128)
+    for (int size : {TILES_128, TILES_256})
         for (int splits = 1; splits <= MAX_SPLITS && (splits == 1 || kt / splits >= 4); ++splits) {
             const int64_t edge = size == TILES_256 ? 256 : 128, at_once = size == TILES_256 ? CUS : 2 * CUS;
             const int64_t work = ((rows + edge - 1) / edge) * ((cols + edge - 1) / edge) * splits, rest = work % at_once;

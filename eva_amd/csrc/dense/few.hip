@@ -139,7 +139,7 @@ __device__ __forceinline__ void few_product(const LinearParams& p, const Tile& t
                 if (GATED) u[i] += s2[i];
             }
         }
-        finish<T, GATED, 4>(p, t.expert, t.row + r, 16 * (CB * t.col + b) + 4 * g, v, u);
+        finish<T, GATED>(p, t.expert, t.row + r, 16 * (CB * t.col + b) + 4 * g, v, u);
     }
 }
 

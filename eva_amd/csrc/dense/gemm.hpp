@@ -2,7 +2,11 @@
 //
 // p runs along a row of the result (so that a lane ends up with four values in a row), q over its rows. A matrix comes either
 // with k along its rows in memory, or (TR) with k over its rows: then LDS holds it as it lies in memory and ds_read_b64_tr_b16
-// turns it on the way to the registers. k-tiles of 64 come to LDS directly, two stages in turn.
+// turns it on the way to the registers. k-tiles of 64 come to LDS directly, into two or three places in turn.
+//
+// 256 by 256 by 64: 2048 cycles of matrix instructions a CU beside 1536 of LDS reads and 512 of its loads. 8192 rows of 7168 -> 4096 in
+// bf16: 365 us, 1320 TFLOP/s (x's gradient 397, w's 383; a large library product 1605): the operands' way from memory, a k-tile ahead,
+// and the clock under such loads bound it. 4096^3: 100 us, 1370 TFLOP/s.
 #pragma once
 #include "dense.hpp"
 
@@ -142,6 +146,9 @@ __device__ __forceinline__ void arrive()                                // all w
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// A wave's place in LDS for results on their way out: 64 rows, OUT_ROW floats apart (rows_of).
+constexpr int OUT_ROW = 68, OUT_BYTES = 64 * OUT_ROW * 4;
+
 // WP by WQ waves of PB by QB blocks each, KW times: with KW = 2 each half of a k-tile is another wave's, and the two's sums meet in
 // LDS at the end. STAGES k-tiles in LDS.
 template <class T, bool PTR, bool QTR, int WP, int WQ, int PB, int QB, int KW, int STAGES>
@@ -151,7 +158,7 @@ struct Gemm {
     typedef Side<QTR, TQ, WAVES> Q;
     static constexpr int STAGE = P::BYTES + Q::BYTES, JOIN = KW == 1 ? 0 : WP * WQ * PB * QB * 1024;
     static constexpr int STAGES_BYTES = STAGES * STAGE;
-    static constexpr int OUT = WP * WQ * (64 * 68 * 4);
+    static constexpr int OUT = WP * WQ * OUT_BYTES;
     static constexpr int LDS = STAGES_BYTES > JOIN ? STAGES_BYTES > OUT ? STAGES_BYTES : OUT : JOIN > OUT ? JOIN : OUT;
 
     static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
@@ -164,6 +171,7 @@ struct Gemm {
     //
     // The barrier of a k-tile lies where a wave has read all it needs of it: its place then takes the k-tile STAGES further, and the
     // next one's first operands are read while the last products of this one run.
+    //
     // begin() asks for the first k-tiles, run() does the rest. under: each wave has made UNDER other requests between the two, which
     // need not be waited for (requests end in their order).
     static __device__ __forceinline__ void begin(const P& p, const Q& q, char* lds, int kt0, int kt1)
@@ -316,27 +324,25 @@ __device__ __forceinline__ u16x8 paired(f32x4 a, f32x4 b)
 template <class T>
 __device__ __forceinline__ void lined(const f32x4 (&a)[4], u16x8 (&v)[2])
 {
+#ifdef __HIP_DEVICE_COMPILE__
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     const u32x4 x = __builtin_bit_cast(u32x4, paired<T>(a[0], a[1])), y = __builtin_bit_cast(u32x4, paired<T>(a[2], a[3]));
     const bool first = (threadIdx.x & 8) == 0;
     u32x4 p, q;
-#ifdef __HIP_DEVICE_COMPILE__
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t got = __builtin_amdgcn_update_dpp(0, first ? y[i] : x[i], 0x128, 0xf, 0xf, true);    // row_ror:8
         p[i] = first ? x[i] : got;
         q[i] = first ? got : y[i];
     }
-#endif
     v[0] = __builtin_bit_cast(u16x8, p);
     v[1] = __builtin_bit_cast(u16x8, q);
+#endif
 }
 
 // A wave's results by way of LDS: 16 PB columns of 64 rows at a time, rows OUT_ROW floats apart, so that neighbours get neighbouring
 // values of a row (whole lines are loaded and stored) and the code that takes them is there once. f(rows in LDS, the first one's
 // number in the wave's 16 QB, how many).
-constexpr int OUT_ROW = 68, OUT_ROWS = 64, OUT_BYTES = OUT_ROWS * OUT_ROW * 4;
-
 template <int PB, int QB, class F>
 __device__ __forceinline__ void rows_of(const f32x4 (&acc)[PB][QB], char* lds, int slot, F f)
 {

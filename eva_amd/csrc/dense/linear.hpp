@@ -23,15 +23,15 @@ struct LinearParams {
 };
 
 // Tiles of 256 by 256, one workgroup a CU, or of 128 by 128, two a CU, and the parts a sum is cut into.
-enum { TILES_128 = 0, TILES_256 = 2 };
+enum { TILES_128 = 0, TILES_256 = 1 };
 struct Plan {
     int size, splits;
 };
-// For a result of rows by cols that sums k values: the plan of the least time as measured for both kinds of tiles: a k-tile of 64 takes
+// For a result of rows by cols that sums k values: the plan of the least time as measured for both kinds of tiles. A k-tile of 64 takes
 // a 256 by 256 tile 1.15 us, 1.5 with all CUs at work, and a 128 by 128 one 0.58, with two on every CU 0.85; a tile's begin and end 5
-// and 4 us; no less than what is read at 4.9 TB/s (with 144 workgroups 2.6, 288 3.8); a cut sum 7 us more for the join and its way through memory at 2.9 TB/s. (us: 1024 rows
-// of 4096 -> 4096 in 128 by 128 tiles 43, cut in two 45, in four 58, in 256 by 256 tiles 79, 56 and 49; 128 rows 39, 29, 22 and 51,
-// 36, 26.)
+// and 4 us; no less than what is read at 4.9 TB/s (by 144 workgroups 2.6, 288 3.8); a cut sum 7 us more for the join, and its way
+// through memory at 2.9 TB/s. (us: 1024 rows of 4096 -> 4096 in 128 by 128 tiles 43, cut in two 45, in four 58, in 256 by 256 tiles 79,
+// 56 and 49; 128 rows 39, 29, 22 and 51, 36, 26.)
 Plan plan_of(int64_t rows, int64_t cols, int64_t k);
 
 // Eight values at p of a row, or as many as there are.
@@ -49,37 +49,32 @@ __device__ __forceinline__ void load8(float (&v)[8], const uint16_t* p, int have
     for (int i = 0; i < 8; ++i) v[i] = bf16 ? Bf16::get(x[i]) : F16::get(x[i]);
 }
 
-// N (4 or 8) consecutive results at column n of row `row`: v as summed, for SwiGLU the gate's, u the up product's.
-template <class T, bool GATED, int N>
-__device__ __forceinline__ void finish(const LinearParams& p, int expert, int row, int n, float (&v)[N], float (&u)[N])
+// Four consecutive results at column n of row `row`: v as summed, for SwiGLU the gate's, u the up product's.
+template <class T, bool GATED>
+__device__ __forceinline__ void finish(const LinearParams& p, int expert, int row, int n, float (&v)[4], float (&u)[4])
 {
-    constexpr bool BF = std::is_same<T, Bf16>::value;
     const int cols = GATED ? p.inter : p.n_out, have = cols - n;
     if (have <= 0) return;
-    auto get = [&](const uint16_t* from, float (&out)[N]) {
-        if (have >= N) {
-            if constexpr (N == 8) {
-                load8(out, from, 8, BF);
-            } else {
-                const u16x4 x = *(const u16x4_loose*)from;
+    auto get = [&](const uint16_t* from, float (&out)[4]) {
+        if (have >= 4) {
+            const u16x4 x = *(const u16x4_loose*)from;
 #pragma unroll
-                for (int i = 0; i < N; ++i) out[i] = T::get(x[i]);
-            }
+            for (int i = 0; i < 4; ++i) out[i] = T::get(x[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) out[i] = i < have ? T::get(from[i]) : 0.0f;
+            for (int i = 0; i < 4; ++i) out[i] = i < have ? T::get(from[i]) : 0.0f;
         }
     };
-    float t[N];
+    float t[4];
     if (p.bias) {
         const uint16_t* b = p.bias + (size_t)expert * p.n_out + n;
         get(b, t);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += t[i];
+        for (int i = 0; i < 4; ++i) v[i] += t[i];
         if (GATED) {
             get(b + p.inter, t);
 #pragma unroll
-            for (int i = 0; i < N; ++i) u[i] += t[i];
+            for (int i = 0; i < 4; ++i) u[i] += t[i];
         }
     }
     if (p.pre) {
@@ -88,28 +83,21 @@ __device__ __forceinline__ void finish(const LinearParams& p, int expert, int ro
         if (GATED) store_floats(at + p.inter, u, have);
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = GATED ? swiglu(v[i], u[i], p.limit) : activate(v[i], p.act);
+    for (int i = 0; i < 4; ++i) v[i] = GATED ? swiglu(v[i], u[i], p.limit) : activate(v[i], p.act);
     if (p.residual) {
         get(p.residual + (size_t)row * p.residual_stride + n, t);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += t[i];
+        for (int i = 0; i < 4; ++i) v[i] += t[i];
     }
     uint16_t* y = p.y + (size_t)row * p.y_stride + n;
-    if (have >= N) {
-        if constexpr (N == 8) {
-            u16x8 o;
+    if (have >= 4) {
+        u16x4 o;
 #pragma unroll
-            for (int i = 0; i < N; ++i) o[i] = T::put(v[i]);
-            *(u16x8_loose*)y = o;
-        } else {
-            u16x4 o;
-#pragma unroll
-            for (int i = 0; i < N; ++i) o[i] = T::put(v[i]);
-            *(u16x4_loose*)y = o;
-        }
+        for (int i = 0; i < 4; ++i) o[i] = T::put(v[i]);
+        *(u16x4_loose*)y = o;
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int i = 0; i < 3; ++i)
             if (i < have) y[i] = T::put(v[i]);
     }
 }

@@ -1,4 +1,5 @@
-// y = act(x W^T + b) + residual in tiles, and x's gradient D W, whose matrix has k over its rows.
+// y = act(x W^T + b) + residual in tiles, and x's gradient D W, whose matrix has k over its rows. With few rows an expert the weights
+// are what is read: 32 experts of 128 rows, 7168 -> 4096, 1.9 GB: 432 us, 4.4 TB/s.
 #include "linear.hpp"
 
 namespace evamx_dense {
@@ -64,7 +65,7 @@ struct TileProduct {
                     store_floats(part, v, have);
                     if (GATED) store_floats(part + p.inter, u, have);
                 } else {
-                    finish<T, GATED, 4>(p, t.expert, t.row + r, n, v, u);
+                    finish<T, GATED>(p, t.expert, t.row + r, n, v, u);
                 }
             }
         });
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(256) void join_kernel(LinearParams p)
             if (GATED) add_floats(u, part + s * next + p.inter, cols - n);
         }
     }
-    finish<T, GATED, 4>(p, 0, row, n, v, u);
+    finish<T, GATED>(p, 0, row, n, v, u);
 }
 
 template <class T, bool GATED, bool PTR, int SIZE>
