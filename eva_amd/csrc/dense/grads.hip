@@ -141,27 +141,29 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void weight_grad_kernel(WeightGrad
 __global__ __launch_bounds__(256) void pad_kernel(const uint16_t* from, size_t stride, size_t matrix_stride, int rows, int64_t all, int n, uint16_t* to)
 {
     const int per = (n + 7) / 8;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / per;
-    const int v = (int)(at % per) * 8;
-    if (row >= all) return;
-    const uint16_t* p = from + (size_t)(row / rows) * matrix_stride + (size_t)(row % rows) * stride + v;
-    u16x8 x = (u16x8)(uint16_t)0;
-    if (v > 0 && v + 10 <= n) {
-        x = load8_shifted(p);
-    } else if (v + 8 <= n) {
-        x = *(const u16x8_loose*)p;
-    } else {
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all * per; at += (int64_t)gridDim.x * 256) {
+        const int64_t row = at / per;
+        const int v = (int)(at - row * per) * 8;
+        const uint16_t* p = from + (size_t)(row / rows) * matrix_stride + (size_t)(row % rows) * stride + v;
+        u16x8 x = (u16x8)(uint16_t)0;
+        if (v > 0 && v + 10 <= n) {
+            x = load8_shifted(p);
+        } else if (v + 8 <= n) {
+            x = *(const u16x8_loose*)p;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 7; ++i)
-            if (v + i < n) x[i] = p[i];
+            for (int i = 0; i < 7; ++i)
+                if (v + i < n) x[i] = p[i];
+        }
+        *(u16x8*)(to + (size_t)row * (8 * per) + v) = x;
     }
-    *(u16x8*)(to + (size_t)row * (8 * per) + v) = x;
 }
 
 int launch_pad(const uint16_t* from, size_t stride, size_t matrix_stride, int rows, int count, int n, uint16_t* to, hipStream_t s)
 {
     const int64_t all = (int64_t)rows * count;
-    pad_kernel<<<(unsigned)ceil_div(all * ((n + 7) / 8), 256), 256, 0, s>>>(from, stride, matrix_stride, rows, all, n, to);
+    const int64_t groups = (all * ((n + 7) / 8) + 255) / 256;
+    pad_kernel<<<(unsigned)(groups < 1 << 22 ? groups : 1 << 22), 256, 0, s>>>(from, stride, matrix_stride, rows, all, n, to);
     return launched("linear");
 }
 

@@ -49,6 +49,8 @@ class DenseExperts:
             raise ValueError(f"x has {x.shape[-1]} features, the experts {self.hidden}")
         if residual is not None and residual.shape != x.shape:
             raise ValueError(f"residual must be {list(x.shape)}, got {list(residual.shape)}")
+        if sel.dtype.is_floating_point or sel.dtype.is_complex or sel.dtype == torch.bool:
+            raise ValueError(f"sel must hold expert indices, got {sel.dtype}")
         flat, topk = _rows(x), sel.shape[-1]
         order = ops.expert_order(sel.reshape(flat.shape[0], topk).to(torch.int64).contiguous(), self.n_local, first_expert=self.first_expert)
         h = ops.expert_linear(ops.sort_tokens(flat, order), self.gate_up, order.starts, activation="swiglu", limit=limit)

@@ -541,7 +541,10 @@ def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
 def sort_tokens_grad(grad: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """The gradient of ``sort_tokens`` in its tokens: each one's rows of ``grad`` added up (in fp32, rounded once)."""
     stride = _token_rows(grad, "grad")
-    return _combine_call(grad, stride, _order_args(order, grad.device)[1], None, None, 0)
+    position = _order_args(order, grad.device)[1]
+    if grad.shape[0] != position.numel():
+        raise ValueError(f"grad has {grad.shape[0]} rows, the order {position.numel()} slots")
+    return _combine_call(grad, stride, position, None, None, 0)
 
 
 class _CombineTokens(torch.autograd.Function):
@@ -570,8 +573,8 @@ class _CombineTokens(torch.autograd.Function):
 def combine_tokens(y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor | None = None, *,
                    residual: torch.Tensor | None = None) -> torch.Tensor:
     """Sorted rows back to their tokens: ``out[t] = sum_k weights[t, k] * y[order.position[t, k]] + residual[t]``, for ``y [rows,
-    hidden]`` (fp16, bf16 or fp32), ``weights`` fp32 ``[T, topk]`` (1 without) and ``residual`` of y's type; slots without a row add
-    nothing. fp32 sums in slot order, rounded once. Differentiable in y, weights and residual (once, and not in a graph capture:
+    hidden]`` (fp16, bf16 or fp32), ``weights`` fp32 ``[T, topk]`` (1 without) and ``residual`` of y's type; slots without a row, or
+    with one that y does not have, add nothing. fp32 sums in slot order, rounded once. Differentiable in y, weights and residual (once, and not in a graph capture:
     there call it under ``torch.no_grad()``, and ``combine_tokens_grad``)."""
     _no_tangent("combine_tokens", y, weights, residual)
     stride = _token_rows(y, "y")
@@ -742,7 +745,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *
     [n_out]`` and ``residual [rows, n_out]`` of its type. ``activation``: None, "silu", "gelu" (x times the normal distribution
     function), "relu" or "swiglu", whose ``w`` holds the gate's rows and then the up product's: ``min(silu(g), limit) * clamp(u, -limit,
     limit)`` of half as many columns, as the routed experts of ``moe_forward`` (``limit`` 0: not clamped; a NaN stays NaN). fp32
-    sums, rounded once, at the end.
+    sums, rounded once, at the end. Up to 2^24 rows, 2^18 features, and below 3.75 GiB of a matrix with "swiglu".
 
     Differentiable in x, w, bias and residual: a call that autograd follows keeps what the activation takes, in fp32. Once, and not
     in a graph capture: there, ``return_pre=True`` gives ``(y, pre)`` outside autograd, for ``linear_grad``."""
@@ -755,7 +758,8 @@ def expert_linear(x: torch.Tensor, w: torch.Tensor, starts: torch.Tensor, bias: 
                   activation: str | None = None, limit: float = 0.0, return_pre: bool = False):
     """``linear`` on rows sorted by expert (``sort_tokens``), each expert's with its own matrix: ``w [experts, n_out, n_in]``, ``bias
     [experts, n_out]``, ``starts`` int32 ``[experts + 1]`` (``expert_order``). Rows behind ``starts[-1]`` are not read, and are zeros in
-    the result and in x's gradient; an expert without rows has gradients of zero."""
+    the result and in x's gradient (in ``pre`` they are left as they were); an expert without rows has gradients of zero. Up to
+    1024 experts."""
     _dev(starts, "starts", torch.int32, 1)
     return _linear(x, w, starts, bias, activation, limit, None, return_pre)
 

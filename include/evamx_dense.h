@@ -24,15 +24,17 @@ int evamx_dense_version(void);
  * with starts == NULL (experts = 1). Rows behind starts[experts] are not read, and zeros in y. act: SiLU, GELU (x Phi(x)),
  * ReLU, or SwiGLU, min(silu(v[n]), limit) * clamp(v[inter + n], -limit, limit) for n < inter = n_out / 2 (limit 0: none; the first
  * half of W's rows are the gate's, the second the up product's). All of dtype (fp16 or bf16); fp32 sums, rounded once. Rows
- * with unit column strides of any alignment; rows of 16-byte addresses and strides are faster, others may be copied first. starts of any content neither read
- * nor write outside of the given rows. No output overlaps an input, but y may be the residual. */
+ * with unit column strides of any alignment; rows of 16-byte addresses and strides are faster, others may be copied first. starts
+ * of any content neither read nor write outside of the given rows. No output overlaps an input, but y may be the residual. A SwiGLU
+ * matrix (with its row stride) of 3.75 GiB or more is refused for more than a few rows. */
 typedef struct evamx_linear_args {
     const void* x;               /* [rows][x_stride] */
     const void* w;               /* [experts][w_expert_stride]: rows [n_out][w_stride] */
     const void* bias;            /* [experts][n_out] or NULL */
     const void* residual;        /* [rows][residual_stride], n_out (inter) values a row, or NULL */
     void* y;                     /* [rows][y_stride] */
-    float* pre;                  /* fp32 [rows][n_out], what the activation takes (for the gradient), or NULL */
+    float* pre;                  /* fp32 [rows][n_out], what the activation takes (for the gradient), or NULL; rows behind
+                                  * starts[experts] stay as they were */
     const int32_t* starts;       /* [experts + 1] or NULL */
     void* workspace;             /* 16-byte aligned, evamx_linear_workspace_bytes bytes; needs no clearing */
     size_t workspace_bytes;
@@ -40,8 +42,8 @@ typedef struct evamx_linear_args {
     int32_t dtype, rows, n_in, n_out, experts, act;
     float limit;
 } evamx_linear_args;
-/* rows 0..2^24, n_in and n_out 1..EVAMX_W4_MAX_DIM, experts 1..1024. May be 0. direct: x and w have 16-byte addresses and strides (w's
- * matrices too), no row stride is above 2^21, n_in (for the gradient also n_out and grad) a multiple of 8 values; otherwise a call may copy them into the workspace. */
+/* rows 0..2^24, n_in and n_out 1..EVAMX_W4_MAX_DIM, experts 1..1024. May be 0. direct: x and w (for the gradient also grad) have 16-byte addresses and strides (w's matrices too), no row stride is above 2^21, and n_in (n_out) is a
+ * multiple of 8 values; otherwise a call may copy them into the workspace. */
 size_t evamx_linear_workspace_bytes(int rows, int n_in, int n_out, int experts, int grouped, int direct);
 int evamx_linear(const evamx_linear_args* args, evamx_stream_t stream);
 

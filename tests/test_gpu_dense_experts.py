@@ -287,3 +287,36 @@ def test_past_32_bits(dev):
         part = ops.linear(rows[:2], big[4])
         size = rows[:2].float().abs() @ big[4].float().abs().t()
         assert ((y[-2:].float() - part.float()).abs() <= 2 * (8192 / 2 + 64) * 2.0 ** -24 * size + 2.0 ** -7 * part.float().abs()).all()
+
+
+def test_long_copies(dev):
+    """Weights of odd rows, 17 GB, which are copied first: the last expert's against a product of its matrix alone."""
+    experts, n_out, n_in = 1024, 8256, 1001
+    w = torch.randn(experts, n_out, n_in, device=dev, dtype=BF16)
+    x = torch.randn(5 * experts, n_in, device=dev, dtype=BF16)
+    y = ops.expert_linear(x, w, torch.arange(experts + 1, device=dev, dtype=torch.int32) * 5)
+    for e in (0, 511, 1023):
+        part = ops.linear(x[5 * e:5 * e + 5], w[e])
+        size = x[5 * e:5 * e + 5].float().abs() @ w[e].float().abs().t()
+        # fp32 sums of 1001 values in another order, then a rounding of 2^-8 each
+        assert ((y[5 * e:5 * e + 5].float() - part.float()).abs() <= 2 * (1001 / 2 + 64) * 2.0 ** -24 * size + 2.0 ** -7 * part.float().abs()).all()
+
+
+def test_rows_far_apart(dev):
+    """Row strides above 2^21 values: copied."""
+    stride = (1 << 21) + 8
+    flat = torch.randn(80 * stride, device=dev, dtype=BF16)
+    x, w = flat.view(80, stride)[:, :64], flat.view(80, stride)[:40, 128:192]
+    assert torch.equal(ops.linear(x, w), ops.linear(x.contiguous(), w.contiguous()))
+    gr = flat.view(80, stride)[:, 256:296]
+    for a, b in zip(ops.linear_grad(gr, x, w), ops.linear_grad(gr.contiguous(), x.contiguous(), w.contiguous())):
+        assert torch.equal(a, b)
+
+
+def test_routes_of_no_indices_are_refused(dev):
+    layer = DenseExperts(torch.zeros(4, 16, 8, dtype=BF16, device=dev), torch.zeros(4, 8, 8, dtype=BF16, device=dev))
+    x, weights = torch.ones(3, 8, dtype=BF16, device=dev), torch.ones(3, 2, device=dev)
+    for dtype in (torch.float32, torch.bool):
+        with pytest.raises(ValueError, match="indices"):
+            layer(x, torch.ones(3, 2, device=dev).to(dtype), weights)
+    assert layer(x, torch.ones(3, 2, dtype=torch.int32, device=dev), weights).shape == x.shape

@@ -228,3 +228,30 @@ def test_refusals(dev, monkeypatch):
         dual = fwd.make_dual(x.detach(), torch.ones_like(x))
         with pytest.raises(ValueError, match="forward-mode"):
             ops.sort_tokens(dual, order)
+
+
+def test_the_most_slots(dev):
+    """2^26 slots, more tokens than a launch has workgroups for: copies are exact, and so are sums of one row."""
+    rows, hidden, n = 1 << 26, 5, 7
+    sel = (torch.arange(rows, device=dev) * 5 + 3).remainder_(n + 1).view(rows, 1) - 1        # 0..n - 1, and -1 in every eighth
+    x = torch.arange(rows, device=dev).view(rows, 1).bitwise_and(2047).half().expand(rows, hidden).contiguous()
+    order = ops.expert_order(sel, n)
+    assert order.starts[-1] == (sel >= 0).sum()
+    xs = ops.sort_tokens(x, order)
+    at = order.position.view(-1).long()
+    here = at >= 0
+    assert torch.equal(xs[at[here]], x[here]) and not xs[order.starts[-1]:].any()
+    weights = torch.full((rows, 1), 0.5, device=dev)
+    out = ops.combine_tokens(xs, order, weights)
+    assert torch.equal(out, x * 0.5 * here.view(-1, 1))
+    dy, dw = ops.combine_tokens_grad(x, xs, order, weights)
+    assert torch.equal(dy, xs * 0.5)
+    want = (x[:, :1].float() ** 2 * here.view(-1, 1)) * hidden                                # whole numbers below 2^24.4, the last bits a rounding
+    assert ((dw - want).abs() <= 2.0 ** -22 * want).all()
+
+
+def test_a_gradient_of_other_rows_is_refused(dev):
+    order = ops.expert_order(routes(4, 2, 8, 1).to(dev), 8)
+    for rows in (7, 9):
+        with pytest.raises(ValueError, match="slots"):
+            ops.sort_tokens_grad(torch.ones(rows, 16, device=dev), order)
