@@ -224,7 +224,7 @@ extern "C" int evamx_linear(const evamx_linear_args* a, evamx_stream_t stream)
     p.g = Groups{a->starts, a->experts, a->rows};
     p.n_in = a->n_in; p.n_out = a->n_out; p.inter = a->act == EVAMX_ACT_SWIGLU ? cols : 0;
     p.act = a->act; p.limit = a->limit;
-    p.splits = 1;
+    p.splits = 1; p.stream = (int64_t)a->rows * cols * 2 > CACHE;
     const hipStream_t s = (hipStream_t)stream;
     const bool few = few_rows(a->rows, a->n_in, a->n_out, a->experts, grouped);
     if (!few) {
@@ -313,12 +313,13 @@ extern "C" int evamx_linear_grad(const evamx_linear_grad_args* a, evamx_stream_t
         p.y = (uint16_t*)a->grad_x; p.y_stride = (size_t)a->grad_x_stride;
         p.g = g; p.n_in = a->n_out; p.n_out = a->n_in; p.x_cols = (int)pad8(a->n_out); p.w_cols = (int)pad8(a->n_in);
         const Plan plan = forward_plan(a->rows, a->n_out, a->n_in, a->experts, grouped);
-        p.size = plan.size; p.splits = plan.splits; p.part = (float*)at;
+        p.size = plan.size; p.splits = plan.splits; p.part = (float*)at; p.stream = (int64_t)a->rows * a->n_in * 2 > CACHE;
         rc = launch_tiles(p, a->dtype, true, s);
         if (rc != EVAMX_OK) return rc;
     }
     if (a->grad_w) {
-        WeightGradParams p = {x.p, d.p, (size_t)x.stride, (size_t)d.stride, (uint16_t*)a->grad_w, g, a->n_in, a->n_out, (int)pad8(a->n_in),
+        WeightGradParams p = {x.p, d.p, (size_t)x.stride, (size_t)d.stride, (uint16_t*)a->grad_w, g,
+                              (int64_t)a->experts * a->n_in * a->n_out * 2 > CACHE, a->n_in, a->n_out, (int)pad8(a->n_in),
                               (int)pad8(a->n_out), (float*)at, weight_plan(a->rows, a->n_in, a->n_out, a->experts, grouped)};
         rc = launch_weight_grad(p, a->dtype, s);
         if (rc != EVAMX_OK) return rc;

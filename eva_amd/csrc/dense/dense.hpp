@@ -234,14 +234,24 @@ struct Tiles {
     }
 };
 
-// Zeros in rows [from, rows) of out: those of workgroup b of n.
+// 16 bytes of a result. STREAM: not to stay in the L2, for results of more than the last-level cache holds, and what nothing reads.
+template <bool STREAM>
+__device__ __forceinline__ void store16(uint16_t* p, u16x8 v)
+{
+    if constexpr (STREAM) __builtin_nontemporal_store(v, (u16x8_loose*)p);
+    else *(u16x8_loose*)p = v;
+}
+constexpr int64_t CACHE = 256 << 20;
+
+// Zeros in rows [from, rows) of out, which nothing needs: those of workgroup b of n (4096 tokens at an eighth of the experts, 8 slots,
+// seven eighths of the rows: y 444 us against 461 with plain stores, x's gradient 497 against 514).
 __device__ __forceinline__ void zero_rows(uint16_t* out, size_t stride, int cols, int64_t from, int64_t rows, int b, int n)
 {
     for (int64_t r = from + b; r < rows; r += n) {
         uint16_t* at = out + (size_t)r * stride;
         for (int c = threadIdx.x * 8; c < cols; c += blockDim.x * 8) {
             if (c + 8 <= cols) {
-                *(u16x8_loose*)(at + c) = (u16x8)(uint16_t)0;
+                store16<true>(at + c, (u16x8)(uint16_t)0);
             } else {
                 for (int i = c; i < cols; ++i) at[i] = 0;
             }

@@ -107,14 +107,18 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void weight_grad_kernel(WeightGrad
         if (u < units) G::begin(a, b, lds, k0, k1);
         if (whole) {
             uint16_t* at = p.out + (row0 + to_q + (c & 7)) * p.n_in + to_p + 32 * (c >> 3) + 16 * (g & 1) + 8 * (g >> 1);
+            auto all = [&](auto stream) {
 #pragma unroll
-            for (int j = 0; j < QB; ++j) {
-                const f32x4 sums[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
-                u16x8 v[2];
-                lined<T>(sums, v);
+                for (int j = 0; j < QB; ++j) {
+                    const f32x4 sums[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+                    u16x8 v[2];
+                    lined<T>(sums, v);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) *(u16x8_loose*)(at + (size_t)(2 * j + i) * 8 * p.n_in) = v[i];
-            }
+                    for (int i = 0; i < 2; ++i) store16<decltype(stream)::value>(at + (size_t)(2 * j + i) * 8 * p.n_in, v[i]);
+                }
+            };
+            if (p.stream) all(std::true_type());
+            else all(std::false_type());
         } else {
 #pragma unroll
             for (int j = 0; j < QB; ++j) {

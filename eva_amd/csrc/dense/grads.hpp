@@ -21,6 +21,7 @@ struct WeightGradParams {
     size_t x_stride, d_stride;
     uint16_t* out;               // [experts][n_out][n_in]
     Groups g;
+    bool stream;                 // out is more than the last-level cache holds
     int n_in, n_out;
     int x_cols, d_cols;          // values in a row of x and d: multiples of 8, zeros behind the last
     float* part;                 // [splits][n_out][n_in] (one expert)

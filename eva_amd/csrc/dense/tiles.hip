@@ -16,6 +16,7 @@ struct TileProduct {
     {
         return p.splits == 1 && !p.bias && !p.residual && !p.pre && (GATED || p.act == EVAMX_ACT_NONE) && COLS * (t.col + 1) <= (GATED ? p.inter : p.n_out);
     }
+    template <bool STREAM>
     static __device__ __forceinline__ void store_plain(const LinearParams& p, const Tile& t, const f32x4 (&acc)[PB][QB])
     {
         const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -31,7 +32,7 @@ struct TileProduct {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) y[b][i] = swiglu(acc[b][j][i], acc[2 + b][j][i], p.limit);
                 const u16x8 v = paired<T>(y[0], y[1]);
-                if (all || r0 + 16 * j < t.have) *(u16x8_loose*)(at + (size_t)(16 * j) * p.y_stride) = v;
+                if (all || r0 + 16 * j < t.have) store16<STREAM>(at + (size_t)(16 * j) * p.y_stride, v);
             }
         } else {
             const int r0 = 16 * QB * G::wq() + (c & 7);
@@ -43,7 +44,7 @@ struct TileProduct {
                 lined<T>(sums, v);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (all || r0 + 16 * j + 8 * i < t.have) *(u16x8_loose*)(at + (size_t)(16 * j + 8 * i) * p.y_stride) = v[i];
+                    if (all || r0 + 16 * j + 8 * i < t.have) store16<STREAM>(at + (size_t)(16 * j + 8 * i) * p.y_stride, v[i]);
             }
         }
     }
@@ -93,8 +94,9 @@ struct TileProduct {
         f32x4 acc[PB][QB] = {};
         G::begin(a, b, lds, k0, k1);
         if (!G::run(acc, a, b, lds, k0, k1)) return;
-        if (plain(p, t)) store_plain(p, t, acc);
-        else store(p, t, acc, lds);
+        if (!plain(p, t)) store(p, t, acc, lds);
+        else if (p.stream) store_plain<true>(p, t, acc);
+        else store_plain<false>(p, t, acc);
     }
 };
 

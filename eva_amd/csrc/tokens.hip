@@ -144,18 +144,25 @@ struct TokPiece {
     typedef vec loose __attribute__((aligned(sizeof(type))));
     vec v;
 
+    // STREAM: what is not read again before the caches have lost it
+    template <bool STREAM = false>
     __device__ __forceinline__ void load(const void* p, size_t at, int have)
     {
         if (have >= N) {
-            v = *(const loose*)((const type*)p + at);
+            const loose* from = (const loose*)((const type*)p + at);
+            if constexpr (STREAM) v = __builtin_nontemporal_load(from);
+            else v = *from;
         } else {
             for (int i = 0; i < N; ++i) v[i] = i < have ? ((const type*)p)[at + i] : 0;
         }
     }
+    template <bool STREAM = false>
     __device__ __forceinline__ void store(void* p, size_t at, int have) const
     {
         if (have >= N) {
-            *(loose*)((type*)p + at) = v;
+            loose* to = (loose*)((type*)p + at);
+            if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+            else *to = v;
         } else {
             for (int i = 0; i < have; ++i) ((type*)p)[at + i] = v[i];
         }
@@ -195,17 +202,18 @@ struct TokenParams {
     float* grad_weights;
 };
 
-// Workgroups of up to eight waves: a row's parts, or a token's slots, over as few workgroups as that takes, evenly.
-constexpr int TOK_WAVES = 8;
+// Workgroups of up to `most` waves: a row's parts, or a token's slots, over as few workgroups as that takes, evenly. Sums that
+// stream take 16 (16384 tokens: 366 us, with 8 372), others 8 (16 tokens: 4.3 us, with 16 5.1).
+constexpr int TOK_WAVES = 8, TOK_SUM_WAVES = 16;
 struct TokGrid {
     int groups, waves;
-    explicit TokGrid(int units) : groups((units + TOK_WAVES - 1) / TOK_WAVES), waves((units + groups - 1) / groups) {}
+    TokGrid(int units, int most) : groups((units + most - 1) / most), waves((units + groups - 1) / groups) {}
 };
 
 __device__ __forceinline__ int tok_unit() { return blockIdx.y * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // Zeros in the sorted rows behind the last one that belongs to a slot, by the workgroups behind those of the tokens.
-template <int DT>
+template <int DT, bool STREAM>
 __device__ __forceinline__ void tok_zero_tail(const TokenParams& p)
 {
     const int b = (blockIdx.x - p.rows) * gridDim.y + blockIdx.y, n = (gridDim.x - p.rows) * gridDim.y;
@@ -214,27 +222,33 @@ __device__ __forceinline__ void tok_zero_tail(const TokenParams& p)
     TokPiece<DT> zero;
     zero.v = 0;
     for (r += b; r < p.sorted_rows; r += n)
-        for (int c = threadIdx.x * zero.N; c < p.hidden; c += blockDim.x * zero.N) zero.store(p.out, (size_t)r * p.out_stride + c, p.hidden - c);
+        for (int c = threadIdx.x * zero.N; c < p.hidden; c += blockDim.x * zero.N) zero.template store<STREAM>(p.out, (size_t)r * p.out_stride + c, p.hidden - c);
 }
 
+// STREAM, of the kernels below: whether what a pass reads and writes is more than the last-level cache holds. Then the rows written
+// (copies, and gradients), or the rows read for a sum, are marked as not used again. One pass leaves the caches to the next, so that
+// they are measured together, bf16 rows of 7168 values, 8 slots a token: copies of 16384 tokens and their sum 817 us (5.2 TB/s, what
+// a large copy reaches) against 846, a sum of 8191 and its gradient 599 against 624; marked loads alone 841 and 610, stores alone
+// 828 and 620. Rows that fit are not marked (3001 tokens of 5120 values, 6 slots: copies 35 against 39, sums 34 against 41).
+
 // A wave takes 64 pieces of a token's row, and writes them topk times.
-template <int DT>
+template <int DT, bool STREAM>
 __global__ __launch_bounds__(64 * TOK_WAVES) void sort_tokens_kernel(TokenParams p)
 {
     const int t = blockIdx.x, c = (tok_unit() * 64 + (threadIdx.x & 63)) * TokPiece<DT>::N;
-    if (t >= p.rows) return tok_zero_tail<DT>(p);
+    if (t >= p.rows) return tok_zero_tail<DT, STREAM>(p);
     if (c >= p.hidden) return;
     TokPiece<DT> x;
     x.load(p.in, (size_t)t * p.in_stride + c, p.hidden - c);
     for (int k = 0; k < p.topk; ++k) {
         const int at = p.position[(size_t)t * p.topk + k];
-        if (at >= 0 && at < p.sorted_rows) x.store(p.out, (size_t)at * p.out_stride + c, p.hidden - c);
+        if (at >= 0 && at < p.sorted_rows) x.template store<STREAM>(p.out, (size_t)at * p.out_stride + c, p.hidden - c);
     }
 }
 
 // A wave takes 64 pieces of a token's sum, all of its rows' at once. fp32 sums in the order of the slots, rounded once.
-template <int DT>
-__global__ __launch_bounds__(64 * TOK_WAVES) void combine_tokens_kernel(TokenParams p)
+template <int DT, bool STREAM>
+__global__ __launch_bounds__(64 * (STREAM ? TOK_SUM_WAVES : TOK_WAVES)) void combine_tokens_kernel(TokenParams p)
 {
     constexpr int N = TokPiece<DT>::N;
     const int t = blockIdx.x, c = (tok_unit() * 64 + (threadIdx.x & 63)) * N;
@@ -250,7 +264,7 @@ __global__ __launch_bounds__(64 * TOK_WAVES) void combine_tokens_kernel(TokenPar
             const int at = k0 + k < p.topk ? p.position[slot] : -1;
             here[k] = at >= 0 && at < p.sorted_rows;
             w[k] = here[k] && p.weights ? p.weights[slot] : 1.0f;
-            if (here[k]) y[k].load(p.in, (size_t)at * p.in_stride + c, p.hidden - c);
+            if (here[k]) y[k].template load<STREAM>(p.in, (size_t)at * p.in_stride + c, p.hidden - c);
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -267,12 +281,12 @@ __global__ __launch_bounds__(64 * TOK_WAVES) void combine_tokens_kernel(TokenPar
 }
 
 // A wave takes a slot: its row's gradient, and its weight's, a sum over the row that no other wave shares.
-template <int DT>
+template <int DT, bool STREAM>
 __global__ __launch_bounds__(64 * TOK_WAVES) void combine_grad_kernel(TokenParams p)
 {
     constexpr int N = TokPiece<DT>::N;
     const int t = blockIdx.x, k = tok_unit(), lane = threadIdx.x & 63;
-    if (t >= p.rows) return tok_zero_tail<DT>(p);
+    if (t >= p.rows) return tok_zero_tail<DT, STREAM>(p);
     if (k >= p.topk) return;
     const size_t slot = (size_t)t * p.topk + k;
     const int at = p.position[slot];
@@ -289,7 +303,7 @@ __global__ __launch_bounds__(64 * TOK_WAVES) void combine_grad_kernel(TokenParam
                 dot = __builtin_fmaf(g.get(i), y.get(i), dot);
                 d.set(i, w * g.get(i));
             }
-            d.store(p.out, (size_t)at * p.out_stride + c, p.hidden - c);
+            d.template store<STREAM>(p.out, (size_t)at * p.out_stride + c, p.hidden - c);
         }
         for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d);
     }
@@ -298,7 +312,8 @@ __global__ __launch_bounds__(64 * TOK_WAVES) void combine_grad_kernel(TokenParam
 
 // Launches of at most so many tokens, whose threads stay below 2^32. (A loop over tokens in the kernels costs the scalar loads of the
 // positions, which the stores before them might have changed: 3001 tokens of 5120 values, 6 slots, are summed in 28 us instead of 18.)
-constexpr int TOK_LAUNCH = 1 << 22;
+constexpr int TOK_LAUNCH = 1 << 21;
+constexpr int64_t TOK_CACHE = 256 << 20;
 static size_t tok_bytes(int dtype) { return dtype == EVAMX_DTYPE_F32 ? 4 : 2; }
 
 // f(p of the tokens of each launch, whether it is the last) for `rows` tokens; in, residual and out are tokens' rows where `sums`,
@@ -325,12 +340,17 @@ static void tok_launches(TokenParams p, int dtype, bool sums, F f)
 // Workgroups that clear the tail: enough to write at the memory's rate where there is one.
 static int tok_tail_groups(int64_t sorted_rows) { return (int)(sorted_rows < 1024 ? sorted_rows : 1024); }
 
+// f(the type, whether a pass of so many values streams)
 template <class F>
-static void tok_dispatch(int dtype, F f)
+static void tok_dispatch(int dtype, int64_t values, F f)
 {
-    if (dtype == EVAMX_DTYPE_F32) f(std::integral_constant<int, EVAMX_DTYPE_F32>());
-    else if (dtype == EVAMX_DTYPE_BF16) f(std::integral_constant<int, EVAMX_DTYPE_BF16>());
-    else f(std::integral_constant<int, EVAMX_DTYPE_F16>());
+    auto as = [&](auto dt) {
+        if (values * (int64_t)tok_bytes(dtype) > TOK_CACHE) f(dt, std::true_type());
+        else f(dt, std::false_type());
+    };
+    if (dtype == EVAMX_DTYPE_F32) as(std::integral_constant<int, EVAMX_DTYPE_F32>());
+    else if (dtype == EVAMX_DTYPE_BF16) as(std::integral_constant<int, EVAMX_DTYPE_BF16>());
+    else as(std::integral_constant<int, EVAMX_DTYPE_F16>());
 }
 
 static bool tok_sizes_ok(const char* who, int rows, int topk, int n_local)
@@ -431,10 +451,10 @@ extern "C" int evamx_sort_tokens(const void* x, int dtype, int64_t x_stride, int
     TokenParams p = tok_params(rows, hidden, topk, position, out_rows);
     p.starts = starts; p.n_local = n_local;
     p.in = x; p.in_stride = (size_t)x_stride; p.out = out; p.out_stride = (size_t)out_stride;
-    const TokGrid g(tok_parts(dtype, hidden));
-    tok_dispatch(dtype, [&](auto dt) {
+    const TokGrid g(tok_parts(dtype, hidden), TOK_WAVES);
+    tok_dispatch(dtype, (out_rows + rows) * hidden, [&](auto dt, auto stream_out) {
         tok_launches(p, dtype, false, [&](const TokenParams& q, bool last) {
-            sort_tokens_kernel<decltype(dt)::value>
+            sort_tokens_kernel<decltype(dt)::value, decltype(stream_out)::value>
                 <<<dim3(q.rows + (last ? tok_tail_groups(out_rows) : 0), g.groups), 64 * g.waves, 0, (hipStream_t)stream>>>(q);
         });
     });
@@ -455,10 +475,12 @@ extern "C" int evamx_combine_tokens(const void* y, int dtype, int64_t y_stride, 
     TokenParams p = tok_params(rows, hidden, topk, position, y_rows);
     p.in = y; p.in_stride = (size_t)y_stride; p.weights = weights; p.residual = residual; p.residual_stride = (size_t)residual_stride;
     p.out = out; p.out_stride = (size_t)out_stride;
-    const TokGrid g(tok_parts(dtype, hidden));
-    tok_dispatch(dtype, [&](auto dt) {
+    tok_dispatch(dtype, ((int64_t)rows * topk + rows) * hidden, [&](auto dt, auto stream_in) {
+        constexpr bool STREAM = decltype(stream_in)::value;
+        const TokGrid g(tok_parts(dtype, hidden), STREAM ? TOK_SUM_WAVES : TOK_WAVES);
         tok_launches(p, dtype, true, [&](const TokenParams& q, bool) {
-            combine_tokens_kernel<decltype(dt)::value><<<dim3(q.rows, g.groups), 64 * g.waves, 0, (hipStream_t)stream>>>(q);
+            combine_tokens_kernel<decltype(dt)::value, STREAM>
+                <<<dim3(q.rows, g.groups), 64 * g.waves, 0, (hipStream_t)stream>>>(q);
         });
     });
     return launched("combine_tokens");
@@ -483,10 +505,10 @@ extern "C" int evamx_combine_tokens_grad(const void* grad, int dtype, int64_t gr
     p.starts = starts; p.n_local = n_local;
     p.in = grad; p.in_stride = (size_t)grad_stride; p.y = y; p.y_stride = (size_t)y_stride; p.weights = weights;
     p.out = grad_y; p.out_stride = (size_t)grad_y_stride; p.grad_weights = grad_weights;
-    const TokGrid g(topk);
-    tok_dispatch(dtype, [&](auto dt) {
+    const TokGrid g(topk, TOK_WAVES);
+    tok_dispatch(dtype, (2 * y_rows + rows) * hidden, [&](auto dt, auto stream_out) {
         tok_launches(p, dtype, false, [&](const TokenParams& q, bool last) {
-            combine_grad_kernel<decltype(dt)::value>
+            combine_grad_kernel<decltype(dt)::value, decltype(stream_out)::value>
                 <<<dim3(q.rows + (last ? tok_tail_groups(y_rows) : 0), g.groups), 64 * g.waves, 0, (hipStream_t)stream>>>(q);
         });
     });
