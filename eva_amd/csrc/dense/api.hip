@@ -64,11 +64,13 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t k)
 
 // Whether few.hip takes a call: for one matrix where its time (6 us, the weights at 5.6 TB/s, and the rows of x, which each workgroup
 // reads, at 8.9) is below the tiles', up to 64 rows (measured, us, at 1, 16 and 64 rows: 7168 -> 2048: 12, 16, 35 against 19, 20, 21;
-// 7168 -> 18432: 53, 82, 188 against 56, 56, 62); for experts up to four rows for each, of which most may be another rank's (64 experts of
-// 4096 by 7168 at 4 rows: 742 against 662; 25 of them at one row: 294, all of it the weights).
+// 7168 -> 18432: 51, 82, 188 against 56, 56, 62). For experts up to four rows for each, of which most may be another rank's, whatever
+// the experts' shares (64 experts, 7168 -> 4096, rows for four each: spread evenly 544 against 664, by Zipf's law 605 against 633, all
+// one expert's 84 against 134), but not for many workgroups that have little to sum (64 experts, 512 -> 1024: 33 against 18; 32, 1024
+// -> 768: 16 against 20).
 static bool few_rows(int rows, int k, int n, int experts, bool grouped)
 {
-    if (grouped) return rows <= 4 * (int64_t)experts;
+    if (grouped) return rows <= 4 * (int64_t)experts && (k >= 1024 || ceil_div(n, 16) * (int64_t)experts <= 1024);
     if (rows > 64) return false;
     double tiles;
     plan_with(rows, n, k, tiles);
@@ -76,12 +78,18 @@ static bool few_rows(int rows, int k, int n, int experts, bool grouped)
     return 6 + (double)n * k * 2 / 5.6e6 + x / 8.9e6 <= tiles;
 }
 
+// More rows than that may still be few of each expert, or most of them other ranks': where the weights are more than the caches hold, few.hip
+// takes the experts of up to 16 rows and the tiles the others (64 experts, 7168 -> 4096, 8 rows each: 568 us against 667 with tiles
+// alone, 16: 635 against 675; a rank's eighth of 32 rows each: 551 against 665; by Zipf's law 32 rows for each: 766 against 876). Where
+// no expert has as few, the launch without work costs 8 to 22 (60 rows each: 708 against 695; 2048 -> 7168: 405 against 383).
+constexpr int FEW_OF_MANY = 16, MANY = 64;
+
 // Experts' rows are known to the device alone: large tiles (which the kernel takes by halves and quarters where an expert ends), if
 // the most there can be fill the GPU.
 static Plan forward_plan(int rows, int k, int n, int experts, bool grouped)
 {
     if (!grouped) return plan_of(rows, n, k);
-    return {most_row_tiles(rows, experts, true, 256) * ceil_div(n, 256) >= CUS * 3 / 4 ? TILES_256 : TILES_128, 1};
+    return {(rows / 256 + (rows < experts ? rows : experts)) * (int64_t)ceil_div(n, 256) >= CUS * 3 / 4 ? TILES_256 : TILES_128, 1};
 }
 static size_t forward_part(int rows, int k, int n, int experts, bool grouped)
 {
@@ -241,10 +249,21 @@ extern "C" int evamx_linear(const evamx_linear_args* a, evamx_stream_t stream)
         }
     }
     p.x = x.p; p.x_stride = (size_t)x.stride; p.w = w.p; p.w_stride = (size_t)w.stride; p.w_expert_stride = (size_t)w.matrix_stride;
-    if (!few) return launch_tiles(p, a->dtype, false, s);
+    const bool large = (int64_t)a->experts * a->n_out * a->n_in * 2 > CACHE;
+    if (!few) {
+        if (grouped && large && xd && wd && a->rows <= MANY * (int64_t)a->experts) {
+            p.g.upto = FEW_OF_MANY;
+            const int rc = launch_few(p, a->dtype, LIE_STREAM, s);
+            if (rc != EVAMX_OK) return rc;
+            p.g.above = FEW_OF_MANY; p.g.upto = Groups::ALL;
+        }
+        return launch_tiles(p, a->dtype, false, s);
+    }
     const int lx = lie_of(a->x, a->x_stride, 0), lw = lie_of(a->w, a->w_stride, a->experts > 1 ? a->w_expert_stride : 0);
-    const int lie = lx > lw ? lx : lw;
-    return launch_few(p, a->dtype, lie == LIE_16 && a->n_in % 8 ? LIE_4 : lie, s);
+    int lie = lx > lw ? lx : lw;
+    if (lie == LIE_16 && a->n_in % 8) lie = LIE_4;
+    if (lie == LIE_16 && large) lie = LIE_STREAM;
+    return launch_few(p, a->dtype, lie, s);
 }
 
 // What a gradient call may copy: D (where there is no activation to write it anew), x and w.

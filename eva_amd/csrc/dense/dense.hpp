@@ -138,8 +138,10 @@ __device__ __forceinline__ float slope(float v, int act)
 // Rows of expert e are [starts[e], starts[e + 1]), cut to the rows there are, whatever the table holds; without a table all rows
 // are one expert's.
 struct Groups {
+    static constexpr int ALL = 1 << 30;
     const int32_t* starts;
     int experts, rows;
+    int above = 0, upto = ALL;    // with a table: the experts of above + 1 to upto rows, others have none
 
     __device__ __forceinline__ int start(int e) const
     {
@@ -177,7 +179,8 @@ struct Tiles {
             for (int i = 0; i < PER; ++i) {
                 const int e = (int)threadIdx.x * per + i;
                 count[i] = i < per && e < g.experts ? g.start(e + 1) - g.start(e) : 0;
-                if (count[i] > 0) mine += (count[i] + TQ - 1) / TQ;
+                if (count[i] <= g.above || count[i] > g.upto) count[i] = 0;
+                mine += (count[i] + TQ - 1) / TQ;
             }
             upto = mine;
             for (int d = 1; d < 64; d <<= 1) {
@@ -209,7 +212,7 @@ struct Tiles {
                 int before = upto - mine;
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
-                    const int n = count[i] > 0 ? (count[i] + TQ - 1) / TQ : 0;
+                    const int n = (count[i] + TQ - 1) / TQ;
                     if (row_tile >= before && row_tile < before + n) {
                         s[0] = (int)threadIdx.x * per + i;
                         s[1] = before;
@@ -260,10 +263,12 @@ __device__ __forceinline__ void zero_rows(uint16_t* out, size_t stride, int cols
 }
 
 static inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
-// Row tiles that the experts' rows can make at most.
-static inline int64_t most_row_tiles(int rows, int experts, bool grouped, int tq)
+// Row tiles that the rows can make at most.
+static inline int64_t most_row_tiles(const Groups& g, int tq)
 {
-    return grouped ? rows / tq + (rows < experts ? rows : experts) : ceil_div(rows, tq);
+    if (!g.starts) return ceil_div(g.rows, tq);
+    const int64_t most = g.rows / (g.above + 1), experts = most < g.experts ? most : g.experts;    // that have rows
+    return (g.upto < tq ? 0 : g.rows / tq) + experts;
 }
 
 }  // namespace evamx_dense

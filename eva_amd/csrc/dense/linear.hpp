@@ -105,7 +105,7 @@ __device__ __forceinline__ void finish(const LinearParams& p, int expert, int ro
 
 int launch_tiles(const LinearParams& p, int dtype, bool transposed, hipStream_t s);
 // How x and w lie: 16-byte addresses and rows, whole words, or single values.
-enum { LIE_16 = 0, LIE_4 = 1, LIE_2 = 2 };
+enum { LIE_16 = 0, LIE_4 = 1, LIE_2 = 2, LIE_STREAM = 3 };
 int launch_few(const LinearParams& p, int dtype, int lie, hipStream_t s);
 // Rows of n values (rows of each of `count` matrices) to rows of a multiple of 8, zeros behind the last.
 int launch_pad(const uint16_t* from, size_t stride, size_t matrix_stride, int rows, int count, int n, uint16_t* to, hipStream_t s);

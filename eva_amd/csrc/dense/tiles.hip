@@ -166,7 +166,7 @@ static void launch_size(const LinearParams& p, hipStream_t s)
 {
     typedef TileShape<SIZE> S;
     const int cols = ceil_div(GATED ? p.inter : p.n_out, GATED ? 32 * S::WP : 64 * S::WP);
-    const int64_t work = 8 * (int64_t)ceil_div(most_row_tiles(p.g.rows, p.g.experts, p.g.starts, S::TQ) * cols, 8);
+    const int64_t work = 8 * (int64_t)ceil_div(most_row_tiles(p.g, S::TQ) * cols, 8);
     tiles_kernel<T, GATED, PTR, SIZE><<<dim3((unsigned)work, p.splits), S::THREADS, 0, s>>>(p, cols);
 }
 

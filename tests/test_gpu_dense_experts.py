@@ -320,3 +320,33 @@ def test_routes_of_no_indices_are_refused(dev):
         with pytest.raises(ValueError, match="indices"):
             layer(x, torch.ones(3, 2, device=dev).to(dtype), weights)
     assert layer(x, torch.ones(3, 2, dtype=torch.int32, device=dev), weights).shape == x.shape
+
+
+@pytest.mark.parametrize("act", [None, "swiglu"])
+def test_few_rows_beside_many(dev, act):
+    """Weights of more than the caches hold, with experts of 0 to some hundred rows: each against a product of its matrix alone."""
+    counts = [0, 1, 16, 17, 3, 0, 130, 15, 64, 18, 2, 300]
+    n_out, n_in, tail = 4096, 4104, 20
+    starts = torch.tensor([0] + counts, dtype=torch.int32).cumsum(0).to(torch.int32).to(dev)
+    g = torch.Generator(device=dev).manual_seed(6)
+    x, w = (torch.randn(*s, generator=g, device=dev, dtype=BF16) for s in ((sum(counts) + tail, n_in), (len(counts), n_out, n_in)))
+    bias = torch.randn(len(counts), n_out, generator=g, device=dev, dtype=BF16)
+    w *= n_in ** -0.5
+    assert w.numel() * 2 > 256 << 20 and sum(counts) + tail <= 64 * len(counts)
+    y, pre = ops.expert_linear(x, w, starts, bias, activation=act, return_pre=True)
+    assert not y[sum(counts):].any()
+    for e, n in enumerate(counts):
+        if n:
+            rows = slice(int(starts[e]), int(starts[e]) + n)
+            part, z = ops.linear(x[rows], w[e], bias[e], activation=act, return_pre=True)
+            # fp32 sums of 4104 values in another order; then an activation whose slope is below 1.1 a factor, and a rounding of 2^-8 each
+            size = x[rows].float().abs() @ w[e].float().abs().t() + bias[e].float().abs()
+            near = 2 * (4104 / 2 + 64) * 2.0 ** -24 * size
+            if act is None:
+                assert pre is None and ((y[rows].float() - part.float()).abs() <= near + 2.0 ** -7 * part.float().abs()).all()
+                continue
+            assert ((pre[rows] - z).abs() <= near).all()
+            (ga, gu), (na, nu) = z.chunk(2, 1), near.chunk(2, 1)
+            silu = torch.nn.functional.silu(ga)
+            near = 1.1 * na * (gu.abs() + nu) + silu.abs() * nu + 2.0 ** -20 * silu.abs() * gu.abs()
+            assert ((y[rows].float() - part.float()).abs() <= near + 2.0 ** -7 * part.float().abs()).all()
