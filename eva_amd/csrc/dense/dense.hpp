@@ -104,6 +104,26 @@ __device__ __forceinline__ u16x8 load8_shifted(const uint16_t* p)
 
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
 
+// The normal distribution function: its smaller side is erfc(z) / 2 = t 2^(P(t) - z^2 / ln 2) at z = |v| / sqrt(2), t = 1 / (1 + 0.4 z),
+// with P fitted here at the Chebyshev points of z = 0 .. 10, to 1.1e-7 of erfc; in these 32 bits 8e-7 of the value for |v| < 3, 8e-6 for 13.
+// (0.5 (1 + erff) loses the lower side, and costs as much as a product of 64 values: 300 rows of 2048 -> 7168 with bias and residual
+// 46 us instead of 39.)
+__device__ __forceinline__ float normal(float v)
+{
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.282842712f, fabsf(v), 1.0f));
+    float e = -0.306892693f;
+    e = __builtin_fmaf(e, t, 1.37083006f);
+    e = __builtin_fmaf(e, t, -2.22021937f);
+    e = __builtin_fmaf(e, t, 1.52885067f);
+    e = __builtin_fmaf(e, t, -0.699879766f);
+    e = __builtin_fmaf(e, t, 0.458745331f);
+    e = __builtin_fmaf(e, t, 0.570344865f);
+    e = __builtin_fmaf(e, t, 1.44602776f);
+    e = __builtin_fmaf(e, t, -3.14780688f);
+    const float low = t * __builtin_amdgcn_exp2f(__builtin_fmaf(-0.72134752f * v, v, e));
+    return v > 0 ? 1.0f - low : low;
+}
+
 // Clamps that leave a NaN as it is.
 __device__ __forceinline__ float at_most(float v, float m) { return v > m ? m : v; }
 __device__ __forceinline__ float within(float v, float m) { return v > m ? m : v < -m ? -m : v; }
@@ -114,22 +134,29 @@ __device__ __forceinline__ float swiglu(float gate, float up, float limit)
     return limit > 0 ? at_most(a, limit) * within(up, limit) : a * up;
 }
 
-__device__ __forceinline__ float activate(float v, int act)
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act)
 {
-    if (act == EVAMX_ACT_SILU) return v * sigmoid(v);
-    if (act == EVAMX_ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-    if (act == EVAMX_ACT_RELU) return v < 0 ? 0.0f : v;
-    return v;
+    if (act == EVAMX_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] * sigmoid(v[i]);
+    } else if (act == EVAMX_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] * normal(v[i]);
+    } else if (act == EVAMX_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] < 0 ? 0.0f : v[i];
+    }
 }
 
-// d activate(v) / dv
+// Its derivative.
 __device__ __forceinline__ float slope(float v, int act)
 {
     if (act == EVAMX_ACT_SILU) {
         const float s = sigmoid(v);
         return s * (1.0f + v * (1.0f - s));
     }
-    if (act == EVAMX_ACT_GELU) return 0.5f * (1.0f + erff(v * 0.70710678f)) + v * 0.39894228f * __expf(-0.5f * v * v);
+    if (act == EVAMX_ACT_GELU) return normal(v) + v * 0.39894228f * __expf(-0.5f * v * v);
     return v > 0 ? 1.0f : v == v ? 0.0f : v;                     // ReLU; a NaN stays one
 }
 

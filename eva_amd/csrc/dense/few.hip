@@ -185,6 +185,9 @@ __device__ __forceinline__ void few_product(const LinearParams& p, const Tile& t
     for (int block = wave; block < CB * MB; block += WAVES) {
         const int m = block % MB, b = block / MB, r = 16 * m + c;
         if (r >= t.have) continue;
+        Finish<T, GATED> end;
+        end.init(p, t.expert, 16 * (CB * t.col + b) + 4 * g);
+        const u16x4 res = end.residual(p, t.row + r);
         float v[4] = {}, u[4] = {};
         for (int q = 0; q < WAVES; ++q) {
             const f32x4 s = part[((q * NB + b) * MB + m) * 64 + lane], s2 = part[((q * NB + NB - CB + b) * MB + m) * 64 + lane];
@@ -194,7 +197,7 @@ __device__ __forceinline__ void few_product(const LinearParams& p, const Tile& t
                 if (GATED) u[i] += s2[i];
             }
         }
-        finish<T, GATED>(p, t.expert, t.row + r, 16 * (CB * t.col + b) + 4 * g, v, u);
+        end.store(p, t.row + r, v, u, res);
     }
 }
 

@@ -50,58 +50,77 @@ __device__ __forceinline__ void load8(float (&v)[8], const uint16_t* p, int have
     for (int i = 0; i < 8; ++i) v[i] = bf16 ? Bf16::get(x[i]) : F16::get(x[i]);
 }
 
-// Four consecutive results at column n of row `row`: v as summed, for SwiGLU the gate's, u the up product's.
+// What follows a sum, for four consecutive columns from n on, of any rows of an expert. v as summed, for SwiGLU the gate's, u the up
+// product's. What it reads is asked for ahead of the stores, since requests end in their order: read in between, 2000 rows of 2048
+// -> 5120 with bias, activation and its input kept take 69 us instead of 62.
 template <class T, bool GATED>
-__device__ __forceinline__ void finish(const LinearParams& p, int expert, int row, int n, float (&v)[4], float (&u)[4])
-{
-    const int cols = GATED ? p.inter : p.n_out, have = cols - n;
-    if (have <= 0) return;
-    auto get = [&](const uint16_t* from, float (&out)[4]) {
-        if (have >= 4) {
-            const u16x4 x = *(const u16x4_loose*)from;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = T::get(x[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = i < have ? T::get(from[i]) : 0.0f;
-        }
-    };
-    float t[4];
-    if (p.bias) {
-        const uint16_t* b = p.bias + (size_t)expert * p.n_out + n;
-        get(b, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += t[i];
-        if (GATED) {
-            get(b + p.inter, t);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] += t[i];
-        }
-    }
-    if (p.pre) {
-        float* at = p.pre + (size_t)row * p.n_out + n;
-        store_floats(at, v, have);
-        if (GATED) store_floats(at + p.inter, u, have);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = GATED ? swiglu(v[i], u[i], p.limit) : activate(v[i], p.act);
-    if (p.residual) {
-        get(p.residual + (size_t)row * p.residual_stride + n, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += t[i];
-    }
-    uint16_t* y = p.y + (size_t)row * p.y_stride + n;
-    if (have >= 4) {
-        u16x4 o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = T::put(v[i]);
-        *(u16x4_loose*)y = o;
-    } else {
+struct Finish {
+    int n, have;
+    float bias[4], bias_up[4];
+
+    __device__ __forceinline__ u16x4 get(const uint16_t* from) const
+    {
+        if (have >= 4) return *(const u16x4_loose*)from;
+        u16x4 x = {};
 #pragma unroll
         for (int i = 0; i < 3; ++i)
-            if (i < have) y[i] = T::put(v[i]);
+            if (i < have) x[i] = from[i];
+        return x;
     }
-}
+    __device__ __forceinline__ void init(const LinearParams& p, int expert, int column)
+    {
+        n = column;
+        have = (GATED ? p.inter : p.n_out) - n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bias[i] = bias_up[i] = 0.0f;
+        if (p.bias && have > 0) {
+            const uint16_t* b = p.bias + (size_t)expert * p.n_out + n;
+            const u16x4 x = get(b), y = get(b + (GATED ? p.inter : 0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bias[i] = T::get(x[i]);
+                bias_up[i] = T::get(y[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ u16x4 residual(const LinearParams& p, int row) const
+    {
+        return p.residual && have > 0 ? get(p.residual + (size_t)row * p.residual_stride + n) : u16x4{};
+    }
+    __device__ __forceinline__ void store(const LinearParams& p, int row, float (&v)[4], float (&u)[4], u16x4 res) const
+    {
+        if (have <= 0) return;
+        if (p.bias) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] += bias[i];
+                if (GATED) u[i] += bias_up[i];
+            }
+        }
+        if (p.pre) {
+            float* at = p.pre + (size_t)row * p.n_out + n;
+            store_floats(at, v, have);
+            if (GATED) store_floats(at + p.inter, u, have);
+        }
+        if (GATED) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = swiglu(v[i], u[i], p.limit);
+        } else {
+            activate(v, p.act);
+        }
+        u16x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = T::put(p.residual ? v[i] + T::get(res[i]) : v[i]);
+        uint16_t* y = p.y + (size_t)row * p.y_stride + n;
+        if (have >= 4) {
+            *(u16x4_loose*)y = o;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (i < have) y[i] = o[i];
+        }
+    }
+};
 
 int launch_tiles(const LinearParams& p, int dtype, bool transposed, hipStream_t s);
 // How x and w lie: 16-byte addresses and rows, whole words, or single values.
