@@ -205,7 +205,8 @@ static void launch_size(const LinearParams& p, hipStream_t s)
 {
     typedef TileShape<SIZE> S;
     const int cols = ceil_div(GATED ? p.inter : p.n_out, GATED ? 32 * S::WP : 64 * S::WP);
-    const int64_t work = 8 * (int64_t)ceil_div(most_row_tiles(p.g, S::TQ) * cols, 8);
+    // one at least, where few.hip takes all experts there can be, for the rows behind the last
+    const int64_t most = most_row_tiles(p.g, S::TQ) * cols, work = 8 * (int64_t)ceil_div(most < 1 ? 1 : most, 8);
     tiles_kernel<T, GATED, PTR, SIZE><<<dim3((unsigned)work, p.splits), S::THREADS, 0, s>>>(p, cols);
 }
 

@@ -350,3 +350,16 @@ def test_few_rows_beside_many(dev, act):
             silu = torch.nn.functional.silu(ga)
             near = 1.1 * na * (gu.abs() + nu) + silu.abs() * nu + 2.0 ** -20 * silu.abs() * gu.abs()
             assert ((y[rows].float() - part.float()).abs() <= near + 2.0 ** -7 * part.float().abs()).all()
+
+
+def test_few_rows_alone_beside_none(dev):
+    """Two matrices of more than the caches hold and more rows than four for each, but none that has more than sixteen."""
+    w = torch.randn(2, 8704, 8192, device=dev, dtype=BF16) * 0.01
+    x = torch.randn(12, 8192, device=dev, dtype=BF16)
+    y = ops.expert_linear(x, w, torch.tensor([0, 4, 9], dtype=torch.int32, device=dev))
+    assert not y[9:].any()
+    for e, rows in ((0, slice(0, 4)), (1, slice(4, 9))):
+        part = ops.linear(x[rows], w[e])
+        size = x[rows].float().abs() @ w[e].float().abs().t()
+        # fp32 sums of 8192 values in another order, then a rounding of 2^-8 each
+        assert ((y[rows].float() - part.float()).abs() <= 2 * (8192 / 2 + 64) * 2.0 ** -24 * size + 2.0 ** -7 * part.float().abs()).all()
