@@ -19,7 +19,9 @@ constexpr int64_t TOK_MAX_SLOTS = 1 << 26;
 
 // ---- the order ---------------------------------------------------------------------------------
 
-// Chunks of consecutive slots, a workgroup each; a workgroup's waves take consecutive segments of it.
+// Chunks of consecutive slots, a workgroup each; a workgroup's waves take consecutive segments of it. Up to 2048 slots one launch (8
+// slots: 3.6 us, of which a launch is 1.6), more in two, whose second sums the first's counts again in every workgroup (131072 slots
+// of 256 experts: 4.7 and 8.2 us).
 constexpr int ORD_WAVES = 16, ORD_THREADS = 64 * ORD_WAVES, ORD_MAX_CHUNKS = 256;
 
 struct OrderParams {
@@ -280,7 +282,8 @@ __global__ __launch_bounds__(64 * (STREAM ? TOK_SUM_WAVES : TOK_WAVES)) void com
     out.store(p.out, (size_t)t * p.out_stride + c, p.hidden - c);
 }
 
-// A wave takes a slot: its row's gradient, and its weight's, a sum over the row that no other wave shares.
+// A wave takes a slot: its row's gradient, and its weight's, a sum over the row that no other wave shares (8191 x 8 rows of 7168: 2 GB in
+// 425 us, 4.8 TB/s).
 template <int DT, bool STREAM>
 __global__ __launch_bounds__(64 * TOK_WAVES) void combine_grad_kernel(TokenParams p)
 {
