@@ -23,8 +23,8 @@ struct LinearParams {
     bool stream;                 // y is more than the last-level cache holds (48000 rows of 7168, 690 MB: 710 us against 718)
 };
 
-// Tiles of 256 by 256, one workgroup a CU, or of 128 by 128, two a CU, and the parts a sum is cut into.
-enum { TILES_128 = 0, TILES_256 = 1 };
+// Tiles of 256 by 256, one workgroup a CU, or of 128 by 128, two a CU or (chosen at the launch) one, and the parts a sum is cut into.
+enum { TILES_128 = 0, TILES_256 = 1, TILES_128_ALONE = 2 };
 struct Plan {
     int size, splits;
 };

@@ -136,18 +136,20 @@ struct TileProduct {
     }
 };
 
-// A workgroup's tile: 256 columns by 256 rows, or 128 by 128, whose waves take half a k-tile each.
+// A workgroup's tile: 256 columns by 256 rows, or 128 by 128, whose waves take half a k-tile each: four, or, where no two workgroups
+// share a CU, eight (2000 rows, x's gradient of 2048 -> 5120: 54.6 us against 57.9; 128 rows of 4096 -> 4096: 19.6 against 21.3).
 template <int SIZE>
 struct TileShape {
     static constexpr bool BIG = SIZE == TILES_256;
-    static constexpr int WP = BIG ? 4 : 2, WQ = BIG ? 2 : 1, KW = BIG ? 1 : 2, TQ = 128 * WQ, THREADS = 64 * WP * WQ * KW;
+    static constexpr int WP = BIG ? 4 : 2, WQ = SIZE == TILES_128 ? 1 : 2, KW = BIG ? 1 : 2, QB = SIZE == TILES_128_ALONE ? 4 : 8;
+    static constexpr int TQ = 16 * QB * WQ, THREADS = 64 * WP * WQ * KW;
 };
 
 template <class T, bool GATED, bool PTR, int SIZE>
 __global__ __launch_bounds__(TileShape<SIZE>::THREADS, 2) void tiles_kernel(LinearParams p, int cols)
 {
     typedef TileShape<SIZE> S;
-    typedef TileProduct<T, GATED, PTR, S::WP, S::WQ, 8, S::KW, 2> Whole;
+    typedef TileProduct<T, GATED, PTR, S::WP, S::WQ, S::QB, S::KW, 2> Whole;
     // an expert's last rows: waves of half a k-tile, three k-tiles in LDS (32 experts of 128 rows, 7168 -> 4096: 438 us against 530
     // with the waves of the whole tile)
     typedef TileProduct<T, GATED, PTR, 4, 1, 8, 2, 3> Half;
@@ -213,7 +215,9 @@ static void launch_size(const LinearParams& p, hipStream_t s)
 template <class T, bool GATED, bool PTR>
 static void launch_by_size(const LinearParams& p, hipStream_t s)
 {
+    const int64_t work = most_row_tiles(p.g, 128) * ceil_div(GATED ? p.inter : p.n_out, GATED ? 64 : 128) * p.splits;
     if (p.size == TILES_256) launch_size<T, GATED, PTR, TILES_256>(p, s);
+    else if (work <= CUS) launch_size<T, GATED, PTR, TILES_128_ALONE>(p, s);
     else launch_size<T, GATED, PTR, TILES_128>(p, s);
 }
 

@@ -189,3 +189,13 @@ def test_the_largest_tiles(dev, act):
     rows = 3333
     check_product(make(g, FP16, rows, 2120), make(g, FP16, 2504, 2120, scale=0.05), None, None, None, act, 0.0,
                   make(g, FP16, rows, 1252 if act else 2504))
+
+
+@pytest.mark.parametrize("act", [None, "swiglu"])
+def test_many_small_tiles(dev, act):
+    """More tiles of 128 by 128 than CUs, in each direction, where those of 256 by 256 would leave CUs idle."""
+    g = torch.Generator().manual_seed(8)
+    counts = [(7 * e + 3) % 31 for e in range(40)] + [150]
+    x, w = make(g, BF16, sum(counts), 1016), make(g, BF16, len(counts), 1024, 1016, scale=0.05)
+    starts = torch.tensor([0] + counts).cumsum(0).int().to(dev)
+    check_product(x, w, make(g, BF16, len(counts), 1024), None, starts, act, 1.0 if act else 0.0, make(g, BF16, sum(counts), 512 if act else 1024))
