@@ -67,10 +67,10 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t k)
 // 7168 -> 18432: 51, 82, 188 against 56, 56, 62). For experts up to four rows for each, of which most may be another rank's, whatever
 // the experts' shares (64 experts, 7168 -> 4096, rows for four each: spread evenly 544 against 664, by Zipf's law 605 against 633, all
 // one expert's 84 against 134), but not for many workgroups that have little to sum (64 experts, 512 -> 1024: 33 against 18; 32, 1024
-// -> 768: 16 against 20).
-static bool few_rows(int rows, int k, int n, int experts, bool grouped)
+// -> 768: 16 against 20), unless tiles had to copy the weights (24, 333 -> 1000: 16 against 26).
+static bool few_rows(int rows, int k, int n, int experts, bool grouped, bool direct)
 {
-    if (grouped) return rows <= 4 * (int64_t)experts && (k >= 1024 || ceil_div(n, 16) * (int64_t)experts <= 1024);
+    if (grouped) return rows <= 4 * (int64_t)experts && (k >= 1024 || ceil_div(n, 16) * (int64_t)experts <= 1024 || !direct);
     if (rows > 64) return false;
     double tiles;
     plan_with(rows, n, k, tiles);
@@ -194,7 +194,7 @@ extern "C" size_t evamx_linear_workspace_bytes(int rows, int n_in, int n_out, in
 {
     set_error("%s", "");
     if (!sizes_ok("evamx_linear_workspace_bytes", rows, n_in, n_out, experts, grouped)) return 0;
-    if (few_rows(rows, n_in, n_out, experts, grouped)) return 0;
+    if (few_rows(rows, n_in, n_out, experts, grouped, direct)) return 0;
     return forward_part(rows, n_in, n_out, experts, grouped) + (direct ? 0 : forward_copies(rows, n_in, n_out, experts));
 }
 
@@ -234,7 +234,7 @@ extern "C" int evamx_linear(const evamx_linear_args* a, evamx_stream_t stream)
     p.act = a->act; p.limit = a->limit;
     p.splits = 1; p.stream = (int64_t)a->rows * cols * 2 > CACHE;
     const hipStream_t s = (hipStream_t)stream;
-    const bool few = few_rows(a->rows, a->n_in, a->n_out, a->experts, grouped);
+    const bool few = few_rows(a->rows, a->n_in, a->n_out, a->experts, grouped, xd && wd);
     if (!few) {
         char* at = (char*)a->workspace;
         int rc = ready(x, xd, a->rows, 1, a->n_in, at, s);
